@@ -22,7 +22,9 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-ta
 SOURCES = {"capi.hip": "fast", "density.hip": "fast", "cprad.hip": "fast", "densfac.hip": "fast", "node.hip": "fast",
            "edge.hip": "fast", "graph.hip": "off",
            "transport.hip": "fast", "radial.hip": "fast", "linear.hip": "fast",
-           "gemm.hip": "fast", "gemm_xs.hip": "fast", "gemm_split.hip": "fast", "gemm_op.hip": "fast", "densmix.hip": "fast"}
+           "gemm.hip": "fast", "gemm_xs.hip": "fast", "gemm_split.hip": "fast", "gemm_op.hip": "fast", "densmix.hip": "fast",
+           "norm.hip": "fast", "route.hip": "fast", "grouped.hip": "fast", "grouped_f32.hip": "fast",
+           "grouped_bf16.hip": "fast", "grouped_f16.hip": "fast", "grouped_e4m3.hip": "fast"}
 
 
 def compile_one(src):
@@ -41,7 +43,7 @@ def stale(src):
         return True
     t = os.path.getmtime(obj)
     return any(os.path.getmtime(os.path.join(HERE, f)) > t
-               for f in (src, "common.h", "edges.h", "densfac.h", "rows_gemm.h", "../../include/face_hip.h"))
+               for f in (src, "common.h", "edges.h", "densfac.h", "rows_gemm.h", "elem.h", "grouped.h", "../../include/face_hip.h"))
 
 
 def build(jobs=None, verbose=False, changed_only=False):

@@ -108,6 +108,23 @@ __device__ __forceinline__ v16f mfma_32x32x16(v8bf a, v8bf b, v16f c) {
 
 __device__ __forceinline__ v4f ld4(const float* p) { return *reinterpret_cast<const v4f*>(p); }
 
+// Logistic function (and one minus it) with the hardware exp2 and reciprocal, each corrected to first order:
+// e = exp(-x) from the rounded exponent t and what its rounding and that of log2(e) left over, 1 / (1 + e) by
+// one Newton step. Uncorrected, x < 0 came out 0.3 to 0.8 ulp too large on average (silu: mean -0.30 ulp,
+// rms 0.90). |x| is cut at 80, where exp(-|x|) is 2e-35 and all intermediate values are finite.
+__device__ __forceinline__ float gemm_sigmoid(float x, float& rest) {
+    constexpr float kL = 0x1.715476p+0f, kLow = 0x1.4ae0cp-26f;           // log2(e) = kL + kLow
+    const float a = __builtin_amdgcn_fmed3f(x, -80.f, 80.f), t = -kL * a;
+    const float lo = fmaf(-kLow, a, fmaf(-kL, a, -t));
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, 0.693147181f * lo, e);
+    const float d = 1.f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.f), r, r);
+    rest = e * r;
+    return r;
+}
+
 // float4 read of an LDS image (16-byte aligned base) at a float offset that is a multiple of 4:
 // one ds_read_b128. A plain pointer cast at a runtime offset leaves the alignment unknown to
 // the compiler, which then splits the read into 32-bit pairs (ds_read2_b32).

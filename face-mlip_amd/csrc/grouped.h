@@ -1,0 +1,753 @@
+// Products of rows with the weights of their group (gfx950): the slots of a plan, sorted by group, against
+// one weight matrix per group, ragged row counts that only the device knows.
+//
+//   forward        y[a] = op(x[a / xdiv]) W[g]^T + b[g]
+//   input gradient d[a] = (dy[a] W[g]) * op'(z[a / zdiv])
+//   weights        dW[g] = sum over the group's slots of dy[a]^T op(x[a / xdiv]),  db[g] = sum of dy[a]
+//
+// with a = order[i] the slot at place i of its group's range [ptr[g], ptr[g + 1]). Slots behind ptr[G] belong to
+// no group; their rows of y and d are written as zeros.
+//
+// A workgroup of four waves owns a tile of rows of ONE group and of output columns; which, it finds from ptr by a
+// wave-wide prefix sum of the groups' tile counts, so no launch waits for a count on the host. The grid holds the most
+// tiles that so many slots and groups can make; what is left over ends at once. Both operands go through
+// LDS in chunks along the sum, the next chunk's loads in registers during the present one's products:
+//   * 16-bit rows as they are, on v_mfma_f32_32x32x16; e4m3 rows on v_mfma_scale_f32_32x32x64_f8f6f4 at unit
+//     scales (twice the bf16 rate; fp32 results: see e4m3_wide), their row and column scales applied to the sum;
+//   * fp32 rows as three bf16 limbs, split once as they are staged, six products each (common.h);
+//   * an operand whose sum runs along its rows is read 16 bytes a lane; one whose sum runs down its columns (the
+//     weights of the input gradient, both operands of the weight gradient) is staged as it lies in memory and
+//     transposed by ds_read_b64_tr_b16 on the way to the matrix cores.
+// Where a launch has few tiles the four waves share one 32 x 32 tile and split every chunk's k among
+// them, joined in LDS at the end in a fixed order: such calls wait for memory, and eight times as many workgroups
+// have loads in flight.
+#pragma once
+#include "elem.h"
+
+namespace face {
+
+// 8-bit rows. The e4m3 instructions align the products of a step to the largest and cut what is below 2^-13 of it
+// (measured: errors up to 2^-10.4 of the largest product, one large among 63 small ones of a sign). Results of 16 bits
+// take them all the same: the operands' own rounding is 2^-4 of that product. Results in fp32 do not: e4m3_wide
+// rows become bf16 as they are staged, exactly, and their sums are fp32 sums, at the bf16 rate.
+struct e4m3 {
+    uint8_t v;
+};
+struct e4m3_wide {
+    uint8_t v;
+};
+
+struct GroupedArgs {
+    const void* x;                 // rows of the left operand (x, or dy of the input gradient)
+    int64_t ld_x;
+    int32_t xdiv;                  // its row of slot a is a / xdiv
+    int32_t x_op;                  // 1: silu as it loads
+    const void* w;
+    int64_t ld_w, w_group;         // strides between weight rows and groups
+    const void* bias;              // (G, ld_b) or null
+    int64_t ld_b;
+    const float *xs, *ws;          // e4m3: scale of every row of x, and (G, n) of the weights' rows
+    void* y;
+    int64_t ld_y;
+    const void* z;                 // op' of the input gradient: rows a / zdiv, or null
+    int64_t ld_z;
+    int32_t zdiv;
+    int32_t n, k;                  // output columns, length of the sum
+    const int32_t *ptr, *order;
+    int64_t slots;
+    int32_t groups;
+    int32_t col_tiles;
+    int64_t tiles;                 // row tiles the grid holds
+};
+
+struct GroupedWArgs {
+    const void* x;                 // (.., k) with silu as it loads if x_op
+    int64_t ld_x;
+    int32_t xdiv, x_op;
+    const void* dy;                // (slots, n)
+    int64_t ld_dy;
+    void* dw;                      // (G, n, k)
+    void* db;                      // (G, n) or null
+    float* part;                   // partial sums of the items of split groups, (n k [+ n]) each
+    int64_t part_items;            // how many it holds
+    int32_t n, k;
+    const int32_t *ptr, *order;
+    int64_t slots;
+    int32_t groups;
+    int32_t col_tiles, row_tiles;
+    int64_t items, chunk;          // (group, chunk of its slots) pairs the grid holds
+};
+
+// ---------------------------------------------------------------- operands
+template <typename T>
+struct Operand {                                 // bf16, f16: one plane of 16-byte chunks of eight
+    static constexpr int kPlanes = 1, kElems = 8;
+};
+template <>
+struct Operand<float> {                          // three bf16 limbs of eight values
+    static constexpr int kPlanes = 3, kElems = 8;
+};
+template <>
+struct Operand<e4m3> {
+    static constexpr int kPlanes = 1, kElems = 16;
+};
+template <typename T>
+constexpr bool kIsQ8 = __is_same(T, e4m3) || __is_same(T, e4m3_wide);
+
+// A 16-byte chunk's worth of a row (two 16-byte loads of fp32), in flight.
+template <typename T>
+struct Held {
+    v4u a;
+};
+template <>
+struct Held<float> {
+    v4u a, b;
+};
+template <>
+struct Held<e4m3_wide> {
+    uint64_t a;
+};
+
+// The elements [0, left) of the chunk at p, zero beyond.
+template <typename T>
+__device__ __forceinline__ Held<T> hold(const T* p, int left) {
+    Held<T> h = {};
+    constexpr int E = Operand<T>::kElems;
+    if (left >= E) {
+        if constexpr (__is_same(T, e4m3_wide)) {
+            typedef uint64_t any __attribute__((aligned(1)));
+            h.a = *reinterpret_cast<const any*>(p);
+        } else {
+            h.a = ld16(p);
+            if constexpr (sizeof(T) == 4) h.b = ld16(p + 4);
+        }
+    } else if (left > 0) {
+        if constexpr (__is_same(T, e4m3_wide)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) h.a |= (uint64_t)p[e].v << (8 * e);
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t v = e < left ? __builtin_bit_cast(uint32_t, p[e]) : 0u;
+                if (e < 4) h.a[e & 3] = v;
+                else h.b[e & 3] = v;
+            }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) h.a[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (e < left) h.a[e >> 2] |= (uint32_t)p[e].v << (8 * (e & 3));
+        }
+    }
+    return h;
+}
+
+__device__ __forceinline__ float silu(float x) {
+    float rest;
+    return x * gemm_sigmoid(x, rest);
+}
+__device__ __forceinline__ float silu_slope(float x) {
+    float rest;
+    const float s = gemm_sigmoid(x, rest);
+    return s * fmaf(x, rest, 1.f);
+}
+
+// silu in fp32; a 16-bit operand is rounded once more, as it enters the matrix cores.
+template <typename T>
+__device__ __forceinline__ void apply_silu(Held<T>& h) {
+    if constexpr (sizeof(T) == 4) {
+        v4f a = __builtin_bit_cast(v4f, h.a), b = __builtin_bit_cast(v4f, h.b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            a[e] = silu(a[e]);
+            b[e] = silu(b[e]);
+        }
+        h.a = __builtin_bit_cast(v4u, a);
+        h.b = __builtin_bit_cast(v4u, b);
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a, b;
+            unpack2<T>(h.a[e], a, b);
+            h.a[e] = pack2<T>(silu(a), silu(b));
+        }
+    }
+}
+
+// Writes the planes of a held chunk `plane` bytes apart.
+template <typename T>
+__device__ __forceinline__ void put(char* at, int plane, const Held<T>& h) {
+    if constexpr (sizeof(T) == 4) {
+        const Split8 s = split8(__builtin_bit_cast(v4f, h.a), __builtin_bit_cast(v4f, h.b));
+        *reinterpret_cast<v8bf*>(at) = s.h;
+        *reinterpret_cast<v8bf*>(at + plane) = s.m;
+        *reinterpret_cast<v8bf*>(at + 2 * plane) = s.l;
+    } else if constexpr (__is_same(T, e4m3_wide)) {
+        const int lo = (int)(uint32_t)h.a, hi = (int)(uint32_t)(h.a >> 32);
+        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
+        const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+        *reinterpret_cast<v4u*>(at) = (v4u){bf16_pair(a[0], a[1]), bf16_pair(b[0], b[1]), bf16_pair(c[0], c[1]), bf16_pair(d[0], d[1])};
+    } else {
+        *reinterpret_cast<v4u*>(at) = h.a;
+    }
+}
+
+// ---------------------------------------------------------------- LDS tiles
+// R rows of C chunks of 16 bytes. Chunks are moved within a row by an XOR with the row number so that the
+// lanes of an access meet different banks: ROWS tiles are read one chunk a lane down 32 rows, COLS tiles by the
+// transposing read, four rows of two chunks per 16 lanes.
+template <int R, int C, bool COLS>
+struct Tile {
+    static constexpr int kBytes = R * C * 16;
+    __device__ static __forceinline__ int at(int row, int chunk) {
+        int f;
+        if constexpr (COLS)
+            f = C >= 16 ? ((row & 1) << 2) ^ ((row & 2) ? 10 : 0) : (row & 2);
+        else
+            f = C >= 16 ? (row & 15) : (C == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1));
+        return (row * C + (chunk ^ f)) * 16;
+    }
+};
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4s read_tr(const char* lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)lds);
+}
+
+// One lane's eight elements of the 32 x 16 operand at (row i0, element k0): lane i + 32 h holds k0 + 8 h .. + 7 of
+// row i0 + i. A COLS tile holds k down its rows: 16 lanes fetch a 4 x 16 block and receive its transpose.
+template <int R, int C, bool COLS>
+__device__ __forceinline__ v4u fragment(const char* tile, int i0, int k0, int lane) {
+    if constexpr (!COLS) {
+        return *reinterpret_cast<const v4u*>(tile + Tile<R, C, false>::at(i0 + (lane & 31), (k0 >> 3) + (lane >> 5)));
+    } else {
+        const int t = lane & 15, q = lane >> 4;
+        const int k = k0 + 8 * (q >> 1) + (t >> 2), col = i0 + 16 * (q & 1) + 4 * (t & 3);
+        const v4s a = read_tr(tile + Tile<R, C, true>::at(k, col >> 3) + 2 * (col & 7));
+        const v4s b = read_tr(tile + Tile<R, C, true>::at(k + 4, col >> 3) + 2 * (col & 7));
+        typedef short v8s __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(v4u, (v8s)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+typedef f16 v8h __attribute__((ext_vector_type(8)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ v16f mfma16(v4u a, v4u b, v16f c) {
+    if constexpr (__is_same(T, f16))
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else
+        return mfma_32x32x16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c);
+}
+
+// The products of one chunk: MT x NT tiles of 32 x 32, elements [k_begin, k_end) of the chunk.
+template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT>
+__device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int k_end,
+                                               int lane, v16f acc[MT][NT]) {
+    constexpr int PA = Tile<RA, CA, COLS_A>::kBytes, PB = Tile<RB, CB, COLS_B>::kBytes;
+    if constexpr (__is_same(T, e4m3)) {
+        for (int k0 = k_begin; k0 < k_end; k0 += 64) {
+            // each half of the wave takes 32 neighbouring elements of its row
+            v8i a[MT], b[NT];
+            const int c = (k0 >> 4) + 2 * (lane >> 5);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int r = m0 + 32 * m + (lane & 31);
+                reinterpret_cast<v4u*>(&a[m])[0] = *reinterpret_cast<const v4u*>(ta + Tile<RA, CA, false>::at(r, c));
+                reinterpret_cast<v4u*>(&a[m])[1] = *reinterpret_cast<const v4u*>(ta + Tile<RA, CA, false>::at(r, c + 1));
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = n0 + 32 * n + (lane & 31);
+                reinterpret_cast<v4u*>(&b[n])[0] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(r, c));
+                reinterpret_cast<v4u*>(&b[n])[1] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(r, c + 1));
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[m], b[n], acc[m][n], 0, 0, 0, 0x7f7f7f7f, 0,
+                                                                                0x7f7f7f7f);
+        }
+    } else {
+        constexpr int P = Operand<T>::kPlanes;
+#pragma unroll
+        for (int k0 = k_begin; k0 < k_end; k0 += 16) {
+            v4u a[P][MT], b[P][NT];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) a[p][m] = fragment<RA, CA, COLS_A>(ta + p * PA, m0 + 32 * m, k0, lane);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) b[p][n] = fragment<RB, CB, COLS_B>(tb + p * PB, n0 + 32 * n, k0, lane);
+            }
+            // limb products from the smallest up; of one instruction after another none waits for the one before
+            constexpr int kProducts = P == 3 ? 6 : 1;
+            constexpr int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};
+#pragma unroll
+            for (int q = 0; q < kProducts; ++q)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[m][n] = mfma16<T>(a[P == 3 ? pa[q] : 0][m], b[P == 3 ? pb[q] : 0][n], acc[m][n]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- which rows a workgroup owns
+__device__ __forceinline__ int64_t clamp_slot(int64_t v, int64_t slots) { return v < 0 ? 0 : (v > slots ? slots : v); }
+
+struct Range {
+    int group;                     // `groups`: the slots of no group; -1: nothing
+    int64_t begin, end;            // its places in order
+    int64_t index;                 // of this piece among the group's
+    int64_t pieces;                // of the group
+    int64_t split_before;          // pieces of the earlier groups that have more than one
+};
+// The t-th piece of `size` places of the groups 0 .. last, at least `least` for each group. The same in all threads.
+__device__ __forceinline__ Range find_piece(const int32_t* ptr, int last, int groups, int64_t slots, int64_t size,
+                                            int least, int64_t t) {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0, split = 0;
+    for (int g0 = 0; g0 <= last; g0 += 64) {
+        const int g = g0 + lane;
+        int64_t b = 0, e = 0;
+        if (g <= last) {
+            b = clamp_slot(ptr[g], slots);
+            e = g < groups ? clamp_slot(ptr[g + 1], slots) : slots;
+        }
+        int c = e > b ? (int)((e - b + size - 1) / size) : 0;
+        if (g <= last && c < least) c = least;
+        int s = c, m = c > 1 ? c : 0;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(s, o, 64), v = __shfl_up(m, o, 64);
+            if (lane >= o) {
+                s += u;
+                m += v;
+            }
+        }
+        const int total = __shfl(s, 63, 64), total_m = __shfl(m, 63, 64);
+        if (t < before + total) {
+            const uint64_t at = __ballot(before + s > t);
+            const int l = __builtin_ctzll(at);
+            const int cl = __shfl(c, l, 64);
+            Range r;
+            r.group = g0 + l;
+            r.begin = __shfl(b, l, 64);
+            r.end = __shfl(e, l, 64);
+            r.index = t - (before + __shfl(s, l, 64) - cl);
+            r.pieces = cl;
+            r.split_before = split + __shfl(m, l, 64) - (cl > 1 ? cl : 0);
+            return r;
+        }
+        before += total;
+        split += total_m;
+    }
+    return {-1, 0, 0, 0, 0, 0};
+}
+
+// Workgroups that follow each other on one XCD (every eighth) take neighbouring items, so that tiles of the same
+// rows and of the same weights meet in its L2.
+__device__ __forceinline__ int64_t xcd_item(int64_t items) {
+    const int64_t b = blockIdx.x, per = items / 8, rest = items % 8, x = b % 8;
+    return x * per + (x < rest ? x : rest) + b / 8;
+}
+
+// ---------------------------------------------------------------- forward and input gradient
+// WM x WN x WK waves of MT x NT tiles. COLS_B: the weights lie (sum, column), as the input gradient reads them.
+template <typename T, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
+struct RowsKernel {
+    using Op = Operand<T>;
+    static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, BK = C * Op::kElems, P = Op::kPlanes;
+    static constexpr int kThreads = 64 * WM * WN * WK;
+    static constexpr int CB = COLS_B ? BN / 8 : C, RB = COLS_B ? BK : BN;
+    using TA = Tile<BM, C, false>;
+    using TB = Tile<RB, CB, COLS_B>;
+    static constexpr int kLdsA = P * TA::kBytes, kLdsB = P * TB::kBytes;
+    static constexpr int kLdsJoin = WK > 1 ? WK * BM * BN * 4 : 0;
+    static constexpr int kLds = kLdsA + kLdsB > kLdsJoin ? kLdsA + kLdsB : kLdsJoin;
+    static constexpr int NA = BM * C / kThreads, NB = RB * CB / kThreads;   // chunks per thread
+    static_assert(NA * kThreads == BM * C && NB * kThreads == RB * CB, "whole rounds of chunks");
+};
+
+// Out-of-range sums of limbs: a value past bf16's largest, or an infinity, has a NaN limb, so a sum that
+// is not finite is formed again from the fp32 operands.
+__device__ inline float plain_sum(const float* x, const float* w, int64_t step, int k, int op) {
+    float s = 0.f;
+    for (int i = 0; i < k; ++i) s = fmaf(op ? silu(x[i]) : x[i], w[i * step], s);
+    return s;
+}
+
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
+__global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThreads), 2) void grouped_rows_kernel(
+    GroupedArgs g) {
+    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
+    __shared__ __attribute__((aligned(256))) char lds[K::kLds];
+    __shared__ int32_t slot_of[K::BM];
+    const int64_t item = xcd_item(g.tiles * g.col_tiles);
+    const int col0 = (int)(item % g.col_tiles) * K::BN;
+    const Range r = find_piece(g.ptr, g.groups, g.groups, g.slots, K::BM, 0, item / g.col_tiles);
+    if (r.group < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t place0 = r.begin + r.index * K::BM;
+    for (int i = tid; i < K::BM; i += K::kThreads) {
+        int32_t a = -1;
+        if (place0 + i < r.end) a = g.order[place0 + i];
+        slot_of[i] = a >= 0 && a < g.slots ? a : -1;
+    }
+    __syncthreads();
+    Out* y = (Out*)g.y;
+    if (r.group == g.groups) {
+        for (int i = wave; i < K::BM; i += K::kThreads / 64) {
+            const int32_t a = slot_of[i];
+            if (a < 0) continue;
+            for (int c = lane; c < K::BN; c += 64)
+                if (col0 + c < g.n) y[a * g.ld_y + col0 + c] = from_f<Out>(0.f);
+        }
+        return;
+    }
+    const T* w = (const T*)g.w + r.group * g.w_group;
+    const T* x = (const T*)g.x;
+
+    // this thread's chunks: rows of x by their slots, rows of the weights by column (or by place in the sum)
+    const T* ap[K::NA];
+    int a_row[K::NA], b_row[K::NB];
+    const int a_col = (tid % C) * K::Op::kElems, b_chunk = tid % K::CB;
+#pragma unroll
+    for (int i = 0; i < K::NA; ++i) {
+        a_row[i] = tid / C + i * (K::kThreads / C);
+        const int32_t a = slot_of[a_row[i]];
+        ap[i] = a < 0 ? nullptr : x + (int64_t)(a / g.xdiv) * g.ld_x + a_col;
+    }
+#pragma unroll
+    for (int i = 0; i < K::NB; ++i) b_row[i] = tid / K::CB + i * (K::kThreads / K::CB);
+
+    Held<T> ha[K::NA], hb[K::NB];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0, ap[i] ? g.k - k0 - a_col : 0);
+#pragma unroll
+        for (int i = 0; i < K::NB; ++i) {
+            if constexpr (COLS_B) {
+                const int col = col0 + 8 * b_chunk, row = k0 + b_row[i];
+                hb[i] = hold(w + row * g.ld_w + col, row < g.k ? g.n - col : 0);
+            } else {
+                const int col = k0 + b_chunk * K::Op::kElems, row = col0 + b_row[i];
+                hb[i] = hold(w + row * g.ld_w + col, row < g.n ? g.k - col : 0);
+            }
+        }
+    };
+    v16f acc[MT][NT] = {};
+    const int wk = wave % WK, wn = wave / WK % WN, wm = wave / WK / WN;
+    fetch(0);
+    for (int k0 = 0; k0 < g.k; k0 += K::BK) {
+        if (g.x_op) {
+#pragma unroll
+            for (int i = 0; i < K::NA; ++i) apply_silu(ha[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < K::NA; ++i) put(lds + K::TA::at(a_row[i], tid % C), K::TA::kBytes, ha[i]);
+#pragma unroll
+        for (int i = 0; i < K::NB; ++i) put(lds + K::kLdsA + K::TB::at(b_row[i], b_chunk), K::TB::kBytes, hb[i]);
+        __syncthreads();
+        if (k0 + K::BK < g.k) fetch(k0 + K::BK);
+        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT>(lds, lds + K::kLdsA, 32 * MT * wm, 32 * NT * wn,
+                                                                        wk * (K::BK / WK), (wk + 1) * (K::BK / WK), lane, acc);
+        __syncthreads();
+    }
+
+    if constexpr (WK > 1) {
+        // one tile per wave: its part of every sum to LDS, then each wave finishes a share of the rows
+        static_assert(WM == 1 && WN == 1 && MT == 1 && NT == 1 && WK == 4, "split chunks: one tile");
+        float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) part[(wave * 16 + q) * 64 + lane] = acc[0][0][q];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float s = 0.f;
+#pragma unroll
+            for (int v = 0; v < WK; ++v) s += part[(v * 16 + 4 * wave + q) * 64 + lane];
+            acc[0][0][q] = s;
+        }
+    }
+    // D[8 (q >> 2) + 4 (lane >> 5) + (q & 3)][lane & 31] in register q; after a join wave w holds registers 4 w .. 4 w + 3
+    constexpr int kRegs = WK > 1 ? 4 : 16;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int col = col0 + 32 * (NT * wn + n) + (lane & 31);
+        if (col >= g.n) continue;
+        const float b = g.bias ? to_f(((const Out*)g.bias)[r.group * g.ld_b + col]) : 0.f;
+        const float sw = kIsQ8<T> ? g.ws[(int64_t)r.group * g.n + col] : 1.f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int q = 0; q < kRegs; ++q) {
+                const int row = 32 * (MT * wm + m) + 8 * (WK > 1 ? wave : q >> 2) + 4 * (lane >> 5) + (q & 3);
+                const int32_t a = slot_of[row];
+                if (a < 0) continue;
+                float v = acc[m][n][q];
+                if constexpr (__is_same(T, float)) {
+                    if (!(__builtin_fabsf(v) <= 0x1.fffffep+127f))
+                        v = plain_sum((const float*)x + (int64_t)(a / g.xdiv) * g.ld_x,
+                                      (const float*)w + (COLS_B ? col : col * g.ld_w), COLS_B ? g.ld_w : 1, g.k, g.x_op);
+                }
+                if constexpr (kIsQ8<T>) v *= g.xs[a / g.xdiv] * sw;
+                v += b;
+                if constexpr (COLS_B)
+                    if (g.z) v *= silu_slope(to_f(((const Out*)g.z)[(int64_t)(a / g.zdiv) * g.ld_z + col]));
+                y[a * g.ld_y + col] = from_f<Out>(v);
+            }
+    }
+}
+
+// ---------------------------------------------------------------- weight gradient
+// 128 x 128 tiles (n, k) of one group, the sum down a chunk of its slots. Groups of one chunk write their result, the
+// others partial sums for grouped_join_kernel, in the order of their slots: no atomics.
+template <typename T>
+struct WeightKernel {
+    using Op = Operand<T>;
+    static constexpr int P = Op::kPlanes, BK = P == 3 ? 32 : 64, kThreads = 256, CT = 16;
+    using TT = Tile<BK, CT, true>;
+    static constexpr int kLds = 2 * P * TT::kBytes, NC = BK * CT / kThreads;
+};
+
+__device__ inline float plain_dot(const float* dy, int64_t ld_dy, const float* x, int64_t ld_x, int xdiv, int op,
+                                  const int32_t* order, int64_t begin, int64_t end, int64_t slots) {
+    float s = 0.f;
+    for (int64_t i = begin; i < end; ++i) {
+        const int32_t a = order[i];
+        if (a < 0 || a >= slots) continue;
+        const float v = x[(int64_t)(a / xdiv) * ld_x];
+        s = fmaf(dy[a * ld_dy], op ? silu(v) : v, s);
+    }
+    return s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupedWArgs g) {
+    using K = WeightKernel<T>;
+    __shared__ __attribute__((aligned(256))) char lds[K::kLds];
+    const int64_t per = (int64_t)g.row_tiles * g.col_tiles;
+    const int64_t item = xcd_item(g.items * per);
+    const Range r = find_piece(g.ptr, g.groups - 1, g.groups, g.slots, g.chunk, 1, item / per);
+    if (r.group < 0) return;
+    const int row0 = (int)(item % per / g.col_tiles) * 128, col0 = (int)(item % g.col_tiles) * 128;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = tid % K::CT;
+    const int64_t p0 = r.begin + r.index * g.chunk;
+    const int64_t p1 = p0 + g.chunk < r.end ? p0 + g.chunk : r.end;
+    const T *x = (const T*)g.x, *dy = (const T*)g.dy;
+    const int ca = row0 + 8 * chunk, cb = col0 + 8 * chunk;
+    const bool sums = g.db && col0 == 0;
+    // a plan whose ranges overlap can name more split pieces than its slots can make: they have no place
+    if (r.pieces > 1 && r.split_before + r.index >= g.part_items) return;
+    float colsum[8] = {};
+
+    Held<T> ha[K::NC], hb[K::NC];
+    int32_t next[K::NC];
+    auto find = [&](int64_t p) {
+#pragma unroll
+        for (int i = 0; i < K::NC; ++i) {
+            const int64_t at = p + tid / K::CT + i * (K::kThreads / K::CT);
+            next[i] = at < p1 ? g.order[at] : -1;
+        }
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < K::NC; ++i) {
+            const int32_t a = next[i];
+            const bool ok = a >= 0 && a < g.slots;
+            ha[i] = hold(dy + (ok ? a * g.ld_dy + ca : 0), ok ? g.n - ca : 0);
+            hb[i] = hold(x + (ok ? (int64_t)(a / g.xdiv) * g.ld_x + cb : 0), ok ? g.k - cb : 0);
+        }
+    };
+    v16f acc[2][2] = {};
+    const int wn = wave & 1, wm = wave >> 1;
+    find(p0);
+    fetch();
+    find(p0 + K::BK);
+    for (int64_t p = p0; p < p1; p += K::BK) {
+        if (g.x_op) {
+#pragma unroll
+            for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+        }
+        if (sums) {
+#pragma unroll
+            for (int i = 0; i < K::NC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (sizeof(T) == 4) {
+                        colsum[e] += __builtin_bit_cast(v4f, ha[i].a)[e];
+                        colsum[4 + e] += __builtin_bit_cast(v4f, ha[i].b)[e];
+                    } else {
+                        float u, v;
+                        unpack2<T>(ha[i].a[e], u, v);
+                        colsum[2 * e] += u;
+                        colsum[2 * e + 1] += v;
+                    }
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < K::NC; ++i) {
+            const int at = K::TT::at(tid / K::CT + i * (K::kThreads / K::CT), chunk);
+            put(lds + at, K::TT::kBytes, ha[i]);
+            put(lds + K::P * K::TT::kBytes + at, K::TT::kBytes, hb[i]);
+        }
+        __syncthreads();
+        if (p + K::BK < p1) {
+            fetch();
+            find(p + 2 * K::BK);
+        }
+        chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2>(lds, lds + K::P * K::TT::kBytes, 64 * wm, 64 * wn, 0,
+                                                                        K::BK, lane, acc);
+        __syncthreads();
+    }
+    const int64_t stride = (int64_t)g.n * g.k + (g.db ? g.n : 0);
+    float* part = r.pieces > 1 ? g.part + (r.split_before + r.index) * stride : nullptr;
+    T* dw = (T*)g.dw + (int64_t)r.group * g.n * g.k;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int col = col0 + 64 * wn + 32 * n + (lane & 31);
+        if (col >= g.k) continue;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const int row = row0 + 64 * wm + 32 * m + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3);
+                if (row >= g.n) continue;
+                float v = acc[m][n][q];
+                if constexpr (__is_same(T, float)) {
+                    if (!(__builtin_fabsf(v) <= 0x1.fffffep+127f))
+                        v = plain_dot((const float*)dy + row, g.ld_dy, (const float*)x + col, g.ld_x, g.xdiv, g.x_op, g.order, p0,
+                                      p1, g.slots);
+                }
+                if (part)
+                    part[(int64_t)row * g.k + col] = v;
+                else
+                    dw[(int64_t)row * g.k + col] = from_f<T>(v);
+            }
+    }
+    if (sums) {
+        float* red = reinterpret_cast<float*>(lds);          // 16 threads per chunk of eight columns
+#pragma unroll
+        for (int e = 0; e < 8; ++e) red[(tid / K::CT) * 128 + 8 * chunk + e] = colsum[e];
+        __syncthreads();
+        if (tid < 128 && row0 + tid < g.n) {
+            float s = 0.f;
+            for (int i = 0; i < K::kThreads / K::CT; ++i) s += red[i * 128 + tid];
+            if (part)
+                part[(int64_t)g.n * g.k + row0 + tid] = s;
+            else
+                ((T*)g.db)[(int64_t)r.group * g.n + row0 + tid] = from_f<T>(s);
+        }
+    }
+}
+
+// dW and db of the groups with several chunks: their partial sums, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_join_kernel(GroupedWArgs g) {
+    __shared__ int64_t first, count;
+    const int group = blockIdx.y;
+    if (threadIdx.x < 64) {
+        int64_t before = 0, mine = 0;
+        for (int e0 = 0; e0 <= group; e0 += 64) {
+            const int e = e0 + (int)threadIdx.x;
+            int64_t c = 0;
+            if (e <= group) {
+                const int64_t b = clamp_slot(g.ptr[e], g.slots), d = clamp_slot(g.ptr[e + 1], g.slots);
+                c = d > b ? (d - b + g.chunk - 1) / g.chunk : 0;
+            }
+            if (e == group) mine = c;
+            int m = c > 1 && e < group ? (int)c : 0;
+            for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
+            before += m;
+        }
+        for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
+        if (threadIdx.x == 0) {
+            first = before;
+            count = mine;
+        }
+    }
+    __syncthreads();
+    if (count <= 1 || first + count > g.part_items) return;
+    const int64_t nk = (int64_t)g.n * g.k, stride = nk + (g.db ? g.n : 0);
+    const float* part = g.part + first * stride;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < stride; i += (int64_t)gridDim.x * 256) {
+        float s = 0.f;
+#pragma unroll 4
+        for (int64_t c = 0; c < count; ++c) s += part[c * stride + i];
+        if (i < nk)
+            ((T*)g.dw)[group * nk + i] = from_f<T>(s);
+        else
+            ((T*)g.db)[(int64_t)group * g.n + i - nk] = from_f<T>(s);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+// Instantiated per element type in a file of its own (grouped_f32.hip, ...).
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
+static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
+    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
+    const int64_t most = g.groups + (int64_t)1;
+    g.tiles = g.slots / K::BM + (most < g.slots ? most : g.slots);
+    g.col_tiles = (g.n + K::BN - 1) / K::BN;
+    const int64_t grid = g.tiles * g.col_tiles;
+    if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C>), dim3((unsigned)grid), dim3(K::kThreads),
+                       0, st, g);
+    FACE_LAUNCH_CHECK();
+    return 0;
+}
+
+// Tiles of 128 x 128 once there is about one for every CU, else of 32 x 32 with the sum split over the waves.
+constexpr int64_t kLargeTiles = 256;
+
+template <typename T, typename Out, bool COLS_B>
+int launch_rows(GroupedArgs g, hipStream_t st) {
+    const int64_t groups = g.groups < g.slots ? g.groups : g.slots;
+    const int64_t large = (g.slots / 128 + groups) * ((g.n + 127) / 128);
+    constexpr int C = sizeof(T) == 4 ? 4 : 8, CS = sizeof(T) == 4 ? 16 : 32;
+    if (large >= kLargeTiles) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C>(g, st);
+    return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, CS>(g, st);
+}
+
+// Slots per chunk of the weight gradient: enough chunks for about 2048 workgroups, at most 64 (each adds a partial
+// result to write and to read), of 512 slots at least.
+static inline int64_t weight_chunk(int64_t slots, int n, int k) {
+    const int64_t tiles = (int64_t)((n + 127) / 128) * ((k + 127) / 128);
+    int64_t chunks = 2048 / tiles;
+    chunks = chunks < 4 ? 4 : (chunks > 64 ? 64 : chunks);
+    const int64_t c = (slots + chunks - 1) / chunks;
+    return c < 512 ? 512 : (c + 127) / 128 * 128;
+}
+// Pieces of the groups with more than one chunk, at most.
+static inline int64_t weight_part_items(int64_t slots, int groups, int64_t chunk) {
+    const int64_t split = slots / (chunk + 1);               // groups of more than a chunk
+    return split ? slots / chunk + (groups < split ? groups : split) : 0;
+}
+
+template <typename T>
+int launch_weight(GroupedWArgs g, hipStream_t st) {
+    g.row_tiles = (g.n + 127) / 128;
+    g.col_tiles = (g.k + 127) / 128;
+    g.items = g.slots / g.chunk + g.groups;
+    const int64_t grid = g.items * g.row_tiles * g.col_tiles;
+    if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(grouped_weight_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, g);
+    FACE_LAUNCH_CHECK();
+    if (g.slots > g.chunk) {
+        const int64_t blocks = ((int64_t)g.n * g.k + 1023) / 1024;
+        hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096), g.groups), dim3(256), 0, st,
+                           g);
+        FACE_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+}  // namespace face

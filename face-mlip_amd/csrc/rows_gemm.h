@@ -74,22 +74,6 @@ __device__ __forceinline__ v4f flip_sign(v4f v, uint32_t sign) {
     return __builtin_bit_cast(v4f, __builtin_bit_cast(v4u, v) ^ sign);
 }
 
-// Logistic function (and one minus it) with the hardware exp2 and reciprocal, each corrected to first order:
-// e = exp(-x) from the rounded exponent t and what its rounding and that of log2(e) left over, 1 / (1 + e) by
-// one Newton step. Uncorrected, x < 0 came out 0.3 to 0.8 ulp too large on average (silu: mean -0.30 ulp,
-// rms 0.90). |x| is cut at 80, where exp(-|x|) is 2e-35 and all intermediate values are finite.
-__device__ __forceinline__ float gemm_sigmoid(float x, float& rest) {
-    constexpr float kL = 0x1.715476p+0f, kLow = 0x1.4ae0cp-26f;           // log2(e) = kL + kLow
-    const float a = __builtin_amdgcn_fmed3f(x, -80.f, 80.f), t = -kL * a;
-    const float lo = fmaf(-kLow, a, fmaf(-kL, a, -t));
-    float e = __builtin_amdgcn_exp2f(t);
-    e = fmaf(e, 0.693147181f * lo, e);
-    const float d = 1.f + e;
-    float r = __builtin_amdgcn_rcpf(d);
-    r = fmaf(fmaf(-d, r, 1.f), r, r);
-    rest = e * r;
-    return r;
-}
 __device__ __forceinline__ float gemm_op(float x, float z, int op) {
     float rest;
     if (op == 1) return x * gemm_sigmoid(x, rest);

@@ -88,9 +88,27 @@ _SIGS = {
     "face_eq_gate_bwd": (ctypes.c_int, [P, P, P, P, P, I64, I32, P, P, P, P]),
     "face_layer_norm_fwd": (ctypes.c_int, [P, I64, I32, P, P, ctypes.c_float, P, P, P, P]),
     "face_layer_norm_bwd": (ctypes.c_int, [P, P, I64, I32, P, P, P, P, P]),
+    "face_rms_norm_fwd": (ctypes.c_int, [P, I64, P, I64, I64, I32, I32, P, F32, P, P, P, P, P]),
+    "face_rms_norm_bwd_work": (I64, [I64, I32]),
+    "face_rms_norm_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, I64, I32, I32, P, F32, P, P, P, I64, P]),
+    "face_quantize_rows": (ctypes.c_int, [P, I64, I64, I32, I32, I32, P, P, P]),
+    "face_route_fwd": (ctypes.c_int, [P, I64, I64, I32, I32, I32, P, P, I32, I32, P, P, P]),
+    "face_route_bwd": (ctypes.c_int, [P, I64, I64, I32, I32, I32, P, P, I32, I32, P, P, P, P, P]),
+    "face_group_plan_work": (I64, [I64, I32]),
+    "face_group_plan": (ctypes.c_int, [P, I64, I32, P, P, P, I64, P]),
+    "face_grouped_linear": (ctypes.c_int, [P, I64, I32, I32, P, I64, I64, P, I64, P, P, I64, I32, I32, I32, I32, P, I64,
+                                           P]),
+    "face_grouped_linear_q8": (ctypes.c_int, [P, I64, P, I32, P, I64, I64, P, P, I64, P, P, I64, I32, I32, I32, I32, P,
+                                              I64, P]),
+    "face_grouped_linear_dx": (ctypes.c_int, [P, I64, P, I64, I64, P, I64, I32, P, P, I64, I32, I32, I32, I32, P, I64,
+                                              P]),
+    "face_grouped_linear_dw_work": (I64, [I64, I32, I32, I32, I32]),
+    "face_grouped_linear_dw": (ctypes.c_int, [P, I64, I32, I32, P, I64, P, P, I64, I32, I32, I32, I32, P, P, P, I64, P]),
+    "face_expert_combine_fwd": (ctypes.c_int, [P, I64, P, P, I64, I64, I32, I32, I32, P, P]),
+    "face_expert_combine_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, I32, I32, I32, P, P, P]),
 }
 
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 
 class LinProblem(ctypes.Structure):

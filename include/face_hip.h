@@ -7,7 +7,8 @@
  *   - Return value: 0 on success, a positive hipError_t from the launch, or a negative
  *     FACE_ERR_* code for an argument the kernels cannot serve. face_hip_error_string()
  *     names either kind.
- *   - Floating point data are fp32, row-major; `ld_*` arguments are row strides in elements.
+ *   - Floating point data are fp32, row-major; `ld_*` arguments are row strides in elements. The expert
+ *     layer's entries (last section) also take 16-bit and e4m3 rows, named by a dtype argument.
  *   - Edge lists are grouped by receiver atom i. `row_ptr` (N+1, int32) gives row i as edges
  *     [row_ptr[i], row_ptr[i+1]); row_ptr == NULL means the reference's padded-dense layout
  *     (N, M): row i is edges [i*M, (i+1)*M), masked slots included (their radial weight is 0).
@@ -543,6 +544,79 @@ int face_edge_geom_bwd_seg(const float* pos, const int32_t* recv, const int32_t*
                            const float* const* gr, float* gvec_rev, float* wsum, void* stream);
 int face_force_scatter_rows(const float* gvec_rev, const float* wsum, const int32_t* row_ptr, int64_t N,
                             int32_t mean_row, float sign, float* grad, void* stream);
+
+/* ---------------------------------------------------------------- expert layer
+ * Layers whose weights depend on the atom's species or on a learned gate: the norm before them, the
+ * gate, the grouping of the rows, the products and the join. No counterpart in the reference, whose
+ * per-element parameters are scale tables (face/model.py:498-501). Rows have unit column stride, any
+ * row stride >= their width and any alignment of their type; widths need not be multiples of anything. `dtype`
+ * names the type of every `void*` operand that no other type is given for. */
+enum { FACE_F32 = 0, FACE_BF16 = 1, FACE_F16 = 2 };
+
+/* s = x + r (rounded to the rows' type; r and s NULL: s is x), then y (N, F) = s w / sqrt(mean(s^2) + eps),
+ * or, with q and scale in place of y, that row in e4m3: scale (N) = max(max|y| / 448, 2^-126), q = y / scale.
+ * Statistics in fp32. w (F); y, s and q dense. F <= 65536. */
+int face_rms_norm_fwd(const void* x, int64_t ld_x, const void* r, int64_t ld_r, int64_t N, int32_t F, int32_t dtype,
+                      const void* w, float eps, void* y, void* s, void* q, float* scale, void* stream);
+/* dx (N, F) = gradient of s (so of x and of r) for dy and the gradient ds that arrives at s itself
+ * (either may be NULL = 0); dw (F). Either output may be NULL. work: face_rms_norm_bwd_work bytes, for dw. Fixed
+ * summation order. */
+int64_t face_rms_norm_bwd_work(int64_t N, int32_t F);
+int face_rms_norm_bwd(const void* s, int64_t ld_s, const void* dy, int64_t ld_dy, const void* ds, int64_t ld_ds,
+                      int64_t N, int32_t F, int32_t dtype, const void* w, float eps, void* dx, void* dw, void* work,
+                      int64_t work_bytes, void* stream);
+/* q (N, F) e4m3 and scale (N) of op(x) as above; x_op 0 none, 1 silu. */
+int face_quantize_rows(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_t dtype, int32_t x_op, void* q,
+                       float* scale, void* stream);
+
+/* Gate: the k <= 16 largest of a row's E <= 1024 logits, in descending order, ties to the lower expert, among
+ * the experts that row group[i] of allowed (n_groups, E) bytes opens (allowed NULL: all; group NULL: row 0 of
+ * one; a group outside [0, n_groups): none) and whose logit is above -inf. weight (N, k) = softmax over
+ * the open experts, or (renorm) over the chosen ones. Where fewer than k are open: expert -1, weight 0. A NaN
+ * counts as the largest logit and makes the row's weights NaN. */
+int face_route_fwd(const void* logits, int64_t ld, int64_t N, int32_t E, int32_t k, int32_t dtype,
+                   const uint8_t* allowed, const int32_t* group, int32_t n_groups, int32_t renorm, int32_t* expert,
+                   float* weight, void* stream);
+/* dlogits (N, E) dense, for dweight (N, k); expert and weight as the forward wrote them. */
+int face_route_bwd(const void* logits, int64_t ld, int64_t N, int32_t E, int32_t k, int32_t dtype,
+                   const uint8_t* allowed, const int32_t* group, int32_t n_groups, int32_t renorm, const int32_t* expert,
+                   const float* weight, const float* dweight, void* dlogits, void* stream);
+
+/* Plan of `slots` < 2^31 slots with a group each: order (slots) = the slots sorted by group, stably, ptr (G + 1) = where
+ * each group's begin in it; those of no group in [0, G) last, from ptr[G] on. G <= 1024. work: face_group_plan_work
+ * bytes. */
+int64_t face_group_plan_work(int64_t slots, int32_t G);
+int face_group_plan(const int32_t* expert, int64_t slots, int32_t G, int32_t* ptr, int32_t* order, void* work,
+                    int64_t work_bytes, void* stream);
+
+/* y[a] (slots, n) = op(x[a / x_div]) W[g]^T + bias[g] for the slots a of group g of a plan, 0 for those of no group.
+ * x has ceil(slots / x_div) rows of k; w (G, n, k) with strides w_group, ld_w; bias (G, n) with row stride ld_b, or
+ * NULL; x_op 0 none, 1 silu. fp32 products are six bf16 products of three-way splits (as face_rows_linear),
+ * 16-bit ones bf16 or fp16 products, sums in fp32. G <= 65535. */
+int face_grouped_linear(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* w, int64_t ld_w,
+                        int64_t w_group, const void* bias, int64_t ld_b, const int32_t* ptr, const int32_t* order,
+                        int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* y, int64_t ld_y, void* stream);
+/* The same of e4m3 x with a scale per row and e4m3 w with a scale w_scale (G, n) per row; bias and y of `dtype`. */
+int face_grouped_linear_q8(const void* x, int64_t ld_x, const float* x_scale, int32_t x_div, const void* w, int64_t ld_w,
+                           int64_t w_group, const float* w_scale, const void* bias, int64_t ld_b, const int32_t* ptr,
+                           const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* y,
+                           int64_t ld_y, void* stream);
+/* dx[a] (slots, k) = (dy[a] W[g]) [* silu'(z[a / z_div])], a row per slot; z NULL: no factor. */
+int face_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ld_w, int64_t w_group, const void* z,
+                           int64_t ld_z, int32_t z_div, const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G,
+                           int32_t n, int32_t k, int32_t dtype, void* dx, int64_t ld_dx, void* stream);
+/* dw (G, n, k) and db (G, n) (may be NULL), dense. work: face_grouped_linear_dw_work bytes. Fixed summation order. */
+int64_t face_grouped_linear_dw_work(int64_t slots, int32_t G, int32_t n, int32_t k, int32_t with_bias);
+int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy, int64_t ld_dy,
+                           const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k,
+                           int32_t dtype, void* dw, void* db, void* work, int64_t work_bytes, void* stream);
+
+/* out[i] (N, F) = r[i] + sum_j weight[i, j] y[i k + j]; r NULL: 0, weight (N, k) NULL: 1. */
+int face_expert_combine_fwd(const void* y, int64_t ld_y, const float* weight, const void* r, int64_t ld_r, int64_t N,
+                            int32_t k, int32_t F, int32_t dtype, void* out, void* stream);
+/* dy (N k, F) = weight dout, dweight (N, k) = dout . y; either may be NULL. */
+int face_expert_combine_bwd(const void* dout, int64_t ld_d, const void* y, int64_t ld_y, const float* weight, int64_t N,
+                            int32_t k, int32_t F, int32_t dtype, void* dy, float* dweight, void* stream);
 
 #ifdef __cplusplus
 }
