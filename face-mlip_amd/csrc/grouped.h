@@ -203,14 +203,12 @@ __device__ __forceinline__ void put(char* at, int plane, const Held<T>& h) {
 template <int R, int C, bool COLS>
 struct Tile {
     static constexpr int kBytes = R * C * 16;
-    __device__ static __forceinline__ int at(int row, int chunk) {
-        int f;
-        if constexpr (COLS)
-            f = C >= 16 ? ((row & 1) << 2) ^ ((row & 2) ? 10 : 0) : (row & 2);
-        else
-            f = C >= 16 ? (row & 15) : (C == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1));
-        return (row * C + (chunk ^ f)) * 16;
+    // The chunk that lies at a place of the row, and the place of a chunk.
+    __device__ static __forceinline__ int chunk(int row, int place) {
+        if constexpr (COLS) return place ^ (C >= 16 ? ((row & 1) << 2) ^ ((row & 2) ? 10 : 0) : (row & 2));
+        return place ^ (C >= 16 ? (row & 15) : (C == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1)));
     }
+    __device__ static __forceinline__ int at(int row, int c) { return (row * C + chunk(row, c)) * 16; }
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -245,7 +243,9 @@ __device__ __forceinline__ v16f mfma16(v4u a, v4u b, v16f c) {
         return mfma_32x32x16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c);
 }
 
-// The products of one chunk: MT x NT tiles of 32 x 32, elements [k_begin, k_end) of the chunk.
+// The products of one chunk: MT x NT tiles of 32 x 32, elements [k_begin, k_end) of the chunk. The column operand
+// comes first, so that a lane ends with four neighbouring columns of one row at a time: register q of acc[m][n] is row
+// lane & 31, column 8 (q >> 2) + 4 (lane >> 5) + (q & 3) of the tile.
 template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT>
 __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int k_end,
                                                int lane, v16f acc[MT][NT]) {
@@ -271,7 +271,7 @@ __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, i
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[m], b[n], acc[m][n], 0, 0, 0, 0x7f7f7f7f, 0,
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[n], a[m], acc[m][n], 0, 0, 0, 0x7f7f7f7f, 0,
                                                                                 0x7f7f7f7f);
         }
     } else {
@@ -295,9 +295,19 @@ __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, i
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
-                        acc[m][n] = mfma16<T>(a[P == 3 ? pa[q] : 0][m], b[P == 3 ? pb[q] : 0][n], acc[m][n]);
+                        acc[m][n] = mfma16<T>(b[P == 3 ? pb[q] : 0][n], a[P == 3 ? pa[q] : 0][m], acc[m][n]);
         }
     }
+}
+
+// ---------------------------------------------------------------- staging without registers
+// Operands whose 16-byte chunks are aligned and whole (launch_rows, launch_weight) go from memory to LDS directly:
+// lane l of a wave fills the 16 bytes at 16 l of a stretch of 1 KB, so the chunk that belongs there by the tile's XOR is
+// the one it loads. Chunks outside the operand come from a block of zeros.
+__device__ const v4u kZeroChunk = {0, 0, 0, 0};
+__device__ __forceinline__ void to_lds(const void* from, char* stretch) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)stretch, 16, 0, 0);
 }
 
 // ---------------------------------------------------------------- which rows a workgroup owns
@@ -361,19 +371,22 @@ __device__ __forceinline__ int64_t xcd_item(int64_t items) {
 
 // ---------------------------------------------------------------- forward and input gradient
 // WM x WN x WK waves of MT x NT tiles. COLS_B: the weights lie (sum, column), as the input gradient reads them.
+// DIRECT_A, DIRECT_B: the operand is staged without registers.
 template <typename T, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
 struct RowsKernel {
     using Op = Operand<T>;
     static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, BK = C * Op::kElems, P = Op::kPlanes;
-    static constexpr int kThreads = 64 * WM * WN * WK;
+    static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
     static constexpr int CB = COLS_B ? BN / 8 : C, RB = COLS_B ? BK : BN;
     using TA = Tile<BM, C, false>;
     using TB = Tile<RB, CB, COLS_B>;
     static constexpr int kLdsA = P * TA::kBytes, kLdsB = P * TB::kBytes;
-    static constexpr int kLdsJoin = WK > 1 ? WK * BM * BN * 4 : 0;
-    static constexpr int kLds = kLdsA + kLdsB > kLdsJoin ? kLdsA + kLdsB : kLdsJoin;
+    // finished sums on their way out: 32 rows of a wave's columns at a time, rows four floats apart in the banks
+    static constexpr int kOutLd = 32 * NT + 4, kOut = 32 * kOutLd * 4;
+    static constexpr int kLds = kLdsA + kLdsB > kWaves * kOut ? kLdsA + kLdsB : kWaves * kOut;
     static constexpr int NA = BM * C / kThreads, NB = RB * CB / kThreads;   // chunks per thread
     static_assert(NA * kThreads == BM * C && NB * kThreads == RB * CB, "whole rounds of chunks");
+    static_assert(WK == 1 || (WM == 1 && WN == 1 && MT == 1 && NT == 1 && WK == 4), "split chunks: one tile");
 };
 
 // Out-of-range sums of limbs: a value past bf16's largest, or an infinity, has a NaN limb, so a sum that
@@ -383,10 +396,49 @@ __device__ inline float plain_sum(const float* x, const float* w, int64_t step, 
     for (int i = 0; i < k; ++i) s = fmaf(op ? silu(x[i]) : x[i], w[i * step], s);
     return s;
 }
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 0x1.fffffep+127f; }
 
-template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
-__global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThreads), 2) void grouped_rows_kernel(
-    GroupedArgs g) {
+// The epilogue of the eight columns from col of slot a, and their store.
+template <typename T, typename Out, bool COLS_B>
+__device__ __forceinline__ void finish(const GroupedArgs& g, int group, int32_t a, int col, float v[8]) {
+    const int left = g.n - col;
+    if (left <= 0) return;
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!finite(v[e]) && e < left) {
+                const float* w = (const float*)g.w + group * g.w_group;
+                v[e] = plain_sum((const float*)g.x + (int64_t)(a / g.xdiv) * g.ld_x,
+                                 COLS_B ? w + col + e : w + (col + e) * g.ld_w, COLS_B ? g.ld_w : 1, g.k, g.x_op);
+            }
+    }
+    if constexpr (kIsQ8<T>) {
+        const float sx = g.xs[a / g.xdiv];
+        float s[8];
+        load_piece(g.ws + (int64_t)group * g.n + col, left, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= sx * s[e];
+    }
+    if (g.bias) {
+        float s[8];
+        load_piece((const Out*)g.bias + group * g.ld_b + col, left, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += s[e];
+    }
+    if constexpr (COLS_B) {
+        if (g.z) {
+            float z[8];
+            load_piece((const Out*)g.z + (int64_t)(a / g.zdiv) * g.ld_z + col, left, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= silu_slope(z[e]);
+        }
+    }
+    store_piece((Out*)g.y + a * g.ld_y + col, left, v);
+}
+
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B>
+__global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThreads), (DIRECT_A ? 4 : 2)) void
+    grouped_rows_kernel(GroupedArgs g) {
     using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
     __shared__ __attribute__((aligned(256))) char lds[K::kLds];
     __shared__ int32_t slot_of[K::BM];
@@ -402,9 +454,9 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
         slot_of[i] = a >= 0 && a < g.slots ? a : -1;
     }
     __syncthreads();
-    Out* y = (Out*)g.y;
     if (r.group == g.groups) {
-        for (int i = wave; i < K::BM; i += K::kThreads / 64) {
+        Out* y = (Out*)g.y;
+        for (int i = wave; i < K::BM; i += K::kWaves) {
             const int32_t a = slot_of[i];
             if (a < 0) continue;
             for (int c = lane; c < K::BN; c += 64)
@@ -414,32 +466,48 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
     }
     const T* w = (const T*)g.w + r.group * g.w_group;
     const T* x = (const T*)g.x;
+    char *lds_a = lds, *lds_b = lds + K::kLdsA;
 
-    // this thread's chunks: rows of x by their slots, rows of the weights by column (or by place in the sum)
-    const T* ap[K::NA];
-    int a_row[K::NA], b_row[K::NB];
-    const int a_col = (tid % C) * K::Op::kElems, b_chunk = tid % K::CB;
+    // This thread's chunks. Through registers: chunk tid % C of row tid / C, the next ones kThreads / C rows on. Directly:
+    // the same places of the tile, and what the XOR puts there.
+    const T *ap[K::NA], *bp[K::NB];
+    int a_col[K::NA], b_col[K::NB];          // element of the chunk along the row; a row that is not there: past its end
 #pragma unroll
     for (int i = 0; i < K::NA; ++i) {
-        a_row[i] = tid / C + i * (K::kThreads / C);
-        const int32_t a = slot_of[a_row[i]];
-        ap[i] = a < 0 ? nullptr : x + (int64_t)(a / g.xdiv) * g.ld_x + a_col;
+        const int row = tid / C + i * (K::kThreads / C);
+        const int chunk = DIRECT_A ? K::TA::chunk(row, tid % C) : tid % C;
+        const int32_t a = slot_of[row];
+        ap[i] = a < 0 ? x : x + (int64_t)(a / g.xdiv) * g.ld_x;
+        a_col[i] = a < 0 ? g.k : chunk * K::Op::kElems;
     }
 #pragma unroll
-    for (int i = 0; i < K::NB; ++i) b_row[i] = tid / K::CB + i * (K::kThreads / K::CB);
-
-    Held<T> ha[K::NA], hb[K::NB];
+    for (int i = 0; i < K::NB; ++i) {
+        const int row = tid / K::CB + i * (K::kThreads / K::CB);
+        const int chunk = DIRECT_B ? K::TB::chunk(row, tid % K::CB) : tid % K::CB;
+        if constexpr (COLS_B) {
+            const int col = col0 + 8 * chunk;
+            bp[i] = col < g.n ? w + row * g.ld_w + col : w;
+            b_col[i] = col < g.n ? row : g.k;                    // place in the sum
+        } else {
+            bp[i] = col0 + row < g.n ? w + (col0 + row) * g.ld_w : w;
+            b_col[i] = col0 + row < g.n ? chunk * K::Op::kElems : g.k;
+        }
+    }
+    Held<T> ha[DIRECT_A ? 1 : K::NA], hb[DIRECT_B ? 1 : K::NB];
     auto fetch = [&](int k0) {
+        if constexpr (!DIRECT_A) {
 #pragma unroll
-        for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0, ap[i] ? g.k - k0 - a_col : 0);
+            for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + a_col[i] + k0, g.k - a_col[i] - k0);
+        }
+        if constexpr (!DIRECT_B) {
 #pragma unroll
-        for (int i = 0; i < K::NB; ++i) {
-            if constexpr (COLS_B) {
-                const int col = col0 + 8 * b_chunk, row = k0 + b_row[i];
-                hb[i] = hold(w + row * g.ld_w + col, row < g.k ? g.n - col : 0);
-            } else {
-                const int col = k0 + b_chunk * K::Op::kElems, row = col0 + b_row[i];
-                hb[i] = hold(w + row * g.ld_w + col, row < g.n ? g.k - col : 0);
+            for (int i = 0; i < K::NB; ++i) {
+                if constexpr (COLS_B) {
+                    const int col = col0 + 8 * (tid % K::CB);
+                    hb[i] = hold(bp[i] + k0 * g.ld_w, b_col[i] + k0 < g.k ? g.n - col : 0);
+                } else {
+                    hb[i] = hold(bp[i] + b_col[i] + k0, g.k - b_col[i] - k0);
+                }
             }
         }
     };
@@ -447,63 +515,75 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
     const int wk = wave % WK, wn = wave / WK % WN, wm = wave / WK / WN;
     fetch(0);
     for (int k0 = 0; k0 < g.k; k0 += K::BK) {
-        if (g.x_op) {
+        if constexpr (DIRECT_A) {
 #pragma unroll
-            for (int i = 0; i < K::NA; ++i) apply_silu(ha[i]);
+            for (int i = 0; i < K::NA; ++i)
+                to_lds(a_col[i] + k0 < g.k ? (const void*)(ap[i] + a_col[i] + k0) : &kZeroChunk,
+                       lds_a + (i * K::kThreads + wave * 64) * 16);
+        } else {
+            if (g.x_op) {
+#pragma unroll
+                for (int i = 0; i < K::NA; ++i) apply_silu(ha[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < K::NA; ++i)
+                put(lds_a + K::TA::at(tid / C + i * (K::kThreads / C), tid % C), K::TA::kBytes, ha[i]);
         }
+        if constexpr (DIRECT_B) {
 #pragma unroll
-        for (int i = 0; i < K::NA; ++i) put(lds + K::TA::at(a_row[i], tid % C), K::TA::kBytes, ha[i]);
+            for (int i = 0; i < K::NB; ++i)
+                to_lds(b_col[i] + k0 < g.k ? (const void*)(COLS_B ? bp[i] + k0 * g.ld_w : bp[i] + b_col[i] + k0) : &kZeroChunk,
+                       lds_b + (i * K::kThreads + wave * 64) * 16);
+        } else {
 #pragma unroll
-        for (int i = 0; i < K::NB; ++i) put(lds + K::kLdsA + K::TB::at(b_row[i], b_chunk), K::TB::kBytes, hb[i]);
+            for (int i = 0; i < K::NB; ++i)
+                put(lds_b + K::TB::at(tid / K::CB + i * (K::kThreads / K::CB), tid % K::CB), K::TB::kBytes, hb[i]);
+        }
         __syncthreads();
         if (k0 + K::BK < g.k) fetch(k0 + K::BK);
-        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT>(lds, lds + K::kLdsA, 32 * MT * wm, 32 * NT * wn,
+        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT>(lds_a, lds_b, 32 * MT * wm, 32 * NT * wn,
                                                                         wk * (K::BK / WK), (wk + 1) * (K::BK / WK), lane, acc);
         __syncthreads();
     }
 
+    // Out through LDS: whole rows of eight columns a lane, so that the stores (and the reads of z) are whole lines
+    float* out = reinterpret_cast<float*>(lds) + wave * (K::kOut / 4);
     if constexpr (WK > 1) {
-        // one tile per wave: its part of every sum to LDS, then each wave finishes a share of the rows
-        static_assert(WM == 1 && WN == 1 && MT == 1 && NT == 1 && WK == 4, "split chunks: one tile");
-        float* part = reinterpret_cast<float*>(lds);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) part[(wave * 16 + q) * 64 + lane] = acc[0][0][q];
+        for (int q = 0; q < 4; ++q)
+            st4(out + (lane & 31) * K::kOutLd + 8 * q + 4 * (lane >> 5),
+                (v4f){acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]});
         __syncthreads();
+        const int row = tid >> 2, c = 8 * (tid & 3);
+        if (tid < 128 && slot_of[row] >= 0) {
+            float v[8] = {};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float s = 0.f;
+            for (int u = 0; u < WK; ++u)
 #pragma unroll
-            for (int v = 0; v < WK; ++v) s += part[(v * 16 + 4 * wave + q) * 64 + lane];
-            acc[0][0][q] = s;
+                for (int e = 0; e < 8; ++e) v[e] += reinterpret_cast<const float*>(lds)[u * (K::kOut / 4) + row * K::kOutLd + c + e];
+            finish<T, Out, COLS_B>(g, r.group, slot_of[row], col0 + c, v);
         }
-    }
-    // D[8 (q >> 2) + 4 (lane >> 5) + (q & 3)][lane & 31] in register q; after a join wave w holds registers 4 w .. 4 w + 3
-    constexpr int kRegs = WK > 1 ? 4 : 16;
+    } else {
+        constexpr int kLanes = 4 * NT;                           // lanes per row, eight columns each
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int col = col0 + 32 * (NT * wn + n) + (lane & 31);
-        if (col >= g.n) continue;
-        const float b = g.bias ? to_f(((const Out*)g.bias)[r.group * g.ld_b + col]) : 0.f;
-        const float sw = kIsQ8<T> ? g.ws[(int64_t)r.group * g.n + col] : 1.f;
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int q = 0; q < kRegs; ++q) {
-                const int row = 32 * (MT * wm + m) + 8 * (WK > 1 ? wave : q >> 2) + 4 * (lane >> 5) + (q & 3);
-                const int32_t a = slot_of[row];
-                if (a < 0) continue;
-                float v = acc[m][n][q];
-                if constexpr (__is_same(T, float)) {
-                    if (!(__builtin_fabsf(v) <= 0x1.fffffep+127f))
-                        v = plain_sum((const float*)x + (int64_t)(a / g.xdiv) * g.ld_x,
-                                      (const float*)w + (COLS_B ? col : col * g.ld_w), COLS_B ? g.ld_w : 1, g.k, g.x_op);
-                }
-                if constexpr (kIsQ8<T>) v *= g.xs[a / g.xdiv] * sw;
-                v += b;
-                if constexpr (COLS_B)
-                    if (g.z) v *= silu_slope(to_f(((const Out*)g.z)[(int64_t)(a / g.zdiv) * g.ld_z + col]));
-                y[a * g.ld_y + col] = from_f<Out>(v);
+                for (int q = 0; q < 4; ++q)
+                    st4(out + (lane & 31) * K::kOutLd + 32 * n + 8 * q + 4 * (lane >> 5),
+                        (v4f){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]});
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 32 * kLanes / 64; ++i) {
+                const int row = lane / kLanes + i * (64 / kLanes), c = 8 * (lane % kLanes);
+                const v4f lo = ld4(out + row * K::kOutLd + c), hi = ld4(out + row * K::kOutLd + c + 4);
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                const int32_t a = slot_of[32 * (MT * wm + m) + row];
+                if (a >= 0) finish<T, Out, COLS_B>(g, r.group, a, col0 + 32 * NT * wn + c, v);
             }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
@@ -530,8 +610,8 @@ __device__ inline float plain_dot(const float* dy, int64_t ld_dy, const float* x
     return s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupedWArgs g) {
+template <typename T, bool DIRECT>
+__global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(GroupedWArgs g) {
     using K = WeightKernel<T>;
     __shared__ __attribute__((aligned(256))) char lds[K::kLds];
     const int64_t per = (int64_t)g.row_tiles * g.col_tiles;
@@ -539,104 +619,151 @@ __global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupedWArgs g) 
     const Range r = find_piece(g.ptr, g.groups - 1, g.groups, g.slots, g.chunk, 1, item / per);
     if (r.group < 0) return;
     const int row0 = (int)(item % per / g.col_tiles) * 128, col0 = (int)(item % g.col_tiles) * 128;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = tid % K::CT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t p0 = r.begin + r.index * g.chunk;
     const int64_t p1 = p0 + g.chunk < r.end ? p0 + g.chunk : r.end;
     const T *x = (const T*)g.x, *dy = (const T*)g.dy;
-    const int ca = row0 + 8 * chunk, cb = col0 + 8 * chunk;
-    const bool sums = g.db && col0 == 0;
+    char *lds_a = lds, *lds_b = lds + K::P * K::TT::kBytes;
     // a plan whose ranges overlap can name more split pieces than its slots can make: they have no place
     if (r.pieces > 1 && r.split_before + r.index >= g.part_items) return;
-    float colsum[8] = {};
 
-    Held<T> ha[K::NC], hb[K::NC];
+    // chunk tid % CT (directly: the one the XOR puts there, the same in all of the thread's rows, four apart)
+    const int row_t = tid / K::CT, chunk = DIRECT ? K::TT::chunk(row_t, tid % K::CT) : tid % K::CT;
+    const int ca = row0 + 8 * chunk, cb = col0 + 8 * chunk;
+    const bool sums = g.db && col0 == 0;
+    float colsum[8] = {};
     int32_t next[K::NC];
     auto find = [&](int64_t p) {
 #pragma unroll
         for (int i = 0; i < K::NC; ++i) {
-            const int64_t at = p + tid / K::CT + i * (K::kThreads / K::CT);
-            next[i] = at < p1 ? g.order[at] : -1;
+            const int64_t at = p + row_t + i * (K::kThreads / K::CT);
+            const int32_t a = at < p1 ? g.order[at] : -1;
+            next[i] = a < g.slots ? a : -1;
         }
     };
+    Held<T> ha[DIRECT ? 1 : K::NC], hb[DIRECT ? 1 : K::NC];
     auto fetch = [&]() {
+        if constexpr (!DIRECT) {
 #pragma unroll
-        for (int i = 0; i < K::NC; ++i) {
-            const int32_t a = next[i];
-            const bool ok = a >= 0 && a < g.slots;
-            ha[i] = hold(dy + (ok ? a * g.ld_dy + ca : 0), ok ? g.n - ca : 0);
-            hb[i] = hold(x + (ok ? (int64_t)(a / g.xdiv) * g.ld_x + cb : 0), ok ? g.k - cb : 0);
+            for (int i = 0; i < K::NC; ++i) {
+                const int32_t a = next[i];
+                ha[i] = hold(dy + (a >= 0 ? a * g.ld_dy + ca : 0), a >= 0 ? g.n - ca : 0);
+                hb[i] = hold(x + (a >= 0 ? (int64_t)(a / g.xdiv) * g.ld_x + cb : 0), a >= 0 ? g.k - cb : 0);
+            }
+        }
+    };
+    auto add_columns = [&](v4u lo, v4u hi) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) {
+                colsum[e] += __builtin_bit_cast(v4f, lo)[e];
+                colsum[4 + e] += __builtin_bit_cast(v4f, hi)[e];
+            } else {
+                float u, v;
+                unpack2<T>(lo[e], u, v);
+                colsum[2 * e] += u;
+                colsum[2 * e + 1] += v;
+            }
         }
     };
     v16f acc[2][2] = {};
     const int wn = wave & 1, wm = wave >> 1;
     find(p0);
     fetch();
-    find(p0 + K::BK);
+    if constexpr (!DIRECT) find(p0 + K::BK);
     for (int64_t p = p0; p < p1; p += K::BK) {
-        if (g.x_op) {
+        if constexpr (DIRECT) {
 #pragma unroll
-            for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
-        }
-        if (sums) {
+            for (int i = 0; i < K::NC; ++i) {
+                const int32_t a = next[i];
+                to_lds(a >= 0 && ca < g.n ? (const void*)(dy + a * g.ld_dy + ca) : &kZeroChunk,
+                       lds_a + (i * K::kThreads + wave * 64) * 16);
+                to_lds(a >= 0 && cb < g.k ? (const void*)(x + (int64_t)(a / g.xdiv) * g.ld_x + cb) : &kZeroChunk,
+                       lds_b + (i * K::kThreads + wave * 64) * 16);
+            }
+            find(p + K::BK);
+        } else {
+            if (g.x_op) {
 #pragma unroll
-            for (int i = 0; i < K::NC; ++i)
+                for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+            }
+            if (sums) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (sizeof(T) == 4) {
-                        colsum[e] += __builtin_bit_cast(v4f, ha[i].a)[e];
-                        colsum[4 + e] += __builtin_bit_cast(v4f, ha[i].b)[e];
-                    } else {
-                        float u, v;
-                        unpack2<T>(ha[i].a[e], u, v);
-                        colsum[2 * e] += u;
-                        colsum[2 * e + 1] += v;
-                    }
+                for (int i = 0; i < K::NC; ++i) {
+                    if constexpr (sizeof(T) == 4) add_columns(ha[i].a, ha[i].b);
+                    else add_columns(ha[i].a, ha[i].a);
                 }
-        }
+            }
 #pragma unroll
-        for (int i = 0; i < K::NC; ++i) {
-            const int at = K::TT::at(tid / K::CT + i * (K::kThreads / K::CT), chunk);
-            put(lds + at, K::TT::kBytes, ha[i]);
-            put(lds + K::P * K::TT::kBytes + at, K::TT::kBytes, hb[i]);
+            for (int i = 0; i < K::NC; ++i) {
+                const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
+                put(lds_a + at, K::TT::kBytes, ha[i]);
+                put(lds_b + at, K::TT::kBytes, hb[i]);
+            }
         }
         __syncthreads();
-        if (p + K::BK < p1) {
+        if constexpr (DIRECT) {
+            if (sums) {                                          // the thread's own chunks again, from LDS
+#pragma unroll
+                for (int i = 0; i < K::NC; ++i) {
+                    const v4u v = *reinterpret_cast<const v4u*>(lds_a + (i * K::kThreads + tid) * 16);
+                    add_columns(v, v);
+                }
+            }
+        } else if (p + K::BK < p1) {
             fetch();
             find(p + 2 * K::BK);
         }
-        chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2>(lds, lds + K::P * K::TT::kBytes, 64 * wm, 64 * wn, 0,
-                                                                        K::BK, lane, acc);
+        chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2>(lds_a, lds_b, 64 * wm, 64 * wn, 0, K::BK, lane, acc);
         __syncthreads();
     }
     const int64_t stride = (int64_t)g.n * g.k + (g.db ? g.n : 0);
     float* part = r.pieces > 1 ? g.part + (r.split_before + r.index) * stride : nullptr;
     T* dw = (T*)g.dw + (int64_t)r.group * g.n * g.k;
+    // out through LDS as in the forward: 32 rows of 64 columns of a wave at a time
+    constexpr int kLd = 68;
+    static_assert(K::kLds >= 2 * 32 * kLd * 4, "room for two waves' rows");
+    float* out = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * kLd;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int col = col0 + 64 * wn + 32 * n + (lane & 31);
-        if (col >= g.k) continue;
+    for (int turn = 0; turn < 2; ++turn) {
+        __syncthreads();
+        if (wm != turn) continue;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int row = row0 + 64 * wm + 32 * m + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3);
-                if (row >= g.n) continue;
-                float v = acc[m][n][q];
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    st4(out + (lane & 31) * kLd + 32 * n + 8 * q + 4 * (lane >> 5),
+                        (v4f){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]});
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (lane >> 3) + 8 * i, row = row0 + 64 * wm + 32 * m + at, c = 8 * (lane & 7);
+                const int col = col0 + 64 * wn + c, left = g.k - col;
+                const v4f lo = ld4(out + at * kLd + c), hi = ld4(out + at * kLd + c + 4);
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                if (row >= g.n || left <= 0) continue;
                 if constexpr (__is_same(T, float)) {
-                    if (!(__builtin_fabsf(v) <= 0x1.fffffep+127f))
-                        v = plain_dot((const float*)dy + row, g.ld_dy, (const float*)x + col, g.ld_x, g.xdiv, g.x_op, g.order, p0,
-                                      p1, g.slots);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!finite(v[e]) && e < left)
+                            v[e] = plain_dot((const float*)dy + row, g.ld_dy, (const float*)x + col + e, g.ld_x, g.xdiv, g.x_op,
+                                             g.order, p0, p1, g.slots);
                 }
                 if (part)
-                    part[(int64_t)row * g.k + col] = v;
+                    store_piece(part + (int64_t)row * g.k + col, left, v);
                 else
-                    dw[(int64_t)row * g.k + col] = from_f<T>(v);
+                    store_piece(dw + (int64_t)row * g.k + col, left, v);
             }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
     if (sums) {
+        __syncthreads();
         float* red = reinterpret_cast<float*>(lds);          // 16 threads per chunk of eight columns
 #pragma unroll
-        for (int e = 0; e < 8; ++e) red[(tid / K::CT) * 128 + 8 * chunk + e] = colsum[e];
+        for (int e = 0; e < 8; ++e) red[row_t * 128 + 8 * chunk + e] = colsum[e];
         __syncthreads();
         if (tid < 128 && row0 + tid < g.n) {
             float s = 0.f;
@@ -691,7 +818,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedWArgs g) {
 
 // ---------------------------------------------------------------- launches
 // Instantiated per element type in a file of its own (grouped_f32.hip, ...).
-template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B>
 static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
     using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
     const int64_t most = g.groups + (int64_t)1;
@@ -699,8 +826,8 @@ static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
     g.col_tiles = (g.n + K::BN - 1) / K::BN;
     const int64_t grid = g.tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C>), dim3((unsigned)grid), dim3(K::kThreads),
-                       0, st, g);
+    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B>), dim3((unsigned)grid),
+                       dim3(K::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     return 0;
 }
@@ -708,13 +835,26 @@ static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
 // Tiles of 128 x 128 once there is about one for every CU, else of 32 x 32 with the sum split over the waves.
 constexpr int64_t kLargeTiles = 256;
 
+// Whether rows of `width` elements at p, `ld` apart, are whole 16-byte chunks at 16-byte addresses.
+template <typename T>
+static inline bool whole_chunks(const void* p, int64_t ld, int64_t width) {
+    constexpr int E = 16 / sizeof(T);
+    return sizeof(T) < 4 && !__is_same(T, e4m3_wide) && (uintptr_t)p % 16 == 0 && ld % E == 0 && width % E == 0;
+}
+
 template <typename T, typename Out, bool COLS_B>
 int launch_rows(GroupedArgs g, hipStream_t st) {
     const int64_t groups = g.groups < g.slots ? g.groups : g.slots;
     const int64_t large = (g.slots / 128 + groups) * ((g.n + 127) / 128);
     constexpr int C = sizeof(T) == 4 ? 4 : 8, CS = sizeof(T) == 4 ? 16 : 32;
-    if (large >= kLargeTiles) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C>(g, st);
-    return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, CS>(g, st);
+    if constexpr (sizeof(T) < 4 && !__is_same(T, e4m3_wide)) {
+        const bool a = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op;
+        const bool b = whole_chunks<T>(g.w, g.ld_w, COLS_B ? g.n : g.k) && g.w_group % (16 / (int)sizeof(T)) == 0;
+        if (large >= kLargeTiles && a && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, true, true>(g, st);
+        if (large >= kLargeTiles && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, false, true>(g, st);
+    }
+    if (large >= kLargeTiles) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, false, false>(g, st);
+    return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, CS, false, false>(g, st);
 }
 
 // Slots per chunk of the weight gradient: enough chunks for about 2048 workgroups, at most 64 (each adds a partial
@@ -739,7 +879,10 @@ int launch_weight(GroupedWArgs g, hipStream_t st) {
     g.items = g.slots / g.chunk + g.groups;
     const int64_t grid = g.items * g.row_tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(grouped_weight_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, g);
+    bool direct = false;
+    if constexpr (sizeof(T) < 4) direct = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n);
+    auto* kernel = direct ? grouped_weight_kernel<T, (sizeof(T) < 4)> : grouped_weight_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, g);
     FACE_LAUNCH_CHECK();
     if (g.slots > g.chunk) {
         const int64_t blocks = ((int64_t)g.n * g.k + 1023) / 1024;
