@@ -23,6 +23,7 @@
 // have loads in flight.
 #pragma once
 #include "elem.h"
+#include <type_traits>
 
 namespace face {
 
@@ -64,18 +65,19 @@ struct GroupedWArgs {
     const void* x;                 // (.., k) with silu as it loads if x_op
     int64_t ld_x;
     int32_t xdiv, x_op;
+    uint32_t div_mul, div_shift;   // a / xdiv = a div_mul >> div_shift for a < 2^31
     const void* dy;                // (slots, n)
     int64_t ld_dy;
     void* dw;                      // (G, n, k)
     void* db;                      // (G, n) or null
-    float* part;                   // partial sums of the items of split groups, (n k [+ n]) each
-    int64_t part_items;            // how many it holds
+    float* part;                   // 2 shares partial results of n k [+ n] sums
     int32_t n, k;
     const int32_t *ptr, *order;
     int64_t slots;
     int32_t groups;
     int32_t col_tiles, row_tiles;
-    int64_t items, chunk;          // (group, chunk of its slots) pairs the grid holds
+    int32_t shares;                // of the places in order, `share` each; 1: a workgroup per group instead
+    int64_t share;
 };
 
 // ---------------------------------------------------------------- operands
@@ -205,7 +207,8 @@ struct Tile {
     static constexpr int kBytes = R * C * 16;
     // The chunk that lies at a place of the row, and the place of a chunk.
     __device__ static __forceinline__ int chunk(int row, int place) {
-        if constexpr (COLS) return place ^ (C >= 16 ? ((row & 1) << 2) ^ ((row & 2) ? 10 : 0) : (row & 2));
+        if constexpr (COLS)
+            return place ^ (C >= 16 ? ((row & 1) << 2) ^ ((row & 2) ? 10 : 0) : (C == 8 ? 2 * (row & 3) : (row & 2)));
         return place ^ (C >= 16 ? (row & 15) : (C == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1)));
     }
     __device__ static __forceinline__ int at(int row, int c) { return (row * C + chunk(row, c)) * 16; }
@@ -233,6 +236,7 @@ __device__ __forceinline__ v4u fragment(const char* tile, int i0, int k0, int la
 }
 
 typedef f16 v8h __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 
 template <typename T>
@@ -243,42 +247,32 @@ __device__ __forceinline__ v16f mfma16(v4u a, v4u b, v16f c) {
         return mfma_32x32x16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c);
 }
 
-// The products of one chunk: MT x NT tiles of 32 x 32, elements [k_begin, k_end) of the chunk. The column operand
-// comes first, so that a lane ends with four neighbouring columns of one row at a time: register q of acc[m][n] is row
-// lane & 31, column 8 (q >> 2) + 4 (lane >> 5) + (q & 3) of the tile.
+// The products of one chunk: MT x NT tiles of 32 x 32, elements [k_begin, k_begin + STEPS * step) of the chunk. The
+// column operand comes first, so that a lane ends with four neighbouring columns of one row at a time: register q of
+// acc[m][n] is row lane & 31, column 8 (q >> 2) + 4 (lane >> 5) + (q & 3) of the tile.
+template <typename T>
+constexpr int kStep = __is_same(T, e4m3) ? 64 : 16;              // elements of the sum per instruction
+
+// One step's operands: 8 (e4m3: 32, each half of the wave its own) neighbouring elements of a row per lane.
 template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT>
-__device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int k_end,
-                                               int lane, v16f acc[MT][NT]) {
-    constexpr int PA = Tile<RA, CA, COLS_A>::kBytes, PB = Tile<RB, CB, COLS_B>::kBytes;
-    if constexpr (__is_same(T, e4m3)) {
-        for (int k0 = k_begin; k0 < k_end; k0 += 64) {
-            // each half of the wave takes 32 neighbouring elements of its row
-            v8i a[MT], b[NT];
+struct Fragments {
+    static constexpr int P = Operand<T>::kPlanes, W = __is_same(T, e4m3) ? 2 : 1;
+    v4u a[P * W][MT], b[P * W][NT];
+
+    __device__ __forceinline__ void load(const char* ta, const char* tb, int m0, int n0, int k0, int lane) {
+        if constexpr (__is_same(T, e4m3)) {
             const int c = (k0 >> 4) + 2 * (lane >> 5);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int r = m0 + 32 * m + (lane & 31);
-                reinterpret_cast<v4u*>(&a[m])[0] = *reinterpret_cast<const v4u*>(ta + Tile<RA, CA, false>::at(r, c));
-                reinterpret_cast<v4u*>(&a[m])[1] = *reinterpret_cast<const v4u*>(ta + Tile<RA, CA, false>::at(r, c + 1));
-            }
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int r = n0 + 32 * n + (lane & 31);
-                reinterpret_cast<v4u*>(&b[n])[0] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(r, c));
-                reinterpret_cast<v4u*>(&b[n])[1] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(r, c + 1));
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
+                for (int m = 0; m < MT; ++m)
+                    a[h][m] = *reinterpret_cast<const v4u*>(ta + Tile<RA, CA, false>::at(m0 + 32 * m + (lane & 31), c + h));
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[n], a[m], acc[m][n], 0, 0, 0, 0x7f7f7f7f, 0,
-                                                                                0x7f7f7f7f);
-        }
-    } else {
-        constexpr int P = Operand<T>::kPlanes;
-#pragma unroll
-        for (int k0 = k_begin; k0 < k_end; k0 += 16) {
-            v4u a[P][MT], b[P][NT];
+                    b[h][n] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(n0 + 32 * n + (lane & 31), c + h));
+            }
+        } else {
+            constexpr int PA = Tile<RA, CA, COLS_A>::kBytes, PB = Tile<RB, CB, COLS_B>::kBytes;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
@@ -286,6 +280,22 @@ __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, i
 #pragma unroll
                 for (int n = 0; n < NT; ++n) b[p][n] = fragment<RB, CB, COLS_B>(tb + p * PB, n0 + 32 * n, k0, lane);
             }
+        }
+    }
+    __device__ __forceinline__ void products(v16f acc[MT][NT]) const {
+        if constexpr (__is_same(T, e4m3)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const v8i x = __builtin_shufflevector(__builtin_bit_cast(v4i, a[0][m]), __builtin_bit_cast(v4i, a[1][m]), 0,
+                                                          1, 2, 3, 4, 5, 6, 7);
+                    const v8i w = __builtin_shufflevector(__builtin_bit_cast(v4i, b[0][n]), __builtin_bit_cast(v4i, b[1][n]), 0,
+                                                          1, 2, 3, 4, 5, 6, 7);
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc[m][n], 0, 0, 0, 0x7f7f7f7f, 0,
+                                                                                0x7f7f7f7f);
+                }
+        } else {
             // limb products from the smallest up; of one instruction after another none waits for the one before
             constexpr int kProducts = P == 3 ? 6 : 1;
             constexpr int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};
@@ -297,6 +307,18 @@ __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, i
                     for (int n = 0; n < NT; ++n)
                         acc[m][n] = mfma16<T>(b[P == 3 ? pb[q] : 0][n], a[P == 3 ? pa[q] : 0][m], acc[m][n]);
         }
+    }
+};
+
+template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT, int STEPS>
+__device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int lane,
+                                               v16f acc[MT][NT]) {
+    using F = Fragments<T, RA, CA, COLS_A, RB, CB, COLS_B, MT, NT>;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        F f;
+        f.load(ta, tb, m0, n0, k_begin + s * kStep<T>, lane);
+        f.products(acc);
     }
 }
 
@@ -317,49 +339,32 @@ struct Range {
     int group;                     // `groups`: the slots of no group; -1: nothing
     int64_t begin, end;            // its places in order
     int64_t index;                 // of this piece among the group's
-    int64_t pieces;                // of the group
-    int64_t split_before;          // pieces of the earlier groups that have more than one
 };
-// The t-th piece of `size` places of the groups 0 .. last, at least `least` for each group. The same in all threads.
-__device__ __forceinline__ Range find_piece(const int32_t* ptr, int last, int groups, int64_t slots, int64_t size,
-                                            int least, int64_t t) {
+// The t-th piece of `size` places of the groups 0 .. groups. The same in all threads.
+__device__ __forceinline__ Range find_piece(const int32_t* ptr, int groups, int64_t slots, int size, int64_t t) {
     const int lane = threadIdx.x & 63;
-    int64_t before = 0, split = 0;
-    for (int g0 = 0; g0 <= last; g0 += 64) {
+    int64_t before = 0;
+    for (int g0 = 0; g0 <= groups; g0 += 64) {
         const int g = g0 + lane;
         int64_t b = 0, e = 0;
-        if (g <= last) {
+        if (g <= groups) {
             b = clamp_slot(ptr[g], slots);
             e = g < groups ? clamp_slot(ptr[g + 1], slots) : slots;
         }
-        int c = e > b ? (int)((e - b + size - 1) / size) : 0;
-        if (g <= last && c < least) c = least;
-        int s = c, m = c > 1 ? c : 0;
+        const int c = e > b ? (int)((e - b + size - 1) / size) : 0;
+        int s = c;
         for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(s, o, 64), v = __shfl_up(m, o, 64);
-            if (lane >= o) {
-                s += u;
-                m += v;
-            }
+            const int u = __shfl_up(s, o, 64);
+            if (lane >= o) s += u;
         }
-        const int total = __shfl(s, 63, 64), total_m = __shfl(m, 63, 64);
+        const int total = __shfl(s, 63, 64);
         if (t < before + total) {
-            const uint64_t at = __ballot(before + s > t);
-            const int l = __builtin_ctzll(at);
-            const int cl = __shfl(c, l, 64);
-            Range r;
-            r.group = g0 + l;
-            r.begin = __shfl(b, l, 64);
-            r.end = __shfl(e, l, 64);
-            r.index = t - (before + __shfl(s, l, 64) - cl);
-            r.pieces = cl;
-            r.split_before = split + __shfl(m, l, 64) - (cl > 1 ? cl : 0);
-            return r;
+            const int l = __builtin_ctzll(__ballot(before + s > t));
+            return {g0 + l, __shfl(b, l, 64), __shfl(e, l, 64), t - (before + __shfl(s, l, 64) - __shfl(c, l, 64))};
         }
         before += total;
-        split += total_m;
     }
-    return {-1, 0, 0, 0, 0, 0};
+    return {-1, 0, 0, 0};
 }
 
 // Workgroups that follow each other on one XCD (every eighth) take neighbouring items, so that tiles of the same
@@ -444,7 +449,7 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
     __shared__ int32_t slot_of[K::BM];
     const int64_t item = xcd_item(g.tiles * g.col_tiles);
     const int col0 = (int)(item % g.col_tiles) * K::BN;
-    const Range r = find_piece(g.ptr, g.groups, g.groups, g.slots, K::BM, 0, item / g.col_tiles);
+    const Range r = find_piece(g.ptr, g.groups, g.slots, K::BM, item / g.col_tiles);
     if (r.group < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t place0 = r.begin + r.index * K::BM;
@@ -466,60 +471,56 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
     }
     const T* w = (const T*)g.w + r.group * g.w_group;
     const T* x = (const T*)g.x;
-    char *lds_a = lds, *lds_b = lds + K::kLdsA;
 
-    // This thread's chunks. Through registers: chunk tid % C of row tid / C, the next ones kThreads / C rows on. Directly:
-    // the same places of the tile, and what the XOR puts there.
-    const T *ap[K::NA], *bp[K::NB];
-    int a_col[K::NA], b_col[K::NB];          // element of the chunk along the row; a row that is not there: past its end
+    // This thread's chunks: chunk tid % C of row tid / C, the next ones kThreads / C rows on (directly: the same places of
+    // the tile, and the chunk that the XOR puts there, the same in all of the thread's rows). Rows of x and columns of the
+    // weights that are not there repeat one that is: what comes of them is not stored.
+    const T* ap[K::NA];
+    uint32_t b_off[K::NB];                   // bytes from the group's weights
+    const int a_col = (DIRECT_A ? K::TA::chunk(tid / C, tid % C) : tid % C) * K::Op::kElems;
+    const int b_chunk = DIRECT_B ? K::TB::chunk(tid / K::CB, tid % K::CB) : tid % K::CB;
+    const int b_col = COLS_B ? col0 + 8 * b_chunk : b_chunk * K::Op::kElems;     // along the row
+    const char* wb = (const char*)w;
 #pragma unroll
     for (int i = 0; i < K::NA; ++i) {
-        const int row = tid / C + i * (K::kThreads / C);
-        const int chunk = DIRECT_A ? K::TA::chunk(row, tid % C) : tid % C;
-        const int32_t a = slot_of[row];
-        ap[i] = a < 0 ? x : x + (int64_t)(a / g.xdiv) * g.ld_x;
-        a_col[i] = a < 0 ? g.k : chunk * K::Op::kElems;
+        const int32_t a = slot_of[tid / C + i * (K::kThreads / C)];
+        ap[i] = x + (int64_t)(a < 0 ? 0 : a / g.xdiv) * g.ld_x + a_col;
     }
+    if constexpr (DIRECT_B) {
 #pragma unroll
-    for (int i = 0; i < K::NB; ++i) {
-        const int row = tid / K::CB + i * (K::kThreads / K::CB);
-        const int chunk = DIRECT_B ? K::TB::chunk(row, tid % K::CB) : tid % K::CB;
-        if constexpr (COLS_B) {
-            const int col = col0 + 8 * chunk;
-            bp[i] = col < g.n ? w + row * g.ld_w + col : w;
-            b_col[i] = col < g.n ? row : g.k;                    // place in the sum
-        } else {
-            bp[i] = col0 + row < g.n ? w + (col0 + row) * g.ld_w : w;
-            b_col[i] = col0 + row < g.n ? chunk * K::Op::kElems : g.k;
+        for (int i = 0; i < K::NB; ++i) {
+            const int row = tid / K::CB + i * (K::kThreads / K::CB);
+            const int wr = COLS_B || col0 + row < g.n ? row : 0, wc = COLS_B && b_col >= g.n ? 0 : b_col;
+            b_off[i] = (uint32_t)(((COLS_B ? wr : col0 + wr) * g.ld_w + wc) * sizeof(T));
         }
     }
+    const int64_t w_step = (COLS_B ? g.ld_w : 1) * (int64_t)sizeof(T);           // one place of the sum
     Held<T> ha[DIRECT_A ? 1 : K::NA], hb[DIRECT_B ? 1 : K::NB];
     auto fetch = [&](int k0) {
         if constexpr (!DIRECT_A) {
 #pragma unroll
-            for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + a_col[i] + k0, g.k - a_col[i] - k0);
+            for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0, g.k - a_col - k0);
         }
         if constexpr (!DIRECT_B) {
 #pragma unroll
             for (int i = 0; i < K::NB; ++i) {
-                if constexpr (COLS_B) {
-                    const int col = col0 + 8 * (tid % K::CB);
-                    hb[i] = hold(bp[i] + k0 * g.ld_w, b_col[i] + k0 < g.k ? g.n - col : 0);
-                } else {
-                    hb[i] = hold(bp[i] + b_col[i] + k0, g.k - b_col[i] - k0);
-                }
+                const int row = tid / K::CB + i * (K::kThreads / K::CB);
+                if constexpr (COLS_B)
+                    hb[i] = hold(w + (k0 + row) * g.ld_w + b_col, k0 + row < g.k ? g.n - b_col : 0);
+                else
+                    hb[i] = hold(w + (col0 + row) * g.ld_w + b_col + k0, col0 + row < g.n ? g.k - b_col - k0 : 0);
             }
         }
     };
     v16f acc[MT][NT] = {};
     const int wk = wave % WK, wn = wave / WK % WN, wm = wave / WK / WN;
-    fetch(0);
-    for (int k0 = 0; k0 < g.k; k0 += K::BK) {
+    // WHOLE: the chunk ends within the sum; else what lies past its end is zeros, in both operands
+    auto stage_a = [&](int k0, char* to, auto whole) {
         if constexpr (DIRECT_A) {
 #pragma unroll
             for (int i = 0; i < K::NA; ++i)
-                to_lds(a_col[i] + k0 < g.k ? (const void*)(ap[i] + a_col[i] + k0) : &kZeroChunk,
-                       lds_a + (i * K::kThreads + wave * 64) * 16);
+                to_lds(decltype(whole)::value || a_col + k0 < g.k ? (const void*)(ap[i] + k0) : &kZeroChunk,
+                       to + (i * K::kThreads + wave * 64) * 16);
         } else {
             if (g.x_op) {
 #pragma unroll
@@ -527,22 +528,43 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
             }
 #pragma unroll
             for (int i = 0; i < K::NA; ++i)
-                put(lds_a + K::TA::at(tid / C + i * (K::kThreads / C), tid % C), K::TA::kBytes, ha[i]);
+                put(to + K::TA::at(tid / C + i * (K::kThreads / C), tid % C), K::TA::kBytes, ha[i]);
         }
+    };
+    auto stage_b = [&](int k0, char* to, auto whole) {
         if constexpr (DIRECT_B) {
+            const char* base = wb + k0 * w_step;
 #pragma unroll
-            for (int i = 0; i < K::NB; ++i)
-                to_lds(b_col[i] + k0 < g.k ? (const void*)(COLS_B ? bp[i] + k0 * g.ld_w : bp[i] + b_col[i] + k0) : &kZeroChunk,
-                       lds_b + (i * K::kThreads + wave * 64) * 16);
+            for (int i = 0; i < K::NB; ++i) {
+                const int at = COLS_B ? tid / K::CB + i * (K::kThreads / K::CB) : b_col;     // place in the chunk
+                to_lds(decltype(whole)::value || at + k0 < g.k ? (const void*)(base + b_off[i]) : &kZeroChunk,
+                       to + (i * K::kThreads + wave * 64) * 16);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < K::NB; ++i)
-                put(lds_b + K::TB::at(tid / K::CB + i * (K::kThreads / K::CB), tid % K::CB), K::TB::kBytes, hb[i]);
+                put(to + K::TB::at(tid / K::CB + i * (K::kThreads / K::CB), tid % K::CB), K::TB::kBytes, hb[i]);
         }
+    };
+    auto stage = [&](int k0, char* to) {
+        if (k0 + K::BK <= g.k) {
+            stage_a(k0, to, std::true_type{});
+            stage_b(k0, to + K::kLdsA, std::true_type{});
+        } else {
+            stage_a(k0, to, std::false_type{});
+            stage_b(k0, to + K::kLdsA, std::false_type{});
+        }
+    };
+    auto products = [&](const char* from) {
+        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
+            from, from + K::kLdsA, 32 * MT * wm, 32 * NT * wn, wk * (K::BK / WK), lane, acc);
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < g.k; k0 += K::BK) {
+        stage(k0, lds);
         __syncthreads();
         if (k0 + K::BK < g.k) fetch(k0 + K::BK);
-        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT>(lds_a, lds_b, 32 * MT * wm, 32 * NT * wn,
-                                                                        wk * (K::BK / WK), (wk + 1) * (K::BK / WK), lane, acc);
+        products(lds);
         __syncthreads();
     }
 
@@ -588,8 +610,11 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 }
 
 // ---------------------------------------------------------------- weight gradient
-// 128 x 128 tiles (n, k) of one group, the sum down a chunk of its slots. Groups of one chunk write their result, the
-// others partial sums for grouped_join_kernel, in the order of their slots: no atomics.
+// 128 x 128 tiles (n, k), the sum down the places of order. The places are cut into equal shares, as many as fill the chip
+// once with a workgroup per share and tile, wherever the groups end: a workgroup goes through the groups of its share.
+// A group that lies within one share is finished there; of the others each share leaves a partial result, two at most (of its
+// first and its last group), which grouped_join_kernel adds in order: no atomics. 100,000 x 2 slots, 512 x 2304, eight
+// groups, bf16: 673 us, against 780 us with chunks of single groups (2.25 rounds of workgroups of unlike length).
 template <typename T>
 struct WeightKernel {
     using Op = Operand<T>;
@@ -615,30 +640,48 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
     using K = WeightKernel<T>;
     __shared__ __attribute__((aligned(256))) char lds[K::kLds];
     const int64_t per = (int64_t)g.row_tiles * g.col_tiles;
-    const int64_t item = xcd_item(g.items * per);
-    const Range r = find_piece(g.ptr, g.groups - 1, g.groups, g.slots, g.chunk, 1, item / per);
-    if (r.group < 0) return;
+    const int64_t item = xcd_item(per * (g.shares > 1 ? g.shares : g.groups));
     const int row0 = (int)(item % per / g.col_tiles) * 128, col0 = (int)(item % g.col_tiles) * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t p0 = r.begin + r.index * g.chunk;
-    const int64_t p1 = p0 + g.chunk < r.end ? p0 + g.chunk : r.end;
     const T *x = (const T*)g.x, *dy = (const T*)g.dy;
     char *lds_a = lds, *lds_b = lds + K::P * K::TT::kBytes;
-    // a plan whose ranges overlap can name more split pieces than its slots can make: they have no place
-    if (r.pieces > 1 && r.split_before + r.index >= g.part_items) return;
+    const int unit = (int)(item / per);                          // share or group
+    int64_t s0 = 0, s1 = g.slots;
+    int group = unit, last = unit;
+    if (g.shares > 1) {
+        const int64_t lo = clamp_slot(g.ptr[0], g.slots), hi = clamp_slot(g.ptr[g.groups], g.slots);
+        s0 = lo + unit * g.share;
+        s1 = s0 + g.share < hi ? s0 + g.share : hi;
+        if (s0 >= s1) return;
+        // the first group that ends behind s0
+        last = g.groups - 1;
+        for (group = 0; group <= last; group += 64) {
+            const int e = group + lane;
+            const uint64_t m = __ballot(e <= last && g.ptr[e + 1] > s0);
+            if (m) {
+                group += __builtin_ctzll(m);
+                break;
+            }
+        }
+    }
 
     // chunk tid % CT (directly: the one the XOR puts there, the same in all of the thread's rows, four apart)
     const int row_t = tid / K::CT, chunk = DIRECT ? K::TT::chunk(row_t, tid % K::CT) : tid % K::CT;
     const int ca = row0 + 8 * chunk, cb = col0 + 8 * chunk;
     const bool sums = g.db && col0 == 0;
-    float colsum[8] = {};
+    const int64_t stride = (int64_t)g.n * g.k + (g.db ? g.n : 0);
+    const int wn = wave & 1, wm = wave >> 1, slots = (int)g.slots;
+    float colsum[8];
     int32_t next[K::NC];
-    auto find = [&](int64_t p) {
+    const uint32_t ld_a = (uint32_t)(g.ld_dy * sizeof(T)), ld_b = (uint32_t)(g.ld_x * sizeof(T));
+    const int32_t* order;
+    int rows;                                                    // of the present group in this share
+    auto find = [&](int p) {                                     // the slots of the rows from p on
 #pragma unroll
         for (int i = 0; i < K::NC; ++i) {
-            const int64_t at = p + row_t + i * (K::kThreads / K::CT);
-            const int32_t a = at < p1 ? g.order[at] : -1;
-            next[i] = a < g.slots ? a : -1;
+            const int at = p + i * (K::kThreads / K::CT);
+            const int32_t a = at + row_t < rows ? order[at] : -1;
+            next[i] = a < slots ? a : -1;
         }
     };
     Held<T> ha[DIRECT ? 1 : K::NC], hb[DIRECT ? 1 : K::NC];
@@ -648,7 +691,8 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
             for (int i = 0; i < K::NC; ++i) {
                 const int32_t a = next[i];
                 ha[i] = hold(dy + (a >= 0 ? a * g.ld_dy + ca : 0), a >= 0 ? g.n - ca : 0);
-                hb[i] = hold(x + (a >= 0 ? (int64_t)(a / g.xdiv) * g.ld_x + cb : 0), a >= 0 ? g.k - cb : 0);
+                const uint32_t ra = (uint32_t)((uint64_t)(uint32_t)a * g.div_mul >> g.div_shift);
+                hb[i] = hold(x + (a >= 0 ? (int64_t)ra * g.ld_x + cb : 0), a >= 0 ? g.k - cb : 0);
             }
         }
     };
@@ -666,149 +710,147 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
             }
         }
     };
-    v16f acc[2][2] = {};
-    const int wn = wave & 1, wm = wave >> 1;
-    find(p0);
-    fetch();
-    if constexpr (!DIRECT) find(p0 + K::BK);
-    for (int64_t p = p0; p < p1; p += K::BK) {
-        if constexpr (DIRECT) {
+    for (; group <= last; ++group) {
+        const int64_t g0 = clamp_slot(g.ptr[group], g.slots), g1 = clamp_slot(g.ptr[group + 1], g.slots);
+        const int64_t p0 = g0 > s0 ? g0 : s0, p1 = g1 < s1 ? g1 : s1;
+        if (g.shares > 1) {
+            if (p0 >= s1) break;
+            if (p0 >= p1) continue;                              // a group without slots: grouped_join_kernel
+        }
+        order = g.order + p0 + row_t;
+        rows = p1 > p0 ? (int)(p1 - p0) : 0;
+        v16f acc[2][2] = {};
 #pragma unroll
-            for (int i = 0; i < K::NC; ++i) {
-                const int32_t a = next[i];
-                to_lds(a >= 0 && ca < g.n ? (const void*)(dy + a * g.ld_dy + ca) : &kZeroChunk,
-                       lds_a + (i * K::kThreads + wave * 64) * 16);
-                to_lds(a >= 0 && cb < g.k ? (const void*)(x + (int64_t)(a / g.xdiv) * g.ld_x + cb) : &kZeroChunk,
-                       lds_b + (i * K::kThreads + wave * 64) * 16);
-            }
-            find(p + K::BK);
-        } else {
-            if (g.x_op) {
-#pragma unroll
-                for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
-            }
-            if (sums) {
+        for (int e = 0; e < 8; ++e) colsum[e] = 0.f;
+        find(0);
+        fetch();
+        if constexpr (!DIRECT) find(K::BK);
+        for (int p = 0; p < rows; p += K::BK) {
+            if constexpr (DIRECT) {
 #pragma unroll
                 for (int i = 0; i < K::NC; ++i) {
-                    if constexpr (sizeof(T) == 4) add_columns(ha[i].a, ha[i].b);
-                    else add_columns(ha[i].a, ha[i].a);
+                    // strides below 2^31 bytes: one multiply-add an address
+                    const uint32_t a = (uint32_t)next[i], ra = (uint32_t)((uint64_t)a * g.div_mul >> g.div_shift);
+                    const char* pa = (const char*)(dy + ca) + (uint64_t)a * ld_a;
+                    const char* pb = (const char*)(x + cb) + (uint64_t)ra * ld_b;
+                    to_lds(next[i] >= 0 && ca < g.n ? pa : (const char*)&kZeroChunk, lds_a + (i * K::kThreads + wave * 64) * 16);
+                    to_lds(next[i] >= 0 && cb < g.k ? pb : (const char*)&kZeroChunk, lds_b + (i * K::kThreads + wave * 64) * 16);
                 }
-            }
+                find(p + K::BK);
+            } else {
+                if (g.x_op) {
 #pragma unroll
-            for (int i = 0; i < K::NC; ++i) {
-                const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
-                put(lds_a + at, K::TT::kBytes, ha[i]);
-                put(lds_b + at, K::TT::kBytes, hb[i]);
-            }
-        }
-        __syncthreads();
-        if constexpr (DIRECT) {
-            if (sums) {                                          // the thread's own chunks again, from LDS
+                    for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+                }
+                if (sums) {
+#pragma unroll
+                    for (int i = 0; i < K::NC; ++i) {
+                        if constexpr (sizeof(T) == 4) add_columns(ha[i].a, ha[i].b);
+                        else add_columns(ha[i].a, ha[i].a);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < K::NC; ++i) {
-                    const v4u v = *reinterpret_cast<const v4u*>(lds_a + (i * K::kThreads + tid) * 16);
-                    add_columns(v, v);
+                    const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
+                    put(lds_a + at, K::TT::kBytes, ha[i]);
+                    put(lds_b + at, K::TT::kBytes, hb[i]);
                 }
             }
-        } else if (p + K::BK < p1) {
-            fetch();
-            find(p + 2 * K::BK);
-        }
-        chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2>(lds_a, lds_b, 64 * wm, 64 * wn, 0, K::BK, lane, acc);
-        __syncthreads();
-    }
-    const int64_t stride = (int64_t)g.n * g.k + (g.db ? g.n : 0);
-    float* part = r.pieces > 1 ? g.part + (r.split_before + r.index) * stride : nullptr;
-    T* dw = (T*)g.dw + (int64_t)r.group * g.n * g.k;
-    // out through LDS as in the forward: 32 rows of 64 columns of a wave at a time
-    constexpr int kLd = 68;
-    static_assert(K::kLds >= 2 * 32 * kLd * 4, "room for two waves' rows");
-    float* out = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * kLd;
+            __syncthreads();
+            if constexpr (DIRECT) {
+                if (sums) {                                          // the thread's own chunks again, from LDS
 #pragma unroll
-    for (int turn = 0; turn < 2; ++turn) {
-        __syncthreads();
-        if (wm != turn) continue;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    st4(out + (lane & 31) * kLd + 32 * n + 8 * q + 4 * (lane >> 5),
-                        (v4f){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]});
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = (lane >> 3) + 8 * i, row = row0 + 64 * wm + 32 * m + at, c = 8 * (lane & 7);
-                const int col = col0 + 64 * wn + c, left = g.k - col;
-                const v4f lo = ld4(out + at * kLd + c), hi = ld4(out + at * kLd + c + 4);
-                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                if (row >= g.n || left <= 0) continue;
-                if constexpr (__is_same(T, float)) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!finite(v[e]) && e < left)
-                            v[e] = plain_dot((const float*)dy + row, g.ld_dy, (const float*)x + col + e, g.ld_x, g.xdiv, g.x_op,
-                                             g.order, p0, p1, g.slots);
+                    for (int i = 0; i < K::NC; ++i) {
+                        const v4u v = *reinterpret_cast<const v4u*>(lds_a + (i * K::kThreads + tid) * 16);
+                        add_columns(v, v);
+                    }
                 }
+            } else if (p + K::BK < rows) {
+                fetch();
+                find(p + 2 * K::BK);
+            }
+            chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2, K::BK / 16>(lds_a, lds_b, 64 * wm, 64 * wn, 0, lane,
+                                                                                      acc);
+            __syncthreads();
+        }
+        float* part = g0 >= s0 && g1 <= s1 ? nullptr : g.part + (2 * (int64_t)unit + (p0 > s0)) * stride;
+        T* dw = (T*)g.dw + (int64_t)group * g.n * g.k;
+        // out through LDS as in the forward: 32 rows of 64 columns of a wave at a time
+        constexpr int kLd = 68;
+        static_assert(K::kLds >= 2 * 32 * kLd * 4, "room for two waves' rows");
+        float* out = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * kLd;
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+            __syncthreads();
+            if (wm != turn) continue;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        st4(out + (lane & 31) * kLd + 32 * n + 8 * q + 4 * (lane >> 5),
+                            (v4f){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]});
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = (lane >> 3) + 8 * i, row = row0 + 64 * wm + 32 * m + at, c = 8 * (lane & 7);
+                    const int col = col0 + 64 * wn + c, left = g.k - col;
+                    const v4f lo = ld4(out + at * kLd + c), hi = ld4(out + at * kLd + c + 4);
+                    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    if (row >= g.n || left <= 0) continue;
+                    if constexpr (__is_same(T, float)) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (!finite(v[e]) && e < left)
+                                v[e] = plain_dot((const float*)dy + row, g.ld_dy, (const float*)x + col + e, g.ld_x, g.xdiv, g.x_op,
+                                                 g.order, p0, p1, g.slots);
+                    }
+                    if (part)
+                        store_piece(part + (int64_t)row * g.k + col, left, v);
+                    else
+                        store_piece(dw + (int64_t)row * g.k + col, left, v);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        if (sums) {
+            __syncthreads();
+            float* red = reinterpret_cast<float*>(lds);          // 16 threads per chunk of eight columns
+#pragma unroll
+            for (int e = 0; e < 8; ++e) red[row_t * 128 + 8 * chunk + e] = colsum[e];
+            __syncthreads();
+            if (tid < 128 && row0 + tid < g.n) {
+                float s = 0.f;
+                for (int i = 0; i < K::kThreads / K::CT; ++i) s += red[i * 128 + tid];
                 if (part)
-                    store_piece(part + (int64_t)row * g.k + col, left, v);
+                    part[(int64_t)g.n * g.k + row0 + tid] = s;
                 else
-                    store_piece(dw + (int64_t)row * g.k + col, left, v);
+                    ((T*)g.db)[(int64_t)group * g.n + row0 + tid] = from_f<T>(s);
             }
-            __builtin_amdgcn_wave_barrier();
         }
-    }
-    if (sums) {
-        __syncthreads();
-        float* red = reinterpret_cast<float*>(lds);          // 16 threads per chunk of eight columns
-#pragma unroll
-        for (int e = 0; e < 8; ++e) red[row_t * 128 + 8 * chunk + e] = colsum[e];
-        __syncthreads();
-        if (tid < 128 && row0 + tid < g.n) {
-            float s = 0.f;
-            for (int i = 0; i < K::kThreads / K::CT; ++i) s += red[i * 128 + tid];
-            if (part)
-                part[(int64_t)g.n * g.k + row0 + tid] = s;
-            else
-                ((T*)g.db)[(int64_t)r.group * g.n + row0 + tid] = from_f<T>(s);
-        }
+        __syncthreads();                                             // LDS is free for the next group
     }
 }
 
-// dW and db of the groups with several chunks: their partial sums, in order.
+// dW and db of the groups that lie in several shares: their partial sums, in order. Zeros for groups without slots.
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedWArgs g) {
-    __shared__ int64_t first, count;
     const int group = blockIdx.y;
-    if (threadIdx.x < 64) {
-        int64_t before = 0, mine = 0;
-        for (int e0 = 0; e0 <= group; e0 += 64) {
-            const int e = e0 + (int)threadIdx.x;
-            int64_t c = 0;
-            if (e <= group) {
-                const int64_t b = clamp_slot(g.ptr[e], g.slots), d = clamp_slot(g.ptr[e + 1], g.slots);
-                c = d > b ? (d - b + g.chunk - 1) / g.chunk : 0;
-            }
-            if (e == group) mine = c;
-            int m = c > 1 && e < group ? (int)c : 0;
-            for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-            before += m;
-        }
-        for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
-        if (threadIdx.x == 0) {
-            first = before;
-            count = mine;
-        }
-    }
-    __syncthreads();
-    if (count <= 1 || first + count > g.part_items) return;
+    const int64_t lo = clamp_slot(g.ptr[0], g.slots), hi = clamp_slot(g.ptr[g.groups], g.slots);
+    int64_t b = clamp_slot(g.ptr[group], g.slots), e = clamp_slot(g.ptr[group + 1], g.slots);
+    b = b > lo ? b : lo;
+    e = e < hi ? e : hi;
+    const bool none = e <= b;
+    const int64_t first = none ? 0 : (b - lo) / g.share, last = none ? 0 : (e - 1 - lo) / g.share;
+    if ((!none && first == last) || last >= g.shares) return;
     const int64_t nk = (int64_t)g.n * g.k, stride = nk + (g.db ? g.n : 0);
-    const float* part = g.part + first * stride;
+    const float* head = g.part + (2 * first + (b > lo + first * g.share)) * stride;
+    const float* rest = g.part + 2 * (first + 1) * stride;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < stride; i += (int64_t)gridDim.x * 256) {
-        float s = 0.f;
+        float s = none ? 0.f : head[i];
 #pragma unroll 4
-        for (int64_t c = 0; c < count; ++c) s += part[c * stride + i];
+        for (int64_t c = 0; c < last - first; ++c) s += rest[2 * c * stride + i];
         if (i < nk)
             ((T*)g.dw)[group * nk + i] = from_f<T>(s);
         else
@@ -826,14 +868,11 @@ static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
     g.col_tiles = (g.n + K::BN - 1) / K::BN;
     const int64_t grid = g.tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B>), dim3((unsigned)grid),
-                       dim3(K::kThreads), 0, st, g);
+    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B>),
+                       dim3((unsigned)grid), dim3(K::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     return 0;
 }
-
-// Tiles of 128 x 128 once there is about one for every CU, else of 32 x 32 with the sum split over the waves.
-constexpr int64_t kLargeTiles = 256;
 
 // Whether rows of `width` elements at p, `ld` apart, are whole 16-byte chunks at 16-byte addresses.
 template <typename T>
@@ -842,49 +881,94 @@ static inline bool whole_chunks(const void* p, int64_t ld, int64_t width) {
     return sizeof(T) < 4 && !__is_same(T, e4m3_wide) && (uintptr_t)p % 16 == 0 && ld % E == 0 && width % E == 0;
 }
 
-template <typename T, typename Out, bool COLS_B>
-int launch_rows(GroupedArgs g, hipStream_t st) {
-    const int64_t groups = g.groups < g.slots ? g.groups : g.slots;
-    const int64_t large = (g.slots / 128 + groups) * ((g.n + 127) / 128);
-    constexpr int C = sizeof(T) == 4 ? 4 : 8, CS = sizeof(T) == 4 ? 16 : 32;
+template <typename T, typename Out, bool COLS_B, int MT, int NT>
+static int launch_rows_large(GroupedArgs g, hipStream_t st) {
+    constexpr int C = sizeof(T) == 4 ? 4 : 8;
     if constexpr (sizeof(T) < 4 && !__is_same(T, e4m3_wide)) {
         const bool a = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op;
-        const bool b = whole_chunks<T>(g.w, g.ld_w, COLS_B ? g.n : g.k) && g.w_group % (16 / (int)sizeof(T)) == 0;
-        if (large >= kLargeTiles && a && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, true, true>(g, st);
-        if (large >= kLargeTiles && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, false, true>(g, st);
+        const bool b = whole_chunks<T>(g.w, g.ld_w, COLS_B ? g.n : g.k) && g.w_group % (16 / (int)sizeof(T)) == 0 &&
+                       (COLS_B ? 64 : (int64_t)g.n) * g.ld_w * (int64_t)sizeof(T) < ((int64_t)1 << 31);
+        if (a && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, true, true>(g, st);
+        if (b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, false, true>(g, st);
     }
-    if (large >= kLargeTiles) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, 2, 2, C, false, false>(g, st);
-    return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, CS, false, false>(g, st);
+    return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, false, false>(g, st);
 }
 
-// Slots per chunk of the weight gradient: enough chunks for about 2048 workgroups, at most 64 (each adds a partial
-// result to write and to read), of 512 slots at least.
-static inline int64_t weight_chunk(int64_t slots, int n, int k) {
-    const int64_t tiles = (int64_t)((n + 127) / 128) * ((k + 127) / 128);
-    int64_t chunks = 2048 / tiles;
-    chunks = chunks < 4 ? 4 : (chunks > 64 ? 64 : chunks);
-    const int64_t c = (slots + chunks - 1) / chunks;
-    return c < 512 ? 512 : (c + 127) / 128 * 128;
+// The tile: of a workgroup's chunks each waits `wait` ns for memory and barriers and takes `work` ns for each of the
+// workgroups that a CU has to do, so a launch takes about chunks (wait + work ceil(tiles / CUs)); the shape with the
+// least is launched. Fitted to 3 x 10 sizes of 21 to 12,000 slots and widths of 97 to 2304 (us; 32 x 32 split four ways, 64 x
+// 64, 128 x 64, 128 x 128):
+//   fp32, 2304 -> 512:    21 slots 24 / 57 / 82 / 120, 3,000 slots 89 / 74 / 89 / 126, 12,000 slots 303 / 199 / 200 / 174
+//   fp32, 1440 -> 320:    1,344 slots 24 / 38 / 54 / 80, 12,000 slots 126 / 84 / 76 / 114
+//   bf16, 2304 -> 512:    21 slots 9.9 / 18 / 21 / 30, 3,000 slots 30 / 27 / 32 / 41, 12,000 slots 88 / 46 / 50 / 48
+//   bf16, 2304 <- 512:    400 slots 11.9 / 8.6 / 9.6 / 12, 12,000 slots 140 / 54 / 48 / 42
+//   e4m3, 2304 -> 512:    21 slots 7.1 / 10 / 12 / 16, 3,000 slots 20 / 14 / 19 / 23, 12,000 slots 57 / 27 / 28 / 29
+struct RowsShape {
+    int rows, cols, bytes, wait, work;       // bytes: of a row's chunk in the 16-bit or 8-bit operand (of 32 bits: half)
+};
+template <typename T, bool COLS_B>
+static inline int rows_shape(int64_t slots, int64_t groups, int n, int k) {
+    constexpr RowsShape f32[4] = {{32, 32, 256, 650, COLS_B ? 900 : 680}, {64, 64, 64, 380, 400}, {128, 64, 64, 320, 810},
+                                  {128, 128, 64, 460, 1200}};
+    constexpr RowsShape low[4] = {{32, 32, 512, 720, COLS_B ? 550 : 380}, {64, 64, 128, 330, 160}, {128, 64, 128, 300, 350},
+                                  {128, 128, 128, 360, 460}};
+    const int64_t cus = device_cu_count();
+    groups = groups < slots ? groups : slots;
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < 4; ++i) {
+        const RowsShape& s = sizeof(T) == 4 ? f32[i] : low[i];
+        // a group ends in the middle of a tile on average
+        int64_t tiles = slots / s.rows + groups / 2;
+        tiles = (tiles > groups ? tiles : groups) * ((n + s.cols - 1) / s.cols);
+        const int64_t chunk = s.bytes / (__is_same(T, e4m3) ? 1 : 2), chunks = (k + chunk - 1) / chunk;
+        const int64_t ns = chunks * (s.wait + s.work * ((tiles + cus - 1) / cus));
+        if (ns < least) {
+            least = ns;
+            best = i;
+        }
+    }
+    return best;
 }
-// Pieces of the groups with more than one chunk, at most.
-static inline int64_t weight_part_items(int64_t slots, int groups, int64_t chunk) {
-    const int64_t split = slots / (chunk + 1);               // groups of more than a chunk
-    return split ? slots / chunk + (groups < split ? groups : split) : 0;
+
+template <typename T, typename Out, bool COLS_B>
+int launch_rows(GroupedArgs g, hipStream_t st) {
+    switch (rows_shape<T, COLS_B>(g.slots, g.groups, g.n, g.k)) {
+        case 0: return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, (sizeof(T) == 4 ? 16 : 32), false, false>(g, st);
+        case 1: return launch_rows_large<T, Out, COLS_B, 1, 1>(g, st);
+        case 2: return launch_rows_large<T, Out, COLS_B, 2, 1>(g, st);
+        default: return launch_rows_large<T, Out, COLS_B, 2, 2>(g, st);
+    }
+}
+
+// Shares of the weight gradient's slots: a workgroup per share and tile fills the chip once (four workgroups per CU of
+// 16-bit rows, two of fp32 rows), of at least 256 slots each. Up to 512 slots one workgroup per group and tile.
+static inline int weight_shares(int64_t slots, int n, int k, int dtype) {
+    const int64_t tiles = (int64_t)((n + 127) / 128) * ((k + 127) / 128), most = (slots + 255) / 256;
+    const int64_t fill = (dtype == FACE_F32 ? 2 : 4) * (int64_t)device_cu_count() / tiles;
+    const int64_t s = fill < most ? fill : most;
+    return slots <= 512 || s < 1 ? 1 : (int)s;
 }
 
 template <typename T>
 int launch_weight(GroupedWArgs g, hipStream_t st) {
     g.row_tiles = (g.n + 127) / 128;
     g.col_tiles = (g.k + 127) / 128;
-    g.items = g.slots / g.chunk + g.groups;
-    const int64_t grid = g.items * g.row_tiles * g.col_tiles;
+    const int64_t grid = (int64_t)(g.shares > 1 ? g.shares : g.groups) * g.row_tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
     bool direct = false;
-    if constexpr (sizeof(T) < 4) direct = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n);
+    if constexpr (sizeof(T) < 4)
+        direct = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n) &&
+                 g.ld_x < ((int64_t)1 << 30) && g.ld_dy < ((int64_t)1 << 30);
+    // ceil(2^(31 + s) / xdiv) with 2^s >= xdiv is exact for every numerator below 2^31
+    uint32_t s = 0;
+    while (((int64_t)1 << s) < g.xdiv) ++s;
+    g.div_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + g.xdiv - 1) / g.xdiv);
+    g.div_shift = 31 + s;
     auto* kernel = direct ? grouped_weight_kernel<T, (sizeof(T) < 4)> : grouped_weight_kernel<T, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, g);
     FACE_LAUNCH_CHECK();
-    if (g.slots > g.chunk) {
+    if (g.shares > 1) {
         const int64_t blocks = ((int64_t)g.n * g.k + 1023) / 1024;
         hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096), g.groups), dim3(256), 0, st,
                            g);

@@ -69,9 +69,10 @@ extern "C" int face_grouped_linear_dx(const void* dy, int64_t ld_dy, const void*
     return with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), decltype(t), true>(g, (hipStream_t)stream); });
 }
 
-extern "C" int64_t face_grouped_linear_dw_work(int64_t slots, int32_t G, int32_t n, int32_t k, int32_t with_bias) {
-    if (slots <= 0 || G <= 0 || n <= 0 || k <= 0) return 0;
-    return weight_part_items(slots, G, weight_chunk(slots, n, k)) * ((int64_t)n * k + (with_bias ? n : 0)) * 4;
+extern "C" int64_t face_grouped_linear_dw_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t with_bias) {
+    if (slots <= 0 || n <= 0 || k <= 0) return 0;
+    const int shares = weight_shares(slots, n, k, dtype);
+    return shares > 1 ? 2 * shares * ((int64_t)n * k + (with_bias ? n : 0)) * 4 : 0;
 }
 
 extern "C" int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy,
@@ -81,10 +82,10 @@ extern "C" int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div
     if (int rc = grouped_args(ptr, order, slots, G, n, k, dtype)) return rc;
     if (x_div <= 0 || (x_op != 0 && x_op != 1) || ld_x < k || ld_dy < n || !ptr || !dw) return FACE_ERR_ARG;
     if (slots && (!x || !dy)) return FACE_ERR_ARG;
-    const int64_t need = face_grouped_linear_dw_work(slots, G, n, k, db != nullptr);
+    const int64_t need = face_grouped_linear_dw_work(slots, n, k, dtype, db != nullptr);
     if (work_bytes < need || (need && !work)) return FACE_ERR_ARG;
-    const int64_t chunk = weight_chunk(slots, n, k);
-    GroupedWArgs g = {x, ld_x, x_div, x_op, dy, ld_dy, dw, db, (float*)work, weight_part_items(slots, G, chunk),
-                      n, k, ptr, order, slots, G, 0, 0, 0, chunk};
+    const int shares = weight_shares(slots, n, k, dtype);
+    GroupedWArgs g = {x, ld_x, x_div, x_op, 0, 0, dy, ld_dy, dw, db, (float*)work, n, k, ptr, order, slots, G, 0, 0,
+                      shares, (slots + shares - 1) / shares};
     return with_dtype(dtype, [&](auto t) { return launch_weight<decltype(t)>(g, (hipStream_t)stream); });
 }

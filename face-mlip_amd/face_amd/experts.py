@@ -408,7 +408,7 @@ class GroupedLinear(torch.autograd.Function):
             if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
                 dw = torch.empty(G, n, k, dtype=x.dtype, device=x.device)
                 db = torch.empty(G, n, dtype=x.dtype, device=x.device) if ctx.bias and ctx.needs_input_grad[2] else None
-                need = _lib.lib().face_grouped_linear_dw_work(plan.slots, G, n, k, int(db is not None))
+                need = _lib.lib().face_grouped_linear_dw_work(plan.slots, n, k, code, int(db is not None))
                 work = _work(need, x.device)
                 call("face_grouped_linear_dw", ptr(x2), _ld(x2), div, op, ptr(dy), _ld(dy), ptr(p), ptr(order), plan.slots,
                      G, n, k, code, ptr(dw), ptr(db), ptr(work), need, stream, label="grouped_linear_dw")

@@ -606,7 +606,7 @@ int face_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t
                            int64_t ld_z, int32_t z_div, const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G,
                            int32_t n, int32_t k, int32_t dtype, void* dx, int64_t ld_dx, void* stream);
 /* dw (G, n, k) and db (G, n) (may be NULL), dense. work: face_grouped_linear_dw_work bytes. Fixed summation order. */
-int64_t face_grouped_linear_dw_work(int64_t slots, int32_t G, int32_t n, int32_t k, int32_t with_bias);
+int64_t face_grouped_linear_dw_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t with_bias);
 int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy, int64_t ld_dy,
                            const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k,
                            int32_t dtype, void* dw, void* db, void* work, int64_t work_bytes, void* stream);

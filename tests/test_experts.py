@@ -132,8 +132,8 @@ def test_entry_points_refuse_bad_arguments():
     assert lin(ldw=7) == lin(ldy=4) == lin(x=None) == -1 and lin(slots=0) == 0
     assert lin(slots=1 << 31) == lin(G=65536) == -2
     dw = lambda slots, work, n: L.face_grouped_linear_dw(ok, 8, 1, 0, ok, 5, ok, ok, slots, 3, 5, 8, 0, ok, None, work, n, None)
-    need = L.face_grouped_linear_dw_work(5000, 3, 5, 8, 0)
+    need = L.face_grouped_linear_dw_work(5000, 5, 8, 0, 0)
     assert need > 0 and dw(5000, None, need) == -1 and dw(5000, ok, need - 1) == -1
-    assert L.face_grouped_linear_dw_work(512, 3, 5, 8, 0) == 0
+    assert L.face_grouped_linear_dw_work(512, 5, 8, 0, 0) == 0
     cmb = lambda N=1, k=2, F=8, dt=0, ld=8, y=ok: L.face_expert_combine_fwd(y, ld, ok, None, 0, N, k, F, dt, ok, None)
     assert cmb(N=-1) == cmb(k=0) == cmb(F=0) == cmb(dt=3) == cmb(ld=7) == cmb(y=None) == -1 and cmb(N=0) == 0
