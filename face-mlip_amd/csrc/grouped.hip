@@ -56,36 +56,51 @@ extern "C" int face_grouped_linear_q8(const void* x, int64_t ld_x, const float* 
     return with_dtype(dtype, [&](auto t) { return launch_rows<q8_rows<decltype(t)>, decltype(t), false>(g, (hipStream_t)stream); });
 }
 
-extern "C" int face_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ld_w, int64_t w_group,
-                                      const void* z, int64_t ld_z, int32_t z_div, const int32_t* ptr, const int32_t* order,
-                                      int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* dx,
-                                      int64_t ld_dx, void* stream) {
-    if (int rc = grouped_args(ptr, order, slots, G, n, k, dtype)) return rc;
-    if (ld_dy < n || ld_w < k || w_group < 0 || (z && (ld_z < k || z_div <= 0)) || ld_dx < k) return FACE_ERR_ARG;
-    if (slots == 0) return 0;
-    if (!dy || !w || !dx) return FACE_ERR_ARG;
-    GroupedArgs g = {dy, ld_dy, 1, 0, w, ld_w, w_group, nullptr, 0, nullptr, nullptr, dx, ld_dx, z, ld_z, z ? z_div : 1,
-                     k, n, ptr, order, slots, G, 0, 0};
-    return with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), decltype(t), true>(g, (hipStream_t)stream); });
+namespace face {
+// Workspace of the backward: a row of dx per slot where the rows of x are shared, then the weights' partial results.
+static int64_t slot_rows_bytes(int64_t slots, int32_t k, int32_t dtype, int32_t x_div) {
+    return x_div > 1 ? (slots * k * (dtype == FACE_F32 ? 4 : 2) + 255) / 256 * 256 : 0;
 }
-
-extern "C" int64_t face_grouped_linear_dw_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t with_bias) {
-    if (slots <= 0 || n <= 0 || k <= 0) return 0;
+static int64_t part_bytes(int64_t slots, int32_t n, int32_t k, int32_t dtype, bool with_bias) {
     const int shares = weight_shares(slots, n, k, dtype);
     return shares > 1 ? 2 * shares * ((int64_t)n * k + (with_bias ? n : 0)) * 4 : 0;
 }
+}  // namespace face
 
-extern "C" int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy,
-                                      int64_t ld_dy, const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G,
-                                      int32_t n, int32_t k, int32_t dtype, void* dw, void* db, void* work,
-                                      int64_t work_bytes, void* stream) {
+extern "C" int64_t face_grouped_linear_bwd_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t x_div,
+                                                int32_t with_dx, int32_t with_dw, int32_t with_db) {
+    if (slots <= 0 || n <= 0 || k <= 0) return 0;
+    return (with_dx ? slot_rows_bytes(slots, k, dtype, x_div) : 0) + (with_dw ? part_bytes(slots, n, k, dtype, with_db) : 0);
+}
+
+extern "C" int face_grouped_linear_bwd(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy,
+                                       int64_t ld_dy, const void* w, int64_t ld_w, int64_t w_group, const int32_t* ptr,
+                                       const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype,
+                                       void* dx, void* dw, void* db, void* work, int64_t work_bytes, void* stream) {
     if (int rc = grouped_args(ptr, order, slots, G, n, k, dtype)) return rc;
-    if (x_div <= 0 || (x_op != 0 && x_op != 1) || ld_x < k || ld_dy < n || !ptr || !dw) return FACE_ERR_ARG;
-    if (slots && (!x || !dy)) return FACE_ERR_ARG;
-    const int64_t need = face_grouped_linear_dw_work(slots, n, k, dtype, db != nullptr);
+    if (x_div <= 0 || slots % x_div || (x_op != 0 && x_op != 1) || ld_x < k || ld_dy < n || (db && !dw)) return FACE_ERR_ARG;
+    if (dx && (ld_w < k || w_group < 0)) return FACE_ERR_ARG;
+    if (dw && !ptr) return FACE_ERR_ARG;
+    if (slots && (!dy || (dx && !w) || ((dw || x_op) && !x))) return FACE_ERR_ARG;
+    const int64_t need = face_grouped_linear_bwd_work(slots, n, k, dtype, x_div, dx != nullptr, dw != nullptr, db != nullptr);
     if (work_bytes < need || (need && !work)) return FACE_ERR_ARG;
-    const int shares = weight_shares(slots, n, k, dtype);
-    GroupedWArgs g = {x, ld_x, x_div, x_op, 0, 0, dy, ld_dy, dw, db, (float*)work, n, k, ptr, order, slots, G, 0, 0,
-                      shares, (slots + shares - 1) / shares};
-    return with_dtype(dtype, [&](auto t) { return launch_weight<decltype(t)>(g, (hipStream_t)stream); });
+    char* part = (char*)work + (dx ? slot_rows_bytes(slots, k, dtype, x_div) : 0);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dx && slots) {
+        void* rows = x_div > 1 ? work : dx;
+        GroupedArgs g = {dy, ld_dy, 1, 0, w, ld_w, w_group, nullptr, 0, nullptr, nullptr, rows, k, x_op ? x : nullptr, ld_x,
+                         x_div, k, n, ptr, order, slots, G, 0, 0};
+        int rc = with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), decltype(t), true>(g, st); });
+        // a slot's row was rounded to the rows' type; the sum of a row's slots is rounded once more
+        if (!rc && x_div > 1)
+            rc = face_expert_combine_fwd(work, k, nullptr, nullptr, 0, slots / x_div, x_div, k, dtype, dx, stream);
+        if (rc) return rc;
+    }
+    if (dw) {
+        const int shares = weight_shares(slots, n, k, dtype);
+        GroupedWArgs g = {x, ld_x, x_div, x_op, 0, 0, dy, ld_dy, dw, db, (float*)part, n, k, ptr, order, slots, G, 0, 0,
+                          shares, (slots + shares - 1) / shares};
+        return with_dtype(dtype, [&](auto t) { return launch_weight<decltype(t)>(g, st); });
+    }
+    return 0;
 }

@@ -100,10 +100,9 @@ _SIGS = {
                                            P]),
     "face_grouped_linear_q8": (ctypes.c_int, [P, I64, P, I32, P, I64, I64, P, P, I64, P, P, I64, I32, I32, I32, I32, P,
                                               I64, P]),
-    "face_grouped_linear_dx": (ctypes.c_int, [P, I64, P, I64, I64, P, I64, I32, P, P, I64, I32, I32, I32, I32, P, I64,
-                                              P]),
-    "face_grouped_linear_dw_work": (I64, [I64, I32, I32, I32, I32]),
-    "face_grouped_linear_dw": (ctypes.c_int, [P, I64, I32, I32, P, I64, P, P, I64, I32, I32, I32, I32, P, P, P, I64, P]),
+    "face_grouped_linear_bwd_work": (I64, [I64, I32, I32, I32, I32, I32, I32, I32]),
+    "face_grouped_linear_bwd": (ctypes.c_int, [P, I64, I32, I32, P, I64, P, I64, I64, P, P, I64, I32, I32, I32, I32, P, P,
+                                               P, P, I64, P]),
     "face_expert_combine_fwd": (ctypes.c_int, [P, I64, P, P, I64, I64, I32, I32, I32, P, P]),
     "face_expert_combine_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, I32, I32, I32, P, P, P]),
 }

@@ -19,7 +19,6 @@ synchronises; none has a CPU path. They differentiate once, in training too: all
 inputs take gradients, except those of the 8-bit forms.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr
@@ -53,31 +52,30 @@ def _check(name, ref, **tensors):
 def _rows(t, width):
     """t as (rows, width) with unit column stride and rows one after the other: a view where its
     strides allow one, else a copy."""
-    t = t if t.dim() == 2 else t.reshape(-1, width)
-    if t.shape[0] > 1 and (t.stride(0) < width or (t.stride(1) != 1 and width > 1)) or \
-            t.shape[0] <= 1 and width > 1 and t.stride(1) != 1:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    if t.stride(1) == 1 and t.stride(0) >= width:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _ld(t):
-    """Row stride of a _rows() tensor (that of a single row does not matter)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-class _on:
-    """The device of a tensor as the current one while a kernel is launched (nothing to do when it is)."""
+def _launch(t, name, label, *args):
+    """Call entry point `name` with args and the current stream of t's device, as the current device."""
+    idx = t.device.index
+    if idx == _get_device():
+        call(name, *args, _lib.stream_of(t), label=label)
+    else:
+        with torch.cuda.device(idx):
+            call(name, *args, _lib.stream_of(t), label=label)
 
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _once():
+    """A backward that is itself recorded would need second derivatives."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError("the expert layer's operators differentiate once (create_graph=False)")
 
 
 def _work(n_bytes, device):
@@ -115,9 +113,8 @@ def _norm_fwd(code, x, w, eps, r, q8):
     y = None if q8 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     q = torch.empty(x.shape, dtype=_E4M3, device=x.device) if q8 else None
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if q8 else None
-    with _on(x):
-        call("face_rms_norm_fwd", ptr(x2), _ld(x2), ptr(r2), F if r2 is None else _ld(r2), N, F, code, ptr(w), eps,
-             ptr(y), ptr(s), ptr(q), ptr(scale), _lib.stream_of(x), label="rms_norm_fwd")
+    _launch(x, "face_rms_norm_fwd", "rms_norm_fwd", x2.data_ptr(), x2.stride(0), ptr(r2), F if r2 is None else r2.stride(0),
+            N, F, code, w.data_ptr(), eps, ptr(y), ptr(s), ptr(q), ptr(scale))
     return (q, scale, s) if q8 else (y, s)
 
 
@@ -128,32 +125,34 @@ class RMSNorm(torch.autograd.Function):
     def forward(ctx, x, w, eps, r):
         y, s = _norm_fwd(_DTYPES[x.dtype], x, w, eps, r, False)
         ctx.save_for_backward(x if s is None else s, w)
-        ctx.eps, ctx.residual = eps, r is not None
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, ds=None):
-        s, w = ctx.saved_tensors
-        need_w = ctx.needs_input_grad[1]
-        need_x = ctx.needs_input_grad[0] or (ctx.residual and ctx.needs_input_grad[3])
-        if dy is None and ds is None or not (need_x or need_w):
+        _once()
+        need_x, need_w, _, need_r = ctx.needs_input_grad
+        if dy is None and ds is None:
             return None, None, None, None
-        F = s.shape[-1]
+        s, w = ctx.saved_tensors
+        F, code = s.shape[-1], _DTYPES[s.dtype]
         s2, w = _rows(s, F), w.contiguous()
-        dy, ds = (None if t is None else _rows(t, F) for t in (dy, ds))
         N = s2.shape[0]
-        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device) if need_x else None
-        dw = torch.empty_like(w) if need_w else None
-        need = _lib.lib().face_rms_norm_bwd_work(N, F) if need_w else 0
-        work = _work(need, s.device)
-        with _on(s):
-            call("face_rms_norm_bwd", ptr(s2), _ld(s2), ptr(dy), F if dy is None else _ld(dy), ptr(ds),
-                 F if ds is None else _ld(ds), N, F, _DTYPES[s.dtype], ptr(w), ctx.eps, ptr(dx), ptr(dw), ptr(work), need,
-                 _lib.stream_of(s), label="rms_norm_bwd")
-        return (dx if ctx.needs_input_grad[0] else None, dw, None,
-                dx if ctx.residual and ctx.needs_input_grad[3] else None)
+        if dy is not None:
+            dy = _rows(dy, F)
+        if ds is not None:
+            ds = _rows(ds, F)
+        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device) if need_x or need_r else None
+        dw = work = None
+        need = 0
+        if need_w:
+            dw = torch.empty_like(w)
+            need = _lib.lib().face_rms_norm_bwd_work(N, F)
+            work = _work(need, s.device)
+        _launch(s, "face_rms_norm_bwd", "rms_norm_bwd", s2.data_ptr(), s2.stride(0), ptr(dy), F if dy is None else dy.stride(0),
+                ptr(ds), F if ds is None else ds.stride(0), N, F, code, w.data_ptr(), ctx.eps, ptr(dx), ptr(dw), ptr(work), need)
+        return dx if need_x else None, dw, None, dx if need_r else None
 
 
 def rms_norm(x, w, eps=1e-6, residual=None):
@@ -192,9 +191,8 @@ def quantize_rows(x, x_op=None):
     x2 = _rows(x, F)
     q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with _on(x):
-        call("face_quantize_rows", ptr(x2), _ld(x2), x2.shape[0], F, code, _X_OPS[x_op], ptr(q), ptr(scale),
-             _lib.stream_of(x), label="quantize_rows")
+    _launch(x, "face_quantize_rows", "quantize_rows", x2.data_ptr(), x2.stride(0), x2.shape[0], F, code, _X_OPS[x_op],
+            q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -204,10 +202,8 @@ def _route_fwd(logits, k, allowed, group, renorm):
     l2 = _rows(logits, E)
     expert = torch.empty(N, k, dtype=torch.int32, device=logits.device)
     weight = torch.empty(N, k, dtype=torch.float32, device=logits.device)
-    with _on(logits):
-        call("face_route_fwd", ptr(l2), _ld(l2), N, E, k, _DTYPES[logits.dtype], ptr(allowed), ptr(group),
-             0 if allowed is None else allowed.shape[0], int(renorm), ptr(expert), ptr(weight), _lib.stream_of(logits),
-             label="route_fwd")
+    _launch(logits, "face_route_fwd", "route_fwd", l2.data_ptr(), l2.stride(0), N, E, k, _DTYPES[logits.dtype], ptr(allowed),
+            ptr(group), 0 if allowed is None else allowed.shape[0], int(renorm), expert.data_ptr(), weight.data_ptr())
     return expert, weight
 
 
@@ -222,18 +218,17 @@ class Route(torch.autograd.Function):
         return expert, weight
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _, dweight):
+        _once()
         if dweight is None:
             return None, None, None, None, None
         logits, allowed, group, expert, weight = ctx.saved_tensors
         N, E = logits.shape
         l2, dweight = _rows(logits, E), dweight.contiguous()
         dl = torch.empty(N, E, dtype=logits.dtype, device=logits.device)
-        with _on(logits):
-            call("face_route_bwd", ptr(l2), _ld(l2), N, E, ctx.k, _DTYPES[logits.dtype], ptr(allowed), ptr(group),
-                 0 if allowed is None else allowed.shape[0], int(ctx.renorm), ptr(expert), ptr(weight), ptr(dweight),
-                 ptr(dl), _lib.stream_of(logits), label="route_bwd")
+        _launch(logits, "face_route_bwd", "route_bwd", l2.data_ptr(), l2.stride(0), N, E, ctx.k, _DTYPES[logits.dtype],
+                ptr(allowed), ptr(group), 0 if allowed is None else allowed.shape[0], int(ctx.renorm), expert.data_ptr(),
+                weight.data_ptr(), dweight.data_ptr(), dl.data_ptr())
         return dl, None, None, None, None
 
 
@@ -326,9 +321,7 @@ def group_plan(expert, n_groups):
     order = torch.empty(slots, dtype=torch.int32, device=e.device)
     need = _lib.lib().face_group_plan_work(slots, n_groups)
     work = _work(need, e.device)
-    with _on(e):
-        call("face_group_plan", ptr(e), slots, n_groups, ptr(p), ptr(order), ptr(work), need, _lib.stream_of(e),
-             label="group_plan")
+    _launch(e, "face_group_plan", "group_plan", e.data_ptr(), slots, n_groups, p.data_ptr(), order.data_ptr(), ptr(work), need)
     return GroupPlan(p, order, e.shape[0], 1 if e.dim() == 1 else e.shape[1])
 
 
@@ -364,10 +357,9 @@ def _linear_fwd(x, w, plan, bias, op):
     G, n, k = w.shape
     x2, w, b = _rows(x, k), _weights(w), None if bias is None else bias.contiguous()
     y = torch.empty(plan.slots, n, dtype=x.dtype, device=x.device)
-    with _on(x):
-        call("face_grouped_linear", ptr(x2), _ld(x2), _div(plan, x.shape[0]), op, ptr(w), w.stride(1), w.stride(0), ptr(b), n,
-             ptr(plan.ptr), ptr(plan.order), plan.slots, G, n, k, _DTYPES[x.dtype], ptr(y), n, _lib.stream_of(x),
-             label="grouped_linear_fwd")
+    _launch(x, "face_grouped_linear", "grouped_linear_fwd", x2.data_ptr(), x2.stride(0), _div(plan, x.shape[0]), op,
+            w.data_ptr(), w.stride(1), w.stride(0), ptr(b), n, plan.ptr.data_ptr(), plan.order.data_ptr(), plan.slots, G, n, k,
+            _DTYPES[x.dtype], y.data_ptr(), n)
     return y
 
 
@@ -376,43 +368,31 @@ class GroupedLinear(torch.autograd.Function):
     def forward(ctx, x, w, bias, p, order, plan, op):
         y = _linear_fwd(x, w, plan, bias, op)
         ctx.save_for_backward(x, w, p, order)
-        ctx.plan, ctx.op, ctx.bias = plan, op, bias is not None
+        ctx.plan, ctx.op = plan, op
         ctx.set_materialize_grads(False)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _once()
         if dy is None:
             return (None,) * 7
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x, w, p, order = ctx.saved_tensors
-        plan, op, code = ctx.plan, ctx.op, _DTYPES[x.dtype]
+        dtype, dev, code = x.dtype, x.device, _DTYPES[x.dtype]
         G, n, k = w.shape
-        div = _div(plan, x.shape[0])
-        x2, dy = _rows(x, k), _rows(dy, n)
-        dx = dw = db = None
-        with _on(x):
-            stream = _lib.stream_of(x)
-            if ctx.needs_input_grad[0]:
-                w2 = _weights(w)
-                dx = torch.empty(plan.slots, k, dtype=x.dtype, device=x.device)
-                z = x2 if op else None
-                call("face_grouped_linear_dx", ptr(dy), _ld(dy), ptr(w2), w2.stride(1), w2.stride(0), ptr(z),
-                     _ld(x2) if op else k, div, ptr(p), ptr(order), plan.slots, G, n, k, code, ptr(dx), k, stream,
-                     label="grouped_linear_dx")
-                if div > 1:
-                    # a row's choices were rounded to the rows' type one by one; their sum is rounded once more
-                    parts, dx = dx, torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                    call("face_expert_combine_fwd", ptr(parts), k, None, None, k, x.shape[0], div, k, code, ptr(dx), stream,
-                         label="expert_combine_fwd")
-            if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-                dw = torch.empty(G, n, k, dtype=x.dtype, device=x.device)
-                db = torch.empty(G, n, dtype=x.dtype, device=x.device) if ctx.bias and ctx.needs_input_grad[2] else None
-                need = _lib.lib().face_grouped_linear_dw_work(plan.slots, n, k, code, int(db is not None))
-                work = _work(need, x.device)
-                call("face_grouped_linear_dw", ptr(x2), _ld(x2), div, op, ptr(dy), _ld(dy), ptr(p), ptr(order), plan.slots,
-                     G, n, k, code, ptr(dw), ptr(db), ptr(work), need, stream, label="grouped_linear_dw")
-        return dx, dw if ctx.needs_input_grad[1] else None, db, None, None, None, None
+        slots = order.shape[0]
+        div = _div(ctx.plan, x.shape[0])
+        x2, dy, w2 = _rows(x, k), _rows(dy, n), _weights(w)
+        dx = torch.empty(x.shape, dtype=dtype, device=dev) if need_x else None
+        dw = torch.empty(G, n, k, dtype=dtype, device=dev) if need_w or need_b else None
+        db = torch.empty(G, n, dtype=dtype, device=dev) if need_b else None
+        need = _lib.lib().face_grouped_linear_bwd_work(slots, n, k, code, div, need_x, need_w or need_b, need_b)
+        work = _work(need, dev)
+        _launch(x, "face_grouped_linear_bwd", "grouped_linear_bwd", x2.data_ptr(), x2.stride(0), div, ctx.op, dy.data_ptr(),
+                dy.stride(0), w2.data_ptr(), w2.stride(1), w2.stride(0), p.data_ptr(), order.data_ptr(), slots, G, n, k, code,
+                ptr(dx), ptr(dw), ptr(db), ptr(work), need)
+        return dx, dw if need_w else None, db, None, None, None, None
 
 
 def grouped_linear(x, w, plan, bias=None, x_op=None):
@@ -452,10 +432,9 @@ def grouped_linear_q8(x, x_scale, w, w_scale, plan, bias=None, dtype=torch.bfloa
     x2, w2 = _rows(x, k), _weights(w)
     xs, ws, b = x_scale.contiguous(), w_scale.contiguous(), None if bias is None else bias.contiguous()
     y = torch.empty(plan.slots, n, dtype=dtype, device=x.device)
-    with _on(x):
-        call("face_grouped_linear_q8", ptr(x2), _ld(x2), ptr(xs), _div(plan, x.shape[0]), ptr(w2), w2.stride(1), w2.stride(0),
-             ptr(ws), ptr(b), n, ptr(plan.ptr), ptr(plan.order), plan.slots, G, n, k, _DTYPES[dtype], ptr(y), n,
-             _lib.stream_of(x), label="grouped_linear_q8")
+    _launch(x, "face_grouped_linear_q8", "grouped_linear_q8", x2.data_ptr(), x2.stride(0), xs.data_ptr(),
+            _div(plan, x.shape[0]), w2.data_ptr(), w2.stride(1), w2.stride(0), ws.data_ptr(), ptr(b), n, plan.ptr.data_ptr(),
+            plan.order.data_ptr(), plan.slots, G, n, k, _DTYPES[dtype], y.data_ptr(), n)
     return y
 
 
@@ -466,9 +445,8 @@ def _combine_fwd(y, weight, residual):
     y2, w = _rows(y, F), weight.contiguous()
     r = None if residual is None else _rows(residual, F)
     out = torch.empty(N, F, dtype=y.dtype, device=y.device)
-    with _on(y):
-        call("face_expert_combine_fwd", ptr(y2), _ld(y2), ptr(w), ptr(r), F if r is None else _ld(r), N, k, F,
-             _DTYPES[y.dtype], ptr(out), _lib.stream_of(y), label="expert_combine_fwd")
+    _launch(y, "face_expert_combine_fwd", "expert_combine_fwd", y2.data_ptr(), y2.stride(0), w.data_ptr(), ptr(r),
+            F if r is None else r.stride(0), N, k, F, _DTYPES[y.dtype], out.data_ptr())
     return out
 
 
@@ -479,19 +457,21 @@ class ExpertCombine(torch.autograd.Function):
         return _combine_fwd(y, weight, residual)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        y, weight = ctx.saved_tensors
-        N, k = weight.shape
-        F = y.shape[1]
+        _once()
         need_y, need_w, need_r = ctx.needs_input_grad
-        dy = torch.empty(N * k, F, dtype=y.dtype, device=y.device) if need_y else None
-        dw = torch.empty(N, k, dtype=torch.float32, device=y.device) if need_w else None
+        dy = dw = None
         if need_y or need_w:
+            y, weight = ctx.saved_tensors
+            N, k = weight.shape
+            F = y.shape[1]
+            if need_y:
+                dy = torch.empty(N * k, F, dtype=y.dtype, device=y.device)
+            if need_w:
+                dw = torch.empty(N, k, dtype=torch.float32, device=y.device)
             y2, w, d = _rows(y, F), weight.contiguous(), _rows(dout, F)
-            with _on(y):
-                call("face_expert_combine_bwd", ptr(d), _ld(d), ptr(y2), _ld(y2), ptr(w), N, k, F, _DTYPES[y.dtype], ptr(dy),
-                     ptr(dw), _lib.stream_of(y), label="expert_combine_bwd")
+            _launch(y, "face_expert_combine_bwd", "expert_combine_bwd", d.data_ptr(), d.stride(0), y2.data_ptr(), y2.stride(0),
+                    w.data_ptr(), N, k, F, _DTYPES[y.dtype], ptr(dy), ptr(dw))
         return dy, dw, dout if need_r else None
 
 

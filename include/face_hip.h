@@ -601,15 +601,16 @@ int face_grouped_linear_q8(const void* x, int64_t ld_x, const float* x_scale, in
                            int64_t w_group, const float* w_scale, const void* bias, int64_t ld_b, const int32_t* ptr,
                            const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* y,
                            int64_t ld_y, void* stream);
-/* dx[a] (slots, k) = (dy[a] W[g]) [* silu'(z[a / z_div])], a row per slot; z NULL: no factor. */
-int face_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ld_w, int64_t w_group, const void* z,
-                           int64_t ld_z, int32_t z_div, const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G,
-                           int32_t n, int32_t k, int32_t dtype, void* dx, int64_t ld_dx, void* stream);
-/* dw (G, n, k) and db (G, n) (may be NULL), dense. work: face_grouped_linear_dw_work bytes. Fixed summation order. */
-int64_t face_grouped_linear_dw_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t with_bias);
-int face_grouped_linear_dw(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy, int64_t ld_dy,
-                           const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k,
-                           int32_t dtype, void* dw, void* db, void* work, int64_t work_bytes, void* stream);
+/* Its gradients for dy (slots, n): dx like x, dense rows (the slots of a shared row rounded to the rows' type, then
+ * summed), dw (G, n, k) and db (G, n) dense; each may be NULL (db only with dw; w is read for dx, x for dw and for
+ * x_op). slots a multiple of x_div. work: face_grouped_linear_bwd_work bytes, 256-byte aligned. Fixed summation
+ * order. */
+int64_t face_grouped_linear_bwd_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t x_div, int32_t with_dx,
+                                     int32_t with_dw, int32_t with_db);
+int face_grouped_linear_bwd(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy, int64_t ld_dy,
+                            const void* w, int64_t ld_w, int64_t w_group, const int32_t* ptr, const int32_t* order,
+                            int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* dx, void* dw, void* db,
+                            void* work, int64_t work_bytes, void* stream);
 
 /* out[i] (N, F) = r[i] + sum_j weight[i, j] y[i k + j]; r NULL: 0, weight (N, k) NULL: 1. */
 int face_expert_combine_fwd(const void* y, int64_t ld_y, const float* weight, const void* r, int64_t ld_r, int64_t N,

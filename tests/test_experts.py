@@ -131,9 +131,13 @@ def test_entry_points_refuse_bad_arguments():
     assert lin(n=0) == lin(k=0) == lin(dt=3) == lin(slots=-1) == lin(G=0) == lin(xd=0) == lin(op=2) == lin(ldx=7) == -1
     assert lin(ldw=7) == lin(ldy=4) == lin(x=None) == -1 and lin(slots=0) == 0
     assert lin(slots=1 << 31) == lin(G=65536) == -2
-    dw = lambda slots, work, n: L.face_grouped_linear_dw(ok, 8, 1, 0, ok, 5, ok, ok, slots, 3, 5, 8, 0, ok, None, work, n, None)
-    need = L.face_grouped_linear_dw_work(5000, 5, 8, 0, 0)
-    assert need > 0 and dw(5000, None, need) == -1 and dw(5000, ok, need - 1) == -1
-    assert L.face_grouped_linear_dw_work(512, 5, 8, 0, 0) == 0
+    bwd = lambda slots=4, work=None, n=0, xd=1, dx=None, dw=None, db=None, w=ok, x=ok, ldy=5, op=0: L.face_grouped_linear_bwd(
+        x, 8, xd, op, ok, ldy, w, 8, 40, ok, ok, slots, 3, 5, 8, 0, dx, dw, db, work, n, None)
+    need = L.face_grouped_linear_bwd_work(5000, 5, 8, 0, 1, 1, 1, 0)
+    assert need > 0 and bwd(5000, None, need, dw=ok) == -1 and bwd(5000, ok, need - 1, dw=ok) == -1
+    assert L.face_grouped_linear_bwd_work(512, 5, 8, 0, 1, 1, 1, 1) == 0
+    assert L.face_grouped_linear_bwd_work(512, 5, 8, 0, 2, 1, 0, 0) == 512 * 8 * 4
+    assert bwd(dx=ok, xd=2) == bwd(dx=ok, xd=3) == bwd(db=ok) == bwd(dx=ok, w=None) == bwd(dw=ok, x=None) == -1
+    assert bwd(dx=ok, x=None, op=1) == bwd(dx=ok, ldy=4) == bwd(dx=ok, op=2) == -1 and bwd() == 0
     cmb = lambda N=1, k=2, F=8, dt=0, ld=8, y=ok: L.face_expert_combine_fwd(y, ld, ok, None, 0, N, k, F, dt, ok, None)
     assert cmb(N=-1) == cmb(k=0) == cmb(F=0) == cmb(dt=3) == cmb(ld=7) == cmb(y=None) == -1 and cmb(N=0) == 0

@@ -796,9 +796,13 @@ def test_two_captured_graphs():
                 assert torch.equal(a, b), turn
 
 
-def test_double_backward_is_refused():
+def test_a_recorded_backward_is_refused():
+    """Second derivatives would be dropped in silence: a backward with create_graph raises, in every operator."""
     g = gen(0)
-    x = rand(g, 4, 8).requires_grad_(True)
-    d, = torch.autograd.grad(ex.rms_norm(x, torch.ones(8, device=DEV)).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        d.sum().backward()
+    x, w = rand(g, 4, 8).requires_grad_(True), rand(g, 2, 4).softmax(1).requires_grad_(True)
+    plan = ex.group_plan(torch.zeros(4, dtype=torch.int32, device=DEV), 1)
+    for out in (ex.rms_norm(x, torch.ones(8, device=DEV)), ex.route(x, 2)[1], ex.grouped_linear(x, rand(g, 1, 3, 8), plan),
+                ex.expert_combine(x, rand(g, 2, 2)), ex.expert_combine(x.detach(), w[:, :2])):
+        leaf = x if out.grad_fn.next_functions[0][0] is not None else w
+        with pytest.raises(NotImplementedError, match="differentiate once"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
