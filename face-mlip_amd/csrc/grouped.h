@@ -314,11 +314,24 @@ template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, 
 __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int lane,
                                                v16f acc[MT][NT]) {
     using F = Fragments<T, RA, CA, COLS_A, RB, CB, COLS_B, MT, NT>;
+    if constexpr (MT * NT > 4) {
+        // few waves per SIMD: the next step's operands are on their way during this one's products, and no more of
+        // them (the barrier), or the accumulators would spill
+        F f[2];
+        f[0].load(ta, tb, m0, n0, k_begin, lane);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        F f;
-        f.load(ta, tb, m0, n0, k_begin + s * kStep<T>, lane);
-        f.products(acc);
+        for (int s = 0; s < STEPS; ++s) {
+            if (s + 1 < STEPS) f[(s + 1) & 1].load(ta, tb, m0, n0, k_begin + (s + 1) * kStep<T>, lane);
+            f[s & 1].products(acc);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            F f;
+            f.load(ta, tb, m0, n0, k_begin + s * kStep<T>, lane);
+            f.products(acc);
+        }
     }
 }
 
@@ -613,12 +626,16 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 // 128 x 128 tiles (n, k), the sum down the places of order. The places are cut into equal shares, as many as fill the chip
 // once with a workgroup per share and tile, wherever the groups end: a workgroup goes through the groups of its share.
 // A group that lies within one share is finished there; of the others each share leaves a partial result, two at most (of its
-// first and its last group), which grouped_join_kernel adds in order: no atomics. 100,000 x 2 slots, 512 x 2304, eight
-// groups, bf16: 673 us, against 780 us with chunks of single groups (2.25 rounds of workgroups of unlike length).
-template <typename T>
+// first and its last group), which grouped_join_kernel adds in order: no atomics. 200,000 slots, 512 x 2304, eight
+// groups, bf16: 673 us in 128 x 128 tiles, against 780 us with chunks of single groups (2.25 rounds of workgroups of
+// unlike length).
+// TILE 256 (16-bit operands staged without registers): 256 x 256 by eight waves of 128 x 64, into two buffers in turn, the next
+// slots on their way during the present ones' products.
+template <typename T, int TILE>
 struct WeightKernel {
     using Op = Operand<T>;
-    static constexpr int P = Op::kPlanes, BK = P == 3 ? 32 : 64, kThreads = 256, CT = 16;
+    static constexpr int P = Op::kPlanes, BK = P == 3 ? 32 : 64, CT = TILE / 8;
+    static constexpr int WM = 2, WN = TILE / 64, MT = TILE / 64, NT = 2, kThreads = 64 * WM * WN;
     using TT = Tile<BK, CT, true>;
     static constexpr int kLds = 2 * P * TT::kBytes, NC = BK * CT / kThreads;
 };
@@ -635,16 +652,21 @@ __device__ inline float plain_dot(const float* dy, int64_t ld_dy, const float* x
     return s;
 }
 
-template <typename T, bool DIRECT>
-__global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(GroupedWArgs g) {
-    using K = WeightKernel<T>;
+template <typename T, bool DIRECT, int TILE>
+__global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE == 128 ? 4 : 2)) void grouped_weight_kernel(
+    GroupedWArgs g) {
+    using K = WeightKernel<T, TILE>;
+    constexpr bool kTwo = TILE == 256;
+    static_assert(DIRECT || !kTwo, "two buffers are filled without registers");
+    // two arrays, not one of twice the size: reads of one need not wait for what is on its way into the other
     __shared__ __attribute__((aligned(256))) char lds[K::kLds];
+    __shared__ __attribute__((aligned(256))) char lds_2[kTwo ? K::kLds : 16];
     const int64_t per = (int64_t)g.row_tiles * g.col_tiles;
     const int64_t item = xcd_item(per * (g.shares > 1 ? g.shares : g.groups));
-    const int row0 = (int)(item % per / g.col_tiles) * 128, col0 = (int)(item % g.col_tiles) * 128;
+    const int row0 = (int)(item % per / g.col_tiles) * TILE, col0 = (int)(item % g.col_tiles) * TILE;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *x = (const T*)g.x, *dy = (const T*)g.dy;
-    char *lds_a = lds, *lds_b = lds + K::P * K::TT::kBytes;
+    constexpr int kB = K::P * K::TT::kBytes;                     // where x lies behind dy
     const int unit = (int)(item / per);                          // share or group
     int64_t s0 = 0, s1 = g.slots;
     int group = unit, last = unit;
@@ -670,7 +692,7 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
     const int ca = row0 + 8 * chunk, cb = col0 + 8 * chunk;
     const bool sums = g.db && col0 == 0;
     const int64_t stride = (int64_t)g.n * g.k + (g.db ? g.n : 0);
-    const int wn = wave & 1, wm = wave >> 1, slots = (int)g.slots;
+    const int wn = wave % K::WN, wm = wave / K::WN, slots = (int)g.slots;
     float colsum[8];
     int32_t next[K::NC];
     const uint32_t ld_a = (uint32_t)(g.ld_dy * sizeof(T)), ld_b = (uint32_t)(g.ld_x * sizeof(T));
@@ -719,74 +741,101 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
         }
         order = g.order + p0 + row_t;
         rows = p1 > p0 ? (int)(p1 - p0) : 0;
-        v16f acc[2][2] = {};
+        v16f acc[K::MT][K::NT] = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) colsum[e] = 0.f;
+        // DIRECT: the rows that `next` names, into LDS
+        auto stage = [&](char* to) {
+#pragma unroll
+            for (int i = 0; i < K::NC; ++i) {
+                // strides below 2^31 bytes: one multiply-add an address
+                const uint32_t a = (uint32_t)next[i], ra = (uint32_t)((uint64_t)a * g.div_mul >> g.div_shift);
+                const char* pa = (const char*)(dy + ca) + (uint64_t)a * ld_a;
+                const char* pb = (const char*)(x + cb) + (uint64_t)ra * ld_b;
+                char* at = to + (i * K::kThreads + wave * 64) * 16;
+                to_lds(next[i] >= 0 && ca < g.n ? pa : (const char*)&kZeroChunk, at);
+                to_lds(next[i] >= 0 && cb < g.k ? pb : (const char*)&kZeroChunk, at + kB);
+            }
+        };
+        auto products = [&](const char* from) {
+            if (DIRECT && sums) {                                // the thread's own chunks again, from LDS
+#pragma unroll
+                for (int i = 0; i < K::NC; ++i) {
+                    const v4u v = *reinterpret_cast<const v4u*>(from + (i * K::kThreads + tid) * 16);
+                    add_columns(v, v);
+                }
+            }
+            chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, K::MT, K::NT, K::BK / 16>(
+                from, from + kB, 32 * K::MT * wm, 32 * K::NT * wn, 0, lane, acc);
+        };
         find(0);
-        fetch();
-        if constexpr (!DIRECT) find(K::BK);
-        for (int p = 0; p < rows; p += K::BK) {
-            if constexpr (DIRECT) {
-#pragma unroll
-                for (int i = 0; i < K::NC; ++i) {
-                    // strides below 2^31 bytes: one multiply-add an address
-                    const uint32_t a = (uint32_t)next[i], ra = (uint32_t)((uint64_t)a * g.div_mul >> g.div_shift);
-                    const char* pa = (const char*)(dy + ca) + (uint64_t)a * ld_a;
-                    const char* pb = (const char*)(x + cb) + (uint64_t)ra * ld_b;
-                    to_lds(next[i] >= 0 && ca < g.n ? pa : (const char*)&kZeroChunk, lds_a + (i * K::kThreads + wave * 64) * 16);
-                    to_lds(next[i] >= 0 && cb < g.k ? pb : (const char*)&kZeroChunk, lds_b + (i * K::kThreads + wave * 64) * 16);
-                }
-                find(p + K::BK);
-            } else {
-                if (g.x_op) {
-#pragma unroll
-                    for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
-                }
-                if (sums) {
-#pragma unroll
-                    for (int i = 0; i < K::NC; ++i) {
-                        if constexpr (sizeof(T) == 4) add_columns(ha[i].a, ha[i].b);
-                        else add_columns(ha[i].a, ha[i].a);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < K::NC; ++i) {
-                    const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
-                    put(lds_a + at, K::TT::kBytes, ha[i]);
-                    put(lds_b + at, K::TT::kBytes, hb[i]);
-                }
-            }
-            __syncthreads();
-            if constexpr (DIRECT) {
-                if (sums) {                                          // the thread's own chunks again, from LDS
-#pragma unroll
-                    for (int i = 0; i < K::NC; ++i) {
-                        const v4u v = *reinterpret_cast<const v4u*>(lds_a + (i * K::kThreads + tid) * 16);
-                        add_columns(v, v);
-                    }
-                }
-            } else if (p + K::BK < rows) {
-                fetch();
+        if constexpr (kTwo) {
+            stage(lds);
+            find(K::BK);
+            int p = 0;
+            for (; p + K::BK < rows; p += 2 * K::BK) {
+                __syncthreads();
+                stage(lds_2);
                 find(p + 2 * K::BK);
+                products(lds);
+                __syncthreads();
+                if (p + 2 * K::BK < rows) {
+                    stage(lds);
+                    find(p + 3 * K::BK);
+                }
+                products(lds_2);
             }
-            chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, 2, 2, K::BK / 16>(lds_a, lds_b, 64 * wm, 64 * wn, 0, lane,
-                                                                                      acc);
             __syncthreads();
+            if (p < rows) products(lds);
+        } else {
+            fetch();
+            if constexpr (!DIRECT) find(K::BK);
+            for (int p = 0; p < rows; p += K::BK) {
+                if constexpr (DIRECT) {
+                    stage(lds);
+                    find(p + K::BK);
+                } else {
+                    if (g.x_op) {
+#pragma unroll
+                        for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+                    }
+                    if (sums) {
+#pragma unroll
+                        for (int i = 0; i < K::NC; ++i) {
+                            if constexpr (sizeof(T) == 4) add_columns(ha[i].a, ha[i].b);
+                            else add_columns(ha[i].a, ha[i].a);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < K::NC; ++i) {
+                        const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
+                        put(lds + at, K::TT::kBytes, ha[i]);
+                        put(lds + kB + at, K::TT::kBytes, hb[i]);
+                    }
+                }
+                __syncthreads();
+                if (!DIRECT && p + K::BK < rows) {
+                    fetch();
+                    find(p + 2 * K::BK);
+                }
+                products(lds);
+                __syncthreads();
+            }
         }
         float* part = g0 >= s0 && g1 <= s1 ? nullptr : g.part + (2 * (int64_t)unit + (p0 > s0)) * stride;
         T* dw = (T*)g.dw + (int64_t)group * g.n * g.k;
         // out through LDS as in the forward: 32 rows of 64 columns of a wave at a time
         constexpr int kLd = 68;
-        static_assert(K::kLds >= 2 * 32 * kLd * 4, "room for two waves' rows");
-        float* out = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * kLd;
+        static_assert(K::kLds >= K::WN * 32 * kLd * 4, "room for the rows of the waves of one turn");
+        float* out = reinterpret_cast<float*>(lds) + wn * 32 * kLd;
 #pragma unroll
-        for (int turn = 0; turn < 2; ++turn) {
+        for (int turn = 0; turn < K::WM; ++turn) {
             __syncthreads();
             if (wm != turn) continue;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            for (int m = 0; m < K::MT; ++m) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < K::NT; ++n)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         st4(out + (lane & 31) * kLd + 32 * n + 8 * q + 4 * (lane >> 5),
@@ -794,7 +843,7 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int at = (lane >> 3) + 8 * i, row = row0 + 64 * wm + 32 * m + at, c = 8 * (lane & 7);
+                    const int at = (lane >> 3) + 8 * i, row = row0 + 32 * (K::MT * wm + m) + at, c = 8 * (lane & 7);
                     const int col = col0 + 64 * wn + c, left = g.k - col;
                     const v4f lo = ld4(out + at * kLd + c), hi = ld4(out + at * kLd + c + 4);
                     float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -818,11 +867,11 @@ __global__ __launch_bounds__(256, (DIRECT ? 4 : 2)) void grouped_weight_kernel(G
             __syncthreads();
             float* red = reinterpret_cast<float*>(lds);          // 16 threads per chunk of eight columns
 #pragma unroll
-            for (int e = 0; e < 8; ++e) red[row_t * 128 + 8 * chunk + e] = colsum[e];
+            for (int e = 0; e < 8; ++e) red[row_t * TILE + 8 * chunk + e] = colsum[e];
             __syncthreads();
-            if (tid < 128 && row0 + tid < g.n) {
+            if (tid < TILE && row0 + tid < g.n) {
                 float s = 0.f;
-                for (int i = 0; i < K::kThreads / K::CT; ++i) s += red[i * 128 + tid];
+                for (int i = 0; i < K::kThreads / K::CT; ++i) s += red[i * TILE + tid];
                 if (part)
                     part[(int64_t)g.n * g.k + row0 + tid] = s;
                 else
@@ -941,32 +990,40 @@ int launch_rows(GroupedArgs g, hipStream_t st) {
     }
 }
 
-// Shares of the weight gradient's slots: a workgroup per share and tile fills the chip once (four workgroups per CU of
-// 16-bit rows, two of fp32 rows), of at least 256 slots each. Up to 512 slots one workgroup per group and tile.
-static inline int weight_shares(int64_t slots, int n, int k, int dtype) {
-    const int64_t tiles = (int64_t)((n + 127) / 128) * ((k + 127) / 128), most = (slots + 255) / 256;
-    const int64_t fill = (dtype == FACE_F32 ? 2 : 4) * (int64_t)device_cu_count() / tiles;
+// Whether the weight gradient of 16-bit rows takes 256 x 256 tiles: half the reads per product, but one workgroup per CU, whose
+// end nothing hides. Both ways (us, 128 / 256, joins included): 100,000 slots 2304 x 512 375 / 352, 200,000 slots 757 / 657,
+// 200,000 slots 2304 x 2304 3767 / 2634; 24,000 slots 2304 x 512 106 / 111, 200,000 slots 512 x 512 188 / 194, 3,000 slots
+// 2304 x 2304 93 / 102.
+static inline bool weight_large(int64_t slots, int n, int k) {
+    auto up = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
+    return n >= 512 && k >= 512 && (double)slots * n * k >= 1e11 &&
+           up(n, 256) * up(k, 256) * 8 <= up(n, 128) * up(k, 128) * 9;          // an eighth more area at most
+}
+// Shares of its slots: a workgroup per share and tile fills the chip once (four workgroups per CU of 16-bit rows, two of fp32
+// rows, one of 256 x 256), of at least 256 slots each. Up to 512 slots one workgroup per group and tile.
+static inline int weight_shares(int64_t slots, int n, int k, int dtype, bool large) {
+    const int tile = large ? 256 : 128;
+    const int64_t tiles = (int64_t)((n + tile - 1) / tile) * ((k + tile - 1) / tile), most = (slots + 255) / 256;
+    const int64_t fill = (large ? 1 : dtype == FACE_F32 ? 2 : 4) * (int64_t)device_cu_count() / tiles;
     const int64_t s = fill < most ? fill : most;
     return slots <= 512 || s < 1 ? 1 : (int)s;
 }
 
-template <typename T>
-int launch_weight(GroupedWArgs g, hipStream_t st) {
-    g.row_tiles = (g.n + 127) / 128;
-    g.col_tiles = (g.k + 127) / 128;
+template <typename T, bool DIRECT, int TILE>
+static int launch_weight_tile(GroupedWArgs g, hipStream_t st) {
+    g.shares = weight_shares(g.slots, g.n, g.k, sizeof(T) == 4 ? FACE_F32 : FACE_BF16, TILE == 256);
+    g.share = (g.slots + g.shares - 1) / g.shares;
+    g.row_tiles = (g.n + TILE - 1) / TILE;
+    g.col_tiles = (g.k + TILE - 1) / TILE;
     const int64_t grid = (int64_t)(g.shares > 1 ? g.shares : g.groups) * g.row_tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    bool direct = false;
-    if constexpr (sizeof(T) < 4)
-        direct = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n) &&
-                 g.ld_x < ((int64_t)1 << 30) && g.ld_dy < ((int64_t)1 << 30);
     // ceil(2^(31 + s) / xdiv) with 2^s >= xdiv is exact for every numerator below 2^31
     uint32_t s = 0;
     while (((int64_t)1 << s) < g.xdiv) ++s;
     g.div_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + g.xdiv - 1) / g.xdiv);
     g.div_shift = 31 + s;
-    auto* kernel = direct ? grouped_weight_kernel<T, (sizeof(T) < 4)> : grouped_weight_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((grouped_weight_kernel<T, DIRECT, TILE>), dim3((unsigned)grid),
+                       dim3(WeightKernel<T, TILE>::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     if (g.shares > 1) {
         const int64_t blocks = ((int64_t)g.n * g.k + 1023) / 1024;
@@ -975,6 +1032,17 @@ int launch_weight(GroupedWArgs g, hipStream_t st) {
         FACE_LAUNCH_CHECK();
     }
     return 0;
+}
+
+template <typename T>
+int launch_weight(GroupedWArgs g, hipStream_t st) {
+    if constexpr (sizeof(T) < 4) {
+        if (whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n) &&
+            g.ld_x < ((int64_t)1 << 30) && g.ld_dy < ((int64_t)1 << 30))
+            return weight_large(g.slots, g.n, g.k) ? launch_weight_tile<T, true, 256>(g, st)
+                                                   : launch_weight_tile<T, true, 128>(g, st);
+    }
+    return launch_weight_tile<T, false, 128>(g, st);
 }
 
 }  // namespace face

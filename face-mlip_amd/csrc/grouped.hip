@@ -62,7 +62,11 @@ static int64_t slot_rows_bytes(int64_t slots, int32_t k, int32_t dtype, int32_t 
     return x_div > 1 ? (slots * k * (dtype == FACE_F32 ? 4 : 2) + 255) / 256 * 256 : 0;
 }
 static int64_t part_bytes(int64_t slots, int32_t n, int32_t k, int32_t dtype, bool with_bias) {
-    const int shares = weight_shares(slots, n, k, dtype);
+    int shares = weight_shares(slots, n, k, dtype, false);
+    if (dtype != FACE_F32 && weight_large(slots, n, k)) {
+        const int large = weight_shares(slots, n, k, dtype, true);       // not known here: which of the two it will be
+        if (large > shares) shares = large;
+    }
     return shares > 1 ? 2 * shares * ((int64_t)n * k + (with_bias ? n : 0)) * 4 : 0;
 }
 }  // namespace face
@@ -97,9 +101,7 @@ extern "C" int face_grouped_linear_bwd(const void* x, int64_t ld_x, int32_t x_di
         if (rc) return rc;
     }
     if (dw) {
-        const int shares = weight_shares(slots, n, k, dtype);
-        GroupedWArgs g = {x, ld_x, x_div, x_op, 0, 0, dy, ld_dy, dw, db, (float*)part, n, k, ptr, order, slots, G, 0, 0,
-                          shares, (slots + shares - 1) / shares};
+        GroupedWArgs g = {x, ld_x, x_div, x_op, 0, 0, dy, ld_dy, dw, db, (float*)part, n, k, ptr, order, slots, G, 0, 0, 0, 0};
         return with_dtype(dtype, [&](auto t) { return launch_weight<decltype(t)>(g, st); });
     }
     return 0;

@@ -468,6 +468,26 @@ def test_grouped_linear_gradient_against_differences():
         assert abs((out[i].double() * v).sum() - want) <= 1e-5 * (out[i].double() * v).abs().sum()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_weight_gradient_of_many_slots(dtype):
+    """Tiles of 256 x 256: a hundred thousand slots in uneven groups, one of them empty, and slots of none."""
+    N, G, ki, n = 100300, 6, 1544, 656
+    g = gen(8)
+    e = torch.randint(-1, 4, (N,), generator=g, device=DEV, dtype=torch.int32)
+    e[:30000] = 5
+    plan = ex.group_plan(e, G)
+    x, w = rand(g, N, ki, dtype=dtype), rand(g, G, n, ki, dtype=dtype).requires_grad_(True)
+    b, dy = rand(g, G, n, dtype=dtype).requires_grad_(True), rand(g, N, n, dtype=dtype)
+    dw, db = torch.autograd.grad(ex.grouped_linear(x, w, plan, bias=b), [w, b], dy)
+    for i in range(G):
+        a = e == i
+        xa, da, m = x[a].double(), dy[a].double(), int(a.sum())
+        near(dw[i], da.t() @ xa, steps(dtype, m) * (da.abs().t() @ xa.abs()), f"dw {i}")
+        near(db[i], da.sum(0), m * U32 * da.abs().sum(0), f"db {i}")
+    again = torch.autograd.grad(ex.grouped_linear(x, w, plan, bias=b), [w, b], dy)
+    assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [50, 4000])
 def test_grouped_linear_strides(dtype, N):
