@@ -698,20 +698,24 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
     const uint32_t ld_a = (uint32_t)(g.ld_dy * sizeof(T)), ld_b = (uint32_t)(g.ld_x * sizeof(T));
     const int32_t* order;
     int rows;                                                    // of the present group in this share
-    auto find = [&](int p) {                                     // the slots of the rows from p on
+    // The slots of the thread's rows from p on: fetched without a branch or a test, either of which would wait for them
+    // (and for the operands on their way before them) at once; slot() tests one where it is used, -1: no row.
+    auto find = [&](int p) {
 #pragma unroll
         for (int i = 0; i < K::NC; ++i) {
-            const int at = p + i * (K::kThreads / K::CT);
-            const int32_t a = at + row_t < rows ? order[at] : -1;
-            next[i] = a < slots ? a : -1;
+            const int at = p + row_t + i * (K::kThreads / K::CT);
+            next[i] = order[at < rows ? at : 0];
         }
     };
+    auto slot = [&](int p, int i) {
+        return p + row_t + i * (K::kThreads / K::CT) < rows && next[i] < slots ? next[i] : -1;
+    };
     Held<T> ha[DIRECT ? 1 : K::NC], hb[DIRECT ? 1 : K::NC];
-    auto fetch = [&]() {
+    auto fetch = [&](int p) {
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int i = 0; i < K::NC; ++i) {
-                const int32_t a = next[i];
+                const int32_t a = slot(p, i);
                 ha[i] = hold(dy + (a >= 0 ? a * g.ld_dy + ca : 0), a >= 0 ? g.n - ca : 0);
                 const uint32_t ra = (uint32_t)((uint64_t)(uint32_t)a * g.div_mul >> g.div_shift);
                 hb[i] = hold(x + (a >= 0 ? (int64_t)ra * g.ld_x + cb : 0), a >= 0 ? g.k - cb : 0);
@@ -739,22 +743,23 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
             if (p0 >= s1) break;
             if (p0 >= p1) continue;                              // a group without slots: grouped_join_kernel
         }
-        order = g.order + p0 + row_t;
         rows = p1 > p0 ? (int)(p1 - p0) : 0;
+        order = rows ? g.order + p0 : g.ptr;                     // something to read where there is nothing
         v16f acc[K::MT][K::NT] = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) colsum[e] = 0.f;
-        // DIRECT: the rows that `next` names, into LDS
-        auto stage = [&](char* to) {
+        // DIRECT: the rows from p on, into LDS
+        auto stage = [&](int p, char* to) {
 #pragma unroll
             for (int i = 0; i < K::NC; ++i) {
                 // strides below 2^31 bytes: one multiply-add an address
-                const uint32_t a = (uint32_t)next[i], ra = (uint32_t)((uint64_t)a * g.div_mul >> g.div_shift);
+                const int32_t s = slot(p, i);
+                const uint32_t a = (uint32_t)s, ra = (uint32_t)((uint64_t)a * g.div_mul >> g.div_shift);
                 const char* pa = (const char*)(dy + ca) + (uint64_t)a * ld_a;
                 const char* pb = (const char*)(x + cb) + (uint64_t)ra * ld_b;
                 char* at = to + (i * K::kThreads + wave * 64) * 16;
-                to_lds(next[i] >= 0 && ca < g.n ? pa : (const char*)&kZeroChunk, at);
-                to_lds(next[i] >= 0 && cb < g.k ? pb : (const char*)&kZeroChunk, at + kB);
+                to_lds(s >= 0 && ca < g.n ? pa : (const char*)&kZeroChunk, at);
+                to_lds(s >= 0 && cb < g.k ? pb : (const char*)&kZeroChunk, at + kB);
             }
         };
         auto products = [&](const char* from) {
@@ -770,17 +775,17 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
         };
         find(0);
         if constexpr (kTwo) {
-            stage(lds);
+            stage(0, lds);
             find(K::BK);
             int p = 0;
             for (; p + K::BK < rows; p += 2 * K::BK) {
                 __syncthreads();
-                stage(lds_2);
+                stage(p + K::BK, lds_2);
                 find(p + 2 * K::BK);
                 products(lds);
                 __syncthreads();
                 if (p + 2 * K::BK < rows) {
-                    stage(lds);
+                    stage(p + 2 * K::BK, lds);
                     find(p + 3 * K::BK);
                 }
                 products(lds_2);
@@ -788,11 +793,11 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
             __syncthreads();
             if (p < rows) products(lds);
         } else {
-            fetch();
+            fetch(0);
             if constexpr (!DIRECT) find(K::BK);
             for (int p = 0; p < rows; p += K::BK) {
                 if constexpr (DIRECT) {
-                    stage(lds);
+                    stage(p, lds);
                     find(p + K::BK);
                 } else {
                     if (g.x_op) {
@@ -815,7 +820,7 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
                 }
                 __syncthreads();
                 if (!DIRECT && p + K::BK < rows) {
-                    fetch();
+                    fetch(p + K::BK);
                     find(p + 2 * K::BK);
                 }
                 products(lds);
