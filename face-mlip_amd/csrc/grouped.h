@@ -8,7 +8,7 @@
 // with a = order[i] the slot at place i of its group's range [ptr[g], ptr[g + 1]). Slots behind ptr[G] belong to
 // no group; their rows of y and d are written as zeros.
 //
-// A workgroup of four waves owns a tile of rows of ONE group and of output columns; which, it finds from ptr by a
+// A workgroup owns a tile of rows of ONE group and of output columns; which, it finds from ptr by a
 // wave-wide prefix sum of the groups' tile counts, so no launch waits for a count on the host. The grid holds the most
 // tiles that so many slots and groups can make; what is left over ends at once. Both operands go through
 // LDS in chunks along the sum, the next chunk's loads in registers during the present one's products:
@@ -18,9 +18,8 @@
 //   * an operand whose sum runs along its rows is read 16 bytes a lane; one whose sum runs down its columns (the
 //     weights of the input gradient, both operands of the weight gradient) is staged as it lies in memory and
 //     transposed by ds_read_b64_tr_b16 on the way to the matrix cores.
-// Where a launch has few tiles the four waves share one 32 x 32 tile and split every chunk's k among
-// them, joined in LDS at the end in a fixed order: such calls wait for memory, and eight times as many workgroups
-// have loads in flight.
+// Where a launch has few tiles eight waves share one 32 x 32 tile and split every chunk's k among them, joined in LDS
+// at the end in a fixed order: such calls wait for memory, and more workgroups have more loads in flight.
 #pragma once
 #include "elem.h"
 #include <type_traits>
@@ -110,19 +109,25 @@ struct Held<e4m3_wide> {
     uint64_t a;
 };
 
+// The chunk at p, all of it.
+template <typename T>
+__device__ __forceinline__ Held<T> hold(const T* p) {
+    Held<T> h;
+    if constexpr (__is_same(T, e4m3_wide)) {
+        typedef uint64_t any __attribute__((aligned(1)));
+        h.a = *reinterpret_cast<const any*>(p);
+    } else {
+        h.a = ld16(p);
+        if constexpr (sizeof(T) == 4) h.b = ld16(p + 4);
+    }
+    return h;
+}
 // The elements [0, left) of the chunk at p, zero beyond.
 template <typename T>
 __device__ __forceinline__ Held<T> hold(const T* p, int left) {
     Held<T> h = {};
-    constexpr int E = Operand<T>::kElems;
-    if (left >= E) {
-        if constexpr (__is_same(T, e4m3_wide)) {
-            typedef uint64_t any __attribute__((aligned(1)));
-            h.a = *reinterpret_cast<const any*>(p);
-        } else {
-            h.a = ld16(p);
-            if constexpr (sizeof(T) == 4) h.b = ld16(p + 4);
-        }
+    if (left >= Operand<T>::kElems) {
+        h = hold(p);
     } else if (left > 0) {
         if constexpr (__is_same(T, e4m3_wide)) {
 #pragma unroll
@@ -180,22 +185,30 @@ __device__ __forceinline__ void apply_silu(Held<T>& h) {
     }
 }
 
-// Writes the planes of a held chunk `plane` bytes apart.
+// The planes of a held chunk.
 template <typename T>
-__device__ __forceinline__ void put(char* at, int plane, const Held<T>& h) {
+__device__ __forceinline__ void planes(const Held<T>& h, v4u o[Operand<T>::kPlanes]) {
     if constexpr (sizeof(T) == 4) {
         const Split8 s = split8(__builtin_bit_cast(v4f, h.a), __builtin_bit_cast(v4f, h.b));
-        *reinterpret_cast<v8bf*>(at) = s.h;
-        *reinterpret_cast<v8bf*>(at + plane) = s.m;
-        *reinterpret_cast<v8bf*>(at + 2 * plane) = s.l;
+        o[0] = __builtin_bit_cast(v4u, s.h);
+        o[1] = __builtin_bit_cast(v4u, s.m);
+        o[2] = __builtin_bit_cast(v4u, s.l);
     } else if constexpr (__is_same(T, e4m3_wide)) {
         const int lo = (int)(uint32_t)h.a, hi = (int)(uint32_t)(h.a >> 32);
         const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
         const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-        *reinterpret_cast<v4u*>(at) = (v4u){bf16_pair(a[0], a[1]), bf16_pair(b[0], b[1]), bf16_pair(c[0], c[1]), bf16_pair(d[0], d[1])};
+        o[0] = (v4u){bf16_pair(a[0], a[1]), bf16_pair(b[0], b[1]), bf16_pair(c[0], c[1]), bf16_pair(d[0], d[1])};
     } else {
-        *reinterpret_cast<v4u*>(at) = h.a;
+        o[0] = h.a;
     }
+}
+// The same to LDS, `plane` bytes apart.
+template <typename T>
+__device__ __forceinline__ void put(char* at, int plane, const Held<T>& h) {
+    v4u o[Operand<T>::kPlanes];
+    planes(h, o);
+#pragma unroll
+    for (int p = 0; p < Operand<T>::kPlanes; ++p) *reinterpret_cast<v4u*>(at + p * plane) = o[p];
 }
 
 // ---------------------------------------------------------------- LDS tiles
@@ -404,7 +417,7 @@ struct RowsKernel {
     static constexpr int kLds = kLdsA + kLdsB > kWaves * kOut ? kLdsA + kLdsB : kWaves * kOut;
     static constexpr int NA = BM * C / kThreads, NB = RB * CB / kThreads;   // chunks per thread
     static_assert(NA * kThreads == BM * C && NB * kThreads == RB * CB, "whole rounds of chunks");
-    static_assert(WK == 1 || (WM == 1 && WN == 1 && MT == 1 && NT == 1 && WK == 4), "split chunks: one tile");
+    static_assert(WK == 1 || (WM == 1 && WN == 1 && MT == 1 && NT == 1), "split chunks: one tile");
 };
 
 // Out-of-range sums of limbs: a value past bf16's largest, or an infinity, has a NaN limb, so a sum that
@@ -454,7 +467,79 @@ __device__ __forceinline__ void finish(const GroupedArgs& g, int group, int32_t 
     store_piece((Out*)g.y + a * g.ld_y + col, left, v);
 }
 
-template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B>
+// A 32 x 32 tile of fp32 rows, where there are few: rows and weights go from memory to the matrix cores without LDS, and
+// without a wait in common. Lane i + 32 h holds 16 values of row i and of weight row i; each wave takes every WK-th 128-byte
+// stretch of all of them (32 whole lines an operand), the next one on its way while it multiplies the last. The order of
+// k within a stretch is the lanes', the same for both operands. 21 rows in three groups (us, staged / so): 864 -> 192 10.9
+// / 8.7, 1440 -> 320 15.8 / 11.7, 2304 -> 512 21.4 / 15.8; 100 rows 2048 -> 2048, 288 workgroups, 27.5 / 33.5: an access of 64
+// lanes touches 32 lines. 16-bit rows gain a tenth up to 1440 columns and lose as much from 2304 on: they are staged.
+template <int WK>
+__device__ __forceinline__ void few_rows(const float* x, const float* w, int k, int x_op, int wave, int lane, v16f acc[1][1]) {
+    constexpr int N = 2, E = 8, kLine = 2 * N * E;
+    using F = Fragments<float, 32, 1, false, 32, 1, false, 1, 1>;
+    const int half = N * E * (lane >> 5);
+    struct Run {
+        Held<float> a[N], b[N];
+    };
+    auto load = [&](Run& r, int turn) {
+        const int p = (turn * WK + wave) * kLine + half;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r.a[i] = hold(x + p + i * E);
+            r.b[i] = hold(w + p + i * E);
+        }
+    };
+    auto multiply = [&](Run& r) {
+        if (x_op) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) apply_silu(r.a[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v4u a[3], b[3];
+            planes(r.a[i], a);
+            planes(r.b[i], b);
+            F f;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                f.a[p][0] = a[p];
+                f.b[p][0] = b[p];
+            }
+            f.products(acc);
+        }
+    };
+    const int whole = k / kLine;                                 // stretches; this wave's: wave, wave + WK, ...
+    const int turns = whole > wave ? (whole - wave + WK - 1) / WK : 0;
+    // no branch between a load and its use: behind one the compiler waits for every load on its way
+    Run r0, r1;
+    int turn = 0;
+    if (turns) load(r0, 0);
+    for (; turn + 2 < turns; turn += 2) {
+        load(r1, turn + 1);
+        multiply(r0);
+        load(r0, turn + 2);
+        multiply(r1);
+    }
+    if (turn + 1 < turns) {
+        load(r1, turn + 1);
+        multiply(r0);
+        multiply(r1);
+    } else if (turn < turns) {
+        multiply(r0);
+    }
+    if (k % kLine && whole % WK == wave) {                       // the last stretch, in part
+        const int p = whole * kLine + half;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r0.a[i] = hold(x + p + i * E, k - p - i * E);
+            r0.b[i] = hold(w + p + i * E, k - p - i * E);
+        }
+        multiply(r0);
+    }
+}
+
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B,
+          bool FEW = false>
 __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThreads), (DIRECT_A ? 4 : 2)) void
     grouped_rows_kernel(GroupedArgs g) {
     using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
@@ -508,20 +593,38 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
         }
     }
     const int64_t w_step = (COLS_B ? g.ld_w : 1) * (int64_t)sizeof(T);           // one place of the sum
+    // the next chunk in registers; whole chunks are loaded without a branch per lane
     Held<T> ha[DIRECT_A ? 1 : K::NA], hb[DIRECT_B ? 1 : K::NB];
+    const bool cols_whole = !COLS_B || col0 + K::BN <= g.n;
     auto fetch = [&](int k0) {
-        if constexpr (!DIRECT_A) {
+        if (k0 >= g.k) return;
+        if (k0 + K::BK <= g.k && cols_whole) {
+            if constexpr (!DIRECT_A) {
 #pragma unroll
-            for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0, g.k - a_col - k0);
-        }
-        if constexpr (!DIRECT_B) {
+                for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0);
+            }
+            if constexpr (!DIRECT_B) {
 #pragma unroll
-            for (int i = 0; i < K::NB; ++i) {
-                const int row = tid / K::CB + i * (K::kThreads / K::CB);
-                if constexpr (COLS_B)
-                    hb[i] = hold(w + (k0 + row) * g.ld_w + b_col, k0 + row < g.k ? g.n - b_col : 0);
-                else
-                    hb[i] = hold(w + (col0 + row) * g.ld_w + b_col + k0, col0 + row < g.n ? g.k - b_col - k0 : 0);
+                for (int i = 0; i < K::NB; ++i) {
+                    const int row = tid / K::CB + i * (K::kThreads / K::CB);
+                    hb[i] = hold(COLS_B ? w + (k0 + row) * g.ld_w + b_col
+                                             : w + (col0 + row < g.n ? col0 + row : col0) * g.ld_w + b_col + k0);
+                }
+            }
+        } else {
+            if constexpr (!DIRECT_A) {
+#pragma unroll
+                for (int i = 0; i < K::NA; ++i) ha[i] = hold(ap[i] + k0, g.k - a_col - k0);
+            }
+            if constexpr (!DIRECT_B) {
+#pragma unroll
+                for (int i = 0; i < K::NB; ++i) {
+                    const int row = tid / K::CB + i * (K::kThreads / K::CB);
+                    if constexpr (COLS_B)
+                        hb[i] = hold(w + (k0 + row) * g.ld_w + b_col, k0 + row < g.k ? g.n - b_col : 0);
+                    else
+                        hb[i] = hold(w + (col0 + row) * g.ld_w + b_col + k0, col0 + row < g.n ? g.k - b_col - k0 : 0);
+                }
             }
         }
     };
@@ -559,26 +662,28 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
                 put(to + K::TB::at(tid / K::CB + i * (K::kThreads / K::CB), tid % K::CB), K::TB::kBytes, hb[i]);
         }
     };
-    auto stage = [&](int k0, char* to) {
-        if (k0 + K::BK <= g.k) {
-            stage_a(k0, to, std::true_type{});
-            stage_b(k0, to + K::kLdsA, std::true_type{});
-        } else {
-            stage_a(k0, to, std::false_type{});
-            stage_b(k0, to + K::kLdsA, std::false_type{});
+    if constexpr (FEW) {
+        static_assert(WK > 1 && !COLS_B, "rows of the sum on both sides");
+        const int32_t a = slot_of[lane & 31];
+        const int col = col0 + (lane & 31);
+        few_rows<WK>(x + (int64_t)(a < 0 ? 0 : a / g.xdiv) * g.ld_x, w + (col < g.n ? col : col0) * g.ld_w, g.k, g.x_op, wave, lane,
+                     acc);
+    } else {
+        fetch(0);
+        for (int k0 = 0; k0 < g.k; k0 += K::BK) {
+            if (k0 + K::BK <= g.k) {
+                stage_a(k0, lds, std::true_type{});
+                stage_b(k0, lds + K::kLdsA, std::true_type{});
+            } else {
+                stage_a(k0, lds, std::false_type{});
+                stage_b(k0, lds + K::kLdsA, std::false_type{});
+            }
+            __syncthreads();
+            fetch(k0 + K::BK);
+            chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
+                lds, lds + K::kLdsA, 32 * MT * wm, 32 * NT * wn, wk * (K::BK / WK), lane, acc);
+            __syncthreads();
         }
-    };
-    auto products = [&](const char* from) {
-        chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
-            from, from + K::kLdsA, 32 * MT * wm, 32 * NT * wn, wk * (K::BK / WK), lane, acc);
-    };
-    fetch(0);
-    for (int k0 = 0; k0 < g.k; k0 += K::BK) {
-        stage(k0, lds);
-        __syncthreads();
-        if (k0 + K::BK < g.k) fetch(k0 + K::BK);
-        products(lds);
-        __syncthreads();
     }
 
     // Out through LDS: whole rows of eight columns a lane, so that the stores (and the reads of z) are whole lines
@@ -628,7 +733,7 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 // A group that lies within one share is finished there; of the others each share leaves a partial result, two at most (of its
 // first and its last group), which grouped_join_kernel adds in order: no atomics. 200,000 slots, 512 x 2304, eight
 // groups, bf16: 673 us in 128 x 128 tiles, against 780 us with chunks of single groups (2.25 rounds of workgroups of
-// unlike length).
+// unlike length), and 578 us in 256 x 256 tiles: 816 TFLOP/s.
 // TILE 256 (16-bit operands staged without registers): 256 x 256 by eight waves of 128 x 64, into two buffers in turn, the next
 // slots on their way during the present ones' products.
 template <typename T, int TILE>
@@ -914,7 +1019,8 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedWArgs g) {
 
 // ---------------------------------------------------------------- launches
 // Instantiated per element type in a file of its own (grouped_f32.hip, ...).
-template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B>
+template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B,
+          bool FEW = false>
 static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
     using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
     const int64_t most = g.groups + (int64_t)1;
@@ -922,7 +1028,7 @@ static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
     g.col_tiles = (g.n + K::BN - 1) / K::BN;
     const int64_t grid = g.tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B>),
+    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B, FEW>),
                        dim3((unsigned)grid), dim3(K::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     return 0;
@@ -950,31 +1056,34 @@ static int launch_rows_large(GroupedArgs g, hipStream_t st) {
 
 // The tile: of a workgroup's chunks each waits `wait` ns for memory and barriers and takes `work` ns for each of the
 // workgroups that a CU has to do, so a launch takes about chunks (wait + work ceil(tiles / CUs)); the shape with the
-// least is launched. Fitted to 3 x 10 sizes of 21 to 12,000 slots and widths of 97 to 2304 (us; 32 x 32 split four ways, 64 x
-// 64, 128 x 64, 128 x 128):
-//   fp32, 2304 -> 512:    21 slots 24 / 57 / 82 / 120, 3,000 slots 89 / 74 / 89 / 126, 12,000 slots 303 / 199 / 200 / 174
-//   fp32, 1440 -> 320:    1,344 slots 24 / 38 / 54 / 80, 12,000 slots 126 / 84 / 76 / 114
-//   bf16, 2304 -> 512:    21 slots 9.9 / 18 / 21 / 30, 3,000 slots 30 / 27 / 32 / 41, 12,000 slots 88 / 46 / 50 / 48
-//   bf16, 2304 <- 512:    400 slots 11.9 / 8.6 / 9.6 / 12, 12,000 slots 140 / 54 / 48 / 42
-//   e4m3, 2304 -> 512:    21 slots 7.1 / 10 / 12 / 16, 3,000 slots 20 / 14 / 19 / 23, 12,000 slots 57 / 27 / 28 / 29
+// least is launched. Fitted to 200 sizes of 21 to 100,000 slots and widths of 97 to 2304, on which its choice is 2 % (fp32)
+// and 1 % slower than the best on average, 30 % at worst (us; 32 x 32 split eight ways / 64 x 64 / 128 x 64 / 128 x 128):
+//   fp32, 2304 -> 512:    21 slots 16 / 60 / 87 / 125, 3,000 slots 90 / 80 / 89 / 129, 12,000 slots 311 / 203 / 211 / 182
+//   fp32, 1440 -> 320:    1,344 slots 23 / 40 / 57 / 83, 12,000 slots 128 / 89 / 82 / 106
+//   bf16, 2304 -> 512:    21 slots 9.0 / 18 / 22 / 30, 3,000 slots 33 / 27 / 32 / 41, 12,000 slots 99 / 47 / 50 / 46
+//   bf16, 2304 <- 512:    400 slots 12.7 / 8.2 / 9.6 / 12, 12,000 slots 182 / 55 / 51 / 42
+//   e4m3, 2304 -> 512:    21 slots 6.5 / 10 / 13 / 16, 3,000 slots 25 / 15 / 18 / 23, 12,000 slots 79 / 28 / 28 / 28
 struct RowsShape {
     int rows, cols, bytes, wait, work;       // bytes: of a row's chunk in the 16-bit or 8-bit operand (of 32 bits: half)
 };
+// Tiles of rows x cols: a group ends in the middle of one on average.
+static inline int64_t expected_tiles(int64_t slots, int64_t groups, int n, int rows, int cols) {
+    groups = groups < slots ? groups : slots;
+    const int64_t t = slots / rows + groups / 2;
+    return (t > groups ? t : groups) * ((n + cols - 1) / cols);
+}
 template <typename T, bool COLS_B>
 static inline int rows_shape(int64_t slots, int64_t groups, int n, int k) {
-    constexpr RowsShape f32[4] = {{32, 32, 256, 650, COLS_B ? 900 : 680}, {64, 64, 64, 380, 400}, {128, 64, 64, 320, 810},
-                                  {128, 128, 64, 460, 1200}};
-    constexpr RowsShape low[4] = {{32, 32, 512, 720, COLS_B ? 550 : 380}, {64, 64, 128, 330, 160}, {128, 64, 128, 300, 350},
-                                  {128, 128, 128, 360, 460}};
+    constexpr RowsShape f32[4] = {{32, 32, 256, 560, COLS_B ? 810 : 730}, {64, 64, 64, 650, 440}, {128, 64, 64, 250, 730},
+                                  {128, 128, 64, 510, 1330}};
+    constexpr RowsShape low[4] = {{32, 32, 512, 640, COLS_B ? 610 : 550}, {64, 64, 128, 330, 250}, {128, 64, 128, 510, 330},
+                                  {128, 128, 128, 690, 500}};
     const int64_t cus = device_cu_count();
-    groups = groups < slots ? groups : slots;
     int best = 0;
     int64_t least = INT64_MAX;
     for (int i = 0; i < 4; ++i) {
         const RowsShape& s = sizeof(T) == 4 ? f32[i] : low[i];
-        // a group ends in the middle of a tile on average
-        int64_t tiles = slots / s.rows + groups / 2;
-        tiles = (tiles > groups ? tiles : groups) * ((n + s.cols - 1) / s.cols);
+        const int64_t tiles = expected_tiles(slots, groups, n, s.rows, s.cols);
         const int64_t chunk = s.bytes / (__is_same(T, e4m3) ? 1 : 2), chunks = (k + chunk - 1) / chunk;
         const int64_t ns = chunks * (s.wait + s.work * ((tiles + cus - 1) / cus));
         if (ns < least) {
@@ -988,7 +1097,11 @@ static inline int rows_shape(int64_t slots, int64_t groups, int n, int k) {
 template <typename T, typename Out, bool COLS_B>
 int launch_rows(GroupedArgs g, hipStream_t st) {
     switch (rows_shape<T, COLS_B>(g.slots, g.groups, g.n, g.k)) {
-        case 0: return launch_rows_shape<T, Out, COLS_B, 1, 1, 4, 1, 1, (sizeof(T) == 4 ? 16 : 32), false, false>(g, st);
+        case 0:
+            if constexpr (sizeof(T) == 4 && !COLS_B)
+                if (expected_tiles(g.slots, g.groups, g.n, 32, 32) <= device_cu_count())
+                    return launch_rows_shape<T, Out, COLS_B, 1, 1, 8, 1, 1, 16, false, false, true>(g, st);
+            return launch_rows_shape<T, Out, COLS_B, 1, 1, 8, 1, 1, (sizeof(T) == 4 ? 16 : 32), false, false>(g, st);
         case 1: return launch_rows_large<T, Out, COLS_B, 1, 1>(g, st);
         case 2: return launch_rows_large<T, Out, COLS_B, 2, 1>(g, st);
         default: return launch_rows_large<T, Out, COLS_B, 2, 2>(g, st);
@@ -996,12 +1109,12 @@ int launch_rows(GroupedArgs g, hipStream_t st) {
 }
 
 // Whether the weight gradient of 16-bit rows takes 256 x 256 tiles: half the reads per product, but one workgroup per CU, whose
-// end nothing hides. Both ways (us, 128 / 256, joins included): 100,000 slots 2304 x 512 375 / 352, 200,000 slots 757 / 657,
-// 200,000 slots 2304 x 2304 3767 / 2634; 24,000 slots 2304 x 512 106 / 111, 200,000 slots 512 x 512 188 / 194, 3,000 slots
-// 2304 x 2304 93 / 102.
+// end nothing hides. Both ways (us, 128 / 256, joins included): 200,000 slots 2304 x 512 730 / 584, 2304 x 2304 3627 / 2327,
+// 512 x 512 186 / 174, 100,000 slots 2304 x 512 361 / 311, 8,000 slots 2304 x 2304 164 / 160; 24,000 slots 2304 x 512 in 16
+// groups 147 / 153, 100,000 slots 512 x 512 109 / 111, 3,000 slots 2304 x 2304 93 / 96, 24,000 slots 512 x 512 52 / 62.
 static inline bool weight_large(int64_t slots, int n, int k) {
     auto up = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
-    return n >= 512 && k >= 512 && (double)slots * n * k >= 1e11 &&
+    return n >= 512 && k >= 512 && (double)slots * n * k >= 4e10 &&
            up(n, 256) * up(k, 256) * 8 <= up(n, 128) * up(k, 128) * 9;          // an eighth more area at most
 }
 // Shares of its slots: a workgroup per share and tile fills the chip once (four workgroups per CU of 16-bit rows, two of fp32
