@@ -21,6 +21,13 @@ __device__ __forceinline__ uint32_t route_key(float l) {
     const uint32_t k = (u >> 31) ? ~u : (u | 0x80000000u);
     return k > 0x007fffffu ? k : 0u;
 }
+__device__ __forceinline__ float route_value(uint32_t key) {
+    return __builtin_bit_cast(float, key == 0xffffffffu ? 0x7fc00000u : (key >> 31) ? key & 0x7fffffffu : ~key);
+}
+
+// e^x of a logit below the largest: one instruction and a product, whose rounding is |x| steps of 2^-24, as the
+// subtraction's is already. Below 2^-126 it may be 0.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 template <int LANES>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
@@ -47,14 +54,16 @@ __device__ __forceinline__ void route_row(const T* __restrict__ l, const uint8_t
                                           const int32_t* __restrict__ group, int n_groups, int64_t n, int E, int lane,
                                           float x[V]) {
     const float kNone = -__builtin_inff();
-    int g = 0;
-    if (allowed) g = group ? group[n] : 0;
-    const bool open = !allowed || (g >= 0 && g < n_groups);
+    // the logits are on their way before the row's mask is known
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = lane + LANES * v < E ? to_f(l[lane + LANES * v]) : kNone;
+    if (!allowed) return;
+    const int g = group ? group[n] : 0;
+    const bool open = g >= 0 && g < n_groups;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int e = lane + LANES * v;
-        x[v] = kNone;
-        if (e < E && open && (!allowed || allowed[(int64_t)g * E + e])) x[v] = to_f(l[e]);
+        if (e < E && !(open && allowed[(int64_t)g * E + e])) x[v] = kNone;
     }
 }
 
@@ -86,27 +95,23 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const T* __restrict__ lo
             at = key[v] == best && c > at ? c : at;
         }
         const int e = (int)~lanes_max<LANES>(at);
-        float l = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (lane + LANES * v == e) {
-                l = x[v];
-                key[v] = 0;
-            }
-        l = __shfl(l, e % LANES, LANES);
+            if (lane + LANES * v == e) key[v] = 0;
+        const float l = route_value(best);
         if (j == 0) {
             top = l;
             if (!renorm) {
                 float s = 0.f;
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (x[v] > -__builtin_inff() || x[v] != x[v]) s += expf(x[v] - top);
+                    if (x[v] > -__builtin_inff() || x[v] != x[v]) s += exp_of(x[v] - top);
                 sum = lanes_sum<LANES>(s);
             }
         }
         if (lane == j) {
             got = e;
-            mine = expf(l - top);
+            mine = exp_of(l - top);
         }
     }
     if (renorm) sum = lanes_sum<LANES>(mine);
@@ -127,9 +132,14 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
     const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (n >= N) return;
     float d[V];
-    float mean = 0.f;
-    if (lane < k && expert[n * k + lane] >= 0) mean = weight[n * k + lane] * dw[n * k + lane];
-    mean = lanes_sum<LANES>(mean);
+    int my_e = -1;                               // lane j: choice j
+    float my_w = 0.f, my_g = 0.f;
+    if (lane < k) {
+        my_e = expert[n * k + lane];
+        my_w = weight[n * k + lane];
+        my_g = dw[n * k + lane];
+    }
+    const float mean = lanes_sum<LANES>(my_e >= 0 ? my_w * my_g : 0.f);
     if (renorm) {
 #pragma unroll
         for (int v = 0; v < V; ++v) d[v] = 0.f;
@@ -143,26 +153,23 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
             best = key > best ? key : best;
         }
         best = lanes_max<LANES>(best);
-        const float top = __builtin_bit_cast(float, best == 0xffffffffu ? 0x7fc00000u
-                                                    : (best >> 31)      ? best & 0x7fffffffu
-                                                                        : ~best);
+        const float top = route_value(best);
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            d[v] = best && (d[v] > -__builtin_inff() || d[v] != d[v]) ? expf(d[v] - top) : 0.f;
+            d[v] = best && (d[v] > -__builtin_inff() || d[v] != d[v]) ? exp_of(d[v] - top) : 0.f;
             s += d[v];
         }
         s = lanes_sum<LANES>(s);
-        if (best) {
+        const float inv = best ? 1.f / s : 0.f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) d[v] = d[v] / s;         // p
-        }
+        for (int v = 0; v < V; ++v) d[v] *= inv;                 // p
     }
     float up[V] = {};                            // g of the chosen, 0 of the others
     for (int j = 0; j < k; ++j) {
-        const int e = expert[n * k + j];
+        const int e = __shfl(my_e, j, LANES);
         if (e < 0) break;
-        const float g = dw[n * k + j], w = weight[n * k + j];
+        const float g = __shfl(my_g, j, LANES), w = __shfl(my_w, j, LANES);
 #pragma unroll
         for (int v = 0; v < V; ++v)
             if (lane + LANES * v == e) {
@@ -184,11 +191,13 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
 // lanes that hold the same expert (one ballot per bit of its number), so equal experts keep their order.
 constexpr int kPlanMaxGroups = 1024;
 constexpr int kPlanThreads = 512, kPlanWaves = kPlanThreads / kWave;
-constexpr int64_t kPlanSegment = 4096;           // slots per workgroup up to 4 M slots, then 1024 workgroups
+constexpr int64_t kPlanOne = 4096;               // one workgroup does it all up to here
 
+// Slots per workgroup: 1024 up to 1 M slots, then 1024 workgroups. 400,000 slots, 64 experts (us, all three launches): segments
+// of 512 18.9, of 1024 15.7, of 2048 16.8, of 4096 22.1; 1,000 experts 39 / 31 / 30 / 35.
 static inline int64_t plan_segment(int64_t A) {
     const int64_t s = (A + 1023) / 1024;
-    return s > kPlanSegment ? (s + 511) / 512 * 512 : kPlanSegment;
+    return s > 1024 ? (s + 511) / 512 * 512 : 1024;
 }
 
 __device__ __forceinline__ int plan_group(const int32_t* expert, int64_t a, int64_t end, int G) {
@@ -472,7 +481,7 @@ extern "C" int face_route_bwd(const void* logits, int64_t ld, int64_t N, int32_t
 }
 
 extern "C" int64_t face_group_plan_work(int64_t slots, int32_t G) {
-    if (slots <= kPlanSegment || G <= 0 || G > kPlanMaxGroups) return 0;
+    if (slots <= kPlanOne || G <= 0 || G > kPlanMaxGroups) return 0;
     const int64_t seg = plan_segment(slots), segs = (slots + seg - 1) / seg;
     return 4 * (int64_t)(G + 1) * (segs + 1);
 }
@@ -486,7 +495,7 @@ extern "C" int face_group_plan(const int32_t* expert, int64_t slots, int32_t G, 
     while ((G + 1) >> bits) ++bits;
     const hipStream_t st = (hipStream_t)stream;
     const size_t lds = 4 * (size_t)(G + 1) * (kPlanWaves + 2);
-    if (slots <= kPlanSegment) {
+    if (slots <= kPlanOne) {
         hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kPlanThreads), lds, st, expert, slots, G, bits, ptr, order);
         FACE_LAUNCH_CHECK();
         return 0;
