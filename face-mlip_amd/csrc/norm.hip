@@ -9,6 +9,9 @@
 // backward are formed again from s, which it has to read anyway, so that nothing but s is kept. Bound by
 // bytes: a row is read once and each result written once. The sum is normalised as it was rounded: the
 // backward reads that value, and the next layer's residual starts from it.
+// A row lies in the registers of 16 lanes up to 256 columns, of a wave up to 4096, of four up to 16384, of 16 beyond.
+// 24,000 x 1440 fp32 with the residual: forward 100 us, backward 121 + 5 us (4.9 TB/s of what they must move, as a large copy);
+// 100,000 x 2304 bf16 to 8 bits 359 us (4.5 TB/s); 21 x 864 3.2 us, the launch.
 #include "elem.h"
 
 namespace face {

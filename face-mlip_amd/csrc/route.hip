@@ -6,8 +6,9 @@
 //   renormalised: dl_e = w_j (g_j - sum_i w_i g_i) of a chosen expert, 0 of others
 //   else:         dl_e = p_e ([e chosen] g_j - sum_i w_i g_i)
 // A group of 16 lanes holds a row in registers (64 lanes from 257 experts on) and finds each maximum with
-// cross-lane moves on the VALU: 64 experts and k = 4 are 16 such steps and no trip through LDS. Bound by the
-// row's latency where there are few, by its bytes else.
+// cross-lane moves on the VALU: 64 experts and k = 4 are 32 such steps and no trip through LDS. Bound by the
+// row's latency where there are few, by these steps else: 100,000 rows x 64 experts, k = 4, masked 15 us (28 MB: 6 us
+// of bytes), the gradient 19 us (55 MB: 11 us), without mask and renormalised 12 and 10 us.
 #include "elem.h"
 
 namespace face {
@@ -348,7 +349,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const int32_t*
 }
 
 // ---------------------------------------------------------------- join
-// out[i] = r[i] + sum_j w[i, j] y[i k + j], one read of each row; a row's pieces are spread over LANES threads.
+// out[i] = r[i] + sum_j w[i, j] y[i k + j], one read of each row; a row's pieces are spread over LANES threads. Bound by
+// bytes: 100,000 x 2 x 512 bf16 89 us forward (410 MB), 91 us backward (512 MB): 4.6 and 5.6 TB/s, part of it from the last
+// level of cache.
 // w null: factors of one.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void combine_fwd_kernel(const T* __restrict__ y, int64_t ld_y,
