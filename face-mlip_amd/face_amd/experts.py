@@ -16,7 +16,8 @@ Rows are float32, bfloat16 or float16 (all tensors of a call alike, gate weights
 softmax and norm statistics are float32. Every operator launches the kernels of
 libface_hip.so on torch's current stream of its tensors' device, allocates its results and workspaces with torch and never
 synchronises; none has a CPU path. They differentiate once, in training too: all of their floating
-inputs take gradients, except those of the 8-bit forms.
+inputs take gradients, except those of the 8-bit forms. Forward and backward are captured into a graph together,
+as with torch's own operators on leaves of which no eager graph is alive (fresh ones, by detach().requires_grad_()).
 """
 import torch
 
@@ -157,7 +158,8 @@ class RMSNorm(torch.autograd.Function):
 
 def rms_norm(x, w, eps=1e-6, residual=None):
     """x (..., F), w (F) -> x w / sqrt(mean(x^2) + eps) over the last axis. With residual (like x): (that of
-    s, s) for s = x + residual, rounded to the rows' type before it is normalised. F <= MAX_WIDTH."""
+    s, s) for s = x + residual, rounded to the rows' type before it is normalised. F <= MAX_WIDTH; the squares of a
+    row are summed in float32."""
     eps = float(eps)
     code = _norm_args("rms_norm", x, w, eps, residual)
     if _wants_grad(x, w, residual):

@@ -414,6 +414,32 @@ def test_grouped_linear(dtype, N, k, G, ki, n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 300, 20000])
+def test_grouped_linear_of_thousands_of_groups(dtype, N):
+    """A plan that a program made itself, of more groups than group_plan takes, most of them without rows."""
+    G, ki, n = 5000, 24, 17
+    g = gen(N)
+    e = torch.randint(0, G, (N,), generator=g, device=DEV)
+    x, w, b = rand(g, N, ki, dtype=dtype), rand(g, G, n, ki, dtype=dtype), rand(g, G, n, dtype=dtype)
+    dy = rand(g, N, n, dtype=dtype)
+    c = torch.bincount(e, minlength=G)
+    plan = ex.GroupPlan(torch.cat([c.new_zeros(1), c.cumsum(0)]).int(), torch.sort(e, stable=True).indices.int(), N)
+    ls = [t.requires_grad_(True) for t in (x, w, b)]
+    y = ex.grouped_linear(x, w, plan, bias=b)
+    dx, dw, db = torch.autograd.grad(y, ls, dy)
+    x64, w64, d64 = x.detach().double(), w.detach().double()[e], dy.double()
+    t = w64 * x64[:, None]
+    bias = b.detach().double()[e]
+    near(y, t.sum(2) + bias, steps(dtype, ki) * (t.abs().sum(2) + bias.abs()), "y")
+    t = w64 * d64[:, :, None]
+    near(dx, t.sum(1), steps(dtype, n) * t.abs().sum(1), "dx")
+    t = d64[:, :, None] * x64[:, None]
+    z = torch.zeros(G, n, ki, dtype=torch.float64, device=DEV)
+    near(dw, z.index_add(0, e, t), steps(dtype, N) * z.index_add(0, e, t.abs()), "dw")
+    near(db, z[:, :, 0].index_add(0, e, d64), N * U32 * z[:, :, 0].index_add(0, e, d64.abs()), "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_linear_uneven_groups(dtype):
     """Groups without rows, one with all, slots of no group, a group of one row."""
     g = gen(1)
@@ -826,3 +852,56 @@ def test_a_recorded_backward_is_refused():
         leaf = x if out.grad_fn.next_functions[0][0] is not None else w
         with pytest.raises(NotImplementedError, match="differentiate once"):
             torch.autograd.grad(out.sum(), leaf, create_graph=True)
+
+
+def test_one_tensor_twice_and_backward_twice():
+    """The same leaf as two operands, the same weights in two products, and a backward run again on a kept graph."""
+    g = gen(5)
+    x, w = rand(g, 70, 40).requires_grad_(True), rand(g, 40).requires_grad_(True)
+    dy, ds = rand(g, 70, 40), rand(g, 70, 40)
+    both = torch.autograd.grad(ex.rms_norm(x, w, 1e-5, residual=x), [x, w], [dy, ds])
+    r = x.detach().clone().requires_grad_(True)
+    apart = torch.autograd.grad(ex.rms_norm(x, w, 1e-5, residual=r), [x, r, w], [dy, ds])
+    assert torch.equal(both[0], apart[0] + apart[1]) and torch.equal(both[1], apart[2])
+    x.grad = r.grad = None
+    torch.autograd.backward(ex.rms_norm(x, w, 1e-5, residual=r), [dy, ds])
+    assert x.grad.data_ptr() != r.grad.data_ptr() and torch.equal(x.grad, apart[0]) and torch.equal(r.grad, apart[1])
+
+    plan = ex.group_plan(torch.randint(0, 3, (70, 1), generator=g, device=DEV, dtype=torch.int32), 3)
+    m = rand(g, 3, 40, 40, scale=0.2).requires_grad_(True)
+    u = ex.grouped_linear(x, m, plan)
+    v = ex.grouped_linear(u, m, plan, x_op="silu")
+    once = torch.autograd.grad(v, [x, m, u], dy, retain_graph=True)
+    again = torch.autograd.grad(v, [x, m, u], dy)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    d1, = torch.autograd.grad(ex.grouped_linear(x, m, plan), m, once[2])
+    d2, = torch.autograd.grad(ex.grouped_linear(u.detach(), m, plan, x_op="silu"), m, dy)
+    assert torch.equal(once[1], d1 + d2) or torch.equal(once[1], d2 + d1)
+    with torch.autograd.set_multithreading_enabled(False):
+        u = ex.grouped_linear(x, m, plan)
+        one = torch.autograd.grad(ex.grouped_linear(u, m, plan, x_op="silu"), [x, m, u], dy)
+    assert all(torch.equal(a, b) for a, b in zip(once, one))
+
+    weight = torch.softmax(rand(g, 35, 2), 1).requires_grad_(True)
+    y = rand(g, 70, 40).requires_grad_(True)
+    d = rand(g, 35, 40)
+    gy, = torch.autograd.grad(ex.expert_combine(y, weight, residual=y[:35]), y, d)
+    a, b = torch.autograd.grad(ex.expert_combine(y, weight, residual=r[:35]), [y, r], d)
+    assert torch.equal(gy, a + b)
+
+
+def test_an_operand_changed_before_its_backward_is_noticed():
+    """What the backward reads is what the forward read: torch's version check covers operands, results and plans."""
+    g = gen(6)
+    x, m = rand(g, 12, 8).requires_grad_(True), rand(g, 2, 8, 8).requires_grad_(True)
+    plan = ex.group_plan(torch.arange(12, device=DEV) % 2, 2)
+    r = rand(g, 12, 8)
+    y, s = ex.rms_norm(x, torch.ones(8, device=DEV), residual=r)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    y = ex.grouped_linear(x, m, plan)
+    plan.order.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), m)
