@@ -355,6 +355,18 @@ __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, i
     }
 }
 
+// Waves at their products go before waves of the CU's other workgroups that split operands into limbs, so that the
+// matrix cores are fed first. fp32 24,000 x 1440 -> 320 (us, without / with): 148 / 143, input gradient 165 / 161, weights 183 /
+// 180; 2304 -> 512 372 / 357, 346 / 333, 344 / 344. Of 16 and 8 bits nothing is split, and it costs 1 %: 271 / 280, 70.8 / 71.7.
+template <typename T>
+__device__ __forceinline__ void before_products() {
+    if constexpr (Operand<T>::kPlanes > 1) __builtin_amdgcn_s_setprio(1);
+}
+template <typename T>
+__device__ __forceinline__ void after_products() {
+    if constexpr (Operand<T>::kPlanes > 1) __builtin_amdgcn_s_setprio(0);
+}
+
 // ---------------------------------------------------------------- staging without registers
 // Operands whose 16-byte chunks are aligned and whole (launch_rows, launch_weight) go from memory to LDS directly:
 // lane l of a wave fills the 16 bytes at 16 l of a stretch of 1 KB, so the chunk that belongs there by the tile's XOR is
@@ -687,8 +699,10 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
             }
             __syncthreads();
             fetch(k0 + K::BK);
+            before_products<T>();
             chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
                 lds, lds + K::kLdsA, 32 * MT * wm, 32 * NT * wn, wk * (K::BK / WK), lane, acc);
+            after_products<T>();
             __syncthreads();
         }
     }
@@ -935,7 +949,9 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
                     fetch(p + K::BK);
                     find(p + 2 * K::BK);
                 }
+                before_products<T>();
                 products(lds);
+                after_products<T>();
                 __syncthreads();
             }
         }
