@@ -79,6 +79,11 @@ def _once():
         raise NotImplementedError("the expert layer's operators differentiate once (create_graph=False)")
 
 
+def _like(t):
+    """A dense tensor of t's shape and type (half the host time of torch.empty(t.shape, ...))."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _work(n_bytes, device):
     return torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
 
@@ -110,8 +115,8 @@ def _norm_fwd(code, x, w, eps, r, q8):
     x2, w = _rows(x, F), w.contiguous()
     r2 = None if r is None else _rows(r, F)
     N = x2.shape[0]
-    s = None if r is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = None if q8 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = None if r is None else _like(x)
+    y = None if q8 else _like(x)
     q = torch.empty(x.shape, dtype=_E4M3, device=x.device) if q8 else None
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if q8 else None
     _launch(x, "face_rms_norm_fwd", "rms_norm_fwd", x2.data_ptr(), x2.stride(0), ptr(r2), F if r2 is None else r2.stride(0),
@@ -144,7 +149,7 @@ class RMSNorm(torch.autograd.Function):
             dy = _rows(dy, F)
         if ds is not None:
             ds = _rows(ds, F)
-        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device) if need_x or need_r else None
+        dx = _like(s) if need_x or need_r else None
         dw = work = None
         need = 0
         if need_w:
@@ -386,7 +391,7 @@ class GroupedLinear(torch.autograd.Function):
         slots = order.shape[0]
         div = _div(ctx.plan, x.shape[0])
         x2, dy, w2 = _rows(x, k), _rows(dy, n), _weights(w)
-        dx = torch.empty(x.shape, dtype=dtype, device=dev) if need_x else None
+        dx = _like(x) if need_x else None
         dw = torch.empty(G, n, k, dtype=dtype, device=dev) if need_w or need_b else None
         db = torch.empty(G, n, dtype=dtype, device=dev) if need_b else None
         need = _lib.lib().face_grouped_linear_bwd_work(slots, n, k, code, div, need_x, need_w or need_b, need_b)
