@@ -1078,9 +1078,10 @@ static int launch_rows_large(GroupedArgs g, hipStream_t st) {
 }
 
 // The tile: of a workgroup's chunks each waits `wait` ns for memory and barriers and takes `work` ns for each of the
-// workgroups that a CU has to do, so a launch takes about chunks (wait + work ceil(tiles / CUs)); the shape with the
-// least is launched. Fitted to 200 sizes of 21 to 100,000 slots and widths of 97 to 2304, on which its choice is 2 % (fp32)
-// and 1 % slower than the best on average, 30 % at worst (us; 32 x 32 split eight ways / 64 x 64 / 128 x 64 / 128 x 128):
+// workgroups that a CU has to do, so a launch takes about chunks (wait + work max(1, tiles / CUs)); the shape with the
+// least is launched. Fitted to 400 sizes of 21 to 100,000 slots and widths of 97 to 2304, on which its choice is 0.7 % slower
+// than the best on average (whole rounds of workgroups in place of the quotient: 2 % for fp32, 0.8 % for the others), 17 %
+// at worst (us; 32 x 32 split eight ways / 64 x 64 / 128 x 64 / 128 x 128):
 //   fp32, 2304 -> 512:    21 slots 16 / 60 / 87 / 125, 3,000 slots 90 / 80 / 89 / 129, 12,000 slots 311 / 203 / 211 / 182
 //   fp32, 1440 -> 320:    1,344 slots 23 / 40 / 57 / 83, 12,000 slots 128 / 89 / 82 / 106
 //   bf16, 2304 -> 512:    21 slots 9.0 / 18 / 22 / 30, 3,000 slots 33 / 27 / 32 / 41, 12,000 slots 99 / 47 / 50 / 46
@@ -1097,19 +1098,18 @@ static inline int64_t expected_tiles(int64_t slots, int64_t groups, int n, int r
 }
 template <typename T, bool COLS_B>
 static inline int rows_shape(int64_t slots, int64_t groups, int n, int k) {
-    constexpr RowsShape f32[4] = {{32, 32, 256, 560, COLS_B ? 810 : 730}, {64, 64, 64, 650, 440}, {128, 64, 64, 250, 730},
-                                  {128, 128, 64, 510, 1330}};
-    constexpr RowsShape low[4] = {{32, 32, 512, 640, COLS_B ? 610 : 550}, {64, 64, 128, 330, 250}, {128, 64, 128, 510, 330},
-                                  {128, 128, 128, 690, 500}};
-    const int64_t cus = device_cu_count();
+    constexpr RowsShape f32[4] = {{32, 32, 256, 320, 570}, {64, 64, 64, 350, 310}, {128, 64, 64, 400, 580}, {128, 128, 64, 440, 1130}};
+    constexpr RowsShape low[4] = {{32, 32, 512, 680, COLS_B ? 550 : 280}, {64, 64, 128, 170, 190}, {128, 64, 128, 720, 190},
+                                  {128, 128, 128, 780, 290}};
+    const double cus = (double)device_cu_count();
     int best = 0;
-    int64_t least = INT64_MAX;
+    double least = 0;
     for (int i = 0; i < 4; ++i) {
         const RowsShape& s = sizeof(T) == 4 ? f32[i] : low[i];
-        const int64_t tiles = expected_tiles(slots, groups, n, s.rows, s.cols);
+        const double load = (double)expected_tiles(slots, groups, n, s.rows, s.cols) / cus;
         const int64_t chunk = s.bytes / (__is_same(T, e4m3) ? 1 : 2), chunks = (k + chunk - 1) / chunk;
-        const int64_t ns = chunks * (s.wait + s.work * ((tiles + cus - 1) / cus));
-        if (ns < least) {
+        const double ns = (double)chunks * (s.wait + s.work * (load > 1 ? load : 1));
+        if (i == 0 || ns < least) {
             least = ns;
             best = i;
         }
