@@ -25,8 +25,8 @@
 // waits (a second buffer per workgroup leaves room for fewer: 128 x 128 of bf16 543 -> 562 us, of e4m3 268 -> 342 us).
 // 200,000 slots of 100,000 x 2304 -> 512, eight groups: bf16 530 us (890 TFLOP/s; the library's product of one matrix 500),
 // e4m3 278 us (1.7 PFLOP/s), bf16 input gradient 625 us (750 TFLOP/s, 0.92 GB written), then 254 us for the sum of a row's
-// slots. 24,000 x 1440 -> 320 in fp32, three groups: 145 us (152 TFLOP/s of the 190 that six bf16 products allow), input
-// gradient 150-170 us. 21 rows x 192 -> 97 in fp32 6.6 us; two rows x 2048 -> 2048 in bf16 8.7 us, 16.8 MB of weights.
+// slots. 24,000 x 1440 -> 320 in fp32, three groups: 143 us (155 TFLOP/s of the 190 that six bf16 products allow), input
+// gradient 156 us. 21 rows x 192 -> 97 in fp32 6.6 us; two rows x 2048 -> 2048 in bf16 8.7 us, 16.8 MB of weights.
 #pragma once
 #include "elem.h"
 #include <type_traits>
