@@ -749,8 +749,8 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 }
 
 // ---------------------------------------------------------------- weight gradient
-// 128 x 128 tiles (n, k), the sum down the places of order. The places are cut into equal shares, as many as fill the chip
-// once with a workgroup per share and tile, wherever the groups end: a workgroup goes through the groups of its share.
+// 128 x 128 tiles (n, k), the sum down the places of order. The places are cut into equal shares (weight_shares),
+// wherever the groups end: a workgroup per share and tile goes through the groups of its share.
 // A group that lies within one share is finished there; of the others each share leaves a partial result, two at most (of its
 // first and its last group), which grouped_join_kernel adds in order: no atomics. 200,000 slots, 512 x 2304, eight
 // groups, bf16: 673 us in 128 x 128 tiles, against 780 us with chunks of single groups (2.25 rounds of workgroups of
@@ -1140,19 +1140,30 @@ static inline bool weight_large(int64_t slots, int n, int k) {
     return n >= 512 && k >= 512 && (double)slots * n * k >= 4e10 &&
            up(n, 256) * up(k, 256) * 8 <= up(n, 128) * up(k, 128) * 9;          // an eighth more area at most
 }
-// Shares of its slots: a workgroup per share and tile fills the chip once (four workgroups per CU of 16-bit rows, two of fp32
-// rows, one of 256 x 256), of at least 256 slots each. Up to 512 slots one workgroup per group and tile.
-static inline int weight_shares(int64_t slots, int n, int k, int dtype, bool large) {
+// Shares of its slots. A workgroup takes about `slot` us a slot, and a share costs 0.08 us and the bytes of a partial result
+// written and read at 4 TB/s, so that s shares take slots slot / s + s (0.08 + 2e-6 n k): the s with the least, and no more
+// than fill the chip once (three workgroups per CU of 16-bit rows, two of fp32 rows, one of 256 x 256). One workgroup per
+// group and tile instead, without partial results, where the largest group (taken as half the slots, or all of one) is done
+// no later than the shares and the 9 us of their join, and up to 512 slots, which need no workspace then. Measured (us,
+// shares of 256 slots or more that fill the chip / this rule):
+//   bf16: 1,600 slots in 16 groups 512 x 512 35 / 10, 800 in one 2304 x 512 28 / 20, 8,000 in three 97 x 192 28 / 26,
+//         24,000 in three 512 x 512 56 / 50, 100,000 in eight 1440 x 320 200 / 208, 97 x 96 46 / 50
+//   fp32: 800 in three 2304 x 512 53 / 30, in one 192 x 97 30 / 24, 8,000 in 32 864 x 192 65 / 58, 100,000 in eight 192 x 97
+//         67 / 71; the same within 1 % from 24,000 slots of 1440 x 320 on
+static inline int weight_shares(int64_t slots, int groups, int n, int k, int dtype, bool large, bool direct) {
     const int tile = large ? 256 : 128;
-    const int64_t tiles = (int64_t)((n + tile - 1) / tile) * ((k + tile - 1) / tile), most = (slots + 255) / 256;
-    const int64_t fill = (large ? 1 : dtype == FACE_F32 ? 2 : 4) * (int64_t)device_cu_count() / tiles;
-    const int64_t s = fill < most ? fill : most;
-    return slots <= 512 || s < 1 ? 1 : (int)s;
+    const double tiles = (double)((n + tile - 1) / tile) * ((k + tile - 1) / tile);
+    const double fill = (large ? 1 : dtype == FACE_F32 ? 2 : 3) * device_cu_count() / tiles;
+    const double slot = dtype == FACE_F32 ? 0.06 : (direct ? 0.0175 : 0.035);
+    const double all = (double)slots * slot, join = 0.08 + 2e-6 * n * k;
+    double s = __builtin_sqrt(all / join);
+    s = __builtin_floor(s < fill ? s : fill);
+    return slots <= 512 || s < 2 || (groups > 1 ? all / 2 : all) <= all / s + s * join + 9 ? 1 : (int)s;
 }
 
 template <typename T, bool DIRECT, int TILE>
 static int launch_weight_tile(GroupedWArgs g, hipStream_t st) {
-    g.shares = weight_shares(g.slots, g.n, g.k, sizeof(T) == 4 ? FACE_F32 : FACE_BF16, TILE == 256);
+    g.shares = weight_shares(g.slots, g.groups, g.n, g.k, sizeof(T) == 4 ? FACE_F32 : FACE_BF16, TILE == 256, DIRECT);
     g.share = (g.slots + g.shares - 1) / g.shares;
     g.row_tiles = (g.n + TILE - 1) / TILE;
     g.col_tiles = (g.k + TILE - 1) / TILE;

@@ -62,10 +62,15 @@ static int64_t slot_rows_bytes(int64_t slots, int32_t k, int32_t dtype, int32_t 
     return x_div > 1 ? (slots * k * (dtype == FACE_F32 ? 4 : 2) + 255) / 256 * 256 : 0;
 }
 static int64_t part_bytes(int64_t slots, int32_t n, int32_t k, int32_t dtype, bool with_bias) {
-    int shares = weight_shares(slots, n, k, dtype, false);
-    if (dtype != FACE_F32 && weight_large(slots, n, k)) {
-        const int large = weight_shares(slots, n, k, dtype, true);       // not known here: which of the two it will be
-        if (large > shares) shares = large;
+    // the most shares of the ways the call may go; one group has them wherever several have
+    int shares = weight_shares(slots, 1, n, k, dtype, false, false);
+    if (dtype != FACE_F32) {
+        auto more = [&](bool large) {
+            const int s = weight_shares(slots, 1, n, k, dtype, large, true);
+            if (s > shares) shares = s;
+        };
+        more(false);
+        if (weight_large(slots, n, k)) more(true);
     }
     return shares > 1 ? 2 * shares * ((int64_t)n * k + (with_bias ? n : 0)) * 4 : 0;
 }
