@@ -4,7 +4,8 @@
 // -inf); the k largest logits in descending order, ties to the lower expert; weight p, or p over the sum
 // of the k. What a row cannot fill has expert -1 and weight 0.
 //   renormalised: dl_e = w_j (g_j - sum_i w_i g_i) of a chosen expert, 0 of others
-//   else:         dl_e = p_e ([e chosen] g_j - sum_i w_i g_i)
+//   else:         dl_e = p_e ([e chosen] g_j - sum_i w_i g_i) of an open expert, 0 of others
+// The zeros are written as such: a product would make NaN of them in a row whose sum is not finite.
 // A group of 16 lanes holds a row in registers (64 lanes from 257 experts on) and finds each maximum with
 // cross-lane moves on the VALU: 64 experts and k = 4 are 32 such steps and no trip through LDS. Bound by the
 // row's latency where there are few, by these steps else: 100,000 rows x 64 experts, k = 4, masked 15 us (28 MB: 6 us
@@ -133,6 +134,7 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
     const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (n >= N) return;
     float d[V];
+    uint32_t reached = 0;                        // bit v: the loss depends on the lane's expert v
     int my_e = -1;                               // lane j: choice j
     float my_w = 0.f, my_g = 0.f;
     if (lane < k) {
@@ -158,7 +160,9 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            d[v] = best && (d[v] > -__builtin_inff() || d[v] != d[v]) ? exp_of(d[v] - top) : 0.f;
+            const bool open = d[v] > -__builtin_inff() || d[v] != d[v];
+            reached |= (uint32_t)open << v;
+            d[v] = open ? exp_of(d[v] - top) : 0.f;
             s += d[v];
         }
         s = lanes_sum<LANES>(s);
@@ -175,13 +179,16 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const T* __restrict__ lo
         for (int v = 0; v < V; ++v)
             if (lane + LANES * v == e) {
                 up[v] = g;
-                if (renorm) d[v] = w;
+                if (renorm) {
+                    d[v] = w;
+                    reached |= 1u << v;
+                }
             }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int e = lane + LANES * v;
-        if (e < E) dl[n * E + e] = from_f<T>(d[v] * (up[v] - mean));
+        if (e < E) dl[n * E + e] = from_f<T>((reached >> v) & 1 ? d[v] * (up[v] - mean) : 0.f);
     }
 }
 

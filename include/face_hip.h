@@ -577,7 +577,8 @@ int face_quantize_rows(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_
 int face_route_fwd(const void* logits, int64_t ld, int64_t N, int32_t E, int32_t k, int32_t dtype,
                    const uint8_t* allowed, const int32_t* group, int32_t n_groups, int32_t renorm, int32_t* expert,
                    float* weight, void* stream);
-/* dlogits (N, E) dense, for dweight (N, k); expert and weight as the forward wrote them. */
+/* dlogits (N, E) dense, for dweight (N, k); expert and weight as the forward wrote them. Exactly 0 for the experts that
+ * the weights do not depend on, whatever the row's other values are. */
 int face_route_bwd(const void* logits, int64_t ld, int64_t N, int32_t E, int32_t k, int32_t dtype,
                    const uint8_t* allowed, const int32_t* group, int32_t n_groups, int32_t renorm, const int32_t* expert,
                    const float* weight, const float* dweight, void* dlogits, void* stream);

@@ -283,6 +283,40 @@ def test_route_gradient_against_differences():
         assert abs((d.double() * v).sum() - want) <= 1e-5 * (d.double() * v).abs().sum()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E", [6, 64, 300])
+def test_route_gradient_of_rows_that_are_not_finite(dtype, E):
+    """A NaN or an infinity among a row's logits or upstream gradients reaches the experts that its weights depend on, and
+    no other: closed ones, and (renormalised) those not chosen, have a gradient of exactly 0."""
+    g = gen(E)
+    k = 2
+    l, dw = rand(g, 40, E, dtype=dtype), rand(g, 40, k)
+    allowed = torch.rand(1, E, generator=g, device=DEV) < 0.5
+    allowed[0, :2], allowed[0, 2] = True, False
+    l[0, 1], l[1, 0], l[2, 3:], l[3, 2] = math.nan, math.inf, -math.inf, math.nan
+    dw[4, 0], dw[5, 1], dw[6] = math.inf, math.nan, -math.inf
+    odd = torch.arange(40, device=DEV) < 7
+    for a in (None, allowed):
+        open_ = (l > -math.inf) | l.isnan()
+        if a is not None:
+            open_ &= a
+        for renorm in (True, False):
+            say("gradient of odd rows", dtype, E, a is not None, renorm)
+            x = l.clone().requires_grad_(True)
+            e, w = ex.route(x, k, allowed=a, renormalise=renorm)
+            d, = torch.autograd.grad(w, x, dw)
+            got = torch.zeros_like(open_).scatter_(1, e.clamp_min(0).long(), e >= 0)
+            reached = got if renorm else open_
+            assert bool((d[~reached] == 0).all())
+            assert bool(torch.isfinite(d[~odd]).all())
+            # the mean of the upstream gradients over the weights is not finite in these rows, and no reached one escapes it
+            hit = [0, 1, 4, 5, 6] + ([3] if a is None else [])
+            for i in hit:
+                assert not torch.isfinite(d[i][reached[i]]).any(), i
+            ok = torch.autograd.grad(ex.route(x, k, allowed=a, renormalise=renorm)[1][7:], x, dw[7:])[0]
+            assert torch.equal(ok[7:], d[7:])
+
+
 # ----------------------------------------------------------------------------- grouping
 @pytest.mark.parametrize("slots", [0, 1, 63, 64, 513, 4096, 4097, 70001, 5000000])
 @pytest.mark.parametrize("G", [1, 3, 64, 1024])
