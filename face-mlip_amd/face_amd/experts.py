@@ -16,10 +16,11 @@ Rows are float32, bfloat16 or float16 (all tensors of a call alike, gate weights
 softmax and norm statistics are float32. Every operator launches the kernels of
 libface_hip.so on torch's current stream of its tensors' device, allocates its results and workspaces with torch and never
 synchronises; none has a CPU path. They differentiate once, in training too: all of their floating
-inputs take gradients, except those of the 8-bit forms. Forward and backward are captured into a graph together,
+inputs take gradients, except those of the 8-bit forms. Forward-mode derivatives are refused. Forward and backward are captured into a graph together,
 as with torch's own operators on leaves of which no eager graph is alive (fresh ones, by detach().requires_grad_()).
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, ptr
@@ -42,8 +43,17 @@ def _dtype(name, t):
     return code
 
 
+def _no_tangents(name, *ts):
+    """The kernels see a tensor's values alone: the tangent of a dual tensor would be dropped in silence."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:            # else no tensor has one
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: no forward-mode derivatives")
+
+
 def _check(name, ref, **tensors):
-    """Every tensor on ref's HIP device."""
+    """Every tensor on ref's HIP device, and none with a tangent."""
+    _no_tangents(name, ref, *tensors.values())
     _lib.require_gpu(ref, *tensors.values())
     for k, t in tensors.items():
         if t is not None and t.device != ref.device:
@@ -73,8 +83,9 @@ def _launch(t, name, label, *args):
             call(name, *args, _lib.stream_of(t), label=label)
 
 
-def _once():
-    """A backward that is itself recorded would need second derivatives."""
+def _once(name, *grads):
+    """A backward that is itself recorded, or whose incoming gradients have tangents, would need second derivatives."""
+    _no_tangents(name + "'s gradient", *grads)
     if torch.is_grad_enabled():
         raise NotImplementedError("the expert layer's operators differentiate once (create_graph=False)")
 
@@ -137,7 +148,7 @@ class RMSNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, ds=None):
-        _once()
+        _once("rms_norm", dy, ds)
         need_x, need_w, _, need_r = ctx.needs_input_grad
         if dy is None and ds is None:
             return None, None, None, None
@@ -226,7 +237,7 @@ class Route(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, _, dweight):
-        _once()
+        _once("route", dweight)
         if dweight is None:
             return None, None, None, None, None
         logits, allowed, group, expert, weight = ctx.saved_tensors
@@ -381,7 +392,7 @@ class GroupedLinear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _once()
+        _once("grouped_linear", dy)
         if dy is None:
             return (None,) * 7
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -465,7 +476,7 @@ class ExpertCombine(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        _once()
+        _once("expert_combine", dout)
         need_y, need_w, need_r = ctx.needs_input_grad
         dy = dw = None
         if need_y or need_w:

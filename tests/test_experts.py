@@ -26,6 +26,27 @@ def test_host_tensors_are_refused():
             f()
 
 
+def test_tangents_are_refused():
+    """Forward mode: the kernels read values alone, so an operand with a tangent raises, whichever it is."""
+    dual, level = torch.autograd.forward_ad.make_dual, torch.autograd.forward_ad.dual_level
+    plan = ex.GroupPlan(torch.tensor([0, 4], dtype=torch.int32), torch.arange(4, dtype=torch.int32), 4)
+    w, m, b, c = torch.ones(8), torch.zeros(1, 3, 8), torch.zeros(1, 3), torch.ones(2, 2)
+    q, mq, s = X.to(torch.float8_e4m3fn), m.to(torch.float8_e4m3fn), torch.ones(4)
+    with level():
+        d = lambda t: dual(t, torch.ones_like(t))
+        for f in (lambda: ex.rms_norm(d(X), w), lambda: ex.rms_norm(X, d(w)), lambda: ex.rms_norm(X, w, residual=d(X)),
+                  lambda: ex.rms_norm_q8(d(X), w), lambda: ex.rms_norm_q8(X, w, residual=d(X)), lambda: ex.quantize_rows(d(X)),
+                  lambda: ex.route(d(X), 2), lambda: ex.grouped_linear(d(X), m, plan),
+                  lambda: ex.grouped_linear(X, d(m), plan), lambda: ex.grouped_linear(X, m, plan, bias=d(b)),
+                  lambda: ex.grouped_linear_q8(q, d(s), mq, b, plan), lambda: ex.grouped_linear_q8(q, s, mq, d(b), plan),
+                  lambda: ex.expert_combine(d(X), c), lambda: ex.expert_combine(X, d(c)),
+                  lambda: ex.expert_combine(X, c, residual=d(X[:2]))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+        with pytest.raises(RuntimeError, match="no CPU path"):       # others are checked as ever
+            ex.rms_norm(X, w)
+
+
 def test_norm_refusals():
     w = torch.ones(8)
     for f in (ex.rms_norm, ex.rms_norm_q8):

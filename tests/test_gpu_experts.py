@@ -904,6 +904,25 @@ def test_a_recorded_backward_is_refused():
             torch.autograd.grad(out.sum(), leaf, create_graph=True)
 
 
+def test_tangents_of_gradients_are_refused():
+    """Forward over reverse: a gradient that comes with a tangent raises in every operator's backward, and calls without
+    one give what they give outside a dual level."""
+    g = gen(3)
+    x, plan = rand(g, 4, 8).requires_grad_(True), ex.group_plan(torch.zeros(4, dtype=torch.int32, device=DEV), 1)
+    w, m, c = rand(g, 8), rand(g, 1, 3, 8), rand(g, 2, 2)
+    ops = [lambda: ex.rms_norm(x, w), lambda: ex.route(x, 2)[1], lambda: ex.grouped_linear(x, m, plan), lambda: ex.expert_combine(x, c)]
+    for f in ops:
+        ones = torch.ones_like(f())
+        want, = torch.autograd.grad(f(), x, ones)
+        with torch.autograd.forward_ad.dual_level():
+            got, = torch.autograd.grad(f(), x, ones)
+            assert torch.equal(got, want)
+            with pytest.raises(NotImplementedError, match="gradient: no forward-mode"):
+                torch.autograd.grad(f(), x, torch.autograd.forward_ad.make_dual(ones, ones))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ex.rms_norm(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()), w)
+
+
 def test_one_tensor_twice_and_backward_twice():
     """The same leaf as two operands, the same weights in two products, and a backward run again on a kept graph."""
     g = gen(5)
