@@ -148,4 +148,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* part) {
     return v;
 }
 
+// out (N, F) of `dtype` = sums of k neighbouring fp32 rows (N k, F), in order (route.hip).
+int sum_slot_rows(const float* rows, int64_t N, int k, int F, int dtype, void* out, hipStream_t st);
+
 }  // namespace face

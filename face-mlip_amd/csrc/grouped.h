@@ -478,7 +478,7 @@ __device__ __forceinline__ void finish(const GroupedArgs& g, int group, int32_t 
     if constexpr (COLS_B) {
         if (g.z) {
             float z[8];
-            load_piece((const Out*)g.z + (int64_t)(a / g.zdiv) * g.ld_z + col, left, z);
+            load_piece((const T*)g.z + (int64_t)(a / g.zdiv) * g.ld_z + col, left, z);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= silu_slope(z[e]);
         }

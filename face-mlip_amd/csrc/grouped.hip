@@ -16,6 +16,8 @@ FACE_GROUPED(float)
 FACE_GROUPED(bf16)
 FACE_GROUPED(f16)
 #undef FACE_GROUPED
+extern template int launch_rows<bf16, float, true>(GroupedArgs, hipStream_t);
+extern template int launch_rows<f16, float, true>(GroupedArgs, hipStream_t);
 
 static int grouped_args(const void* ptr, const void* order, int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype) {
     if (slots < 0 || G <= 0 || n <= 0 || k <= 0) return FACE_ERR_ARG;
@@ -57,9 +59,10 @@ extern "C" int face_grouped_linear_q8(const void* x, int64_t ld_x, const float* 
 }
 
 namespace face {
-// Workspace of the backward: a row of dx per slot where the rows of x are shared, then the weights' partial results.
-static int64_t slot_rows_bytes(int64_t slots, int32_t k, int32_t dtype, int32_t x_div) {
-    return x_div > 1 ? (slots * k * (dtype == FACE_F32 ? 4 : 2) + 255) / 256 * 256 : 0;
+// Workspace of the backward: a row of dx per slot where the rows of x are shared, then the weights' partial results. The
+// slots' rows are fp32 whatever the rows' type: their sum is rounded once, and a part past fp16's largest is no infinity.
+static int64_t slot_rows_bytes(int64_t slots, int32_t k, int32_t x_div) {
+    return x_div > 1 ? (slots * k * 4 + 255) / 256 * 256 : 0;
 }
 static int64_t part_bytes(int64_t slots, int32_t n, int32_t k, int32_t dtype, bool with_bias) {
     // the most shares of the ways the call may go; one group has them wherever several have
@@ -79,7 +82,7 @@ static int64_t part_bytes(int64_t slots, int32_t n, int32_t k, int32_t dtype, bo
 extern "C" int64_t face_grouped_linear_bwd_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t x_div,
                                                 int32_t with_dx, int32_t with_dw, int32_t with_db) {
     if (slots <= 0 || n <= 0 || k <= 0) return 0;
-    return (with_dx ? slot_rows_bytes(slots, k, dtype, x_div) : 0) + (with_dw ? part_bytes(slots, n, k, dtype, with_db) : 0);
+    return (with_dx ? slot_rows_bytes(slots, k, x_div) : 0) + (with_dw ? part_bytes(slots, n, k, dtype, with_db) : 0);
 }
 
 extern "C" int face_grouped_linear_bwd(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* dy,
@@ -93,16 +96,17 @@ extern "C" int face_grouped_linear_bwd(const void* x, int64_t ld_x, int32_t x_di
     if (slots && (!dy || (dx && !w) || ((dw || x_op) && !x))) return FACE_ERR_ARG;
     const int64_t need = face_grouped_linear_bwd_work(slots, n, k, dtype, x_div, dx != nullptr, dw != nullptr, db != nullptr);
     if (work_bytes < need || (need && !work)) return FACE_ERR_ARG;
-    char* part = (char*)work + (dx ? slot_rows_bytes(slots, k, dtype, x_div) : 0);
+    char* part = (char*)work + (dx ? slot_rows_bytes(slots, k, x_div) : 0);
     const hipStream_t st = (hipStream_t)stream;
     if (dx && slots) {
         void* rows = x_div > 1 ? work : dx;
         GroupedArgs g = {dy, ld_dy, 1, 0, w, ld_w, w_group, nullptr, 0, nullptr, nullptr, rows, k, x_op ? x : nullptr, ld_x,
                          x_div, k, n, ptr, order, slots, G, 0, 0};
-        int rc = with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), decltype(t), true>(g, st); });
-        // a slot's row was rounded to the rows' type; the sum of a row's slots is rounded once more
-        if (!rc && x_div > 1)
-            rc = face_expert_combine_fwd(work, k, nullptr, nullptr, 0, slots / x_div, x_div, k, dtype, dx, stream);
+        int rc = with_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            return x_div > 1 ? launch_rows<T, float, true>(g, st) : launch_rows<T, T, true>(g, st);
+        });
+        if (!rc && x_div > 1) rc = sum_slot_rows((const float*)work, slots / x_div, x_div, k, dtype, dx, st);
         if (rc) return rc;
     }
     if (dw) {

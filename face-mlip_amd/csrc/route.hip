@@ -359,9 +359,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const int32_t*
 // out[i] = r[i] + sum_j w[i, j] y[i k + j], one read of each row; a row's pieces are spread over LANES threads. Bound by
 // bytes: 100,000 x 2 x 512 bf16 89 us forward (410 MB), 91 us backward (512 MB): 4.6 and 5.6 TB/s, part of it from the last
 // level of cache.
-// w null: factors of one.
-template <typename T, int LANES>
-__global__ __launch_bounds__(256) void combine_fwd_kernel(const T* __restrict__ y, int64_t ld_y,
+// w null: factors of one. Y: the type of y's rows, T or float.
+template <typename Y, typename T, int LANES>
+__global__ __launch_bounds__(256) void combine_fwd_kernel(const Y* __restrict__ y, int64_t ld_y,
                                                           const float* __restrict__ w, const T* __restrict__ r,
                                                           int64_t ld_r, int64_t N, int k, int F, T* __restrict__ out) {
     const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -429,6 +429,25 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(const T* __restrict__ 
 
 // Threads per row of the join: about four pieces each.
 static inline int join_lanes(int F) { return F <= 512 ? 16 : (F <= 4096 ? 64 : 256); }
+
+template <typename Y, typename T>
+static int launch_combine_fwd(const Y* y, int64_t ld_y, const float* w, const T* r, int64_t ld_r, int64_t N, int k, int F, T* out,
+                              hipStream_t st) {
+    const int L = join_lanes(F), rows = 256 / L;
+    const dim3 grid((unsigned)((N + rows - 1) / rows));
+    auto* kern = L == 16 ? combine_fwd_kernel<Y, T, 16> : (L == 64 ? combine_fwd_kernel<Y, T, 64> : combine_fwd_kernel<Y, T, 256>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, y, ld_y, w, r, ld_r, N, k, F, out);
+    FACE_LAUNCH_CHECK();
+    return 0;
+}
+
+int sum_slot_rows(const float* rows, int64_t N, int k, int F, int dtype, void* out, hipStream_t st) {
+    if (F > (1 << 30) || N > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        return launch_combine_fwd<float, T>(rows, F, nullptr, nullptr, 0, N, k, F, (T*)out, st);
+    });
+}
 
 }  // namespace face
 
@@ -534,15 +553,9 @@ extern "C" int face_expert_combine_fwd(const void* y, int64_t ld_y, const float*
     if (ld_y < F || (r && ld_r < F)) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!y || !out) return FACE_ERR_ARG;
-    const int L = join_lanes(F), rows = 256 / L;
-    const dim3 grid((unsigned)((N + rows - 1) / rows));
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        auto* kern = L == 16 ? combine_fwd_kernel<T, 16> : (L == 64 ? combine_fwd_kernel<T, 64> : combine_fwd_kernel<T, 256>);
-        hipLaunchKernelGGL(kern, grid, dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, weight, (const T*)r, ld_r, N,
-                           k, F, (T*)out);
-        FACE_LAUNCH_CHECK();
-        return 0;
+        return launch_combine_fwd<T, T>((const T*)y, ld_y, weight, (const T*)r, ld_r, N, k, F, (T*)out, (hipStream_t)stream);
     });
 }
 

@@ -602,8 +602,7 @@ int face_grouped_linear_q8(const void* x, int64_t ld_x, const float* x_scale, in
                            int64_t w_group, const float* w_scale, const void* bias, int64_t ld_b, const int32_t* ptr,
                            const int32_t* order, int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* y,
                            int64_t ld_y, void* stream);
-/* Its gradients for dy (slots, n): dx like x, dense rows (the slots of a shared row rounded to the rows' type, then
- * summed), dw (G, n, k) and db (G, n) dense; each may be NULL (db only with dw; w is read for dx, x for dw and for
+/* Its gradients for dy (slots, n): dx like x, dense rows (the slots of a shared row summed in fp32), dw (G, n, k) and db (G, n) dense; each may be NULL (db only with dw; w is read for dx, x for dw and for
  * x_op). slots a multiple of x_div. work: face_grouped_linear_bwd_work bytes, 256-byte aligned. Fixed summation
  * order. */
 int64_t face_grouped_linear_bwd_work(int64_t slots, int32_t n, int32_t k, int32_t dtype, int32_t x_div, int32_t with_dx,

@@ -544,6 +544,32 @@ def test_grouped_linear_gradient_against_differences():
         assert abs((out[i].double() * v).sum() - want) <= 1e-5 * (out[i].double() * v).abs().sum()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,k,G,ki,n", [(1, 2, 3, 40, 24), (50, 4, 8, 257, 31), (700, 3, 4, 96, 130), (3000, 4, 8, 256, 192)])
+def test_input_gradient_of_shared_rows_is_rounded_once(dtype, N, k, G, ki, n):
+    """A row's choices are summed in 32 bits: one rounding to the rows' type, in the result."""
+    g = gen(N + k)
+    e = torch.randint(-1, G, (N, k), generator=g, device=DEV, dtype=torch.int32)
+    plan = ex.group_plan(e, G)
+    w, dy = rand(g, G, n, ki, dtype=dtype, scale=n ** -0.5), rand(g, N * k, n, dtype=dtype)
+    for silu in (False, True):
+        say("shared rows", dtype, N, k, silu)
+        x = rand(g, N, ki, dtype=dtype).requires_grad_(True)
+        d, = torch.autograd.grad(ex.grouped_linear(x, w, plan, x_op="silu" if silu else None), x, dy)
+        _, _, d64, ad, *_ = linear64(x.detach(), w, e, None, silu, dy)
+        lim = (steps(dtype, n) + 8 * U32) * ad + k * U32 * ad
+        near(d, d64.view(N, k, ki).sum(1), lim.view(N, k, ki).sum(1), "dx")
+
+
+def test_input_gradient_whose_parts_pass_the_types_largest():
+    """Choices whose parts pass float16's 65504 and cancel: 300 * 250 - 300 * 240."""
+    x = torch.zeros(40, 8, device=DEV, dtype=F16, requires_grad=True)
+    w = torch.tensor([250.0, -240.0], device=DEV, dtype=F16).view(2, 1, 1).expand(2, 1, 8)
+    plan = ex.group_plan(torch.tensor([[0, 1]], device=DEV).expand(40, 2), 2)
+    d, = torch.autograd.grad(ex.grouped_linear(x, w, plan), x, torch.full((80, 1), 300.0, device=DEV, dtype=F16))
+    assert bool((d == 3000).all())
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_weight_gradient_of_many_slots(dtype):
     """Tiles of 256 x 256: a hundred thousand slots in uneven groups, one of them empty, and slots of none."""
