@@ -160,16 +160,6 @@ __device__ __forceinline__ Held<T> hold(const T* p, int left) {
     return h;
 }
 
-__device__ __forceinline__ float silu(float x) {
-    float rest;
-    return x * gemm_sigmoid(x, rest);
-}
-__device__ __forceinline__ float silu_slope(float x) {
-    float rest;
-    const float s = gemm_sigmoid(x, rest);
-    return s * fmaf(x, rest, 1.f);
-}
-
 // silu in fp32; a 16-bit operand is rounded once more, as it enters the matrix cores.
 template <typename T>
 __device__ __forceinline__ void apply_silu(Held<T>& h) {

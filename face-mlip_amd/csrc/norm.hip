@@ -87,10 +87,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_fwd_kernel
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) {
-                float rest;
-                v[u][e] *= gemm_sigmoid(v[u][e], rest);
-            }
+            for (int e = 0; e < kPiece; ++e) v[u][e] = silu(v[u][e]);
     }
     if constexpr (MODE == kNorm) {
 #pragma unroll

@@ -525,6 +525,48 @@ def test_grouped_linear_float32_accuracy():
             assert (a.double() - b).norm() < 1e-6 * b.norm()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu_of_far_values(dtype):
+    """SiLU and its slope over the types' whole range: x sigmoid(x) falls to 0 on the left and is x on the right, the slope 0
+    and 1; an infinity gives what the formula gives, NaN or itself. Left of -87 both are 0: |x| e^x < 87 e^-87 = 2^-118.9 there,
+    the only difference that the 8-bit rows (scales down to 2^-126) could show."""
+    far = [-104.0, -100.0, -90.0, -81.0, -80.5, -80.0, -79.5, -20.0, 0.0, 20.0, 79.5, 80.0, 80.5, 81.0, 90.0, 104.0, 1000.0, -1000.0,
+           6e4, -6e4, math.inf, -math.inf, math.nan]
+    far += [] if dtype == F16 else [v * 10.0 ** e for e in (10, 20, 30, 35, 38) for v in (-3.0, 3.0)]
+    x = torch.tensor(far, device=DEV).to(dtype)[:, None]
+    N = x.shape[0]
+    x64 = x.double()
+    sg = torch.sigmoid(x64)
+    for reps in (1, 100):                                # few slots, and tiles of many
+        say("far values", dtype, reps)
+        xs = x.repeat(reps, 1).requires_grad_(True)
+        plan = ex.group_plan(torch.arange(N, device=DEV).repeat(reps), N)
+        w = torch.ones(N, 1, 1, device=DEV, dtype=dtype, requires_grad=True)
+        y = ex.grouped_linear(xs, w, plan, x_op="silu")
+        dy = torch.zeros(N * reps, 1, device=DEV, dtype=dtype)
+        dy[:N] = 1
+        d, dw = torch.autograd.grad(y, [xs, w], dy)
+        want, slope = (x64 * sg)[:, 0], (sg * (1 + x64 * (1 - sg)))[:, 0]
+        ok = torch.isfinite(want)
+        pre = 4 * U32 + (0 if dtype == F32 else u(dtype))                     # as in check_linear
+        # below 2^-126 a float32 product may be cut: 2^-126 |x|, and 2^-25 of a float16 operand
+        tiny = 2.0 ** -126 * x64[:, 0].abs().clamp_max(1e4) + (2.0 ** -25 if dtype == F16 else 0.0)
+        for got in (y[:N, 0], y[-N:, 0]):
+            near(got[ok], want[ok], ((steps(dtype, 1) + pre) * want.abs() + tiny)[ok], "silu")
+            assert torch.equal(got[~ok].double().nan_to_num(7.0), want[~ok].nan_to_num(7.0))
+        fin = torch.isfinite(slope)
+        mag = (sg * (1 + x64.abs() * (1 - sg)))[:, 0]
+        near(d[:N, 0][fin], slope[fin], ((steps(dtype, 1) + 8 * U32) * mag + tiny)[fin], "slope")
+        assert d[:N, 0][~fin].isnan().all()
+        one = torch.autograd.grad(ex.grouped_linear(xs[:N], w, ex.group_plan(torch.arange(N, device=DEV), N), x_op="silu"), w,
+                                  dy[:N])[0][:, 0, 0]
+        near(one[ok], want[ok], ((steps(dtype, 1) + pre) * want.abs() + tiny)[ok], "dw")
+    q, scale = ex.quantize_rows(x, "silu")
+    left = x64 < -87
+    assert bool(((x64 * sg)[left & ok[:, None]].abs() < 2.0 ** -118.9).all())
+    check_q8(q[ok], scale[ok], torch.where(left, 0.0, x64 * sg)[ok], 4 * U32)
+
+
 def test_grouped_linear_gradient_against_differences():
     g = gen(9)
     e = torch.randint(-1, 3, (15, 2), generator=g, device=DEV, dtype=torch.int32)
