@@ -457,7 +457,11 @@ __device__ __forceinline__ void finish(const GroupedArgs& g, int group, int32_t 
         float s[8];
         load_piece(g.ws + (int64_t)group * g.n + col, left, s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= sx * s[e];
+        for (int e = 0; e < 8; ++e) {
+            // one after the other where their product leaves the normal range, in which the result may still lie
+            const float f = sx * s[e];
+            v[e] = __builtin_amdgcn_classf(f, 0x108) ? v[e] * f : v[e] * sx * s[e];
+        }
     }
     if (g.bias) {
         float s[8];

@@ -740,6 +740,25 @@ def test_grouped_linear_q8(out, N, k, G, ki, n):
                        ex.grouped_linear_q8(q, xs, wq, ws, plan, dtype=out))
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("N,n", [(3, 5), (2000, 300)])
+def test_grouped_linear_q8_of_far_scales(out, N, n):
+    """Scales whose product leaves float32's range while the result does not: sums of 0 stay 0, tiny and huge ones keep
+    their digits."""
+    k = 48
+    plan = ex.group_plan(torch.zeros(N, dtype=torch.int32, device=DEV), 1)
+    fill = lambda v, *shape: torch.full(shape, v, device=DEV).to(E4M3)
+    for xv, wv, xs, ws in ((448.0, 416.0, 1.2345 * 2.0 ** -70, 1.7 * 2.0 ** -72), (2.0 ** -9, 3 * 2.0 ** -9, 1.3 * 2.0 ** 90, 1.1 * 2.0 ** 40),
+                           (448.0, 0.0, 2.0 ** 100, 2.0 ** 40), (0.0, 448.0, 2.0 ** 40, 2.0 ** 100), (448.0, 448.0, 2.0 ** 100, 1.1 * 2.0 ** -120),
+                           (448.0, 448.0, 1.3 * 2.0 ** -120, 2.0 ** 110)):
+        y = ex.grouped_linear_q8(fill(xv, N, k), torch.full((N,), xs, device=DEV), fill(wv, 1, n, k), torch.full((1, n), ws, device=DEV),
+                                 plan, dtype=out)
+        f32 = lambda v: torch.tensor(v, dtype=F32).double().item()
+        want = torch.full((N, n), k * xv * wv * f32(xs) * f32(ws), device=DEV, dtype=torch.float64)
+        # equal products, whose partial sums are whole multiples below 2^24 of one: exact; three roundings of scales
+        near(y, want, 3 * U32 * want.abs(), f"{xs:.3g} {ws:.3g}")
+
+
 def test_rows_past_two_to_the_31_elements():
     """Rows of x, y and the gradient whose offsets pass 32 bits."""
     N, n = 70000, 33000
