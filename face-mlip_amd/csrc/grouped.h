@@ -1136,7 +1136,7 @@ static inline bool weight_large(int64_t slots, int n, int k) {
 }
 // Shares of its slots. A workgroup takes about `slot` us a slot, and a share costs 0.08 us and the bytes of a partial result
 // written and read at 4 TB/s, so that s shares take slots slot / s + s (0.08 + 2e-6 n k): the s with the least, and no more
-// than fill the chip once (three workgroups per CU of 16-bit rows, two of fp32 rows, one of 256 x 256). One workgroup per
+// than fill the chip once (three workgroups per CU of 16-bit rows staged without registers, two of others, one of 256 x 256). One workgroup per
 // group and tile instead, without partial results, where the largest group (taken as half the slots, or all of one) is done
 // no later than the shares and the 9 us of their join, and up to 512 slots, which need no workspace then. Measured (us,
 // shares of 256 slots or more that fill the chip / this rule):
@@ -1144,10 +1144,12 @@ static inline bool weight_large(int64_t slots, int n, int k) {
 //         24,000 in three 512 x 512 56 / 50, 100,000 in eight 1440 x 320 200 / 208, 97 x 96 46 / 50
 //   fp32: 800 in three 2304 x 512 53 / 30, in one 192 x 97 30 / 24, 8,000 in 32 864 x 192 65 / 58, 100,000 in eight 192 x 97
 //         67 / 71; the same within 1 % from 24,000 slots of 1440 x 320 on
+// 16-bit rows staged through registers take 195 of them, two workgroups per CU; shares for three / for two (us): 200,000 slots in
+// eight 2304 x 512 1650 / 1452, 100,000 512 x 512 198 / 168, 1440 x 320 411 / 368, 513 x 97 111 / 89, 321 x 1440 420 / 433.
 static inline int weight_shares(int64_t slots, int groups, int n, int k, int dtype, bool large, bool direct) {
     const int tile = large ? 256 : 128;
     const double tiles = (double)((n + tile - 1) / tile) * ((k + tile - 1) / tile);
-    const double fill = (large ? 1 : dtype == FACE_F32 ? 2 : 3) * device_cu_count() / tiles;
+    const double fill = (large ? 1 : dtype != FACE_F32 && direct ? 3 : 2) * device_cu_count() / tiles;
     const double slot = dtype == FACE_F32 ? 0.06 : (direct ? 0.0175 : 0.035);
     const double all = (double)slots * slot, join = 0.08 + 2e-6 * n * k;
     double s = __builtin_sqrt(all / join);
