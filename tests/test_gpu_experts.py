@@ -690,6 +690,75 @@ def test_grouped_linear_values_that_are_not_finite(N):
     assert bool((ex.grouped_linear(x, w, plan) == torch.tensor(big, device=DEV) * 0.5).all())
 
 
+@pytest.mark.parametrize("N,G,ki,n", [(21, 3, 300, 97), (21, 3, 33, 65), (100, 3, 2048, 2048), (700, 3, 1440, 320), (3000, 3, 96, 70),
+                                      (12000, 3, 520, 330)])
+def test_float32_values_past_the_range_of_bfloat16(N, G, ki, n):
+    """Products of fp32 values past bfloat16's largest (3.39e38), in one row and column or everywhere, and of infinities and
+    NaN everywhere, in every tile and direction: as plain float32 products, whose sums of m terms are off by m u of them."""
+    say("past bfloat16", N, G, ki, n)
+    g = gen(N + ki)
+    e = torch.randint(0, G, (N, 1), generator=g, device=DEV, dtype=torch.int32)
+    plan = ex.group_plan(e, G)
+    big = lambda *s: (3.395e38 + 5e35 * torch.rand(*s, generator=g, device=DEV)) * (torch.randint(0, 2, s, generator=g, device=DEV) * 2 - 1)
+    tiny = lambda *s: rand(g, *s, scale=2.0 ** -100)
+    for where in ("rows", "weights", "all"):
+        x, w, dy = rand(g, N, ki), rand(g, G, n, ki), tiny(N, n)
+        if where == "rows":
+            x, w = tiny(N, ki), tiny(G, n, ki)
+            x[N // 2, ki // 3], x[0, 0], dy[N // 3, n // 2] = 3.4e38, -3.4e38, 3.4e38
+        elif where == "weights":
+            x, w = tiny(N, ki), tiny(G, n, ki)
+            w[G - 1, n // 2, ki // 2] = w[0, 0, 0] = 3.4e38
+        else:
+            x, w = big(N, ki), tiny(G, n, ki) if N > 100 else tiny(G, n, ki) * 2.0 ** -20
+        y64, ay, d64, ad, dw64, adw, *_ = linear64(x, w, e, None, False, dy)
+        x.requires_grad_(True), w.requires_grad_(True)
+        y = ex.grouped_linear(x, w, plan)
+        d, dw = torch.autograd.grad(y, [x, w], dy)
+        for got, want, terms, m, what in ((y, y64, ay, ki, "y"), (d, d64, ad, n, "dx"), (dw, dw64, adw, N, "dw")):
+            assert bool(torch.isfinite(got).all()), (where, what)
+            near(got, want, (m * U32 + steps(F32, m)) * terms + 2.0 ** -126, (where, what))
+    for v in (math.nan, math.inf):
+        x, w, dy = torch.full((N, ki), v, device=DEV), rand(g, G, n, ki), rand(g, N, n)
+        dy[:, 0], w[:, 0] = dy[:, 0].abs(), w[:, 0].abs()                  # a column whose infinities agree
+        y64, _, d64, *_ = linear64(x, w, e, None, False, torch.full_like(dy, v))
+        x.requires_grad_(True), w.requires_grad_(True)
+        y = ex.grouped_linear(x, w, plan)
+        dw64 = linear64(x.detach(), w.detach(), e, None, False, dy)[4]
+        dw, = torch.autograd.grad(y, w, dy)
+        d, = torch.autograd.grad(ex.grouped_linear(x, w, plan), x, torch.full_like(dy, v))
+        for got, want in ((y, y64), (d, d64), (dw, dw64)):
+            assert torch.equal(got.double().nan_to_num(7.0), want.nan_to_num(7.0)), v
+
+
+def test_float32_values_that_are_not_finite_cost_a_bounded_time():
+    """A diverged step: every value NaN or infinite takes some ten times a finite step's time, where sums formed again one by
+    one take hundreds."""
+    g = gen(1)
+    N, G, ki, n = 24000, 3, 1440, 320
+    plan = ex.group_plan(torch.randint(0, G, (N,), generator=g, device=DEV, dtype=torch.int32), G)
+    w, dy = rand(g, G, n, ki).requires_grad_(True), rand(g, N, n)
+
+    def ms(v):
+        x = (rand(g, N, ki) if v is None else torch.full((N, ki), v, device=DEV)).requires_grad_(True)
+        up = dy if v is None else torch.full_like(dy, v)
+        best = math.inf
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            torch.autograd.grad(ex.grouped_linear(x, w, plan), [x, w], up)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    fine = ms(None)
+    for v in (math.nan, math.inf):
+        t = ms(v)
+        say("ms: finite", fine, "of", v, t)
+        assert t < 60 * fine
+
+
 def test_plans_that_name_no_slot_are_bounded():
     """Ranges and slots outside the plan are left out: no access outside the operands."""
     g = gen(4)
