@@ -403,14 +403,25 @@ class GroupedLinear(torch.autograd.Function):
         div = _div(ctx.plan, x.shape[0])
         x2, dy, w2 = _rows(x, k), _rows(dy, n), _weights(w)
         dx = _like(x) if need_x else None
-        dw = torch.empty(G, n, k, dtype=dtype, device=dev) if need_w or need_b else None
         db = torch.empty(G, n, dtype=dtype, device=dev) if need_b else None
-        need = _lib.lib().face_grouped_linear_bwd_work(slots, n, k, code, div, need_x, need_w or need_b, need_b)
-        work = _work(need, dev)
-        _launch(x, "face_grouped_linear_bwd", "grouped_linear_bwd", x2.data_ptr(), x2.stride(0), div, ctx.op, dy.data_ptr(),
-                dy.stride(0), w2.data_ptr(), w2.stride(1), w2.stride(0), p.data_ptr(), order.data_ptr(), slots, G, n, k, code,
-                ptr(dx), ptr(dw), ptr(db), ptr(work), need)
-        return dx, dw if need_w else None, db, None, None, None, None
+
+        def launch(k, op, dx, dw, db):
+            need = _lib.lib().face_grouped_linear_bwd_work(slots, n, k, code, div, dx is not None, dw is not None, db is not None)
+            work = _work(need, dev)
+            _launch(x, "face_grouped_linear_bwd", "grouped_linear_bwd", x2.data_ptr(), x2.stride(0), div, op, dy.data_ptr(),
+                    dy.stride(0), w2.data_ptr(), w2.stride(1), w2.stride(0), p.data_ptr(), order.data_ptr(), slots, G, n, k, code,
+                    ptr(dx), ptr(dw), ptr(db), ptr(work), need)
+
+        if need_w or not need_b:
+            dw = torch.empty(G, n, k, dtype=dtype, device=dev) if need_w else None
+            launch(k, ctx.op, dx, dw, db)
+        else:                                        # db comes with dw: that of eight columns, not of all
+            dw = None
+            if need_x:
+                launch(k, ctx.op, dx, None, None)
+            few = min(k, 8)
+            launch(few, 0, None, torch.empty(G, n, few, dtype=dtype, device=dev), db)
+        return dx, dw, db, None, None, None, None
 
 
 def grouped_linear(x, w, plan, bias=None, x_op=None):

@@ -464,6 +464,37 @@ def test_weight_gradient_by_shares_or_by_group(dtype, N, G, ki, n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,k,ki,n", [(30, 2, 5, 17), (700, 1, 200, 97), (20000, 2, 2304, 256)])
+def test_bias_gradient_alone(dtype, N, k, ki, n):
+    """Frozen weights with a trained bias, with and without rows that take gradients: no weight gradient is formed, nor room
+    for one."""
+    G = 64
+    g = gen(ki)
+    e = torch.randint(-1, G, (N, k), generator=g, device=DEV, dtype=torch.int32)
+    e[e == 3] = 4                                        # a group without slots
+    plan = ex.group_plan(e, G)
+    x, w, dy = rand(g, N, ki, dtype=dtype), rand(g, G, n, ki, dtype=dtype, scale=n ** -0.5), rand(g, N * k, n, dtype=dtype)
+    b = rand(g, G, n, dtype=dtype).requires_grad_(True)
+    i = torch.where(e < 0, G, e).reshape(-1).long()
+    want = torch.zeros(G + 1, n, dtype=torch.float64, device=DEV).index_add_(0, i, dy.double())[:G]
+    mag = torch.zeros(G + 1, n, dtype=torch.float64, device=DEV).index_add_(0, i, dy.double().abs())[:G]
+    for op in (None, "silu"):
+        say("bias alone", dtype, N, op)
+        y = ex.grouped_linear(x, w, plan, bias=b, x_op=op)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        db, = torch.autograd.grad(y, b, dy)
+        if ki > 2000:
+            assert torch.cuda.max_memory_allocated() - before < w.numel() * w.element_size()
+        near(db, want, N * k * U32 * mag, "db")
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        d, db1 = torch.autograd.grad(ex.grouped_linear(xl, w, plan, bias=b, x_op=op), [xl, b], dy)
+        d0, _, _ = torch.autograd.grad(ex.grouped_linear(xl, wl, plan, bias=b, x_op=op), [xl, wl, b], dy)
+        assert torch.equal(db1, db) and torch.equal(d, d0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [1, 300, 20000])
 def test_grouped_linear_of_thousands_of_groups(dtype, N):
     """A plan that a program made itself, of more groups than group_plan takes, most of them without rows."""
