@@ -643,6 +643,45 @@ def test_input_gradient_whose_parts_pass_the_types_largest():
     assert bool((d == 3000).all())
 
 
+# Sizes (N, G, ki, n) that take tiles of 128 x 64 (the first four, in both directions) and 128 x 128 (the next three in one
+# direction, the last two in both) of 16-bit rows on 256 CUs: sums that end within a chunk of 64, groups that end within a tile, last columns of 8 to 128; both operands whole chunks of 16
+# bytes, one of them or neither.
+LARGE = [(24000, 3, 264, 320), (24000, 3, 320, 319), (24000, 3, 257, 264), (24000, 3, 319, 257), (24000, 3, 136, 200),
+         (24000, 3, 200, 135), (24000, 3, 135, 200), (12000, 3, 520, 520), (16000, 3, 2304, 392)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,G,ki,n", LARGE)
+def test_large_tiles(dtype, N, G, ki, n):
+    say("large tiles", dtype, N, ki, n)
+    g = gen(ki)
+    e = torch.randint(-1, G, (N, 1), generator=g, device=DEV, dtype=torch.int32)
+    check_linear(N, 1, G, ki, n, dtype, expert=e)
+    check_linear(N, 1, G, ki, n, dtype, expert=e, silu=True, bias=False)
+    if ki < 300:                                          # odd addresses of either operand
+        wide, ww = rand(g, N, ki + 9, dtype=dtype), rand(g, G, n, ki + 8, dtype=dtype, scale=ki ** -0.5)
+        check_linear(N, 1, G, ki, n, dtype, expert=e, x=wide[:, 1:ki + 1].detach(), w=ww[..., :ki].detach())
+        check_linear(N, 1, G, ki, n, dtype, expert=e, x=wide[:, :ki].detach(), w=ww[..., 1:ki + 1].detach())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_products_of_many_slots(dtype):
+    """The forward and the input gradient of a hundred thousand slots, one row each and two of a row."""
+    N, G, ki, n = 100300, 6, 1544, 656
+    g = gen(18)
+    w = rand(g, G, n, ki, dtype=dtype, scale=ki ** -0.5)
+    for k, rows in ((1, N), (2, N // 2)):
+        e = torch.randint(-1, 5, (rows, k), generator=g, device=DEV, dtype=torch.int32)
+        plan = ex.group_plan(e, G)
+        x, dy = rand(g, rows, ki, dtype=dtype).requires_grad_(True), rand(g, rows * k, n, dtype=dtype)
+        y = ex.grouped_linear(x, w, plan)
+        d, = torch.autograd.grad(y, x, dy)
+        y64, ay, d64, ad, *_ = linear64(x.detach(), w, e, None, False, dy)
+        near(y, y64, steps(dtype, ki) * ay, "y")
+        lim = (steps(dtype, n) + k * U32) * ad.view(rows, k, ki).sum(1)
+        near(d, d64.view(rows, k, ki).sum(1), lim, "dx")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_weight_gradient_of_many_slots(dtype):
     """Tiles of 256 x 256: a hundred thousand slots in uneven groups, one of them empty, and slots of none."""
@@ -840,6 +879,45 @@ def test_grouped_linear_q8(out, N, k, G, ki, n):
                        ex.grouped_linear_q8(q, xs, wq, ws, plan, dtype=out))
 
 
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("N,G,ki,n", [(24000, 3, 272, 320), (24000, 3, 136, 264), (24000, 3, 144, 200), (24000, 3, 200, 135),
+                                      (12000, 3, 528, 520), (16000, 3, 2304, 392)])
+def test_large_tiles_q8(out, N, G, ki, n):
+    """Tiles of 128 x 64 and 128 x 128 in 8 bits: chunks of 128, whole or not, either operand at an odd address."""
+    say("large tiles q8", out, N, ki, n)
+    g = gen(ki)
+    e = torch.randint(-1, G, (N, 1), generator=g, device=DEV, dtype=torch.int32)
+    plan = ex.group_plan(e, G)
+    q, xs = ex.quantize_rows(rand(g, N, ki))
+    wq, ws = ex.quantize_rows(rand(g, G, n, ki))
+    b = rand(g, G, n, dtype=out)
+    y = ex.grouped_linear_q8(q, xs, wq, ws, plan, bias=b, dtype=out)
+    y64, ay, *_ = linear64(q.double() * xs.double()[:, None], wq.double() * ws.double()[..., None], e, b, False)
+    # 16 bits: each of a step's 64 products cut below 2^-13 of the largest of them, which is at most the terms' sum
+    cut = 0.0 if out == F32 else 2.0 ** -13 * math.ceil(ki / 64)
+    near(y, y64, (2 * U32 * (ki / 16 + 16) + cut) * ay, "y")
+    assert bool((y[e[:, 0] < 0] == 0).all())
+    wide, ww = torch.zeros(N, ki + 16, device=DEV, dtype=E4M3), torch.zeros(G, n, ki + 16, device=DEV, dtype=E4M3)
+    for at, bt in ((5, 0), (0, 3), (16, 16)):
+        wide[:, at:at + ki], ww[..., bt:bt + ki] = q, wq
+        assert torch.equal(ex.grouped_linear_q8(wide[:, at:at + ki], xs, ww[..., bt:bt + ki], ws, plan, bias=b, dtype=out), y)
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("N,n", [(40, 64), (3000, 512), (24000, 320), (24000, 200)])
+def test_q8_sums_of_one_sign(out, N, n):
+    """The cut of the 8-bit instruction goes by the products of a step, not by the sum so far: a sum of 2304 positive products
+    keeps its digits. Operands in [1/2, 1], so that no product is below a quarter of a step's largest: the cut, 2^-13 of that
+    largest for each, is at most 2^-11 of each product. By the sum so far it would be up to 64 2^-13 of it in each of 36 steps."""
+    g = gen(n)
+    q = (0.5 + 0.5 * torch.rand(N, 2304, generator=g, device=DEV)).to(E4M3)
+    wq = (0.5 + 0.5 * torch.rand(1, n, 2304, generator=g, device=DEV)).to(E4M3)
+    ones, plan = torch.ones(N, device=DEV), ex.group_plan(torch.zeros(N, dtype=torch.int32, device=DEV), 1)
+    y = ex.grouped_linear_q8(q, ones, wq, torch.full((1, n), 2.0 ** -5, device=DEV), plan, dtype=out)
+    want = q.double() @ wq[0].double().t() / 32
+    near(y, want, (2 * U32 * (2304 / 16 + 16) + (0.0 if out == F32 else 2.0 ** -11)) * want, "y")
+
+
 @pytest.mark.parametrize("out", [F32, BF16])
 @pytest.mark.parametrize("N,n", [(3, 5), (2000, 300)])
 def test_grouped_linear_q8_of_far_scales(out, N, n):
@@ -882,6 +960,58 @@ def test_rows_past_two_to_the_31_elements():
     near(d[rows], want, steps(BF16, n) * mag)
     out = ex.expert_combine(y, torch.full((N, 1), 2.0, device=DEV))
     assert torch.equal(out[rows], 2 * y[rows])
+
+
+def test_gradients_past_two_to_the_31_elements():
+    """Offsets that pass 32 bits in the backwards: the weight gradient's and the norm's rows, the join's slots."""
+    N, n = 70000, 33000
+    g = gen(2)
+    e = (torch.arange(N, device=DEV) % 2).to(torch.int32)
+    plan = ex.group_plan(e, 2)
+    x, w = rand(g, N, 16, dtype=BF16), rand(g, 2, n, 16, dtype=BF16).requires_grad_(True)
+    b = torch.zeros(2, n, device=DEV, dtype=BF16, requires_grad=True)
+    dy = rand(g, N, n, dtype=BF16)
+    for op in (None, "silu"):                             # staged without and through registers
+        say("weight gradient past 2^31", op)
+        dw, db = torch.autograd.grad(ex.grouped_linear(x, w, plan, bias=b, x_op=op), [w, b], dy)
+        cols = torch.tensor([0, 1, 16500, n - 2, n - 1], device=DEV)
+        h = x.double() * (torch.sigmoid(x.double()) if op else 1)
+        pre = (4 * U32 + u(BF16)) if op else 0
+        for i in range(2):
+            da, ha = dy[i::2, cols].double(), h[i::2]
+            near(dw[i, cols], da.t() @ ha, (steps(BF16, N) + pre) * (da.abs().t() @ ha.abs()), f"dw {i}")
+            near(db[i, cols], da.sum(0), N * U32 * da.abs().sum(0), f"db {i}")
+    # x rows past 2^31, gathered by the weight gradient
+    wt = rand(g, 2, 8, n, dtype=BF16, scale=0.01).requires_grad_(True)
+    up = rand(g, N, 8, dtype=BF16)
+    dw, = torch.autograd.grad(ex.grouped_linear(dy, wt, plan), wt, up)
+    for i in range(2):
+        da, ha = up[i::2].double(), dy[i::2, cols].double()
+        near(dw[i][:, cols], da.t() @ ha, steps(BF16, N) * (da.abs().t() @ ha.abs()), f"dw of wide rows {i}")
+    del dw, db
+    say("norm past 2^31")
+    rows = torch.tensor([0, 1, 35001, N - 2, N - 1], device=DEV)
+    wn = torch.ones(n, device=DEV, dtype=BF16, requires_grad=True)
+    xs = dy.detach().requires_grad_(True)
+    up = torch.ones(1, 1, device=DEV, dtype=BF16).expand(N, n)
+    d, dwn = torch.autograd.grad(ex.rms_norm(xs, wn, 1e-5), [xs, wn], up)
+    s = dy[rows].double()
+    rstd = 1 / torch.sqrt((s * s).mean(-1, keepdim=True) + 1e-5)
+    m = s.mean(-1, keepdim=True)
+    mag = rstd * (1 + s.abs() * rstd ** 2 * s.abs().mean(-1, keepdim=True))
+    near(d[rows], rstd * (1 - s * rstd ** 2 * m), 3 * (norm_terms(n) + 4) * U32 * mag, "dx")
+    rstd = 1 / torch.sqrt(torch.stack([(dy[i:i + 10000].double() ** 2).mean(1) for i in range(0, N, 10000)]).reshape(-1, 1) + 1e-5)
+    t = dy[:, cols].double() * rstd
+    near(dwn[cols], t.sum(0), (N + norm_terms(n) + 8) * U32 * t.abs().sum(0), "dw")
+    del d, xs, up
+    say("join past 2^31")
+    y, wc = dy.detach().requires_grad_(True), rand(g, N // 2, 2).requires_grad_(True)
+    dout = rand(g, N // 2, n, dtype=BF16)
+    gy, gw = torch.autograd.grad(ex.expert_combine(y, wc), [y, wc], dout)
+    at, j = rows // 2, rows % 2
+    near(gy[rows], wc.detach().double()[at, j][:, None] * dout[at].double(), torch.zeros((), device=DEV).double(), "dy")
+    t = dy[rows].double() * dout[at].double()
+    near(gw[at, j], t.sum(1), (n + 8) * U32 * t.abs().sum(1), "dweight")
 
 
 # ----------------------------------------------------------------------------- join
