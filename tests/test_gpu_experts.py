@@ -644,8 +644,8 @@ def test_input_gradient_whose_parts_pass_the_types_largest():
 
 
 # Sizes (N, G, ki, n) that take tiles of 128 x 64 (the first four, in both directions) and 128 x 128 (the next three in one
-# direction, the last two in both) of 16-bit rows on 256 CUs: sums that end within a chunk of 64, groups that end within a tile, last columns of 8 to 128; both operands whole chunks of 16
-# bytes, one of them or neither.
+# direction, the last two in both) of 16-bit rows on 256 CUs: sums that end within a chunk of 64, groups that end within a
+# tile, last columns of 8 to 128; both operands whole chunks of 16 bytes, one of them or neither.
 LARGE = [(24000, 3, 264, 320), (24000, 3, 320, 319), (24000, 3, 257, 264), (24000, 3, 319, 257), (24000, 3, 136, 200),
          (24000, 3, 200, 135), (24000, 3, 135, 200), (12000, 3, 520, 520), (16000, 3, 2304, 392)]
 
@@ -1238,6 +1238,33 @@ def test_tangents_of_gradients_are_refused():
                 torch.autograd.grad(f(), x, torch.autograd.forward_ad.make_dual(ones, ones))
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 ex.rms_norm(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()), w)
+
+
+def test_gradients_of_some_operands():
+    """Every subset of the leaves: the gradients that all leaves together get, and nothing for the others."""
+    import itertools
+    g = gen(12)
+    N, k, F, G = 40, 2, 96, 5
+    e = torch.randint(-1, G, (N, k), generator=g, device=DEV, dtype=torch.int32)
+    plan = ex.group_plan(e, G)
+    for dtype in TYPES:
+        r = lambda *s: rand(g, *s, dtype=dtype)
+        cases = [(lambda x, w, q: ex.rms_norm(x, w, 1e-5, residual=q), [r(N, F), r(F), r(N, F)], [r(N, F), r(N, F)]),
+                 (lambda x, w, b: (ex.grouped_linear(x, w, plan, bias=b, x_op="silu"),), [r(N, F), r(G, 33, F), r(G, 33)], [r(N * k, 33)]),
+                 (lambda y, c, q: (ex.expert_combine(y, c, residual=q),), [r(N * k, F), rand(g, N, k), r(N, F)], [r(N, F)])]
+        for f, ops, ups in cases:
+            fresh = lambda on: [t.detach().requires_grad_(i in on) for i, t in enumerate(ops)]
+            ls = fresh((0, 1, 2))
+            full = torch.autograd.grad(f(*ls), ls, ups)
+            for m in (1, 2):
+                for on in itertools.combinations(range(3), m):
+                    ls = fresh(on)
+                    for i, d in zip(on, torch.autograd.grad(f(*ls), [ls[j] for j in on], ups)):
+                        assert torch.equal(d, full[i]) and d.dtype == ops[i].dtype, (dtype, on)
+        x, w, q = (t.detach().requires_grad_(True) for t in cases[0][1])
+        _, s = ex.rms_norm(x, w, residual=q)
+        d = torch.autograd.grad(s, [x, w, q], cases[0][2][0])                # of the sum alone
+        assert torch.equal(d[0], cases[0][2][0]) and torch.equal(d[2], d[0]) and not d[1].any()
 
 
 def test_one_tensor_twice_and_backward_twice():
