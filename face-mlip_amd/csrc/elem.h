@@ -114,9 +114,9 @@ static inline int with_dtype(int dtype, Fn f) {
     }
 }
 
-// Rows of a row-wise kernel: `lanes` threads work on one row, each on up to kRowUnits pieces that stay in
-// registers from the first read to the last store, so that a row is read once. Few lanes for short
-// rows (four rows to a wave), a workgroup of 1024 for the longest.
+// Rows of a row-wise kernel: `lanes` threads work on one row, each on up to kRowUnits pieces that it keeps
+// from the first read to the last store, so that a row is read once: in registers, but for part of the rows of a
+// workgroup of 1024 (norm.hip). Few lanes for short rows (four rows to a wave), that workgroup for the longest.
 constexpr int kRowUnits = 8;
 struct RowShape {
     int lanes, units;

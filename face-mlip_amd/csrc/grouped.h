@@ -23,10 +23,13 @@
 //
 // Large calls are bound by the matrix cores and the power they may draw, up to four workgroups per CU covering each other's
 // waits (a second buffer per workgroup leaves room for fewer: 128 x 128 of bf16 543 -> 562 us, of e4m3 268 -> 342 us).
-// 200,000 slots of 100,000 x 2304 -> 512, eight groups: bf16 530 us (890 TFLOP/s; the library's product of one matrix 500),
-// e4m3 278 us (1.7 PFLOP/s), bf16 input gradient 625 us (750 TFLOP/s, 0.92 GB written), then 254 us for the sum of a row's
-// slots. 24,000 x 1440 -> 320 in fp32, three groups: 143 us (155 TFLOP/s of the 190 that six bf16 products allow), input
-// gradient 156 us. 21 rows x 192 -> 97 in fp32 6.6 us; two rows x 2048 -> 2048 in bf16 8.7 us, 16.8 MB of weights.
+// 200,000 slots of 100,000 x 2304 -> 512, eight groups: bf16 534 us (883 TFLOP/s; the library's product of one matrix 500),
+// e4m3 287 us (1.6 PFLOP/s), bf16 input gradient 799 us (590 TFLOP/s, 1.84 GB of fp32 rows written), then 461 us for the sum of
+// a row's slots; with a row per slot, in 16 bits, 625 us. 200,000 slots 512 -> 2304 in bf16 647 us, with SiLU on load 1226:
+// it keeps the rows from going to LDS directly and is formed again for each of 18 column tiles.
+// 24,000 x 1440 -> 320 in fp32, three groups: 142 us (155 TFLOP/s of the 190 that six bf16 products allow), input
+// gradient 156 us. 21 rows x 192 -> 97 in fp32 6.1 us; two rows x 2048 -> 2048 in bf16 8.8 us, 16.8 MB of weights, by 128
+// workgroups on 256 CUs.
 #pragma once
 #include "elem.h"
 #include <type_traits>
@@ -34,7 +37,8 @@
 namespace face {
 
 // 8-bit rows. The e4m3 instructions align the products of a step to the largest and cut what is below 2^-13 of it
-// (measured: errors up to 2^-10.4 of the largest product, one large among 63 small ones of a sign). Results of 16 bits
+// (measured: errors up to 2^-10.4 of the largest product, one large among 63 small ones of a sign). The sum so far takes no
+// part in it: sums of 2304 positive products are off by no more than their rounding to 16 bits. Results of 16 bits
 // take them all the same: the operands' own rounding is 2^-4 of that product. Results in fp32 do not: e4m3_wide
 // rows become bf16 as they are staged, exactly, and their sums are fp32 sums, at the bf16 rate.
 struct e4m3 {
@@ -800,7 +804,9 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 // groups, bf16: 673 us in 128 x 128 tiles, against 780 us with chunks of single groups (2.25 rounds of workgroups of
 // unlike length), and 578 us in 256 x 256 tiles: 816 TFLOP/s.
 // TILE 256 (16-bit operands staged without registers): 256 x 256 by eight waves of 128 x 64, into two buffers in turn, the next
-// slots on their way during the present ones' products.
+// slots on their way during the present ones' products. It spills 46 registers, the 128 x 128 tile staged so 25 to 27: places of
+// the results, stored before the loop over the groups and read where the results are, none in the loop over the slots.
+// The tile's padding is multiplied too: 1440 x 320 becomes 1536 x 384, 28 % more.
 template <typename T, int TILE>
 struct WeightKernel {
     using Op = Operand<T>;

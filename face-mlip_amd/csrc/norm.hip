@@ -5,13 +5,16 @@
 //   ds = rstd (g - s rstd^2 mean(g s)) + ds_in,  g = dy w,  rstd = 1 / sqrt(mean(s^2) + eps)
 //   dw = sum over rows of dy s rstd
 //
-// Everything between the first read of a row and its last store is fp32 in registers; the statistics of the
-// backward are formed again from s, which it has to read anyway, so that nothing but s is kept. Bound by
+// Everything between the first read of a row and its last store is fp32 in registers (up to 16384 columns); the statistics
+// of the backward are formed again from s, which it has to read anyway, so that nothing but s is kept. Bound by
 // bytes: a row is read once and each result written once. The sum is normalised as it was rounded: the
 // backward reads that value, and the next layer's residual starts from it.
-// A row lies in the registers of 16 lanes up to 256 columns, of a wave up to 4096, of four up to 16384, of 16 beyond.
+// A row lies in the registers of 16 lanes up to 256 columns, of a wave up to 4096, of four up to 16384. Longer ones are
+// shared by 16 waves, which leaves 128 registers to a lane: the backward spills 13 to 648 of them to scratch, the forward 4 to
+// 246 from 40,961 columns on.
 // 24,000 x 1440 fp32 with the residual: forward 100 us, backward 121 + 5 us (4.9 TB/s of what they must move, as a large copy);
-// 100,000 x 2304 bf16 to 8 bits 359 us (4.5 TB/s); 21 x 864 3.2 us, the launch.
+// 100,000 x 2304 bf16 to 8 bits 359 us (4.5 TB/s), in 16 bits forward 382 us (4.8 TB/s), backward 644 us (2.9 TB/s); 21 x 864
+// 3.2 us, the launch. TB/s of long bf16 rows, forward / backward: 16,384 columns 4.6 / 1.7, 32,768 5.0 / 1.2, 65,536 3.0 / 0.5.
 #include "elem.h"
 
 namespace face {
@@ -235,7 +238,9 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restric
     if (ry == 0 && c < F) out[c] = from_f<T>(sums[0][cx]);
 }
 
-// Workgroups of the backward: four per CU keep enough rows in flight, and each adds a row of partial sums.
+// Workgroups of the backward, each of which adds a row of partial sums. 1024 are four per CU, of which the registers let four
+// run at once at 1 and 2 units of 64 lanes, three at 3 (141 registers in fp32), two at 4 and 5, one from 257 registers on: the others
+// follow in a second round.
 constexpr int64_t kNormBwdGroups = 1024;
 static inline int64_t norm_bwd_grid(int64_t N, int F) {
     const RowShape sh = row_shape(F);

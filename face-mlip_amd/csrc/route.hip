@@ -8,8 +8,8 @@
 // The zeros are written as such: a product would make NaN of them in a row whose sum is not finite.
 // A group of 16 lanes holds a row in registers (64 lanes from 257 experts on) and finds each maximum with
 // cross-lane moves on the VALU: 64 experts and k = 4 are 32 such steps and no trip through LDS. Bound by the
-// row's latency where there are few, by these steps else: 100,000 rows x 64 experts, k = 4, masked 15 us (28 MB: 6 us
-// of bytes), the gradient 19 us (55 MB: 11 us), without mask and renormalised 12 and 10 us.
+// row's latency where there are few, by these steps else: 100,000 rows x 64 experts, k = 4, masked 16 us (28 MB: 6 us
+// of bytes), the gradient 18 us (55 MB: 11 us), without mask and renormalised 12 and 10 us.
 #include "elem.h"
 
 namespace face {

@@ -1,7 +1,8 @@
 """Operators of an expert layer over atoms: layers whose weights depend on the atom.
 
 The readout of a FACE model is a norm, linear layers and a residual, the same weights for every
-atom. Here the weights are chosen per atom, by its species or by a learned gate:
+atom. Here the weights are chosen per atom, by its species or by a learned gate (for models built of these
+operators: the FACE model itself calls none of them):
 
     y, s = rms_norm(x, w, eps, residual=r)                s = x + r and its normalised rows
     expert, weight = route(gate, k)                        the k experts of every atom (or its species)
@@ -430,7 +431,8 @@ def grouped_linear(x, w, plan, bias=None, x_op=None):
     x (plan.rows, k), each row multiplied by the weights of all its choices, or (plan.slots, k), a row per
     slot; w (G, n, k), bias (G, n); x_op "silu" applies SiLU to x as it loads. float32 rows: products as of
     exact three-way bfloat16 splits (float32 accuracy); 16-bit rows: one product each, op(x) rounded to the
-    rows' type. Differentiable in x, w and bias; gradients are bitwise reproducible."""
+    rows' type, sums in float32 (over a shared row's choices too). Differentiable in x, w and bias; gradients are
+    bitwise reproducible."""
     code_op = _X_OPS.get(x_op)
     if code_op is None:
         _fail("grouped_linear", f"x_op None or 'silu', got {x_op!r}")
@@ -446,7 +448,8 @@ def grouped_linear(x, w, plan, bias=None, x_op=None):
 def grouped_linear_q8(x, x_scale, w, w_scale, plan, bias=None, dtype=torch.bfloat16):
     """grouped_linear of 8-bit operands, for serving: x float8_e4m3fn with x_scale (rows of x,), w (G, n, k)
     float8_e4m3fn with w_scale (G, n), as rms_norm_q8 and quantize_rows make them; y[a] = x_scale w_scale
-    sum_k(x w) + bias, in `dtype` (bias too). No gradients."""
+    sum_k(x w) + bias, in `dtype` (bias too). A float32 result sums the exact products, at half the rate; for 16-bit
+    results the matrix instruction cuts each of 64 neighbouring products below 2^-13 of the largest. No gradients."""
     name = "grouped_linear_q8"
     if x.dtype != _E4M3:
         _fail(name, f"float8_e4m3fn rows, got {x.dtype}")
