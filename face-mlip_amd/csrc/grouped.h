@@ -12,7 +12,7 @@
 // wave-wide prefix sum of the groups' tile counts, so no launch waits for a count on the host. The grid holds the most
 // tiles that so many slots and groups can make; what is left over ends at once. Both operands go through
 // LDS in chunks along the sum, the next chunk's loads in registers during the present one's products:
-//   * 16-bit rows as they are, on v_mfma_f32_32x32x16; e4m3 rows on v_mfma_scale_f32_32x32x64_f8f6f4 at unit
+//   * 16-bit rows as they are, on v_mfma_f32_32x32x16, or through silu, in two limbs of their type and twice the products; e4m3 rows on v_mfma_scale_f32_32x32x64_f8f6f4 at unit
 //     scales (twice the bf16 rate; fp32 results: see e4m3_wide), their row and column scales applied to the sum;
 //   * fp32 rows as three bf16 limbs, split once as they are staged, six products each (common.h);
 //   * an operand whose sum runs along its rows is read 16 bytes a lane; one whose sum runs down its columns (the
@@ -25,8 +25,9 @@
 // waits (a second buffer per workgroup leaves room for fewer: 128 x 128 of bf16 543 -> 562 us, of e4m3 268 -> 342 us).
 // 200,000 slots of 100,000 x 2304 -> 512, eight groups: bf16 534 us (883 TFLOP/s; the library's product of one matrix 500),
 // e4m3 287 us (1.6 PFLOP/s), bf16 input gradient 799 us (590 TFLOP/s, 1.84 GB of fp32 rows written), then 461 us for the sum of
-// a row's slots; with a row per slot, in 16 bits, 625 us. 200,000 slots 512 -> 2304 in bf16 647 us, with SiLU on load 1226:
-// it keeps the rows from going to LDS directly and is formed again for each of 18 column tiles.
+// a row's slots; with a row per slot, in 16 bits, 625 us. 200,000 slots 512 -> 2304 in bf16 647 us, with SiLU on load 1570 (1230
+// in one limb, of sqrt 2 of the error): it keeps the rows from going to LDS directly and is formed again for each of 18 column
+// tiles.
 // 24,000 x 1440 -> 320 in fp32, three groups: 142 us (155 TFLOP/s of the 190 that six bf16 products allow), input
 // gradient 156 us. 21 rows x 192 -> 97 in fp32 6.1 us; two rows x 2048 -> 2048 in bf16 8.8 us, 16.8 MB of weights, by 128
 // workgroups on 256 CUs.
@@ -164,26 +165,16 @@ __device__ __forceinline__ Held<T> hold(const T* p, int left) {
     return h;
 }
 
-// silu in fp32; a 16-bit operand is rounded once more, as it enters the matrix cores.
-template <typename T>
-__device__ __forceinline__ void apply_silu(Held<T>& h) {
-    if constexpr (sizeof(T) == 4) {
-        v4f a = __builtin_bit_cast(v4f, h.a), b = __builtin_bit_cast(v4f, h.b);
+// silu of fp32 rows as they are held.
+__device__ __forceinline__ void apply_silu(Held<float>& h) {
+    v4f a = __builtin_bit_cast(v4f, h.a), b = __builtin_bit_cast(v4f, h.b);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            a[e] = silu(a[e]);
-            b[e] = silu(b[e]);
-        }
-        h.a = __builtin_bit_cast(v4u, a);
-        h.b = __builtin_bit_cast(v4u, b);
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float a, b;
-            unpack2<T>(h.a[e], a, b);
-            h.a[e] = pack2<T>(silu(a), silu(b));
-        }
+    for (int e = 0; e < 4; ++e) {
+        a[e] = silu(a[e]);
+        b[e] = silu(b[e]);
     }
+    h.a = __builtin_bit_cast(v4u, a);
+    h.b = __builtin_bit_cast(v4u, b);
 }
 
 // The planes of a held chunk.
@@ -203,13 +194,30 @@ __device__ __forceinline__ void planes(const Held<T>& h, v4u o[Operand<T>::kPlan
         o[0] = h.a;
     }
 }
-// The same to LDS, `plane` bytes apart.
-template <typename T>
+// The same to LDS, `plane` bytes apart. SILU, of 16-bit rows: silu in fp32 as two limbs of the rows' type, its rounding and what
+// that left over (0 of an infinity), so that the product is as of the fp32 value and not of one rounded once more.
+template <typename T, bool SILU = false>
 __device__ __forceinline__ void put(char* at, int plane, const Held<T>& h) {
-    v4u o[Operand<T>::kPlanes];
-    planes(h, o);
+    constexpr int P = SILU ? 2 : Operand<T>::kPlanes;
+    v4u o[P];
+    if constexpr (SILU) {
 #pragma unroll
-    for (int p = 0; p < Operand<T>::kPlanes; ++p) *reinterpret_cast<v4u*>(at + p * plane) = o[p];
+        for (int e = 0; e < 4; ++e) {
+            float a, b, ha, hb;
+            unpack2<T>(h.a[e], a, b);
+            a = silu(a);
+            b = silu(b);
+            o[0][e] = pack2<T>(a, b);
+            unpack2<T>(o[0][e], ha, hb);
+            a -= ha;
+            b -= hb;
+            o[1][e] = pack2<T>(a == a ? a : 0.f, b == b ? b : 0.f);
+        }
+    } else {
+        planes(h, o);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<v4u*>(at + p * plane) = o[p];
 }
 
 // ---------------------------------------------------------------- LDS tiles
@@ -268,10 +276,12 @@ template <typename T>
 constexpr int kStep = __is_same(T, e4m3) ? 64 : 16;              // elements of the sum per instruction
 
 // One step's operands: 8 (e4m3: 32, each half of the wave its own) neighbouring elements of a row per lane.
-template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT>
+// PA, PB: planes of the operands, one each, three each, or two of one of them.
+template <typename T, int PA, int PB, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT>
 struct Fragments {
-    static constexpr int P = Operand<T>::kPlanes, W = __is_same(T, e4m3) ? 2 : 1;
-    v4u a[P * W][MT], b[P * W][NT];
+    static constexpr int W = __is_same(T, e4m3) ? 2 : 1;
+    static_assert((PA == 3 && PB == 3) || PA * PB <= 2, "no other order of products is written");
+    v4u a[PA * W][MT], b[PB * W][NT];
 
     __device__ __forceinline__ void load(const char* ta, const char* tb, int m0, int n0, int k0, int lane) {
         if constexpr (__is_same(T, e4m3)) {
@@ -286,13 +296,15 @@ struct Fragments {
                     b[h][n] = *reinterpret_cast<const v4u*>(tb + Tile<RB, CB, false>::at(n0 + 32 * n + (lane & 31), c + h));
             }
         } else {
-            constexpr int PA = Tile<RA, CA, COLS_A>::kBytes, PB = Tile<RB, CB, COLS_B>::kBytes;
+            constexpr int kA = Tile<RA, CA, COLS_A>::kBytes, kB = Tile<RB, CB, COLS_B>::kBytes;
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
+            for (int p = 0; p < (PA > PB ? PA : PB); ++p) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) a[p][m] = fragment<RA, CA, COLS_A>(ta + p * PA, m0 + 32 * m, k0, lane);
+                for (int m = 0; m < MT; ++m)
+                    if (p < PA) a[p][m] = fragment<RA, CA, COLS_A>(ta + p * kA, m0 + 32 * m, k0, lane);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) b[p][n] = fragment<RB, CB, COLS_B>(tb + p * PB, n0 + 32 * n, k0, lane);
+                for (int n = 0; n < NT; ++n)
+                    if (p < PB) b[p][n] = fragment<RB, CB, COLS_B>(tb + p * kB, n0 + 32 * n, k0, lane);
             }
         }
     }
@@ -311,7 +323,7 @@ struct Fragments {
                 }
         } else {
             // limb products from the smallest up; of one instruction after another none waits for the one before
-            constexpr int kProducts = P == 3 ? 6 : 1;
+            constexpr int kProducts = PA == 3 ? 6 : PA * PB;
             constexpr int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};
 #pragma unroll
             for (int q = 0; q < kProducts; ++q)
@@ -319,15 +331,16 @@ struct Fragments {
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
-                        acc[m][n] = mfma16<T>(b[P == 3 ? pb[q] : 0][n], a[P == 3 ? pa[q] : 0][m], acc[m][n]);
+                        acc[m][n] = mfma16<T>(b[PA == 3 ? pb[q] : PB - 1 - q > 0 ? PB - 1 - q : 0][n],
+                                              a[PA == 3 ? pa[q] : PA - 1 - q > 0 ? PA - 1 - q : 0][m], acc[m][n]);
         }
     }
 };
 
-template <typename T, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT, int STEPS>
+template <typename T, int PA, int PB, int RA, int CA, bool COLS_A, int RB, int CB, bool COLS_B, int MT, int NT, int STEPS>
 __device__ __forceinline__ void chunk_products(const char* ta, const char* tb, int m0, int n0, int k_begin, int lane,
                                                v16f acc[MT][NT]) {
-    using F = Fragments<T, RA, CA, COLS_A, RB, CB, COLS_B, MT, NT>;
+    using F = Fragments<T, PA, PB, RA, CA, COLS_A, RB, CB, COLS_B, MT, NT>;
     if constexpr (MT * NT > 4) {
         // few waves per SIMD: the next step's operands are on their way during this one's products, and no more of
         // them (the barrier), or the accumulators would spill
@@ -415,16 +428,17 @@ __device__ __forceinline__ int64_t xcd_item(int64_t items) {
 
 // ---------------------------------------------------------------- forward and input gradient
 // WM x WN x WK waves of MT x NT tiles. COLS_B: the weights lie (sum, column), as the input gradient reads them.
-// DIRECT_A, DIRECT_B: the operand is staged without registers.
-template <typename T, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C>
+// DIRECT_A, DIRECT_B: the operand is staged without registers. SILU: 16-bit rows through silu, in two limbs.
+template <typename T, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool SILU>
 struct RowsKernel {
     using Op = Operand<T>;
-    static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, BK = C * Op::kElems, P = Op::kPlanes;
+    static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, BK = C * Op::kElems;
+    static constexpr int PA = SILU ? 2 : Op::kPlanes, PB = Op::kPlanes;
     static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
     static constexpr int CB = COLS_B ? BN / 8 : C, RB = COLS_B ? BK : BN;
     using TA = Tile<BM, C, false>;
     using TB = Tile<RB, CB, COLS_B>;
-    static constexpr int kLdsA = P * TA::kBytes, kLdsB = P * TB::kBytes;
+    static constexpr int kLdsA = PA * TA::kBytes, kLdsB = PB * TB::kBytes;
     // finished sums on their way out: 32 rows of a wave's columns at a time, rows four floats apart in the banks
     static constexpr int kOutLd = 32 * NT + 4, kOut = 32 * kOutLd * 4;
     static constexpr int kLds = kLdsA + kLdsB > kWaves * kOut ? kLdsA + kLdsB : kWaves * kOut;
@@ -510,7 +524,7 @@ __device__ __forceinline__ void finish(const GroupedArgs& g, int group, int32_t 
 template <int WK>
 __device__ __forceinline__ void few_rows(const float* x, const float* w, int k, int x_op, int wave, int lane, v16f acc[1][1]) {
     constexpr int N = 2, E = 8, kLine = 2 * N * E;
-    using F = Fragments<float, 32, 1, false, 32, 1, false, 1, 1>;
+    using F = Fragments<float, 3, 3, 32, 1, false, 32, 1, false, 1, 1>;
     const int half = N * E * (lane >> 5);
     struct Run {
         Held<float> a[N], b[N];
@@ -573,10 +587,11 @@ __device__ __forceinline__ void few_rows(const float* x, const float* w, int k, 
 }
 
 template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B,
-          bool FEW = false>
-__global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThreads), (DIRECT_A ? 4 : 2)) void
+          bool FEW = false, bool SILU = false>
+__global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C, SILU>::kThreads), (DIRECT_A ? 4 : 2)) void
     grouped_rows_kernel(GroupedArgs g) {
-    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
+    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C, SILU>;
+    static_assert(!SILU || (sizeof(T) == 2 && !DIRECT_A && !COLS_B), "rows of 16 bits, through registers");
     __shared__ __attribute__((aligned(256))) char lds[K::kLds];
     __shared__ int32_t slot_of[K::BM];
     const int64_t item = xcd_item(g.tiles * g.col_tiles);
@@ -672,13 +687,15 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
                 to_lds(decltype(whole)::value || a_col + k0 < g.k ? (const void*)(ap[i] + k0) : &kZeroChunk,
                        to + (i * K::kThreads + wave * 64) * 16);
         } else {
-            if (g.x_op) {
+            if constexpr (__is_same(T, float)) {
+                if (g.x_op) {
 #pragma unroll
-                for (int i = 0; i < K::NA; ++i) apply_silu(ha[i]);
+                    for (int i = 0; i < K::NA; ++i) apply_silu(ha[i]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < K::NA; ++i)
-                put(to + K::TA::at(tid / C + i * (K::kThreads / C), tid % C), K::TA::kBytes, ha[i]);
+                put<T, SILU>(to + K::TA::at(tid / C + i * (K::kThreads / C), tid % C), K::TA::kBytes, ha[i]);
         }
     };
     auto stage_b = [&](int k0, char* to, auto whole) {
@@ -715,7 +732,7 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
             __syncthreads();
             fetch(k0 + K::BK);
             before_products<T>();
-            chunk_products<T, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
+            chunk_products<T, K::PA, K::PB, K::BM, C, false, K::RB, K::CB, COLS_B, MT, NT, K::BK / WK / kStep<T>>(
                 lds, lds + K::kLdsA, 32 * MT * wm, 32 * NT * wn, wk * (K::BK / WK), lane, acc);
             after_products<T>();
             __syncthreads();
@@ -807,19 +824,21 @@ __global__ __launch_bounds__((RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>::kThr
 // slots on their way during the present ones' products. It spills 46 registers, the 128 x 128 tile staged so 25 to 27: places of
 // the results, stored before the loop over the groups and read where the results are, none in the loop over the slots.
 // The tile's padding is multiplied too: 1440 x 320 becomes 1536 x 384, 28 % more.
-template <typename T, int TILE>
+// SILU: x through silu, in two limbs.
+template <typename T, int TILE, bool SILU>
 struct WeightKernel {
     using Op = Operand<T>;
-    static constexpr int P = Op::kPlanes, BK = P == 3 ? 32 : 64, CT = TILE / 8;
+    static constexpr int P = Op::kPlanes, PX = SILU ? 2 : P, BK = P == 3 ? 32 : 64, CT = TILE / 8;
     static constexpr int WM = 2, WN = TILE / 64, MT = TILE / 64, NT = 2, kThreads = 64 * WM * WN;
     using TT = Tile<BK, CT, true>;
-    static constexpr int kLds = 2 * P * TT::kBytes, NC = BK * CT / kThreads;
+    static constexpr int kLds = (P + PX) * TT::kBytes, NC = BK * CT / kThreads;
 };
 
-template <typename T, bool DIRECT, int TILE>
-__global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE == 128 ? 4 : 2)) void grouped_weight_kernel(
+template <typename T, bool DIRECT, int TILE, bool SILU>
+__global__ __launch_bounds__((WeightKernel<T, TILE, SILU>::kThreads), (DIRECT && TILE == 128 ? 4 : 2)) void grouped_weight_kernel(
     GroupedWArgs g) {
-    using K = WeightKernel<T, TILE>;
+    using K = WeightKernel<T, TILE, SILU>;
+    static_assert(!SILU || (sizeof(T) == 2 && !DIRECT), "rows of 16 bits, through registers");
     constexpr bool kTwo = TILE == 256;
     static_assert(DIRECT || !kTwo, "two buffers are filled without registers");
     // two arrays, not one of twice the size: reads of one need not wait for what is on its way into the other
@@ -934,7 +953,7 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
                     add_columns(v, v);
                 }
             }
-            chunk_products<T, K::BK, K::CT, true, K::BK, K::CT, true, K::MT, K::NT, K::BK / 16>(
+            chunk_products<T, K::P, K::PX, K::BK, K::CT, true, K::BK, K::CT, true, K::MT, K::NT, K::BK / 16>(
                 from, from + kB, 32 * K::MT * wm, 32 * K::NT * wn, 0, lane, acc);
         };
         find(0);
@@ -964,9 +983,11 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
                     stage(p, lds);
                     find(p + K::BK);
                 } else {
-                    if (g.x_op) {
+                    if constexpr (__is_same(T, float)) {
+                        if (g.x_op) {
 #pragma unroll
-                        for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+                            for (int i = 0; i < K::NC; ++i) apply_silu(hb[i]);
+                        }
                     }
                     if (sums) {
 #pragma unroll
@@ -979,7 +1000,7 @@ __global__ __launch_bounds__((WeightKernel<T, TILE>::kThreads), (DIRECT && TILE 
                     for (int i = 0; i < K::NC; ++i) {
                         const int at = K::TT::at(row_t + i * (K::kThreads / K::CT), chunk);
                         put(lds + at, K::TT::kBytes, ha[i]);
-                        put(lds + kB + at, K::TT::kBytes, hb[i]);
+                        put<T, SILU>(lds + kB + at, K::TT::kBytes, hb[i]);
                     }
                 }
                 __syncthreads();
@@ -1099,15 +1120,15 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedWArgs g) {
 // ---------------------------------------------------------------- launches
 // Instantiated per element type in a file of its own (grouped_f32.hip, ...).
 template <typename T, typename Out, bool COLS_B, int WM, int WN, int WK, int MT, int NT, int C, bool DIRECT_A, bool DIRECT_B,
-          bool FEW = false>
+          bool FEW = false, bool SILU = false>
 static int launch_rows_shape(GroupedArgs g, hipStream_t st) {
-    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C>;
+    using K = RowsKernel<T, COLS_B, WM, WN, WK, MT, NT, C, SILU>;
     const int64_t most = g.groups + (int64_t)1;
     g.tiles = g.slots / K::BM + (most < g.slots ? most : g.slots);
     g.col_tiles = (g.n + K::BN - 1) / K::BN;
     const int64_t grid = g.tiles * g.col_tiles;
     if (grid > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B, FEW>),
+    hipLaunchKernelGGL((grouped_rows_kernel<T, Out, COLS_B, WM, WN, WK, MT, NT, C, DIRECT_A, DIRECT_B, FEW, SILU>),
                        dim3((unsigned)grid), dim3(K::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     return 0;
@@ -1124,9 +1145,14 @@ template <typename T, typename Out, bool COLS_B, int MT, int NT>
 static int launch_rows_large(GroupedArgs g, hipStream_t st) {
     constexpr int C = sizeof(T) == 4 ? 4 : 8;
     if constexpr (sizeof(T) < 4 && !__is_same(T, e4m3_wide)) {
-        const bool a = whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op;
+        const bool a = whole_chunks<T>(g.x, g.ld_x, g.k);
         const bool b = whole_chunks<T>(g.w, g.ld_w, COLS_B ? g.n : g.k) && g.w_group % (16 / (int)sizeof(T)) == 0 &&
                        (COLS_B ? 64 : (int64_t)g.n) * g.ld_w * (int64_t)sizeof(T) < ((int64_t)1 << 31);
+        if constexpr (sizeof(T) == 2 && !COLS_B) {
+            if (g.x_op)
+                return b ? launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, false, true, false, true>(g, st)
+                         : launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, false, false, false, true>(g, st);
+        }
         if (a && b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, true, true>(g, st);
         if (b) return launch_rows_shape<T, Out, COLS_B, 2, 2, 1, MT, NT, C, false, true>(g, st);
     }
@@ -1180,6 +1206,8 @@ int launch_rows(GroupedArgs g, hipStream_t st) {
             if constexpr (sizeof(T) == 4 && !COLS_B)
                 if (expected_tiles(g.slots, g.groups, g.n, 32, 32) <= device_cu_count())
                     return launch_rows_shape<T, Out, COLS_B, 1, 1, 8, 1, 1, 16, false, false, true>(g, st);
+            if constexpr (sizeof(T) == 2 && !COLS_B)
+                if (g.x_op) return launch_rows_shape<T, Out, COLS_B, 1, 1, 8, 1, 1, 32, false, false, false, true>(g, st);
             return launch_rows_shape<T, Out, COLS_B, 1, 1, 8, 1, 1, (sizeof(T) == 4 ? 16 : 32), false, false>(g, st);
         case 1: return launch_rows_large<T, Out, COLS_B, 1, 1>(g, st);
         case 2: return launch_rows_large<T, Out, COLS_B, 2, 1>(g, st);
@@ -1206,8 +1234,9 @@ static inline bool weight_large(int64_t slots, int n, int k) {
 //         24,000 in three 512 x 512 56 / 50, 100,000 in eight 1440 x 320 200 / 208, 97 x 96 46 / 50
 //   fp32: 800 in three 2304 x 512 53 / 30, in one 192 x 97 30 / 24, 8,000 in 32 864 x 192 65 / 58, 100,000 in eight 192 x 97
 //         67 / 71; the same within 1 % from 24,000 slots of 1440 x 320 on
-// 16-bit rows staged through registers take 195 of them, two workgroups per CU; shares for three / for two (us): 200,000 slots in
-// eight 2304 x 512 1650 / 1452, 100,000 512 x 512 198 / 168, 1440 x 320 411 / 368, 513 x 97 111 / 89, 321 x 1440 420 / 433.
+// 16-bit rows staged through registers take 195 of them, two workgroups per CU; shares for three / for two (us, SiLU on load in
+// one limb): 200,000 slots in eight 2304 x 512 1650 / 1452, 100,000 512 x 512 198 / 168, 1440 x 320 411 / 368; without SiLU
+// 513 x 97 111 / 89, 321 x 1440 420 / 433.
 static inline int weight_shares(int64_t slots, int groups, int n, int k, int dtype, bool large, bool direct) {
     const int tile = large ? 256 : 128;
     const double tiles = (double)((n + tile - 1) / tile) * ((k + tile - 1) / tile);
@@ -1219,7 +1248,7 @@ static inline int weight_shares(int64_t slots, int groups, int n, int k, int dty
     return slots <= 512 || s < 2 || (groups > 1 ? all / 2 : all) <= all / s + s * join + 9 ? 1 : (int)s;
 }
 
-template <typename T, bool DIRECT, int TILE>
+template <typename T, bool DIRECT, int TILE, bool SILU = false>
 static int launch_weight_tile(GroupedWArgs g, hipStream_t st) {
     g.shares = weight_shares(g.slots, g.groups, g.n, g.k, sizeof(T) == 4 ? FACE_F32 : FACE_BF16, TILE == 256, DIRECT);
     g.share = (g.slots + g.shares - 1) / g.shares;
@@ -1232,8 +1261,8 @@ static int launch_weight_tile(GroupedWArgs g, hipStream_t st) {
     while (((int64_t)1 << s) < g.xdiv) ++s;
     g.div_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + g.xdiv - 1) / g.xdiv);
     g.div_shift = 31 + s;
-    hipLaunchKernelGGL((grouped_weight_kernel<T, DIRECT, TILE>), dim3((unsigned)grid),
-                       dim3(WeightKernel<T, TILE>::kThreads), 0, st, g);
+    hipLaunchKernelGGL((grouped_weight_kernel<T, DIRECT, TILE, SILU>), dim3((unsigned)grid),
+                       dim3(WeightKernel<T, TILE, SILU>::kThreads), 0, st, g);
     FACE_LAUNCH_CHECK();
     if (g.shares > 1) {
         const int64_t blocks = ((int64_t)g.n * g.k + 1023) / 1024;
@@ -1247,7 +1276,8 @@ static int launch_weight_tile(GroupedWArgs g, hipStream_t st) {
 template <typename T>
 int launch_weight(GroupedWArgs g, hipStream_t st) {
     if constexpr (sizeof(T) < 4) {
-        if (whole_chunks<T>(g.x, g.ld_x, g.k) && !g.x_op && whole_chunks<T>(g.dy, g.ld_dy, g.n) &&
+        if (g.x_op) return launch_weight_tile<T, false, 128, true>(g, st);
+        if (whole_chunks<T>(g.x, g.ld_x, g.k) && whole_chunks<T>(g.dy, g.ld_dy, g.n) &&
             g.ld_x < ((int64_t)1 << 30) && g.ld_dy < ((int64_t)1 << 30))
             return weight_large(g.slots, g.n, g.k) ? launch_weight_tile<T, true, 256>(g, st)
                                                    : launch_weight_tile<T, true, 128>(g, st);

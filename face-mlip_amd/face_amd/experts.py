@@ -430,8 +430,8 @@ def grouped_linear(x, w, plan, bias=None, x_op=None):
 
     x (plan.rows, k), each row multiplied by the weights of all its choices, or (plan.slots, k), a row per
     slot; w (G, n, k), bias (G, n); x_op "silu" applies SiLU to x as it loads. float32 rows: products as of
-    exact three-way bfloat16 splits (float32 accuracy); 16-bit rows: one product each, op(x) rounded to the
-    rows' type, sums in float32 (over a shared row's choices too). Differentiable in x, w and bias; gradients are
+    exact three-way bfloat16 splits (float32 accuracy); 16-bit rows: one product each, or with SiLU two, of its
+    rounding to the rows' type and of the rest; sums in float32 (over a shared row's choices too). Differentiable in x, w and bias; gradients are
     bitwise reproducible."""
     code_op = _X_OPS.get(x_op)
     if code_op is None:

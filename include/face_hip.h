@@ -593,7 +593,7 @@ int face_group_plan(const int32_t* expert, int64_t slots, int32_t G, int32_t* pt
 /* y[a] (slots, n) = op(x[a / x_div]) W[g]^T + bias[g] for the slots a of group g of a plan, 0 for those of no group.
  * x has ceil(slots / x_div) rows of k; w (G, n, k) with strides w_group, ld_w; bias (G, n) with row stride ld_b, or
  * NULL; x_op 0 none, 1 silu. fp32 products are six bf16 products of three-way splits (as face_rows_linear),
- * 16-bit ones bf16 or fp16 products, sums in fp32. G <= 65535. */
+ * 16-bit ones bf16 or fp16 products (with silu two: of its rounding and of the rest), sums in fp32. G <= 65535. */
 int face_grouped_linear(const void* x, int64_t ld_x, int32_t x_div, int32_t x_op, const void* w, int64_t ld_w,
                         int64_t w_group, const void* bias, int64_t ld_b, const int32_t* ptr, const int32_t* order,
                         int64_t slots, int32_t G, int32_t n, int32_t k, int32_t dtype, void* y, int64_t ld_y, void* stream);

@@ -665,6 +665,34 @@ def test_large_tiles(dtype, N, G, ki, n):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,k,G,ki,n", [(1, 1, 1, 1, 1), (21, 2, 3, 192, 97), (40, 1, 3, 2048, 300), (700, 1, 3, 1440, 320),
+                                        (3000, 2, 4, 257, 65)] + [(N, 1, G, ki, n) for N, G, ki, n in LARGE])
+def test_silu_on_load_adds_no_rounding(dtype, N, k, G, ki, n):
+    """silu of 16-bit rows enters the products in two limbs, h = T(s) and T(s - h): off by u^2 of it (2^-16, 2^-22), and in
+    float16, whose values are 2^-24 apart at the least, by 2^-25 whatever its size. One limb would be off by u."""
+    say("two limbs", dtype, N, k, ki, n)
+    g = gen(N + ki)
+    e = torch.randint(-1, G, (N, k), generator=g, device=DEV, dtype=torch.int32)
+    plan = ex.group_plan(e, G)
+    x, w = rand(g, N * k, ki, dtype=dtype), rand(g, G, n, ki, dtype=dtype, scale=ki ** -0.5)
+    dy = rand(g, N * k, n, dtype=dtype)
+    y64, ay, _, _, dw64, adw, _, adb = linear64(x, w, e, None, True, dy)
+    w.requires_grad_(True)
+    y = ex.grouped_linear(x, w, plan, x_op="silu")
+    dw, = torch.autograd.grad(y, w, dy)
+    pre = 4 * U32 + u(dtype) ** 2
+    tiny = 2.0 ** -25 if dtype == F16 else 0.0
+    sums = torch.cat([w.detach().double().abs().sum(2), torch.zeros(1, n, device=DEV).double()])
+    rows = sums[torch.where(e < 0, G, e).reshape(-1).long()]
+    near(y, y64, (steps(dtype, 2 * ki) + pre) * ay + tiny * rows, "y")
+    near(dw, dw64, (steps(dtype, 2 * N * k) + pre) * adw + tiny * adb[:, :, None], "dw")
+    if min(ki, n) > 90 and N > 20:
+        # the norm of the error: that of the result's rounding, uniform within a step, u / sqrt 3 of a value at the most
+        for got, want in ((y, y64), (dw, dw64)):
+            assert (got.double() - want).norm() <= 1.02 * (want.to(dtype).double() - want).norm()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 def test_products_of_many_slots(dtype):
     """The forward and the input gradient of a hundred thousand slots, one row each and two of a row."""
     N, G, ki, n = 100300, 6, 1544, 656
