@@ -23,7 +23,7 @@ SOURCES = {"capi.hip": "fast", "density.hip": "fast", "cprad.hip": "fast", "dens
            "edge.hip": "fast", "graph.hip": "off",
            "transport.hip": "fast", "radial.hip": "fast", "linear.hip": "fast",
            "gemm.hip": "fast", "gemm_xs.hip": "fast", "gemm_split.hip": "fast", "gemm_op.hip": "fast", "densmix.hip": "fast",
-           "norm.hip": "fast", "route.hip": "fast", "grouped.hip": "fast", "grouped_f32.hip": "fast",
+           "norm.hip": "fast", "lnorm.hip": "fast", "kept.hip": "fast", "embed.hip": "fast", "sorted.hip": "fast", "route.hip": "fast", "grouped.hip": "fast", "grouped_f32.hip": "fast",
            "grouped_bf16.hip": "fast", "grouped_f16.hip": "fast", "grouped_e4m3.hip": "fast"}
 
 
@@ -43,7 +43,7 @@ def stale(src):
         return True
     t = os.path.getmtime(obj)
     return any(os.path.getmtime(os.path.join(HERE, f)) > t
-               for f in (src, "common.h", "edges.h", "densfac.h", "rows_gemm.h", "elem.h", "grouped.h", "../../include/face_hip.h"))
+               for f in (src, "common.h", "edges.h", "densfac.h", "rows_gemm.h", "elem.h", "kept.h", "grouped.h", "../../include/face_hip.h"))
 
 
 def build(jobs=None, verbose=False, changed_only=False):

@@ -1,0 +1,173 @@
+// Rows kept in 8 bits: e4m3 with a power of two for each 32 neighbouring columns of a row.
+//
+//   e = the least with max|x| <= 448 2^e over the block's finite values (2^e >= 2^-126),  q = e4m3(x 2^-e)
+//
+// The scale is a byte, e + 127, which is a float's exponent field: x 2^-e and q 2^e are exact, so what a value is
+// kept as hangs on no order of operations, and the rounding to e4m3 (to nearest, ties to even, half a step 2^-4) is the only
+// one. It may pass a type's largest value by half a step: what it stands for is cut to that. A NaN or an infinity is kept as NaN
+// and leaves the others of its block as they are. A block's 32 columns lie in a quad
+// of lanes, a piece each: its maximum is two cross-lane moves.
+#pragma once
+#include "elem.h"
+
+namespace face {
+
+constexpr int kKeptBlock = 32;
+static __host__ __device__ __forceinline__ int64_t kept_blocks(int64_t F) { return (F + kKeptBlock - 1) / kKeptBlock; }
+
+// The scale's byte of the quad's 32 values (zeros beyond the row's end). All lanes of a quad are active.
+__device__ __forceinline__ uint32_t kept_scale(const float x[kPiece]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+        const uint32_t m = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu;
+        top = m < 0x7f800000u && m > top ? m : top;
+    }
+    const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false);   // lane ^ 1
+    top = a > top ? a : top;
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false);   // lane ^ 2
+    top = b > top ? b : top;
+    const int s = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);     // 448 = 1.75 2^8
+    return (uint32_t)(s < 1 ? 1 : s);
+}
+
+// Eight values times `inv` in e4m3. The instruction turns what rounds past 448 (infinities) into NaN.
+__device__ __forceinline__ void store_e4m3(uint8_t* p, int left, const float x[kPiece], float inv) {
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, lo, true);
+    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * inv, x[5] * inv, 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * inv, x[7] * inv, hi, true);
+    if (left >= kPiece) {
+        typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
+        *reinterpret_cast<v2i_any*>(p) = (v2i_any){lo, hi};
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e)
+            if (e < left) p[e] = (uint8_t)((uint32_t)(e < 4 ? lo : hi) >> (8 * (e & 3)));
+    }
+}
+
+// Piece c / 8 of a row: its eight bytes at q + c, and its block's scale, written by the first lane of the quad.
+__device__ __forceinline__ void store_kept(uint8_t* q, uint8_t* scale, int c, int F, const float x[kPiece]) {
+    const uint32_t s = kept_scale(x);
+    store_e4m3(q + c, F - c, x, __builtin_bit_cast(float, (254u - s) << 23));
+    if ((c & (kKeptBlock - 1)) == 0 && c < F) scale[c / kKeptBlock] = (uint8_t)s;
+}
+
+// v within [-top, top]; a NaN stays one.
+__device__ __forceinline__ float within(float v, float top) { return v > top ? top : (v < -top ? -top : v); }
+
+// A kept piece on its way: its bytes and its scale.
+struct KeptPiece {
+    uint32_t lo, hi, scale;
+};
+__device__ __forceinline__ KeptPiece hold_kept(const uint8_t* q, const uint8_t* scale, int c, int F) {
+    KeptPiece k = {0, 0, 0};
+    if (c + kPiece <= F) {
+        typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(1)));
+        const v2u_any v = *reinterpret_cast<const v2u_any*>(q + c);
+        k.lo = v[0];
+        k.hi = v[1];
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e)
+            if (c + e < F) (e < 4 ? k.lo : k.hi) |= (uint32_t)q[c + e] << (8 * (e & 3));
+    }
+    if (c < F) k.scale = scale[c / kKeptBlock];
+    return k;
+}
+// Its values; zeros beyond the row's end. Of the bytes that store_kept does not write, 0 stands for 2^-127 and 255 for NaN.
+__device__ __forceinline__ void kept_values(const KeptPiece& k, float x[kPiece]) {
+    const float s = __builtin_bit_cast(float, k.scale - 1 < 254u ? k.scale << 23 : (k.scale ? 0x7fc00000u : 0x00400000u));
+    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, true);
+    const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, true);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        x[e] = a[e] * s;
+        x[2 + e] = b[e] * s;
+        x[4 + e] = c[e] * s;
+        x[6 + e] = d[e] * s;
+    }
+    if (k.scale >= 247u) {                       // 256 2^120: what the largest floats round to
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) x[e] = within(x[e], 0x1.fffffep127f);
+    }
+}
+
+// A piece of a row in its memory's type, on its way: half the registers of its values where they are 16-bit.
+template <typename T>
+struct RawPiece {
+    v4u a[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ RawPiece<T> hold_raw(const T* p, int left) {
+    RawPiece<T> r = {};
+    if (left >= kPiece) {
+        r.a[0] = ld16(p);
+        if constexpr (sizeof(T) == 4) r.a[1] = ld16(p + 4);
+    } else if (left > 0) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e)
+                if (e < left) r.a[e >> 2][e & 3] = __builtin_bit_cast(uint32_t, p[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e)
+                if (e < left) r.a[0][e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void raw_values(const RawPiece<T>& r, float x[kPiece]) {
+    if constexpr (sizeof(T) == 4) {
+        const v4f a = __builtin_bit_cast(v4f, r.a[0]), b = __builtin_bit_cast(v4f, r.a[1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = a[e];
+            x[4 + e] = b[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpack2<T>(r.a[0][e], x[2 * e], x[2 * e + 1]);
+    }
+}
+
+// Sum over a wave in a fixed order, the same in every lane, without a trip through LDS.
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row16_sum(v);
+    const int i = __builtin_bit_cast(int, v);
+    const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0));
+    const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16));
+    const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32));
+    const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
+    return (a + b) + (c + d);
+}
+// Sums of two values over the LANES threads of a row (row_sum of elem.h for two). `part`: LDS, LANES / 32 floats.
+template <int LANES>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* part) {
+    if constexpr (LANES == 16) {
+        a = row16_sum(a);
+        b = row16_sum(b);
+        return;
+    }
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (LANES > 64) {
+        constexpr int W = LANES / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            part[threadIdx.x >> 6] = a;
+            part[W + (threadIdx.x >> 6)] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            a += part[i];
+            b += part[W + i];
+        }
+    }
+}
+
+}  // namespace face

@@ -1,0 +1,202 @@
+// Rows to 8 bits and back (kept.h), and the gated activation whose backward reads its inputs in 8 bits:
+//
+//   y = silu(a) b,  a = x[:F], b = x[F:]
+//   da = dy b silu'(a),  db = dy silu(a);   kept: of a and b as 8 bits hold them, each half in blocks of its own
+//
+// A row's pieces are spread over a power of two of threads; a block's four pieces lie in a quad of lanes. Bound by bytes.
+#include "kept.h"
+
+namespace face {
+
+// Threads per row (a power of two, whole quads): about four pieces each.
+static inline int kept_lanes_log2(int64_t F) {
+    const int64_t p = 4 * kept_blocks(F);
+    int lg = 2;
+    while (lg < 8 && ((int64_t)4 << lg) < p) ++lg;
+    return lg;
+}
+
+struct RowAt {
+    int64_t n;
+    int lane, lanes;
+};
+__device__ __forceinline__ RowAt row_at(int lg) {
+    return {(int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg), (int)threadIdx.x & ((1 << lg) - 1), 1 << lg};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
+                                                   uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+    const RowAt r = row_at(lg);
+    if (r.n >= N) return;
+    const int end = kKeptBlock * (int)kept_blocks(F);                    // whole quads
+    x += r.n * ld;
+    q += r.n * F;
+    scale += r.n * kept_blocks(F);
+    for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
+        float v[kPiece];
+        load_piece(x + c, F - c, v);
+        store_kept(q, scale, c, F, v);
+    }
+}
+
+// The type's largest value.
+template <typename T>
+constexpr float kLargest = __is_same(T, f16) ? 65504.f : (__is_same(T, bf16) ? 0x1.fep127f : 0x1.fffffep127f);
+
+template <typename T>
+__global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__ q, int64_t ld_q,
+                                                     const uint8_t* __restrict__ scale, int64_t ld_s, int64_t N, int F, int lg,
+                                                     T* __restrict__ x) {
+    const RowAt r = row_at(lg);
+    if (r.n >= N) return;
+    q += r.n * ld_q;
+    scale += r.n * ld_s;
+    x += r.n * F;
+#pragma unroll 4
+    for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
+        float v[kPiece];
+        kept_values(hold_kept(q, scale, c, F), v);
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) v[e] = within(v[e], kLargest<T>);
+        store_piece(x + c, F - c, v);
+    }
+}
+
+// q (N, 2 F) and scale (N, 2, blocks of F), or null.
+template <typename T, bool KEEP>
+__global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
+                                                        T* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+    const RowAt r = row_at(lg);
+    if (r.n >= N) return;
+    const int blocks = (int)kept_blocks(F), end = KEEP ? kKeptBlock * blocks : F;
+    x += r.n * ld;
+    y += r.n * F;
+    q += r.n * 2 * F;
+    scale += r.n * 2 * blocks;
+    for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
+        float a[kPiece], b[kPiece];
+        load_piece(x + c, F - c, a);
+        load_piece(x + F + c, F - c, b);
+        if constexpr (KEEP) {
+            store_kept(q, scale, c, F, a);
+            store_kept(q + F, scale + blocks, c, F, b);
+        }
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) a[e] = silu(a[e]) * b[e];
+        store_piece(y + c, F - c, a);
+    }
+}
+
+template <typename T, bool KEPT>
+__global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x, int64_t ld, const uint8_t* __restrict__ q,
+                                                        const uint8_t* __restrict__ scale, const T* __restrict__ dy,
+                                                        int64_t ld_dy, int64_t N, int F, int lg, T* __restrict__ dx) {
+    const RowAt r = row_at(lg);
+    if (r.n >= N) return;
+    const int blocks = (int)kept_blocks(F);
+    x += r.n * ld;
+    q += r.n * 2 * F;
+    scale += r.n * 2 * blocks;
+    dy += r.n * ld_dy;
+    dx += r.n * 2 * F;
+#pragma unroll 2
+    for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
+        float a[kPiece], b[kPiece], d[kPiece];
+        load_piece(dy + c, F - c, d);
+        if constexpr (KEPT) {
+            kept_values(hold_kept(q, scale, c, F), a);
+            kept_values(hold_kept(q + F, scale + blocks, c, F), b);
+        } else {
+            load_piece(x + c, F - c, a);
+            load_piece(x + F + c, F - c, b);
+        }
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) {
+            const float t = a[e];
+            a[e] = d[e] * b[e] * silu_slope(t);
+            b[e] = d[e] * silu(t);
+        }
+        store_piece(dx + c, F - c, a);
+        store_piece(dx + F + c, F - c, b);
+    }
+}
+
+constexpr int32_t kKeptMax = 1 << 28;            // longest row
+static int kept_args(int64_t N, int32_t F, int32_t dtype) {
+    if (N < 0 || F <= 0) return FACE_ERR_ARG;
+    if (dtype != FACE_F32 && dtype != FACE_BF16 && dtype != FACE_F16) return FACE_ERR_ARG;
+    if (F > kKeptMax || N > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    return 0;
+}
+static dim3 kept_grid(int64_t N, int lg) { return dim3((unsigned)((N + (256 >> lg) - 1) >> (8 - lg))); }
+
+}  // namespace face
+
+using namespace face;
+
+extern "C" int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_t dtype, void* q, void* scale,
+                              void* stream) {
+    if (int rc = kept_args(N, F, dtype)) return rc;
+    if (ld_x < F) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!x || !q || !scale) return FACE_ERR_ARG;
+    const int lg = kept_lanes_log2(F);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(pack_kernel<T>, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
+                           (uint8_t*)q, (uint8_t*)scale);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
+extern "C" int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, int64_t ld_s, int64_t N, int32_t F,
+                                int32_t dtype, void* x, void* stream) {
+    if (int rc = kept_args(N, F, dtype)) return rc;
+    if (ld_q < F || ld_s < kept_blocks(F)) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!x || !q || !scale) return FACE_ERR_ARG;
+    const int lg = kept_lanes_log2(F);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(unpack_kernel<T>, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
+                           (const uint8_t*)scale, ld_s, N, F, lg, (T*)x);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
+extern "C" int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_t dtype, void* y, void* q,
+                                   void* scale, void* stream) {
+    if (int rc = kept_args(N, F, dtype)) return rc;
+    if (ld_x < 2 * (int64_t)F || !q != !scale) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!x || !y) return FACE_ERR_ARG;
+    const int lg = kept_lanes_log2(F);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto* kern = q ? gated_fwd_kernel<T, true> : gated_fwd_kernel<T, false>;
+        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg, (T*)y,
+                           (uint8_t*)q, (uint8_t*)scale);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
+extern "C" int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, const void* scale, const void* dy,
+                                   int64_t ld_dy, int64_t N, int32_t F, int32_t dtype, void* dx, void* stream) {
+    if (int rc = kept_args(N, F, dtype)) return rc;
+    if ((x && ld_x < 2 * (int64_t)F) || ld_dy < F) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if ((x ? q || scale : !q || !scale) || !dy || !dx) return FACE_ERR_ARG;
+    const int lg = kept_lanes_log2(F);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto* kern = q ? gated_bwd_kernel<T, true> : gated_bwd_kernel<T, false>;
+        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, (const uint8_t*)q,
+                           (const uint8_t*)scale, (const T*)dy, ld_dy, N, F, lg, (T*)dx);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}

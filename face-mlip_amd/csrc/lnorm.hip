@@ -1,0 +1,550 @@
+// Layer norm of atom rows with the residual's addition, its backward with the gradients of weight and bias, rows
+// in 8 bits for serving, and normalised rows kept in 8 bits for the backward:
+//
+//   s = x + r (rounded to the rows' type, as the residual stream holds it)
+//   h = (s - mean s) rstd,  rstd = 1 / sqrt(mean((s - mean s)^2) + eps),  y = h w + b
+//   ds = rstd (g - mean g - h mean(g h)) + ds_in,  g = dy w;   dw = sum over rows of dy h,  db = sum of dy
+//
+// Everything between the first read of a row and its last store is fp32 in registers up to 16384 columns: the mean
+// first, then the squares around it, and with them the sum of the differences, which corrects the mean's own rounding.
+// Longer rows are read three times by a workgroup of 1024. The backward takes mean and rstd (8 bytes a row) from the
+// forward, so that its one reduction follows its only reads. Bound by bytes.
+#include "kept.h"
+
+namespace face {
+
+enum { kLn = 0, kLnQ8 = 1, kLnKept = 2 };
+
+struct LnFwdArgs {
+    const void *x, *r;
+    int64_t ld_x, ld_r, N;
+    int F;
+    const void *w, *b;
+    float eps;
+    void *y, *s;
+    uint8_t* q;                        // kLnQ8: the row in 8 bits; kLnKept: h kept
+    float* scale;                      // kLnQ8: of each row
+    uint8_t* block_scale;              // kLnKept
+    float *mean, *rstd;                // may be null
+};
+
+// f(e, inside) of the piece at column c: `inside` false beyond the row.
+template <int LANES>
+__device__ __forceinline__ bool whole_unit(int u, int F) { return kPiece * LANES * (u + 1) <= F; }
+
+template <typename T>
+__device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, float rs, const T* w, const T* b, int left,
+                                         float h[kPiece], float y[kPiece]) {
+    float g[kPiece], o[kPiece] = {};
+    load_piece(w, left, g);
+    if (b) load_piece(b, left, o);
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+        h[e] = e < left ? (v[e] - mean) * rs : 0.f;
+        y[e] = fmaf(h[e], g[e], o[e]);
+    }
+}
+
+template <typename T, int LANES, int U, int MODE>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
+    constexpr int kRows = 256 / LANES;
+    __shared__ float part[LANES / 32 + 1];
+    const int lane = threadIdx.x % LANES, F = a.F;
+    const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
+    if (n >= a.N) return;                        // a whole row's threads; rows of several waves have a workgroup each
+    const T* x = (const T*)a.x + n * a.ld_x;
+    const T *w = (const T*)a.w, *b = (const T*)a.b;
+    float v[U][kPiece];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = kPiece * (lane + LANES * u);
+        load_piece(x + c, F - c, v[u]);
+    }
+    if (a.r) {
+        const T* r = (const T*)a.r + n * a.ld_r;
+        T* s = (T*)a.s + n * F;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = kPiece * (lane + LANES * u);
+            float t[kPiece];
+            load_piece(r + c, F - c, t);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) v[u][e] = to_f(from_f<T>(v[u][e] + t[e]));
+            store_piece(s + c, F - c, v[u]);
+        }
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) sum += v[u][e];
+    const float inv_f = 1.f / (float)F;
+    float mean = row_sum<LANES>(sum, part) * inv_f;
+    float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int left = F - kPiece * (lane + LANES * u);
+        if (whole_unit<LANES>(u, F)) {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const float d = v[u][e] - mean;
+                d1 += d;
+                d2 = fmaf(d, d, d2);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const float d = e < left ? v[u][e] - mean : 0.f;
+                d1 += d;
+                d2 = fmaf(d, d, d2);
+            }
+        }
+    }
+    row_sum2<LANES>(d1, d2, part);
+    d1 *= inv_f;
+    mean += d1;
+    const float var = fmaf(-d1, d1, d2 * inv_f);
+    const float rs = 1.f / sqrtf(fmaxf(var, 0.f) + a.eps);
+    if (lane == 0 && a.rstd) {
+        a.rstd[n] = rs;
+        if (a.mean) a.mean[n] = mean;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = kPiece * (lane + LANES * u);
+        float h[kPiece], y[kPiece];
+        ln_piece(v[u], mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
+        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
+        if constexpr (MODE == kLnQ8) {
+            // the magnitudes compare as integers, a NaN above everything: its row gets a NaN scale and no number
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                v[u][e] = y[e];
+                const uint32_t m = __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu;
+                top = m > top ? m : top;
+            }
+        } else {
+            store_piece((T*)a.y + n * F + c, F - c, y);
+        }
+    }
+    if constexpr (MODE == kLnQ8) {
+        const float amax = __builtin_bit_cast(float, row_max<LANES>(top, part));
+        float sc = amax / 448.f;
+        if (sc < 0x1p-126f) sc = 0x1p-126f;
+        const float inv = 1.f / sc;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = kPiece * (lane + LANES * u);
+            if (c < F) store_e4m3(a.q + n * F + c, F - c, v[u], inv);
+        }
+        if (lane == 0) a.scale[n] = sc;
+    }
+}
+
+// Rows of any length, a workgroup each: read for the mean, for the squares and for the result (and for the largest
+// magnitude of rows in 8 bits); a thread reads back only what it wrote itself.
+template <typename T, int MODE>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
+    constexpr int LANES = 1024;
+    __shared__ float part[LANES / 32 + 1];
+    const int lane = threadIdx.x, F = a.F;
+    const int64_t n = blockIdx.x;
+    const T *w = (const T*)a.w, *b = (const T*)a.b;
+    const T* x = (const T*)a.x + n * a.ld_x;
+    const int end = (F + kKeptBlock - 1) / kKeptBlock * kKeptBlock;      // whole quads
+    float sum = 0.f;
+    if (a.r) {
+        const T* r = (const T*)a.r + n * a.ld_r;
+        T* s = (T*)a.s + n * F;
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float v[kPiece], t[kPiece];
+            load_piece(x + c, F - c, v);
+            load_piece(r + c, F - c, t);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                v[e] = to_f(from_f<T>(v[e] + t[e]));
+                sum += v[e];
+            }
+            store_piece(s + c, F - c, v);
+        }
+        x = s;
+    } else {
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float v[kPiece];
+            load_piece(x + c, F - c, v);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) sum += v[e];
+        }
+    }
+    const float inv_f = 1.f / (float)F;
+    float mean = row_sum<LANES>(sum, part) * inv_f, d1 = 0.f, d2 = 0.f;
+    for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+        float v[kPiece];
+        load_piece(x + c, F - c, v);
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) {
+            const float d = c + e < F ? v[e] - mean : 0.f;
+            d1 += d;
+            d2 = fmaf(d, d, d2);
+        }
+    }
+    row_sum2<LANES>(d1, d2, part);
+    d1 *= inv_f;
+    mean += d1;
+    const float rs = 1.f / sqrtf(fmaxf(fmaf(-d1, d1, d2 * inv_f), 0.f) + a.eps);
+    if (lane == 0 && a.rstd) {
+        a.rstd[n] = rs;
+        if (a.mean) a.mean[n] = mean;
+    }
+    uint32_t top = 0;
+    for (int c = kPiece * lane; c < end; c += kPiece * LANES) {
+        float v[kPiece], h[kPiece], y[kPiece];
+        load_piece(x + c, F - c, v);
+        ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
+        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
+        if constexpr (MODE == kLnQ8) {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const uint32_t m = __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu;
+                top = m > top ? m : top;
+            }
+        } else {
+            store_piece((T*)a.y + n * F + c, F - c, y);
+        }
+    }
+    if constexpr (MODE == kLnQ8) {
+        const float amax = __builtin_bit_cast(float, row_max<LANES>(top, part));
+        float sc = amax / 448.f;
+        if (sc < 0x1p-126f) sc = 0x1p-126f;
+        const float inv = 1.f / sc;
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float v[kPiece], h[kPiece], y[kPiece];
+            load_piece(x + c, F - c, v);
+            ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
+            store_e4m3(a.q + n * F + c, F - c, y, inv);
+        }
+        if (lane == 0) a.scale[n] = sc;
+    }
+}
+
+struct LnBwdArgs {
+    const void* s;                     // rows that were normalised, or null: h as it was kept
+    int64_t ld_s;
+    const uint8_t *q, *block_scale;
+    const float *mean, *rstd;
+    const void *dy, *ds;               // may be null: zeros
+    int64_t ld_dy, ld_ds, N;
+    int F;
+    const void* w;
+    void* dx;                          // may be null
+    float* part;                       // (workgroups, 2 F): sums of dw, of db; may be null
+};
+
+// h of a piece, from the row as it was normalised or as it was kept.
+template <typename T, bool KEPT>
+struct LnRow {
+    RawPiece<T> a;
+    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c) {
+        a = hold_raw((const T*)g.s + n * g.ld_s + c, g.F - c);
+    }
+    __device__ __forceinline__ void values(float mean, float rs, float h[kPiece]) const {
+        raw_values<T>(a, h);
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) h[e] = (h[e] - mean) * rs;
+    }
+};
+template <typename T>
+struct LnRow<T, true> {
+    KeptPiece a;
+    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c) {
+        a = hold_kept(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, g.F);
+    }
+    __device__ __forceinline__ void values(float, float, float h[kPiece]) const { kept_values(a, h); }
+};
+
+// A workgroup takes rows blockIdx, blockIdx + grid, ... and keeps its columns' sums of dw and db in registers over
+// all of them; its row of partial sums is joined with the others' by ln_column_sum_kernel in a fixed order: no
+// atomics. All of a row's reads are issued before the first is used. Beyond a row's end dy is 0, and h is finite where
+// the row's is.
+template <typename T, int LANES, int U, bool KEPT>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
+    constexpr int kRows = 256 / LANES;
+    __shared__ float part[LANES / 32 + 1];
+    __shared__ float sums[kRows > 1 ? 2 * LANES * U * kPiece : 1];
+    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, F = a.F;
+    const float inv_f = 1.f / (float)F;
+    float aw[U][kPiece] = {}, ab[U][kPiece] = {};
+    for (int64_t n = (int64_t)blockIdx.x * kRows + slot; n < a.N; n += (int64_t)gridDim.x * kRows) {
+        LnRow<T, KEPT> row[U];
+        RawPiece<T> dy[U], ds[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = kPiece * (lane + LANES * u);
+            row[u].hold(a, n, c);
+            dy[u] = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
+            ds[u] = a.ds && a.dx ? hold_raw((const T*)a.ds + n * a.ld_ds + c, F - c) : RawPiece<T>{};
+        }
+        const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
+        float sg = 0.f, sh = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = kPiece * (lane + LANES * u);
+            float h[kPiece], d[kPiece], w[kPiece];
+            row[u].values(mean, rs, h);
+            raw_values<T>(dy[u], d);
+            load_piece((const T*)a.w + c, F - c, w);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                ab[u][e] += d[e];
+                aw[u][e] = fmaf(d[e], h[e], aw[u][e]);
+                const float g = d[e] * w[e];
+                sg += g;
+                sh = fmaf(g, h[e], sh);
+            }
+        }
+        if (!a.dx) continue;
+        row_sum2<LANES>(sg, sh, part);
+        sg *= inv_f;
+        sh *= inv_f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = kPiece * (lane + LANES * u);
+            float h[kPiece], d[kPiece], w[kPiece], o[kPiece];
+            row[u].values(mean, rs, h);
+            raw_values<T>(dy[u], d);
+            raw_values<T>(ds[u], o);
+            load_piece((const T*)a.w + c, F - c, w);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
+            store_piece((T*)a.dx + n * F + c, F - c, o);
+        }
+    }
+    if (!a.part) return;
+    if constexpr (kRows > 1) {
+        for (int k = 0; k < kRows; ++k) {
+            __syncthreads();
+            if (slot == k) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e) {
+                        float& t = sums[(u * kPiece + e) * LANES + lane];
+                        float& o = sums[(U * kPiece + u * kPiece + e) * LANES + lane];
+                        t = k ? t + aw[u][e] : aw[u][e];
+                        o = k ? o + ab[u][e] : ab[u][e];
+                    }
+            }
+        }
+        if (slot != kRows - 1) return;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                aw[u][e] = sums[(u * kPiece + e) * LANES + lane];
+                ab[u][e] = sums[(U * kPiece + u * kPiece + e) * LANES + lane];
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = kPiece * (lane + LANES * u);
+        float* p = a.part + (int64_t)blockIdx.x * 2 * F;
+        if (c < F) {
+            store_piece(p + c, F - c, aw[u]);
+            store_piece(p + F + c, F - c, ab[u]);
+        }
+    }
+}
+
+// The same for rows of any length, a workgroup per row, each read twice; a thread adds to its own columns of the
+// workgroup's partial sums in memory.
+template <typename T, bool KEPT>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnBwdArgs a) {
+    constexpr int LANES = 1024;
+    __shared__ float part[LANES / 32 + 1];
+    const int lane = threadIdx.x, F = a.F;
+    const float inv_f = 1.f / (float)F;
+    float* sums = a.part ? a.part + (int64_t)blockIdx.x * 2 * F : nullptr;
+    bool first = true;
+    for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
+        const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
+        float sg = 0.f, sh = 0.f;
+        auto load = [&](int c, float h[kPiece], float d[kPiece], float w[kPiece]) {
+            LnRow<T, KEPT> row;
+            row.hold(a, n, c);
+            row.values(mean, rs, h);
+            RawPiece<T> r = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
+            raw_values<T>(r, d);
+            load_piece((const T*)a.w + c, F - c, w);
+        };
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float h[kPiece], d[kPiece], w[kPiece];
+            load(c, h, d, w);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const float g = d[e] * w[e];
+                sg += g;
+                sh = fmaf(g, h[e], sh);
+            }
+            if (sums) {
+                float p[kPiece] = {}, o[kPiece] = {};
+                if (!first) {
+                    load_piece(sums + c, F - c, p);
+                    load_piece(sums + F + c, F - c, o);
+                }
+#pragma unroll
+                for (int e = 0; e < kPiece; ++e) {
+                    p[e] = fmaf(d[e], h[e], p[e]);
+                    o[e] += d[e];
+                }
+                store_piece(sums + c, F - c, p);
+                store_piece(sums + F + c, F - c, o);
+            }
+        }
+        first = false;
+        if (!a.dx) continue;
+        row_sum2<LANES>(sg, sh, part);
+        sg *= inv_f;
+        sh *= inv_f;
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float h[kPiece], d[kPiece], w[kPiece], o[kPiece] = {};
+            load(c, h, d, w);
+            if (a.ds) load_piece((const T*)a.ds + n * a.ld_ds + c, F - c, o);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
+            store_piece((T*)a.dx + n * F + c, F - c, o);
+        }
+    }
+}
+
+// dw[c], db[c] = sums over `rows` of part (rows, 2 F): 64 threads per column, each a sum of every 64th row, then a
+// tree.
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_column_sum_kernel(const float* __restrict__ part, int rows, int F,
+                                                             T* __restrict__ dw, T* __restrict__ db) {
+    __shared__ float sums[64][17];
+    const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + cx;
+    float a = 0.f;
+    if (c < 2 * F) {
+#pragma unroll 8
+        for (int r = ry; r < rows; r += 64) a += part[(int64_t)r * 2 * F + c];
+    }
+    sums[ry][cx] = a;
+    __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) {
+        if (ry < o) sums[ry][cx] += sums[ry + o][cx];
+        __syncthreads();
+    }
+    if (ry == 0 && c < 2 * F) {
+        T* out = c < F ? dw : db;
+        if (out) out[c < F ? c : c - F] = from_f<T>(sums[0][cx]);
+    }
+}
+
+constexpr int kLnHeld = 16384;                   // longest row that stays in registers
+constexpr int kLnMax = 65536;
+constexpr int64_t kLnBwdGroups = 1024;
+static inline int64_t ln_bwd_grid(int64_t N, int F) {
+    const RowShape sh = row_shape(F);
+    const int64_t rows = F > kLnHeld ? 1 : 256 / sh.lanes, need = (N + rows - 1) / rows;
+    return need < kLnBwdGroups ? need : kLnBwdGroups;
+}
+
+// The variants: lanes per row and pieces per lane.
+#define FACE_LN_ROWS                                                                                               \
+    FACE_ROW(16, 1) FACE_ROW(16, 2) FACE_ROW(64, 1) FACE_ROW(64, 2) FACE_ROW(64, 3) FACE_ROW(64, 4) FACE_ROW(64, 5) \
+    FACE_ROW(64, 6) FACE_ROW(64, 8) FACE_ROW(256, 3) FACE_ROW(256, 4) FACE_ROW(256, 5) FACE_ROW(256, 6) FACE_ROW(256, 8)
+
+template <typename T, int MODE>
+static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
+    const RowShape sh = row_shape(a.F);
+    const int rows = a.F > kLnHeld ? 1 : 256 / sh.lanes;
+    const int64_t blocks = (a.N + rows - 1) / rows;
+    if (blocks > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)blocks);
+    if (a.F > kLnHeld) {
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);
+    }
+#define FACE_ROW(L_, U_) \
+    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, U_, MODE>), grid, dim3(256), 0, st, a);
+    FACE_LN_ROWS
+#undef FACE_ROW
+    FACE_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T, bool KEPT>
+static int launch_ln_bwd(const LnBwdArgs& a, T* dw, T* db, hipStream_t st) {
+    const RowShape sh = row_shape(a.F);
+    const int64_t blocks = ln_bwd_grid(a.N, a.F);
+    if (blocks) {
+        const dim3 grid((unsigned)blocks);
+        if (a.F > kLnHeld) {
+            hipLaunchKernelGGL((ln_bwd_long_kernel<T, KEPT>), grid, dim3(1024), 0, st, a);
+        }
+#define FACE_ROW(L_, U_) \
+    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, U_, KEPT>), grid, dim3(256), 0, st, a);
+        FACE_LN_ROWS
+#undef FACE_ROW
+        FACE_LAUNCH_CHECK();
+    }
+    if (dw || db) {
+        hipLaunchKernelGGL(ln_column_sum_kernel<T>, dim3((unsigned)((2 * a.F + 15) / 16)), dim3(1024), 0, st, a.part,
+                           (int)blocks, a.F, dw, db);
+        FACE_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+static int ln_args(int64_t N, int32_t F, int32_t dtype) {
+    if (N < 0 || F <= 0) return FACE_ERR_ARG;
+    if (dtype != FACE_F32 && dtype != FACE_BF16 && dtype != FACE_F16) return FACE_ERR_ARG;
+    if (F > kLnMax) return FACE_ERR_UNSUPPORTED;
+    return 0;
+}
+
+}  // namespace face
+
+using namespace face;
+
+extern "C" int face_layer_norm_rows_fwd(const void* x, int64_t ld_x, const void* r, int64_t ld_r, int64_t N, int32_t F,
+                                 int32_t dtype, const void* w, const void* b, float eps, void* y, void* s, void* q,
+                                 float* scale, void* block_scale, float* mean, float* rstd, void* stream) {
+    if (int rc = ln_args(N, F, dtype)) return rc;
+    if (ld_x < F || (r && ld_r < F) || !(eps >= 0.f)) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!x || !w || (!r != !s) || (scale && block_scale) || (!q != !(scale || block_scale))) return FACE_ERR_ARG;
+    if (!y != (scale != nullptr) || (block_scale && !rstd) || (mean && !rstd)) return FACE_ERR_ARG;
+    const LnFwdArgs a = {x, r, ld_x, ld_r, N, F, w, b, eps, y, s, (uint8_t*)q, scale, (uint8_t*)block_scale, mean, rstd};
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const hipStream_t st = (hipStream_t)stream;
+        return scale ? launch_ln_fwd<T, kLnQ8>(a, st) : block_scale ? launch_ln_fwd<T, kLnKept>(a, st) : launch_ln_fwd<T, kLn>(a, st);
+    });
+}
+
+extern "C" int64_t face_layer_norm_rows_bwd_work(int64_t N, int32_t F) {
+    if (N <= 0 || F <= 0 || F > kLnMax) return 0;
+    return ln_bwd_grid(N, F) * F * 8;
+}
+
+extern "C" int face_layer_norm_rows_bwd(const void* s, int64_t ld_s, const void* q, const void* block_scale, const float* mean,
+                                 const float* rstd, const void* dy, int64_t ld_dy, const void* ds, int64_t ld_ds, int64_t N,
+                                 int32_t F, int32_t dtype, const void* w, void* dx, void* dw, void* db, void* work,
+                                 int64_t work_bytes, void* stream) {
+    if (int rc = ln_args(N, F, dtype)) return rc;
+    if ((s && ld_s < F) || (dy && ld_dy < F) || (ds && ld_ds < F)) return FACE_ERR_ARG;
+    if (!dx && !dw && !db) return 0;
+    if (N && (!w || !rstd || (s ? !mean || q : !q || !block_scale))) return FACE_ERR_ARG;
+    const bool sums = dw || db;
+    if (sums && N && (!work || work_bytes < face_layer_norm_rows_bwd_work(N, F))) return FACE_ERR_ARG;
+    if (N == 0 && !sums) return 0;
+    const LnBwdArgs a = {s, ld_s, (const uint8_t*)q, (const uint8_t*)block_scale, mean, rstd, dy, ds, ld_dy, ld_ds, N, F, w, dx,
+                         sums ? (float*)work : nullptr};
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const hipStream_t st = (hipStream_t)stream;
+        return s || !q ? launch_ln_bwd<T, false>(a, (T*)dw, (T*)db, st) : launch_ln_bwd<T, true>(a, (T*)dw, (T*)db, st);
+    });
+}

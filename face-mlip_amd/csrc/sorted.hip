@@ -1,0 +1,269 @@
+// Rows laid out by expert and joined again, for the slots a = order[p] of a plan at the places p < ptr[G] (slot a is
+// choice a % k of row a / k):
+//
+//   out     xs[p] = x[a / k], 0 behind ptr[G];   dx[i] = sum over the row's slots of dxs[place(a)]
+//   back    y[i] = r[i] + sum_j w[i, j] xs[place(i k + j)];   dxs[p] = w[a] dy[a / k], dw[a] = dy[a / k] . xs[p]
+//
+// place is order's inverse, -1 for slots that have none: what leaves rows of x, or gathers into rows of y, goes by
+// rows, reads or writes each of those once, and its other side by whole rows. With one choice per row there is nothing to share:
+// xs is gathered by order, without the inverse. Bound by bytes.
+#include "elem.h"
+
+namespace face {
+
+constexpr int64_t kPlacesOne = 8192;             // one workgroup inverts the order up to here
+
+__device__ __forceinline__ int64_t places_of(const int32_t* ptr, int G, int64_t slots) {
+    const int64_t m = ptr[G];
+    return m < 0 ? 0 : (m < slots ? m : slots);
+}
+
+// The inverse in LDS, then written once.
+__global__ __launch_bounds__(1024) void places_one_kernel(const int32_t* __restrict__ ptr, const int32_t* __restrict__ order,
+                                                          int slots, int G, int32_t* __restrict__ place) {
+    __shared__ int32_t at[kPlacesOne];
+    const int m = (int)places_of(ptr, G, slots);
+    for (int a = threadIdx.x; a < slots; a += 1024) at[a] = -1;
+    __syncthreads();
+    for (int p = threadIdx.x; p < m; p += 1024) {
+        const int a = order[p];
+        if (a >= 0 && a < slots) at[a] = p;
+    }
+    __syncthreads();
+    for (int a = threadIdx.x; a < slots; a += 1024) place[a] = at[a];
+}
+__global__ __launch_bounds__(256) void places_none_kernel(int64_t slots, int32_t* __restrict__ place) {
+    const int64_t a = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (a < slots) place[a] = -1;
+}
+__global__ __launch_bounds__(256) void places_kernel(const int32_t* __restrict__ ptr, const int32_t* __restrict__ order,
+                                                     int64_t slots, int G, int32_t* __restrict__ place) {
+    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p >= places_of(ptr, G, slots)) return;
+    const int a = order[p];
+    if (a >= 0 && a < slots) place[a] = (int32_t)p;
+}
+
+// Threads per row: about four pieces each.
+static inline int sorted_lanes_log2(int64_t F) {
+    const int64_t p = (F + kPiece - 1) / kPiece;
+    int lg = 4;
+    while (lg < 8 && ((int64_t)4 << lg) < p) ++lg;
+    return lg;
+}
+
+// xs[p] = x[order[p] / k].
+template <typename T>
+__global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restrict__ x, int64_t ld,
+                                                              const int32_t* __restrict__ ptr,
+                                                              const int32_t* __restrict__ order, int64_t slots, int k, int G,
+                                                              int F, int lg, T* __restrict__ xs) {
+    const int64_t p = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    if (p >= slots) return;
+    const int a = p < places_of(ptr, G, slots) ? order[p] : -1;
+    const bool some = a >= 0 && a < slots;
+    const T* from = x + (int64_t)(some ? a / k : 0) * ld;
+#pragma unroll 4
+    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
+        float v[kPiece] = {};
+        if (some) load_piece(from + c, F - c, v);
+        store_piece(xs + p * F + c, F - c, v);
+    }
+}
+
+// A row's threads write it to the places of its k slots, and zeros to those of the places i k .. i k + k - 1 that
+// have no slot.
+template <typename T>
+__global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restrict__ x, int64_t ld,
+                                                               const int32_t* __restrict__ ptr,
+                                                               const int32_t* __restrict__ order,
+                                                               const int32_t* __restrict__ place, int64_t slots, int k, int G,
+                                                               int F, int lg, T* __restrict__ xs) {
+    const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    if (n * k >= slots) return;
+    const int64_t m = places_of(ptr, G, slots);
+#pragma unroll 2
+    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
+        float v[kPiece];
+        const float none[kPiece] = {};
+        load_piece(x + n * ld + c, F - c, v);
+        for (int j = 0; j < k; ++j) {
+            const int64_t i = n * k + j;
+            const int p = place[i];
+            if (p >= 0) store_piece(xs + (int64_t)p * F + c, F - c, v);
+            const int a = i < m ? order[i] : -1;
+            if (a < 0 || a >= slots || place[a] != i) store_piece(xs + i * F + c, F - c, none);
+        }
+    }
+}
+
+// out[i] = r[i] + sum_j w[i, j] y[place(i k + j)], in order; w null: ones.
+template <typename T>
+__global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ place,
+                                                         const float* __restrict__ w, const T* __restrict__ r, int64_t ld_r,
+                                                         int64_t N, int k, int F, int lg, T* __restrict__ out) {
+    const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    if (n >= N) return;
+    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
+        float s[kPiece] = {};
+        if (r) load_piece(r + n * ld_r + c, F - c, s);
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) {
+            const int p = place[n * k + j];
+            if (p < 0) continue;
+            float v[kPiece];
+            load_piece(y + (int64_t)p * ld_y + c, F - c, v);
+            const float f = w ? w[n * k + j] : 1.f;
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) s[e] = fmaf(f, v[e], s[e]);
+        }
+        store_piece(out + n * F + c, F - c, s);
+    }
+}
+
+// dy[p] = w dout and dw = dout . y[p] at the places of the row's slots; zeros at places without a slot.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ dout, int64_t ld_d, const T* __restrict__ y,
+                                                         int64_t ld_y, const int32_t* __restrict__ ptr,
+                                                         const int32_t* __restrict__ order,
+                                                         const int32_t* __restrict__ place, const float* __restrict__ w,
+                                                         int64_t N, int k, int G, int F, T* __restrict__ dy,
+                                                         float* __restrict__ dw) {
+    __shared__ float part[LANES / 64 + 1];
+    const int lane = threadIdx.x % LANES;
+    const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (n >= N) return;
+    const int64_t slots = N * k, m = places_of(ptr, G, slots);
+    constexpr int J = 4;
+    for (int j0 = 0; j0 < k; j0 += J) {
+        float s[J] = {}, f[J];
+        int p[J];
+        bool bare[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int64_t i = n * k + j0 + j;
+            const bool in = j0 + j < k;
+            f[j] = in && w ? w[i] : 1.f;
+            p[j] = in ? place[i] : -1;
+            const int a = in && i < m ? order[i] : -1;
+            bare[j] = in && (a < 0 || a >= slots || place[a] != i);
+        }
+        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
+            float d[kPiece];
+            load_piece(dout + n * ld_d + c, F - c, d);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                float v[kPiece];
+                if (dw && p[j] >= 0) {
+                    load_piece(y + (int64_t)p[j] * ld_y + c, F - c, v);
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e) s[j] = fmaf(d[e], v[e], s[j]);
+                }
+                if (!dy) continue;
+                if (p[j] >= 0) {
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e) v[e] = f[j] * d[e];
+                    store_piece(dy + (int64_t)p[j] * F + c, F - c, v);
+                }
+                if (bare[j]) {
+                    const float none[kPiece] = {};
+                    store_piece(dy + (n * k + j0 + j) * F + c, F - c, none);
+                }
+            }
+        }
+        if (dw) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float t = row_sum<LANES>(s[j], part);
+                if (lane == 0 && j0 + j < k) dw[n * k + j0 + j] = t;
+            }
+        }
+    }
+}
+
+static int sorted_args(int64_t N, int32_t k, int32_t G, int32_t F, int32_t dtype) {
+    if (N < 0 || k <= 0 || G <= 0 || F <= 0) return FACE_ERR_ARG;
+    if (dtype != FACE_F32 && dtype != FACE_BF16 && dtype != FACE_F16) return FACE_ERR_ARG;
+    if (F > (1 << 28) || N > (int64_t)0x7fffffff || N * k > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    return 0;
+}
+static dim3 sorted_grid(int64_t rows, int lg) { return dim3((unsigned)((rows + (256 >> lg) - 1) >> (8 - lg))); }
+
+}  // namespace face
+
+using namespace face;
+
+extern "C" int face_expert_places(const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t* place,
+                                  void* stream) {
+    if (slots < 0 || G <= 0) return FACE_ERR_ARG;
+    if (slots > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
+    if (slots == 0) return 0;
+    if (!ptr || !order || !place) return FACE_ERR_ARG;
+    const hipStream_t st = (hipStream_t)stream;
+    if (slots <= kPlacesOne) {
+        hipLaunchKernelGGL(places_one_kernel, dim3(1), dim3(1024), 0, st, ptr, order, (int)slots, G, place);
+    } else {
+        const dim3 grid((unsigned)((slots + 255) / 256));
+        hipLaunchKernelGGL(places_none_kernel, grid, dim3(256), 0, st, slots, place);
+        hipLaunchKernelGGL(places_kernel, grid, dim3(256), 0, st, ptr, order, slots, G, place);
+    }
+    FACE_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, const int32_t* ptr, const int32_t* order,
+                                    const int32_t* place, int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs,
+                                    void* stream) {
+    if (int rc = sorted_args(N, k, G, F, dtype)) return rc;
+    if (ld_x < F) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!x || !ptr || !order || !xs) return FACE_ERR_ARG;
+    const int lg = sorted_lanes_log2(F);
+    const int64_t slots = N * k;
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (place)
+            hipLaunchKernelGGL(dispatch_scatter_kernel<T>, sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x,
+                               ld_x, ptr, order, place, slots, k, G, F, lg, (T*)xs);
+        else
+            hipLaunchKernelGGL(dispatch_gather_kernel<T>, sorted_grid(slots, lg), dim3(256), 0, (hipStream_t)stream,
+                               (const T*)x, ld_x, ptr, order, slots, k, G, F, lg, (T*)xs);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
+extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* place, const float* weight, const void* r,
+                                      int64_t ld_r, int64_t N, int32_t k, int32_t F, int32_t dtype, void* out, void* stream) {
+    if (int rc = sorted_args(N, k, 1, F, dtype)) return rc;
+    if (ld_y < F || (r && ld_r < F)) return FACE_ERR_ARG;
+    if (N == 0) return 0;
+    if (!y || !place || !out) return FACE_ERR_ARG;
+    const int lg = sorted_lanes_log2(F);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(return_fwd_kernel<T>, sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, place,
+                           weight, (const T*)r, ld_r, N, k, F, lg, (T*)out);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
+extern "C" int face_expert_return_bwd(const void* dout, int64_t ld_d, const void* y, int64_t ld_y, const int32_t* ptr,
+                                      const int32_t* order, const int32_t* place, const float* weight, int64_t N, int32_t k,
+                                      int32_t G, int32_t F, int32_t dtype, void* dy, float* dweight, void* stream) {
+    if (int rc = sorted_args(N, k, G, F, dtype)) return rc;
+    if (ld_d < F || (dweight && ld_y < F)) return FACE_ERR_ARG;
+    if (N == 0 || (!dy && !dweight)) return 0;
+    if (!dout || !ptr || !order || !place || (dweight && !y)) return FACE_ERR_ARG;
+    const int L = F <= 512 ? 16 : (F <= 4096 ? 64 : 256), rows = 256 / L;
+    const dim3 grid((unsigned)((N + rows - 1) / rows));
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto* kern = L == 16 ? return_bwd_kernel<T, 16> : (L == 64 ? return_bwd_kernel<T, 64> : return_bwd_kernel<T, 256>);
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, (hipStream_t)stream, (const T*)dout, ld_d, (const T*)y, ld_y, ptr, order,
+                           place, weight, N, k, G, F, (T*)dy, dweight);
+        FACE_LAUNCH_CHECK();
+        return 0;
+    });
+}

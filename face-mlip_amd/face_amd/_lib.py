@@ -105,9 +105,23 @@ _SIGS = {
                                                P, P, I64, P]),
     "face_expert_combine_fwd": (ctypes.c_int, [P, I64, P, P, I64, I64, I32, I32, I32, P, P]),
     "face_expert_combine_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, I32, I32, I32, P, P, P]),
+    "face_layer_norm_rows_fwd": (ctypes.c_int, [P, I64, P, I64, I64, I32, I32, P, P, F32, P, P, P, P, P, P, P, P]),
+    "face_layer_norm_rows_bwd_work": (I64, [I64, I32]),
+    "face_layer_norm_rows_bwd": (ctypes.c_int, [P, I64, P, P, P, P, P, I64, P, I64, I64, I32, I32, P, P, P, P, P, I64, P]),
+    "face_pack_rows": (ctypes.c_int, [P, I64, I64, I32, I32, P, P, P]),
+    "face_unpack_rows": (ctypes.c_int, [P, I64, P, I64, I64, I32, I32, P, P]),
+    "face_gated_silu_fwd": (ctypes.c_int, [P, I64, I64, I32, I32, P, P, P, P]),
+    "face_gated_silu_bwd": (ctypes.c_int, [P, I64, P, P, P, I64, I64, I32, I32, P, P]),
+    "face_embed_fwd": (ctypes.c_int, [P, I64, P, I32, I64, I64, I32, I32, F32, P, P, P]),
+    "face_embed_bwd_work": (I64, [I64, I64, I32]),
+    "face_embed_bwd": (ctypes.c_int, [P, P, I64, I64, I64, I32, I32, F32, P, P, I64, P]),
+    "face_expert_places": (ctypes.c_int, [P, P, I64, I32, P, P]),
+    "face_expert_dispatch": (ctypes.c_int, [P, I64, I32, P, P, P, I64, I32, I32, I32, P, P]),
+    "face_expert_return_fwd": (ctypes.c_int, [P, I64, P, P, P, I64, I64, I32, I32, I32, P, P]),
+    "face_expert_return_bwd": (ctypes.c_int, [P, I64, P, I64, P, P, P, P, I64, I32, I32, I32, I32, P, P, P]),
 }
 
-ABI_VERSION = 27
+ABI_VERSION = 28
 
 
 class LinProblem(ctypes.Structure):

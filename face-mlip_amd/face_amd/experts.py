@@ -27,9 +27,10 @@ from . import _lib
 from ._lib import call, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_E4M3 = torch.float8_e4m3fn
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _X_OPS = {None: 0, "silu": 1}
-MAX_WIDTH = 65536                   # widest row of rms_norm and quantize_rows
+MAX_WIDTH = 65536                   # widest row of the norms, quantize_rows and embed
+MAX_PACKED = 1 << 28                # of pack_rows, gated_silu and rows by expert
 MAX_EXPERTS, MAX_K = 1024, 16       # of route; group_plan takes as many groups
 
 
@@ -105,7 +106,7 @@ def _wants_grad(*ts):
 
 
 # ----------------------------------------------------------------------------- norm
-def _norm_args(name, x, w, eps, residual):
+def _norm_args(name, x, w, eps, residual, b=None):
     code = _dtype(name, x)
     if x.dim() < 1 or w.dim() != 1 or x.shape[-1] != w.shape[0]:
         _fail(name, f"x (..., F) and w (F), got {tuple(x.shape)} and {tuple(w.shape)}")
@@ -113,11 +114,13 @@ def _norm_args(name, x, w, eps, residual):
         _fail(name, f"rows of 1 to {MAX_WIDTH} columns, got {x.shape[-1]}")
     if w.dtype != x.dtype:
         _fail(name, f"w of the rows' type {x.dtype}, got {w.dtype}")
+    if b is not None and (b.shape != w.shape or b.dtype != x.dtype):
+        _fail(name, f"b like w, {tuple(w.shape)} {x.dtype}, got {tuple(b.shape)} {b.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         _fail(name, f"residual like x, {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
     if not 0 <= eps < float("inf"):
         _fail(name, f"eps >= 0, got {eps}")
-    _check(name, x, w=w, residual=residual)
+    _check(name, x, w=w, b=b, residual=residual)
     return code
 
 
@@ -196,6 +199,95 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None):
     return (q, scale) if s is None else (q, scale, s)
 
 
+def _layer_norm_fwd(code, x, w, b, eps, r, q8=False, grad=False, keep8=False):
+    """(y, s, kept): kept holds what the backward reads, (mean, rstd), (q, block scales, rstd) or nothing. y is
+    (q, scale) with q8; s is None without a residual."""
+    F = x.shape[-1]
+    x2, w = _rows(x, F), w.contiguous()
+    r2 = None if r is None else _rows(r, F)
+    b = None if b is None else b.contiguous()
+    N, dev = x2.shape[0], x.device
+    s = None if r is None else _like(x)
+    y = None if q8 else _like(x)
+    q = torch.empty(x.shape, dtype=_E4M3, device=dev) if q8 or keep8 else None
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if q8 else None
+    block = _work(N * _blocks(F), dev) if keep8 else None
+    stat = torch.empty((1 if keep8 else 2) * N, dtype=torch.float32, device=dev) if grad else None
+    rstd = ptr(stat)
+    mean = None if stat is None or keep8 else rstd + 4 * N
+    _launch(x, "face_layer_norm_rows_fwd", "layer_norm_fwd", x2.data_ptr(), x2.stride(0), ptr(r2),
+            F if r2 is None else r2.stride(0), N, F, code, w.data_ptr(), ptr(b), eps, ptr(y), ptr(s), ptr(q), ptr(scale),
+            ptr(block), mean, rstd)
+    return (q, scale) if q8 else y, s, (q, block, stat) if keep8 else (stat,)
+
+
+class LayerNorm(torch.autograd.Function):
+    """Keeps the rows it normalised and each one's mean and rstd; with keep8 the normalised rows in 8 bits and rstd."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, r, keep8):
+        y, s, kept = _layer_norm_fwd(_DTYPES[x.dtype], x, w, b, eps, r, grad=True, keep8=keep8)
+        ctx.save_for_backward(None if keep8 else x if s is None else s, w, *kept)
+        ctx.keep8 = keep8
+        ctx.set_materialize_grads(False)
+        return y if s is None else (y, s)
+
+    @staticmethod
+    def backward(ctx, dy, ds=None):
+        _once("layer_norm", dy, ds)
+        need_x, need_w, need_b, _, need_r, _ = ctx.needs_input_grad
+        if dy is None and ds is None:
+            return (None,) * 6
+        some = dy if dy is not None else ds
+        if ctx.keep8:
+            _, w, q, block, stat = ctx.saved_tensors
+            s2, mean = None, None
+        else:
+            s, w, stat = ctx.saved_tensors
+            q = block = None
+            s2 = _rows(s, s.shape[-1])
+        F, code, w = w.shape[0], _DTYPES[w.dtype], w.contiguous()
+        N = some.numel() // F
+        if not ctx.keep8:
+            mean = stat.data_ptr() + 4 * N
+        dx = _like(some) if need_x or need_r else None
+        dw = torch.empty_like(w) if need_w else None
+        db = torch.empty_like(w) if need_b else None
+        if dy is not None:
+            dy = _rows(dy, F)
+        if ds is not None:
+            ds = _rows(ds, F)
+        need = _lib.lib().face_layer_norm_rows_bwd_work(N, F) if need_w or need_b else 0
+        work = _work(need, some.device)
+        _launch(some, "face_layer_norm_rows_bwd", "layer_norm_bwd", ptr(s2), F if s2 is None else s2.stride(0), ptr(q), ptr(block),
+                mean, stat.data_ptr(), ptr(dy), F if dy is None else dy.stride(0), ptr(ds), F if ds is None else ds.stride(0), N, F,
+                code, w.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(work), need)
+        return dx if need_x else None, dw, db, None, dx if need_r else None, None
+
+
+def layer_norm(x, w, b=None, eps=1e-5, residual=None, keep8=False):
+    """x (..., F), w (F), b (F) or None -> (x - mean) w / sqrt(var + eps) + b over the last axis, var the mean square of
+    x - mean. With residual (like x): (that of s, s) for s = x + residual, rounded to the rows' type before it is
+    normalised. F <= MAX_WIDTH; sums in float32. keep8: the backward reads the normalised rows as 8 bits hold them
+    (pack_rows), 1.03 bytes a value, in place of s."""
+    eps = float(eps)
+    code = _norm_args("layer_norm", x, w, eps, residual, b)
+    if _wants_grad(x, w, b, residual):
+        return LayerNorm.apply(x, w, b, eps, residual, bool(keep8))
+    y, s, _ = _layer_norm_fwd(code, x, w, b, eps, residual)
+    return y if s is None else (y, s)
+
+
+@torch.no_grad()
+def layer_norm_q8(x, w, b=None, eps=1e-5, residual=None):
+    """layer_norm whose rows leave in 8 bits, for serving, as those of rms_norm_q8: (q, scale), and s with a residual.
+    No gradients."""
+    eps = float(eps)
+    code = _norm_args("layer_norm_q8", x, w, eps, residual, b)
+    y, s, _ = _layer_norm_fwd(code, x, w, b, eps, residual, q8=True)
+    return y if s is None else (*y, s)
+
+
 @torch.no_grad()
 def quantize_rows(x, x_op=None):
     """x (..., F) -> (q float8_e4m3fn, scale (...) float32) of op(x), x_op None or "silu", each row scaled as in
@@ -213,6 +305,164 @@ def quantize_rows(x, x_op=None):
     _launch(x, "face_quantize_rows", "quantize_rows", x2.data_ptr(), x2.stride(0), x2.shape[0], F, code, _X_OPS[x_op],
             q.data_ptr(), scale.data_ptr())
     return q, scale
+
+
+# ----------------------------------------------------------------------------- rows kept in 8 bits
+def _blocks(F):
+    """Scales of a kept row: one for each 32 columns."""
+    return (F + 31) // 32
+
+
+def _pack(x):
+    F = x.shape[-1]
+    x2 = _rows(x, F)
+    q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
+    scale = torch.empty(*x.shape[:-1], _blocks(F), dtype=_E8M0, device=x.device)
+    _launch(x, "face_pack_rows", "pack_rows", x2.data_ptr(), x2.stride(0), x2.shape[0], F, _DTYPES[x.dtype], q.data_ptr(),
+            scale.data_ptr())
+    return q, scale
+
+
+def _unpack(q, scale, dtype):
+    F = q.shape[-1]
+    q2, s2 = _rows(q, F), _rows(scale, scale.shape[-1])
+    x = torch.empty(q.shape, dtype=dtype, device=q.device)
+    _launch(q, "face_unpack_rows", "unpack_rows", q2.data_ptr(), q2.stride(0), s2.data_ptr(), s2.stride(0), q2.shape[0], F,
+            _DTYPES[dtype], x.data_ptr())
+    return x
+
+
+@torch.no_grad()
+def pack_rows(x):
+    """x (..., F) -> (q (..., F) float8_e4m3fn, scale (..., ceil(F / 32)) float8_e8m0fnu): rows as a backward pass
+    keeps them in 8 bits, 1.03 bytes a value. Each 32 columns share a power of two, the least (>= 2^-126) that
+    keeps their largest magnitude within 448: a value is off by at most 2^-4 of itself or 2^-18 of the block's
+    largest. A NaN or an infinity is kept as NaN and leaves the others as they are. No gradients."""
+    _dtype("pack_rows", x)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_PACKED:
+        _fail("pack_rows", f"rows of 1 to {MAX_PACKED} columns, got {tuple(x.shape)}")
+    _check("pack_rows", x)
+    return _pack(x)
+
+
+@torch.no_grad()
+def unpack_rows(q, scale, dtype=torch.bfloat16):
+    """The values that (q, scale) of pack_rows stand for, in `dtype`; one past its largest is that. No gradients."""
+    name = "unpack_rows"
+    if q.dtype != _E4M3 or q.dim() < 1 or not 1 <= q.shape[-1] <= MAX_PACKED:
+        _fail(name, f"float8_e4m3fn rows of 1 to {MAX_PACKED} columns, got {tuple(q.shape)} {q.dtype}")
+    if dtype not in _DTYPES:
+        _fail(name, f"dtype float32, bfloat16 or float16, got {dtype}")
+    shape = (*q.shape[:-1], _blocks(q.shape[-1]))
+    if scale.shape != shape or scale.dtype != _E8M0:
+        _fail(name, f"scale {shape} float8_e8m0fnu, got {tuple(scale.shape)} {scale.dtype}")
+    _check(name, q, scale=scale)
+    return _unpack(q, scale, dtype)
+
+
+# ----------------------------------------------------------------------------- gated activation
+def _gated_fwd(x, keep8=False):
+    F = x.shape[-1] // 2
+    x2 = _rows(x, 2 * F)
+    N = x2.shape[0]
+    y = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
+    q = _work(N * 2 * F, x.device) if keep8 else None
+    scale = _work(N * 2 * _blocks(F), x.device) if keep8 else None
+    _launch(x, "face_gated_silu_fwd", "gated_silu_fwd", x2.data_ptr(), x2.stride(0), N, F, _DTYPES[x.dtype], y.data_ptr(), ptr(q),
+            ptr(scale))
+    return y, q, scale
+
+
+class GatedSiLU(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, keep8):
+        y, q, scale = _gated_fwd(x, keep8)
+        ctx.save_for_backward(*((q, scale) if keep8 else (x,)))
+        ctx.keep8 = keep8
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _once("gated_silu", dy)
+        F = dy.shape[-1]
+        d2 = _rows(dy, F)
+        x2 = q = scale = None
+        if ctx.keep8:
+            q, scale = ctx.saved_tensors
+        else:
+            x2 = _rows(ctx.saved_tensors[0], 2 * F)
+        dx = torch.empty(*dy.shape[:-1], 2 * F, dtype=dy.dtype, device=dy.device)
+        _launch(dy, "face_gated_silu_bwd", "gated_silu_bwd", ptr(x2), 2 * F if x2 is None else x2.stride(0), ptr(q), ptr(scale),
+                d2.data_ptr(), d2.stride(0), d2.shape[0], F, _DTYPES[dy.dtype], dx.data_ptr())
+        return dx, None
+
+
+def gated_silu(x, keep8=False):
+    """x (..., 2 F) -> silu(x[..., :F]) x[..., F:], the hidden rows between two products whose first makes gates and
+    values side by side. keep8: the backward reads x as 8 bits hold it (pack_rows, each half in blocks of its own)
+    in place of x, written as the forward reads it. Differentiable in x."""
+    _dtype("gated_silu", x)
+    if x.dim() < 1 or x.shape[-1] % 2 or not 2 <= x.shape[-1] <= 2 * MAX_PACKED:
+        _fail("gated_silu", f"x (..., 2 F), F <= {MAX_PACKED}, got {tuple(x.shape)}")
+    _check("gated_silu", x)
+    if _wants_grad(x):
+        return GatedSiLU.apply(x, bool(keep8))
+    return _gated_fwd(x)[0]
+
+
+# ----------------------------------------------------------------------------- rows of a table
+def _embed_fwd(table, index, factor, keys):
+    V, F = table.shape
+    t2, i = _rows(table, F), index.contiguous()
+    y = torch.empty(*index.shape, F, dtype=table.dtype, device=table.device)
+    key = None
+    wide = i.dtype == torch.int64
+    if keys:
+        key = torch.empty(i.shape, dtype=torch.int32, device=i.device) if wide else i
+    _launch(table, "face_embed_fwd", "embed_fwd", t2.data_ptr(), t2.stride(0), i.data_ptr(), int(wide), i.numel(), V, F,
+            _DTYPES[table.dtype], factor, y.data_ptr(), key.data_ptr() if keys and wide else None)
+    return y, key
+
+
+class Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, factor):
+        y, key = _embed_fwd(table, index, factor, True)
+        ctx.save_for_backward(key)
+        ctx.rows, ctx.factor = table.shape[0], factor
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _once("embed", dy)
+        key, = ctx.saved_tensors
+        V, F, N = ctx.rows, dy.shape[-1], key.numel()
+        d2 = _rows(dy, F)
+        dt = torch.empty(V, F, dtype=dy.dtype, device=dy.device)
+        need = _lib.lib().face_embed_bwd_work(N, V, F)
+        work = _work(need, dy.device)
+        _launch(dy, "face_embed_bwd", "embed_bwd", key.data_ptr(), d2.data_ptr(), d2.stride(0), N, V, F, _DTYPES[dy.dtype], ctx.factor,
+                dt.data_ptr(), ptr(work), need)
+        return dt, None, None
+
+
+def embed(table, index, scale=1.0):
+    """table (V, F), index (...) int32 or int64 -> (..., F): scale times the table's rows, zeros where an index lies outside
+    [0, V): the rows of every atom's species, or of every pair's. F <= MAX_WIDTH. Differentiable in the table: a
+    dense gradient, each row's sum in float32 in a fixed order, rounded once."""
+    name = "embed"
+    _dtype(name, table)
+    if table.dim() != 2 or not 1 <= table.shape[1] <= MAX_WIDTH or not 1 <= table.shape[0] < (1 << 31) - 1:
+        _fail(name, f"table (V, F) with 1 <= V < 2^31 - 1 and 1 <= F <= {MAX_WIDTH}, got {tuple(table.shape)}")
+    if index.dtype not in (torch.int32, torch.int64):
+        _fail(name, f"int32 or int64 index, got {index.dtype}")
+    if index.numel() >= 1 << 31:
+        _fail(name, f"fewer than 2^31 rows, got {index.numel()}")
+    factor = float(scale)
+    _check(name, table, index=index)
+    if _wants_grad(table):
+        return Embed.apply(table, index, factor)
+    return _embed_fwd(table, index, factor, False)[0]
 
 
 # ----------------------------------------------------------------------------- gate and grouping
@@ -384,9 +634,9 @@ def _linear_fwd(x, w, plan, bias, op):
 
 class GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, p, order, plan, op):
+    def forward(ctx, x, w, bias, p, order, plan, op, keep8):
         y = _linear_fwd(x, w, plan, bias, op)
-        ctx.save_for_backward(x, w, p, order)
+        ctx.save_for_backward(w, p, order, *(_pack(x) if keep8 else (x,)))
         ctx.plan, ctx.op = plan, op
         ctx.set_materialize_grads(False)
         return y
@@ -395,9 +645,10 @@ class GroupedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         _once("grouped_linear", dy)
         if dy is None:
-            return (None,) * 7
+            return (None,) * 8
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        x, w, p, order = ctx.saved_tensors
+        w, p, order, *x = ctx.saved_tensors
+        x = x[0] if len(x) == 1 else _unpack(*x, w.dtype)
         dtype, dev, code = x.dtype, x.device, _DTYPES[x.dtype]
         G, n, k = w.shape
         slots = order.shape[0]
@@ -422,17 +673,17 @@ class GroupedLinear(torch.autograd.Function):
                 launch(k, ctx.op, dx, None, None)
             few = min(k, 8)
             launch(few, 0, None, torch.empty(G, n, few, dtype=dtype, device=dev), db)
-        return dx, dw, db, None, None, None, None
+        return dx, dw, db, None, None, None, None, None
 
 
-def grouped_linear(x, w, plan, bias=None, x_op=None):
+def grouped_linear(x, w, plan, bias=None, x_op=None, keep8=False):
     """y (plan.slots, n), y[a] = op(x[row(a)]) w[g]^T + bias[g] for the slots a of group g, 0 for slots of no group.
 
     x (plan.rows, k), each row multiplied by the weights of all its choices, or (plan.slots, k), a row per
     slot; w (G, n, k), bias (G, n); x_op "silu" applies SiLU to x as it loads. float32 rows: products as of
     exact three-way bfloat16 splits (float32 accuracy); 16-bit rows: one product each, or with SiLU two, of its
     rounding to the rows' type and of the rest; sums in float32 (over a shared row's choices too). Differentiable in x, w and bias; gradients are
-    bitwise reproducible."""
+    bitwise reproducible. keep8: the backward reads x as 8 bits hold it (pack_rows) in place of x."""
     code_op = _X_OPS.get(x_op)
     if code_op is None:
         _fail("grouped_linear", f"x_op None or 'silu', got {x_op!r}")
@@ -440,7 +691,7 @@ def grouped_linear(x, w, plan, bias=None, x_op=None):
     _linear_args("grouped_linear", x, w, plan, bias, x.dtype)
     _check("grouped_linear", x, w=w, bias=bias, plan=plan.ptr)
     if _wants_grad(x, w, bias):
-        return GroupedLinear.apply(x, w, bias, plan.ptr, plan.order, plan, code_op)
+        return GroupedLinear.apply(x, w, bias, plan.ptr, plan.order, plan, code_op, bool(keep8))
     return _linear_fwd(x, w, plan, bias, code_op)
 
 
@@ -523,3 +774,121 @@ def expert_combine(y, weight, residual=None):
     if _wants_grad(y, weight, residual):
         return ExpertCombine.apply(y, weight, residual)
     return _combine_fwd(y, weight, residual)
+
+
+# ----------------------------------------------------------------------------- rows by expert and back
+def _places(like, p, order, slots):
+    """The inverse of a plan's order: the place of every slot, -1 of one that has none."""
+    place = torch.empty(slots, dtype=torch.int32, device=order.device)
+    _launch(like, "face_expert_places", "expert_places", p.data_ptr(), order.data_ptr(), slots, p.shape[0] - 1, place.data_ptr())
+    return place
+
+
+def _by_rows(slots, k, F):
+    """Whether rows are read once and written to their k places, which takes the order's inverse first, or gathered by
+    the order, read k times."""
+    return k > 1 and slots * F >= 1 << 22
+
+
+def _dispatch_fwd(x, p, order, k):
+    F, slots = x.shape[1], order.shape[0]
+    x2 = _rows(x, F)
+    place = _places(x, p, order, slots) if _by_rows(slots, k, F) else None
+    xs = torch.empty(slots, F, dtype=x.dtype, device=x.device)
+    _launch(x, "face_expert_dispatch", "expert_dispatch", x2.data_ptr(), x2.stride(0), k, p.data_ptr(), order.data_ptr(), ptr(place),
+            x.shape[0], p.shape[0] - 1, F, _DTYPES[x.dtype], xs.data_ptr())
+    return xs, place
+
+
+class ExpertDispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, order, k):
+        xs, place = _dispatch_fwd(x, p, order, k)
+        ctx.save_for_backward(p, order, place)
+        ctx.k, ctx.rows = k, x.shape[0]
+        return xs
+
+    @staticmethod
+    def backward(ctx, dxs):
+        _once("expert_dispatch", dxs)
+        p, order, place = ctx.saved_tensors
+        if place is None:
+            place = _places(dxs, p, order, order.shape[0])
+        return _return_fwd(dxs, place, None, None, ctx.rows, ctx.k), None, None, None
+
+
+def expert_dispatch(x, plan):
+    """xs (plan.slots, F): the rows of x laid out by group, xs[i] = x[row(plan.order[i])], zeros at the places of no
+    group, behind plan.ptr[G]: rows of one expert one after the other, for code of the user's own, or an exchange.
+    x (plan.rows, F), each row to the places of all its choices, or (plan.slots, F), a row per slot. Differentiable in x."""
+    name = "expert_dispatch"
+    _dtype(name, x)
+    if not isinstance(plan, GroupPlan):
+        _fail(name, f"plan: a GroupPlan, got {type(plan).__name__}")
+    if x.dim() != 2 or x.shape[0] not in (plan.rows, plan.slots) or not 1 <= x.shape[1] <= MAX_PACKED:
+        _fail(name, f"x of {plan.rows} rows or {plan.slots} slots and 1 to {MAX_PACKED} columns, got {tuple(x.shape)}")
+    _check(name, x, plan=plan.ptr)
+    k = _div(plan, x.shape[0])
+    if _wants_grad(x):
+        return ExpertDispatch.apply(x, plan.ptr, plan.order, k)
+    return _dispatch_fwd(x, plan.ptr, plan.order, k)[0]
+
+
+def _return_fwd(y, place, weight, residual, N, k):
+    F = y.shape[1]
+    y2, w = _rows(y, F), None if weight is None else weight.contiguous()
+    r = None if residual is None else _rows(residual, F)
+    out = torch.empty(N, F, dtype=y.dtype, device=y.device)
+    _launch(y, "face_expert_return_fwd", "expert_return_fwd", y2.data_ptr(), y2.stride(0), place.data_ptr(), ptr(w), ptr(r),
+            F if r is None else r.stride(0), N, k, F, _DTYPES[y.dtype], out.data_ptr())
+    return out
+
+
+class ExpertReturn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weight, residual, p, order, rows, k):
+        place = _places(y, p, order, order.shape[0])
+        # without a gradient of the weights the backward reads no row of y
+        ctx.save_for_backward(y if weight is not None and ctx.needs_input_grad[1] else None, weight, p, order, place)
+        ctx.rows, ctx.k = rows, k
+        return _return_fwd(y, place, weight, residual, rows, k)
+
+    @staticmethod
+    def backward(ctx, dout):
+        _once("expert_return", dout)
+        need_y, need_w, need_r = ctx.needs_input_grad[:3]
+        dy = dw = None
+        if need_y or need_w:
+            y, weight, p, order, place = ctx.saved_tensors
+            N, k, F = ctx.rows, ctx.k, dout.shape[1]
+            if need_y:
+                dy = torch.empty(N * k, F, dtype=dout.dtype, device=dout.device)
+            if need_w:
+                dw = torch.empty(N, k, dtype=torch.float32, device=dout.device)
+            d2, w = _rows(dout, F), None if weight is None else weight.contiguous()
+            y2 = _rows(y, F) if need_w else None
+            _launch(dout, "face_expert_return_bwd", "expert_return_bwd", d2.data_ptr(), d2.stride(0), ptr(y2),
+                    F if y2 is None else y2.stride(0), p.data_ptr(), order.data_ptr(), place.data_ptr(), ptr(w), N, k,
+                    p.shape[0] - 1, F, _DTYPES[dout.dtype], ptr(dy), ptr(dw))
+        return dy, dw, dout if need_r else None, None, None, None, None
+
+
+def expert_return(y, plan, weight=None, residual=None):
+    """out (plan.rows, F) = residual + the sum of a row's choices, weight[i, j] y[place of slot i k + j]: rows laid out by
+    expert_dispatch joined in the order of the rows. y (plan.slots, F), weight (plan.rows, plan.k) float32 or None (ones),
+    residual (plan.rows, F) like y or None. Slots of no group add nothing, and their rows of y are not read. Differentiable
+    in y, weight and residual."""
+    name = "expert_return"
+    _dtype(name, y)
+    if not isinstance(plan, GroupPlan):
+        _fail(name, f"plan: a GroupPlan, got {type(plan).__name__}")
+    if y.dim() != 2 or y.shape[0] != plan.slots or not 1 <= y.shape[1] <= MAX_PACKED:
+        _fail(name, f"y of {plan.slots} slots and 1 to {MAX_PACKED} columns, got {tuple(y.shape)}")
+    if weight is not None and (weight.shape != (plan.rows, plan.k) or weight.dtype != torch.float32):
+        _fail(name, f"weight ({plan.rows}, {plan.k}) float32, got {tuple(weight.shape)} {weight.dtype}")
+    if residual is not None and (residual.shape != (plan.rows, y.shape[1]) or residual.dtype != y.dtype):
+        _fail(name, f"residual ({plan.rows}, {y.shape[1]}) {y.dtype}, got {tuple(residual.shape)} {residual.dtype}")
+    _check(name, y, plan=plan.ptr, weight=weight, residual=residual)
+    if _wants_grad(y, weight, residual):
+        return ExpertReturn.apply(y, weight, residual, plan.ptr, plan.order, plan.rows, plan.k)
+    return _return_fwd(y, _places(y, plan.ptr, plan.order, plan.slots), weight, residual, plan.rows, plan.k)

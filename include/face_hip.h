@@ -619,6 +619,60 @@ int face_expert_combine_fwd(const void* y, int64_t ld_y, const float* weight, co
 int face_expert_combine_bwd(const void* dout, int64_t ld_d, const void* y, int64_t ld_y, const float* weight, int64_t N,
                             int32_t k, int32_t F, int32_t dtype, void* dy, float* dweight, void* stream);
 
+/* Layer norm: s = x + r (rounded to the rows' type; r and s NULL: s is x), h = (s - mean s) rstd with rstd = 1 /
+ * sqrt(mean((s - mean s)^2) + eps), y (N, F) = h w + b (b NULL: 0). With scale (and q in place of y) that row in e4m3 as of
+ * face_rms_norm_fwd; with block_scale (and q beside y) h is kept as of face_pack_rows. mean and rstd (N), for
+ * the backward, may be NULL (rstd not with block_scale or mean). F <= 65536. */
+int face_layer_norm_rows_fwd(const void* x, int64_t ld_x, const void* r, int64_t ld_r, int64_t N, int32_t F, int32_t dtype,
+                             const void* w, const void* b, float eps, void* y, void* s, void* q, float* scale,
+                             void* block_scale, float* mean, float* rstd, void* stream);
+/* dx (N, F) = gradient of s for dy and the gradient ds that arrives at s itself (either may be NULL = 0); dw, db (F).
+ * Each output may be NULL. From s and mean, or (s NULL) from h as it was kept, q and block_scale. work:
+ * face_layer_norm_rows_bwd_work bytes, for dw and db. Fixed summation order. */
+int64_t face_layer_norm_rows_bwd_work(int64_t N, int32_t F);
+int face_layer_norm_rows_bwd(const void* s, int64_t ld_s, const void* q, const void* block_scale, const float* mean,
+                             const float* rstd, const void* dy, int64_t ld_dy, const void* ds, int64_t ld_ds, int64_t N,
+                             int32_t F, int32_t dtype, const void* w, void* dx, void* dw, void* db, void* work,
+                             int64_t work_bytes, void* stream);
+
+/* Rows in 8 bits: q (N, F) e4m3, scale (N, ceil(F / 32)) e8m0 (2^(byte - 127)), one for each 32 columns, the least power
+ * of two >= 2^-126 that keeps their largest finite magnitude within 448; NaN and infinities become NaN. And back; values
+ * past the type's largest become it. */
+int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_t dtype, void* q, void* scale, void* stream);
+int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, int64_t ld_s, int64_t N, int32_t F, int32_t dtype,
+                     void* x, void* stream);
+
+/* y (N, F) = silu(a) b for the halves a and b of x (N, 2 F); with q (N, 2 F) and scale (N, 2, ceil(F / 32)) x is kept
+ * in 8 bits as above, each half in blocks of its own. dx (N, 2 F) for dy, from x or (x NULL) from q and scale. */
+int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32_t F, int32_t dtype, void* y, void* q, void* scale,
+                        void* stream);
+int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, const void* scale, const void* dy, int64_t ld_dy,
+                        int64_t N, int32_t F, int32_t dtype, void* dx, void* stream);
+
+/* y[i] (N, F) = factor table[index[i]], 0 where index (int32, or int64 if wide) lies outside [0, V). key (N) or NULL: the
+ * index in 32 bits, -1 outside. dtable (V, F) = factor times the sums of the rows of dy by key, 0 for entries without
+ * one; sums in fp32 in a fixed order. work: face_embed_bwd_work bytes, 256-byte aligned. */
+int face_embed_fwd(const void* table, int64_t ld_t, const void* index, int32_t wide, int64_t N, int64_t V, int32_t F,
+                   int32_t dtype, float factor, void* y, int32_t* key, void* stream);
+int64_t face_embed_bwd_work(int64_t N, int64_t V, int32_t F);
+int face_embed_bwd(const int32_t* key, const void* dy, int64_t ld_dy, int64_t N, int64_t V, int32_t F, int32_t dtype,
+                   float factor, void* dtable, void* work, int64_t work_bytes, void* stream);
+
+/* place (slots) = the inverse of a plan's order: where in it, before ptr[G], a slot is, -1 for slots that are not. */
+int face_expert_places(const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t* place, void* stream);
+/* xs[p] (N k, F) = x[order[p] / k], 0 for the places that hold no slot, from ptr[G] on; place NULL: gathered by order, else
+ * scattered by it. */
+int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, const int32_t* ptr, const int32_t* order,
+                         const int32_t* place, int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs, void* stream);
+/* out[i] (N, F) = r[i] + sum_j weight[i, j] y[place[i k + j]]; r NULL: 0, weight (N, k) NULL: 1. With weight and r NULL
+ * the gradient of face_expert_dispatch. */
+int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* place, const float* weight, const void* r,
+                           int64_t ld_r, int64_t N, int32_t k, int32_t F, int32_t dtype, void* out, void* stream);
+/* dy (N k, F) = weight dout at the slots' places, 0 elsewhere, dweight (N, k) = dout . y; either may be NULL. */
+int face_expert_return_bwd(const void* dout, int64_t ld_d, const void* y, int64_t ld_y, const int32_t* ptr,
+                           const int32_t* order, const int32_t* place, const float* weight, int64_t N, int32_t k, int32_t G,
+                           int32_t F, int32_t dtype, void* dy, float* dweight, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
