@@ -68,7 +68,7 @@ __device__ __forceinline__ KeptPiece hold_kept(const uint8_t* q, const uint8_t* 
         const v2u_any v = *reinterpret_cast<const v2u_any*>(q + c);
         k.lo = v[0];
         k.hi = v[1];
-    } else {
+    } else if (c < F) {
 #pragma unroll
         for (int e = 0; e < kPiece; ++e)
             if (c + e < F) (e < 4 ? k.lo : k.hi) |= (uint32_t)q[c + e] << (8 * (e & 3));
@@ -76,9 +76,8 @@ __device__ __forceinline__ KeptPiece hold_kept(const uint8_t* q, const uint8_t* 
     if (c < F) k.scale = scale[c / kKeptBlock];
     return k;
 }
-// Its values; zeros beyond the row's end. Of the bytes that store_kept does not write, 0 stands for 2^-127 and 255 for NaN.
-__device__ __forceinline__ void kept_values(const KeptPiece& k, float x[kPiece]) {
-    const float s = __builtin_bit_cast(float, k.scale - 1 < 254u ? k.scale << 23 : (k.scale ? 0x7fc00000u : 0x00400000u));
+// Its values at scale s; zeros beyond the row's end.
+__device__ __forceinline__ void kept_values_at(const KeptPiece& k, float s, float x[kPiece]) {
     const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, true);
     const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, true);
 #pragma unroll
@@ -88,10 +87,25 @@ __device__ __forceinline__ void kept_values(const KeptPiece& k, float x[kPiece])
         x[4 + e] = c[e] * s;
         x[6 + e] = d[e] * s;
     }
+}
+// Those of a row that a kernel kept, far from the largest float.
+__device__ __forceinline__ void kept_values_near(const KeptPiece& k, float x[kPiece]) {
+    kept_values_at(k, __builtin_bit_cast(float, k.scale << 23), x);
+}
+// Those of any row. Of the scales that store_kept does not write, 0 stands for 2^-127 and 255 for NaN.
+__device__ __forceinline__ void kept_values(const KeptPiece& k, float x[kPiece]) {
+    kept_values_at(k, __builtin_bit_cast(float, k.scale - 1 < 254u ? k.scale << 23 : (k.scale ? 0x7fc00000u : 0x00400000u)), x);
     if (k.scale >= 247u) {                       // 256 2^120: what the largest floats round to
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) x[e] = within(x[e], 0x1.fffffep127f);
     }
+}
+
+// The same of a whole piece.
+__device__ __forceinline__ KeptPiece hold_kept(const uint8_t* q, const uint8_t* scale, int c) {
+    typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(1)));
+    const v2u_any v = *reinterpret_cast<const v2u_any*>(q + c);
+    return {v[0], v[1], scale[c / kKeptBlock]};
 }
 
 // A piece of a row in its memory's type, on its way: half the registers of its values where they are 16-bit.
@@ -100,11 +114,17 @@ struct RawPiece {
     v4u a[sizeof(T) / 2];
 };
 template <typename T>
+__device__ __forceinline__ RawPiece<T> hold_raw(const T* p) {
+    RawPiece<T> r;
+    r.a[0] = ld16(p);
+    if constexpr (sizeof(T) == 4) r.a[1] = ld16(p + 4);
+    return r;
+}
+template <typename T>
 __device__ __forceinline__ RawPiece<T> hold_raw(const T* p, int left) {
     RawPiece<T> r = {};
     if (left >= kPiece) {
-        r.a[0] = ld16(p);
-        if constexpr (sizeof(T) == 4) r.a[1] = ld16(p + 4);
+        r = hold_raw(p);
     } else if (left > 0) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll

@@ -9,6 +9,9 @@
 // first, then the squares around it, and with them the sum of the differences, which corrects the mean's own rounding.
 // Longer rows are read three times by a workgroup of 1024. The backward takes mean and rstd (8 bytes a row) from the
 // forward, so that its one reduction follows its only reads. Bound by bytes.
+// A row lies in the registers of 16 lanes up to 256 columns, of a wave up to 2560, of four up to 10240, of eight up to 16384,
+// in as few pieces a lane as hold it: only the last of them may end before the lane's, so the others are loaded and stored
+// without a test. With a test at each (and rounded-up shapes) the backward of 100,000 x 2304 bf16 took 615 us for 354.
 #include "kept.h"
 
 namespace face {
@@ -28,9 +31,9 @@ struct LnFwdArgs {
     float *mean, *rstd;                // may be null
 };
 
-// f(e, inside) of the piece at column c: `inside` false beyond the row.
-template <int LANES>
-__device__ __forceinline__ bool whole_unit(int u, int F) { return kPiece * LANES * (u + 1) <= F; }
+// Columns of a row that are left at a lane's piece u of U: only its last may be cut short.
+template <int U>
+__device__ __forceinline__ int left_at(int u, int c, int F) { return u + 1 < U ? kPiece : F - c; }
 
 template <typename T>
 __device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, float rs, const T* w, const T* b, int left,
@@ -46,8 +49,8 @@ __device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, floa
 }
 
 template <typename T, int LANES, int U, int MODE>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
-    constexpr int kRows = 256 / LANES;
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwdArgs a) {
+    constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
     __shared__ float part[LANES / 32 + 1];
     const int lane = threadIdx.x % LANES, F = a.F;
     const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
@@ -58,19 +61,19 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int c = kPiece * (lane + LANES * u);
-        load_piece(x + c, F - c, v[u]);
+        load_piece(x + c, left_at<U>(u, c, F), v[u]);
     }
     if (a.r) {
         const T* r = (const T*)a.r + n * a.ld_r;
         T* s = (T*)a.s + n * F;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u);
+            const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
             float t[kPiece];
-            load_piece(r + c, F - c, t);
+            load_piece(r + c, left, t);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) v[u][e] = to_f(from_f<T>(v[u][e] + t[e]));
-            store_piece(s + c, F - c, v[u]);
+            store_piece(s + c, left, v[u]);
         }
     }
     float sum = 0.f;
@@ -83,21 +86,12 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
     float d1 = 0.f, d2 = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int left = F - kPiece * (lane + LANES * u);
-        if (whole_unit<LANES>(u, F)) {
+        const int left = left_at<U>(u, kPiece * (lane + LANES * u), F);
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) {
-                const float d = v[u][e] - mean;
-                d1 += d;
-                d2 = fmaf(d, d, d2);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < kPiece; ++e) {
-                const float d = e < left ? v[u][e] - mean : 0.f;
-                d1 += d;
-                d2 = fmaf(d, d, d2);
-            }
+        for (int e = 0; e < kPiece; ++e) {
+            const float d = e < left ? v[u][e] - mean : 0.f;
+            d1 += d;
+            d2 = fmaf(d, d, d2);
         }
     }
     row_sum2<LANES>(d1, d2, part);
@@ -112,10 +106,10 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
     uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int c = kPiece * (lane + LANES * u);
+        const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
         float h[kPiece], y[kPiece];
-        ln_piece(v[u], mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
-        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
+        ln_piece(v[u], mean, rs, w + c, b ? b + c : nullptr, left, h, y);
+        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, c + left, h);
         if constexpr (MODE == kLnQ8) {
             // the magnitudes compare as integers, a NaN above everything: its row gets a NaN scale and no number
 #pragma unroll
@@ -125,7 +119,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
                 top = m > top ? m : top;
             }
         } else {
-            store_piece((T*)a.y + n * F + c, F - c, y);
+            store_piece((T*)a.y + n * F + c, left, y);
         }
     }
     if constexpr (MODE == kLnQ8) {
@@ -136,7 +130,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = kPiece * (lane + LANES * u);
-            if (c < F) store_e4m3(a.q + n * F + c, F - c, v[u], inv);
+            store_e4m3(a.q + n * F + c, left_at<U>(u, c, F), v[u], inv);
         }
         if (lane == 0) a.scale[n] = sc;
     }
@@ -245,8 +239,8 @@ struct LnBwdArgs {
 template <typename T, bool KEPT>
 struct LnRow {
     RawPiece<T> a;
-    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c) {
-        a = hold_raw((const T*)g.s + n * g.ld_s + c, g.F - c);
+    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
+        a = hold_raw((const T*)g.s + n * g.ld_s + c, left);
     }
     __device__ __forceinline__ void values(float mean, float rs, float h[kPiece]) const {
         raw_values<T>(a, h);
@@ -257,10 +251,10 @@ struct LnRow {
 template <typename T>
 struct LnRow<T, true> {
     KeptPiece a;
-    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c) {
-        a = hold_kept(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, g.F);
+    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
+        a = hold_kept(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, c + left);
     }
-    __device__ __forceinline__ void values(float, float, float h[kPiece]) const { kept_values(a, h); }
+    __device__ __forceinline__ void values(float, float, float h[kPiece]) const { kept_values_near(a, h); }
 };
 
 // A workgroup takes rows blockIdx, blockIdx + grid, ... and keeps its columns' sums of dw and db in registers over
@@ -268,8 +262,8 @@ struct LnRow<T, true> {
 // atomics. All of a row's reads are issued before the first is used. Beyond a row's end dy is 0, and h is finite where
 // the row's is.
 template <typename T, int LANES, int U, bool KEPT>
-__global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
-    constexpr int kRows = 256 / LANES;
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwdArgs a) {
+    constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
     __shared__ float part[LANES / 32 + 1];
     __shared__ float sums[kRows > 1 ? 2 * LANES * U * kPiece : 1];
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, F = a.F;
@@ -280,10 +274,10 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
         RawPiece<T> dy[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u);
-            row[u].hold(a, n, c);
-            dy[u] = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
-            ds[u] = a.ds && a.dx ? hold_raw((const T*)a.ds + n * a.ld_ds + c, F - c) : RawPiece<T>{};
+            const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
+            row[u].hold(a, n, c, left);
+            dy[u] = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, left) : RawPiece<T>{};
+            ds[u] = a.ds && a.dx ? hold_raw((const T*)a.ds + n * a.ld_ds + c, left) : RawPiece<T>{};
         }
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
@@ -293,7 +287,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
             float h[kPiece], d[kPiece], w[kPiece];
             row[u].values(mean, rs, h);
             raw_values<T>(dy[u], d);
-            load_piece((const T*)a.w + c, F - c, w);
+            load_piece((const T*)a.w + c, left_at<U>(u, c, F), w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
                 ab[u][e] += d[e];
@@ -314,10 +308,10 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
             row[u].values(mean, rs, h);
             raw_values<T>(dy[u], d);
             raw_values<T>(ds[u], o);
-            load_piece((const T*)a.w + c, F - c, w);
+            load_piece((const T*)a.w + c, left_at<U>(u, c, F), w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
-            store_piece((T*)a.dx + n * F + c, F - c, o);
+            store_piece((T*)a.dx + n * F + c, left_at<U>(u, c, F), o);
         }
     }
     if (!a.part) return;
@@ -349,10 +343,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
     for (int u = 0; u < U; ++u) {
         const int c = kPiece * (lane + LANES * u);
         float* p = a.part + (int64_t)blockIdx.x * 2 * F;
-        if (c < F) {
-            store_piece(p + c, F - c, aw[u]);
-            store_piece(p + F + c, F - c, ab[u]);
-        }
+        store_piece(p + c, left_at<U>(u, c, F), aw[u]);
+        store_piece(p + F + c, left_at<U>(u, c, F), ab[u]);
     }
 }
 
@@ -371,7 +363,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnBwdArgs a) {
         float sg = 0.f, sh = 0.f;
         auto load = [&](int c, float h[kPiece], float d[kPiece], float w[kPiece]) {
             LnRow<T, KEPT> row;
-            row.hold(a, n, c);
+            row.hold(a, n, c, F - c);
             row.values(mean, rs, h);
             RawPiece<T> r = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
             raw_values<T>(r, d);
@@ -444,30 +436,37 @@ __global__ __launch_bounds__(1024) void ln_column_sum_kernel(const float* __rest
 
 constexpr int kLnHeld = 16384;                   // longest row that stays in registers
 constexpr int kLnMax = 65536;
-constexpr int64_t kLnBwdGroups = 1024;
-static inline int64_t ln_bwd_grid(int64_t N, int F) {
-    const RowShape sh = row_shape(F);
-    const int64_t rows = F > kLnHeld ? 1 : 256 / sh.lanes, need = (N + rows - 1) / rows;
-    return need < kLnBwdGroups ? need : kLnBwdGroups;
-}
 
-// The variants: lanes per row and pieces per lane.
-#define FACE_LN_ROWS                                                                                               \
+// The variants: lanes per row and pieces per lane, the fewest that hold the row.
+#define FACE_LN_ROWS                                                                                                 \
     FACE_ROW(16, 1) FACE_ROW(16, 2) FACE_ROW(64, 1) FACE_ROW(64, 2) FACE_ROW(64, 3) FACE_ROW(64, 4) FACE_ROW(64, 5) \
-    FACE_ROW(64, 6) FACE_ROW(64, 8) FACE_ROW(256, 3) FACE_ROW(256, 4) FACE_ROW(256, 5) FACE_ROW(256, 6) FACE_ROW(256, 8)
+    FACE_ROW(256, 2) FACE_ROW(256, 3) FACE_ROW(256, 4) FACE_ROW(256, 5) FACE_ROW(512, 3) FACE_ROW(512, 4)
+static inline RowShape ln_shape(int F) {
+    const int p = (F + kPiece - 1) / kPiece, lanes = p <= 32 ? 16 : (p <= 320 ? 64 : (p <= 1280 ? 256 : 512));
+    return {lanes, (p + lanes - 1) / lanes};
+}
+static inline int64_t ln_rows(int F) { return F > 2560 ? 1 : 256 / ln_shape(F).lanes; }
+
+// Workgroups of the backward: as many as the registers of its pieces let run at once on 256 CUs, so that all of them
+// start together and end together (100,000 x 1440 bf16: 768 take 226 us, 512 238, 1024 259).
+static inline int64_t ln_bwd_grid(int64_t N, int F, bool wide) {
+    const RowShape sh = ln_shape(F);
+    const int per = F > kLnHeld ? 2 : sh.lanes == 512 ? 1 : sh.units <= 2 ? (wide ? 3 : 4) : sh.units == 3 && !wide ? 3 : 2;
+    const int64_t need = (N + ln_rows(F) - 1) / ln_rows(F);
+    return need < 256 * per ? need : 256 * per;
+}
 
 template <typename T, int MODE>
 static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
-    const RowShape sh = row_shape(a.F);
-    const int rows = a.F > kLnHeld ? 1 : 256 / sh.lanes;
-    const int64_t blocks = (a.N + rows - 1) / rows;
+    const RowShape sh = ln_shape(a.F);
+    const int64_t rows = ln_rows(a.F), blocks = (a.N + rows - 1) / rows;
     if (blocks > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks);
     if (a.F > kLnHeld) {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);
     }
 #define FACE_ROW(L_, U_) \
-    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, U_, MODE>), grid, dim3(256), 0, st, a);
+    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, U_, MODE>), grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
     FACE_LN_ROWS
 #undef FACE_ROW
     FACE_LAUNCH_CHECK();
@@ -476,15 +475,15 @@ static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
 
 template <typename T, bool KEPT>
 static int launch_ln_bwd(const LnBwdArgs& a, T* dw, T* db, hipStream_t st) {
-    const RowShape sh = row_shape(a.F);
-    const int64_t blocks = ln_bwd_grid(a.N, a.F);
+    const RowShape sh = ln_shape(a.F);
+    const int64_t blocks = ln_bwd_grid(a.N, a.F, sizeof(T) == 4);
     if (blocks) {
         const dim3 grid((unsigned)blocks);
         if (a.F > kLnHeld) {
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, KEPT>), grid, dim3(1024), 0, st, a);
         }
 #define FACE_ROW(L_, U_) \
-    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, U_, KEPT>), grid, dim3(256), 0, st, a);
+    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, U_, KEPT>), grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
         FACE_LN_ROWS
 #undef FACE_ROW
         FACE_LAUNCH_CHECK();
@@ -526,7 +525,7 @@ extern "C" int face_layer_norm_rows_fwd(const void* x, int64_t ld_x, const void*
 
 extern "C" int64_t face_layer_norm_rows_bwd_work(int64_t N, int32_t F) {
     if (N <= 0 || F <= 0 || F > kLnMax) return 0;
-    return ln_bwd_grid(N, F) * F * 8;
+    return ln_bwd_grid(N, F, false) * F * 8;
 }
 
 extern "C" int face_layer_norm_rows_bwd(const void* s, int64_t ld_s, const void* q, const void* block_scale, const float* mean,
