@@ -14,26 +14,90 @@
 
 namespace face {
 
-template <typename T, typename I>
+// Sixteen bytes of a row, so that neighbouring lanes move neighbouring bytes whatever the type.
+template <typename T>
+struct Sixteen {
+    static constexpr int E = 16 / (int)sizeof(T);
+    v4u a;
+};
+template <typename T>
+__device__ __forceinline__ Sixteen<T> hold16(const T* p, int left) {
+    Sixteen<T> r = {};
+    if (left >= Sixteen<T>::E) {
+        r.a = ld16(p);
+    } else if (left > 0) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) r.a[e] = __builtin_bit_cast(uint32_t, p[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) r.a[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void values16(const Sixteen<T>& r, float x[Sixteen<T>::E]) {
+    if constexpr (sizeof(T) == 4) {
+        const v4f v = __builtin_bit_cast(v4f, r.a);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpack2<T>(r.a[e], x[2 * e], x[2 * e + 1]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int left, const float x[Sixteen<T>::E]) {
+    if (left >= Sixteen<T>::E) {
+        if constexpr (sizeof(T) == 4) {
+            st16(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
+        } else {
+            v4u a;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
+            st16(p, a);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < Sixteen<T>::E; ++e)
+            if (e < left) p[e] = from_f<T>(x[e]);
+    }
+}
+
+// R rows per group of lanes, a workgroup's groups side by side, so that the rows' indices, then their entries, are on
+// their way together.
+template <typename T, typename I, int R>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t ld, const I* __restrict__ index,
                                                         int64_t N, int64_t V, int F, float factor, int lg, T* __restrict__ y,
                                                         int32_t* __restrict__ key) {
-    const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
-    if (n >= N) return;
-    const int lane = threadIdx.x & ((1 << lg) - 1);
-    const I v = index[n];
-    const bool in = v >= 0 && v < V;
-    if (key && lane == 0 && blockIdx.y == 0) key[n] = in ? (int32_t)v : -1;
-    const T* from = table + (in ? (int64_t)v : 0) * ld;
-#pragma unroll 4
-    for (int c = kPiece * lane; c < F; c += kPiece << lg) {
-        float x[kPiece] = {};
-        if (in) {
-            load_piece(from + c, F - c, x);
+    constexpr int E = Sixteen<T>::E;
+    const int groups = 256 >> lg, lane = threadIdx.x & ((1 << lg) - 1);
+    const int64_t n0 = (int64_t)blockIdx.x * groups * R + (threadIdx.x >> lg);
+    I v[R];
+    bool in[R];
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) x[e] *= factor;
+    for (int i = 0; i < R; ++i) {
+        const int64_t n = n0 + i * groups;
+        v[i] = n < N ? index[n] : (I)-1;
+        in[i] = v[i] >= 0 && v[i] < V;
+        if (key && lane == 0 && n < N) key[n] = in[i] ? (int32_t)v[i] : -1;
+    }
+    for (int c = E * lane; c < F; c += E << lg) {
+        Sixteen<T> r[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) r[i] = hold16(table + (in[i] ? (int64_t)v[i] : 0) * ld + c, in[i] ? F - c : 0);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t n = n0 + i * groups;
+            float x[E];
+            values16<T>(r[i], x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = in[i] ? x[e] * factor : 0.f;
+            if (n < N) store16(y + n * F + c, F - c, x);
         }
-        store_piece(y + n * F + c, F - c, x);
     }
 }
 
@@ -155,51 +219,115 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool some, int bits) 
     }
     return m;
 }
-// Counts of each wave's share of a segment's digits, cnt[wave][digits] in LDS.
-__device__ __forceinline__ void sort_count(const int32_t* key, int64_t a0, int64_t a1, uint32_t V, int shift, int bits, int* cnt) {
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, D = 1 << bits;
-    for (int i = threadIdx.x; i < kSortWaves * D; i += kSortThreads) cnt[i] = 0;
-    __syncthreads();
+// A segment is shared out to the waves, a wave's share taken 64 keys at a time; up to kSortHeld of these are loaded together
+// (each load by itself was a trip to memory: 15 us a pass for 9 with a million keys).
+constexpr int kSortHeld = 8;
+struct SortShare {
+    int64_t begin, end;
+};
+__device__ __forceinline__ SortShare sort_share(int64_t a0, int64_t a1) {
     const int64_t per = (a1 - a0 + kSortThreads - 1) / kSortThreads * kWave;
-    const int64_t b0 = a0 + wave * per, b1 = b0 + per < a1 ? b0 + per : a1;
-    for (int64_t a = b0; a < b1; a += kWave) {
-        const bool some = a + lane < b1;
-        const uint32_t d = some ? (sort_key(key, a + lane, V) >> shift) & (D - 1) : 0;
-        const uint64_t m = same_digit(d, some, bits);
-        if (some && (m & ((1ull << lane) - 1)) == 0) cnt[wave * D + d] += __popcll(m);
-        __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
+    const int64_t b = a0 + threadIdx.x / kWave * per;
+    return {b, b + per < a1 ? b + per : a1};
 }
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int32_t* __restrict__ key, int64_t N, int64_t seg,
-                                                                  uint32_t V, int shift, int bits, int32_t* __restrict__ count) {
+__device__ __forceinline__ void sort_hold(const int32_t* key, int64_t a, const SortShare& s, uint32_t V, uint32_t k[kSortHeld]) {
+#pragma unroll
+    for (int i = 0; i < kSortHeld; ++i) {
+        const int64_t at = a + i * kWave + threadIdx.x % kWave;
+        k[i] = at < s.end ? sort_key(key, at, V) : 0;
+    }
+}
+// Counts of the wave's share's digits, cnt[digits] in LDS. `k`: the share's first kSortHeld loads.
+__device__ __forceinline__ void sort_count(const int32_t* key, const SortShare& s, uint32_t V, int shift, int bits, int* cnt,
+                                           const uint32_t k0[kSortHeld]) {
+    const int lane = threadIdx.x % kWave;
+    uint32_t k[kSortHeld];
+#pragma unroll
+    for (int i = 0; i < kSortHeld; ++i) k[i] = k0[i];
+    for (int64_t a = s.begin; a < s.end; a += kSortHeld * kWave) {
+        if (a != s.begin) sort_hold(key, a, s, V, k);
+#pragma unroll
+        for (int i = 0; i < kSortHeld; ++i) {
+            if (a + i * kWave >= s.end) break;
+            const bool some = a + i * kWave + lane < s.end;
+            const uint32_t d = some ? (k[i] >> shift) & ((1u << bits) - 1) : 0;
+            const uint64_t m = same_digit(d, some, bits);
+            if (some && (m & ((1ull << lane) - 1)) == 0) cnt[d] += __popcll(m);
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+// Workgroups behind the segments' clear the table's gradient, `zero` of 16-byte pieces each.
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int32_t* __restrict__ key, int64_t N, int64_t seg, int segs,
+                                                                  uint32_t V, int shift, int bits, int32_t* __restrict__ count,
+                                                                  char* __restrict__ out, int64_t out_bytes) {
     __shared__ int cnt[kSortWaves << kSortBits];
+    if ((int)blockIdx.x >= segs) {
+        const int64_t begin = ((int64_t)(blockIdx.x - segs) * kSortThreads + threadIdx.x) * 16;
+        for (int64_t at = begin; at < out_bytes; at += (int64_t)(gridDim.x - segs) * kSortThreads * 16) {
+            if (at + 16 <= out_bytes)
+                st16(out + at, (v4u){0, 0, 0, 0});
+            else
+                for (int64_t i = at; i < out_bytes; i += 2) *(uint16_t*)(out + i) = 0;
+        }
+        return;
+    }
     const int D = 1 << bits;
     const int64_t a0 = blockIdx.x * seg, a1 = a0 + seg < N ? a0 + seg : N;
-    sort_count(key, a0, a1, V, shift, bits, cnt);
+    const SortShare s = sort_share(a0, a1);
+    uint32_t k[kSortHeld];
+    sort_hold(key, s.begin, s, V, k);
+    for (int i = threadIdx.x; i < kSortWaves * D; i += kSortThreads) cnt[i] = 0;
+    __syncthreads();
+    sort_count(key, s, V, shift, bits, cnt + threadIdx.x / kWave * D, k);
+    __syncthreads();
     for (int d = threadIdx.x; d < D; d += kSortThreads) {
-        int s = 0;
-        for (int w = 0; w < kSortWaves; ++w) s += cnt[w * D + d];
-        count[(int64_t)d * gridDim.x + blockIdx.x] = s;
+        int c = 0;
+        for (int w = 0; w < kSortWaves; ++w) c += cnt[w * D + d];
+        count[(int64_t)d * segs + blockIdx.x] = c;
     }
 }
-// count (D, segs): every digit's row becomes its exclusive sums, tot its total. One wave per digit.
-__global__ __launch_bounds__(256) void sort_rows_kernel(int32_t* __restrict__ count, int segs, int D, int32_t* __restrict__ tot) {
-    const int d = blockIdx.x * 4 + threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    if (d >= D) return;
-    int32_t* row = count + (int64_t)d * segs;
-    int run = 0;
-    for (int b0 = 0; b0 < segs; b0 += kWave) {
-        const int b = b0 + lane, c = b < segs ? row[b] : 0;
-        int s = c;
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int t = __shfl_up(s, o, kWave);
-            if (lane >= o) s += t;
-        }
-        if (b < segs) row[b] = run + s - c;
-        run += __shfl(s, kWave - 1, kWave);
+// Exclusive sums of a value per thread over a workgroup of 256, and the total. `part`: LDS, 4.
+__device__ __forceinline__ int sums_before(int c, int* part, int& total) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    int s = c;
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int t = __shfl_up(s, o, kWave);
+        if (lane >= o) s += t;
     }
-    if (lane == 0) tot[d] = run;
+    __syncthreads();
+    if (lane == kWave - 1) part[wave] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int w = 0; w < 4; ++w) {
+        before += w < wave ? part[w] : 0;
+        total += part[w];
+    }
+    return before + s - c;
+}
+// count (D, segs): every digit's row becomes its exclusive sums, tot its total. A workgroup per digit, four segments a
+// thread at a time.
+__global__ __launch_bounds__(256) void sort_rows_kernel(int32_t* __restrict__ count, int segs, int32_t* __restrict__ tot) {
+    __shared__ int part[4];
+    int32_t* row = count + (int64_t)blockIdx.x * segs;
+    int run = 0;
+    for (int b0 = 0; b0 < segs; b0 += 1024) {
+        const int b = b0 + 4 * threadIdx.x;
+        int c[4], sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = b + i < segs ? row[b + i] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += c[i];
+        int at = run + sums_before(sum, part, total);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + i < segs) row[b + i] = at;
+            at += c[i];
+        }
+        run += total;
+    }
+    if (threadIdx.x == 0) tot[blockIdx.x] = run;
 }
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t* __restrict__ key, const int32_t* __restrict__ row,
                                                                   int64_t N, int64_t seg, uint32_t V, int shift, int bits,
@@ -209,46 +337,70 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
     __shared__ int cnt[kSortWaves << kSortBits], begin[1 << kSortBits];
     const int D = 1 << bits, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const int64_t a0 = blockIdx.x * seg, a1 = a0 + seg < N ? a0 + seg : N;
-    sort_count(key, a0, a1, V, shift, bits, cnt);
+    const SortShare s = sort_share(a0, a1);
+    uint32_t k[kSortHeld];
+    int32_t r[kSortHeld];
+    auto hold_rows = [&](int64_t a) {
+#pragma unroll
+        for (int i = 0; i < kSortHeld; ++i) {
+            const int64_t at = a + i * kWave + lane;
+            r[i] = row && at < s.end ? row[at] : (int32_t)at;
+        }
+    };
+    sort_hold(key, s.begin, s, V, k);
+    hold_rows(s.begin);
+    const int mine_tot = (int)threadIdx.x < D ? tot[threadIdx.x] : 0;
+    const int mine_count = (int)threadIdx.x < D ? count[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] : 0;
+    for (int i = threadIdx.x; i < kSortWaves * D; i += kSortThreads) cnt[i] = 0;
+    __syncthreads();
+    sort_count(key, s, V, shift, bits, cnt + wave * D, k);
+    if ((int)threadIdx.x < D) begin[threadIdx.x] = mine_tot;
+    __syncthreads();
     if (wave == 0) {                             // exclusive sums of the digits' totals
         int run = 0;
         for (int d0 = 0; d0 < D; d0 += kWave) {
-            const int d = d0 + lane, c = d < D ? tot[d] : 0;
-            int s = c;
+            const int d = d0 + lane, c = d < D ? begin[d] : 0;
+            int t = c;
             for (int o = 1; o < kWave; o <<= 1) {
-                const int t = __shfl_up(s, o, kWave);
-                if (lane >= o) s += t;
+                const int w = __shfl_up(t, o, kWave);
+                if (lane >= o) t += w;
             }
-            if (d < D) begin[d] = run + s - c;
-            run += __shfl(s, kWave - 1, kWave);
+            if (d < D) begin[d] = run + t - c;
+            run += __shfl(t, kWave - 1, kWave);
         }
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kSortThreads) {
-        int at = begin[d] + count[(int64_t)d * gridDim.x + blockIdx.x];
+    if ((int)threadIdx.x < D) {
+        int at = begin[threadIdx.x] + mine_count;
         for (int w = 0; w < kSortWaves; ++w) {
-            const int c = cnt[w * D + d];
-            cnt[w * D + d] = at;
+            const int c = cnt[w * D + threadIdx.x];
+            cnt[w * D + threadIdx.x] = at;
             at += c;
         }
     }
     __syncthreads();
-    const int64_t per = (a1 - a0 + kSortThreads - 1) / kSortThreads * kWave;
-    const int64_t b0 = a0 + wave * per, b1 = b0 + per < a1 ? b0 + per : a1;
     volatile int* mine = cnt + wave * D;
-    for (int64_t a = b0; a < b1; a += kWave) {
-        const bool some = a + lane < b1;
-        const uint32_t k = some ? sort_key(key, a + lane, V) : 0, d = (k >> shift) & (D - 1);
-        const uint64_t m = same_digit(d, some, bits);
-        const int rank = __popcll(m & ((1ull << lane) - 1));
-        if (some) {
-            const int at = mine[d];
-            key_out[at + rank] = (int32_t)k;
-            row_out[at + rank] = row ? row[a + lane] : (int32_t)(a + lane);
-            __builtin_amdgcn_wave_barrier();     // every lane has read the place before the first one moves it on
-            if (rank == 0) mine[d] = at + __popcll(m);
+    for (int64_t a = s.begin; a < s.end; a += kSortHeld * kWave) {
+        if (s.end - s.begin > kSortHeld * kWave) {
+            sort_hold(key, a, s, V, k);
+            hold_rows(a);
         }
-        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kSortHeld; ++i) {
+            if (a + i * kWave >= s.end) break;
+            const bool some = a + i * kWave + lane < s.end;
+            const uint32_t d = some ? (k[i] >> shift) & (D - 1) : 0;
+            const uint64_t m = same_digit(d, some, bits);
+            const int rank = __popcll(m & ((1ull << lane) - 1));
+            if (some) {
+                const int at = mine[d];
+                key_out[at + rank] = (int32_t)k[i];
+                row_out[at + rank] = r[i];
+                __builtin_amdgcn_wave_barrier(); // every lane has read the place before the first one moves it on
+                if (rank == 0) mine[d] = at + __popcll(m);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
@@ -262,39 +414,49 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(T* __restrict__ out, in
 }
 
 // Groups of LC lanes, C sorted rows each. part (shares, 2, F): a run that comes from the share before (0), one that begins
-// here and goes on (1).
+// here and goes on (1). The next rows' numbers are on their way while the present ones are added.
 template <typename T, int LC>
 __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restrict__ key, const int32_t* __restrict__ row,
                                                          const T* __restrict__ dy, int64_t ld, int64_t N, int64_t C, int V, int F,
                                                          float factor, float* __restrict__ part, T* __restrict__ out) {
+    constexpr int E = Sixteen<T>::E, U = 8;
     const int64_t s = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LC;
     const int64_t begin = s * C, end = begin + C < N ? begin + C : N;
-    const int c = kPiece * ((int)(threadIdx.x % LC) + LC * (int)blockIdx.y), left = F - c;
+    const int c = E * ((int)(threadIdx.x % LC) + LC * (int)blockIdx.y), left = F - c;
     if (begin >= N || left <= 0) return;
     int cur = key[begin];
     if (cur >= V) return;
     bool from_before = begin > 0 && key[begin - 1] == cur;
-    float acc[kPiece] = {};
+    float acc[E] = {};
     auto flush = [&](bool goes_on) {
         if (from_before || goes_on) {
-            store_piece(part + (2 * s + (from_before ? 0 : 1)) * F + c, left, acc);
-        } else {
-            float o[kPiece];
+            float* p = part + (2 * s + (from_before ? 0 : 1)) * F + c;
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) o[e] = factor * acc[e];
-            store_piece(out + (int64_t)cur * F + c, left, o);
+            for (int e = 0; e < E; ++e)
+                if (e < left) p[e] = acc[e];
+        } else {
+            float o[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = factor * acc[e];
+            store16(out + (int64_t)cur * F + c, left, o);
         }
     };
-    constexpr int U = 8;
-    for (int64_t p = begin; p < end; p += U) {
-        int k[U];
-        RawPiece<T> r[U];
+    int k[U], next_k[U];
+    int32_t at[U], next_at[U];
+    auto numbers = [&](int64_t p, int kk[U], int32_t rr[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t q = p + u < end ? p + u : end - 1;
-            k[u] = key[q];
-            r[u] = hold_raw(dy + (int64_t)row[q] * ld + c, left);
+            kk[u] = key[q];
+            rr[u] = row[q];
         }
+    };
+    numbers(begin, k, at);
+    for (int64_t p = begin; p < end; p += U) {
+        Sixteen<T> r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = hold16(dy + (int64_t)at[u] * ld + c, left);
+        if (p + U < end) numbers(p + U, next_k, next_at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (p + u >= end) break;
@@ -304,12 +466,17 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restri
                 from_before = false;
                 if (cur >= V) return;
 #pragma unroll
-                for (int e = 0; e < kPiece; ++e) acc[e] = 0.f;
+                for (int e = 0; e < E; ++e) acc[e] = 0.f;
             }
-            float x[kPiece];
-            raw_values<T>(r[u], x);
+            float x[E];
+            values16<T>(r[u], x);
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) acc[e] += x[e];
+            for (int e = 0; e < E; ++e) acc[e] += x[e];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = next_k[u];
+            at[u] = next_at[u];
         }
     }
     flush(end < N && key[end] == cur);
@@ -334,12 +501,19 @@ __global__ __launch_bounds__(1024) void embed_runs_join_kernel(const int32_t* __
     if (s + 1 < shares) {
         const int64_t begin = s * C, end = begin + C;                    // not the last share: a whole one
         const int k = key[end - 1];
-        if (k < V && key[end] == k && (key[begin] != k || begin == 0 || key[begin - 1] != k)) {
-            int64_t lo = s + 1, hi = shares - 1;                         // the last share that begins with k
-            while (lo < hi) {
-                const int64_t mid = (lo + hi + 1) >> 1;
-                if (key[mid * C] == k) lo = mid;
-                else hi = mid - 1;
+        // how many of the next shares begin with k: their first keys together, then by halves
+        const int64_t probe = s + 1 + lane < shares ? s + 1 + lane : shares - 1;
+        const int first = key[probe * C], at_begin = key[begin], before = begin > 0 ? key[begin - 1] : -1;
+        const uint32_t same = (uint32_t)(__ballot(first == k && s + 1 + lane < shares) >> (threadIdx.x & 48)) & 0xffffu;
+        if (k < V && (same & 1) && (at_begin != k || before != k)) {
+            int64_t lo = s + __builtin_ctz(~same);                       // the last of the next sixteen
+            if (same == 0xffffu) {
+                int64_t hi = shares - 1;
+                while (lo < hi) {
+                    const int64_t mid = (lo + hi + 1) >> 1;
+                    if (key[mid * C] == k) lo = mid;
+                    else hi = mid - 1;
+                }
             }
             if (lo - s > kJoinShort) {
                 if (lane == 0) {
@@ -404,9 +578,9 @@ struct EmbedPlan {
 };
 static inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-static EmbedPlan embed_plan(int64_t N, int64_t V, int F) {
+static EmbedPlan embed_plan(int64_t N, int64_t V, int F, int size) {
     EmbedPlan p = {};
-    const int64_t pieces = (F + kPiece - 1) / kPiece;
+    const int64_t pieces = (F + kPiece - 1) / kPiece, sixteens = ((int64_t)F * size + 15) / 16;
     if (V <= 16 || N <= 512) {
         p.scan = true;
         if (N <= 512) {
@@ -424,8 +598,8 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int F) {
         return p;
     }
     p.lanes = 8;
-    while (p.lanes < 64 && p.lanes < pieces) p.lanes *= 2;
-    p.tiles = (int)((pieces + p.lanes - 1) / p.lanes);
+    while (p.lanes < 64 && p.lanes < sixteens) p.lanes *= 2;
+    p.tiles = (int)((sixteens + p.lanes - 1) / p.lanes);
     const int64_t c = N * p.tiles * p.lanes / 64 / 2048;
     p.C = c < 16 ? 16 : (c > 512 ? 512 : (c + 7) / 8 * 8);
     p.shares = (N + p.C - 1) / p.C;
@@ -435,9 +609,11 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int F) {
     return p;
 }
 
-// Sorted pairs of `key` in work; returns their place.
-static void embed_sort(const int32_t* key, int64_t N, int64_t V, char* work, const int32_t*& key_out, const int32_t*& row_out,
-                       hipStream_t st) {
+// Sorted pairs of `key` in work, where key_out and row_out point then; out (V, F) is cleared on the way.
+template <typename T>
+static void embed_sort(const int32_t* key, int64_t N, int64_t V, int F, T* out, char* work, const int32_t*& key_out,
+                       const int32_t*& row_out, hipStream_t st) {
+    constexpr int size = (int)sizeof(T);
     const int64_t n = up256(4 * N);
     int32_t* k[2] = {(int32_t*)work, (int32_t*)(work + n)};
     int32_t* r[2] = {(int32_t*)(work + 2 * n), (int32_t*)(work + 3 * n)};
@@ -445,6 +621,8 @@ static void embed_sort(const int32_t* key, int64_t N, int64_t V, char* work, con
         int n2 = 2;
         while (n2 < N) n2 *= 2;
         hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(1024), 0, st, key, (int)N, (uint32_t)V, n2, k[0], r[0]);
+        hipLaunchKernelGGL(embed_zero_kernel<T>, dim3((unsigned)((V * F + 256 * kPiece - 1) / (256 * kPiece))), dim3(256), 0, st, out,
+                           V * F);
         key_out = k[0];
         row_out = r[0];
         return;
@@ -452,14 +630,15 @@ static void embed_sort(const int32_t* key, int64_t N, int64_t V, char* work, con
     int bits = 1;
     while (V >> bits) ++bits;                    // keys up to V
     const int passes = (bits + kSortBits - 1) / kSortBits, per = (bits + passes - 1) / passes;
-    const int64_t seg = sort_segment(N);
+    const int64_t seg = sort_segment(N), bytes = V * F * size, zeros = (bytes + 16 * kSortThreads - 1) / (16 * kSortThreads);
     const int segs = (int)((N + seg - 1) / seg);
     int32_t *tot = (int32_t*)(work + 4 * n), *count = tot + (1 << kSortBits);
     const int32_t *from = key, *rows = nullptr;
     for (int i = 0; i < passes; ++i) {
         const int D = 1 << per;
-        hipLaunchKernelGGL(sort_count_kernel, dim3(segs), dim3(kSortThreads), 0, st, from, N, seg, (uint32_t)V, i * per, per, count);
-        hipLaunchKernelGGL(sort_rows_kernel, dim3((D + 3) / 4), dim3(256), 0, st, count, segs, D, tot);
+        hipLaunchKernelGGL(sort_count_kernel, dim3(segs + (i ? 0 : (unsigned)(zeros < 2048 ? zeros : 2048))), dim3(kSortThreads), 0, st,
+                           from, N, seg, segs, (uint32_t)V, i * per, per, count, (char*)out, bytes);
+        hipLaunchKernelGGL(sort_rows_kernel, dim3(D), dim3(256), 0, st, count, segs, tot);
         hipLaunchKernelGGL(sort_place_kernel, dim3(segs), dim3(kSortThreads), 0, st, from, rows, N, seg, (uint32_t)V, i * per, per,
                            count, tot, k[i & 1], r[i & 1]);
         from = k[i & 1];
@@ -472,7 +651,7 @@ static void embed_sort(const int32_t* key, int64_t N, int64_t V, char* work, con
 template <typename T>
 static int launch_embed_bwd(const int32_t* key, const T* dy, int64_t ld, int64_t N, int64_t V, int F, float factor, T* out,
                             char* work, hipStream_t st) {
-    const EmbedPlan p = embed_plan(N, V, F);
+    const EmbedPlan p = embed_plan(N, V, F, (int)sizeof(T));
     if (p.scan) {
         float* part = p.chunks > 1 ? (float*)work : nullptr;
         const dim3 grid((unsigned)((p.chunks * p.blocks + 3) / 4), (unsigned)((F + 64 * kPiece - 1) / (64 * kPiece)));
@@ -485,10 +664,8 @@ static int launch_embed_bwd(const int32_t* key, const T* dy, int64_t ld, int64_t
         return 0;
     }
     const int32_t *keys, *rows;
-    embed_sort(key, N, V, work, keys, rows, st);
+    embed_sort<T>(key, N, V, F, out, work, keys, rows, st);
     float* part = (float*)(work + p.sort_bytes);
-    hipLaunchKernelGGL(embed_zero_kernel<T>, dim3((unsigned)((V * F + 256 * kPiece - 1) / (256 * kPiece))), dim3(256), 0, st, out,
-                       V * F);
     const dim3 grid((unsigned)((p.shares * p.lanes + 255) / 256), (unsigned)p.tiles);
 #define FACE_RUNS(L_)                                                                                                     \
     if (p.lanes == L_)                                                                                                    \
@@ -520,19 +697,21 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
     if (ld_t < F || (wide != 0 && wide != 1)) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!table || !index || !y) return FACE_ERR_ARG;
-    const int64_t pieces = (F + kPiece - 1) / kPiece;
-    int lg = 2;
-    while (lg < 8 && ((int64_t)4 << lg) < pieces) ++lg;
-    const dim3 grid((unsigned)((N + (256 >> lg) - 1) >> (8 - lg)));
     const hipStream_t st = (hipStream_t)stream;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int64_t sixteens = ((int64_t)F * sizeof(T) + 15) / 16;
+        int lg = 0;
+        while (lg < 6 && (1 << lg) < sixteens) ++lg;
+        const int64_t groups = 256 >> lg, many = N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
+        const dim3 grid((unsigned)((N + groups * many - 1) / (groups * many)));
+        auto launch = [&](auto* kern, auto* i) {
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T*)table, ld_t, i, N, V, F, factor, lg, (T*)y, key);
+        };
         if (wide)
-            hipLaunchKernelGGL((embed_fwd_kernel<T, int64_t>), grid, dim3(256), 0, st, (const T*)table, ld_t, (const int64_t*)index, N,
-                               V, F, factor, lg, (T*)y, key);
+            launch(many > 1 ? embed_fwd_kernel<T, int64_t, 4> : embed_fwd_kernel<T, int64_t, 1>, (const int64_t*)index);
         else
-            hipLaunchKernelGGL((embed_fwd_kernel<T, int32_t>), grid, dim3(256), 0, st, (const T*)table, ld_t, (const int32_t*)index, N,
-                               V, F, factor, lg, (T*)y, key);
+            launch(many > 1 ? embed_fwd_kernel<T, int32_t, 4> : embed_fwd_kernel<T, int32_t, 1>, (const int32_t*)index);
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -540,7 +719,8 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
 
 extern "C" int64_t face_embed_bwd_work(int64_t N, int64_t V, int32_t F) {
     if (N <= 0 || V <= 0 || F <= 0 || embed_args(N, V, F, FACE_F32)) return 0;
-    return embed_plan(N, V, F).bytes;
+    const int64_t a = embed_plan(N, V, F, 2).bytes, b = embed_plan(N, V, F, 4).bytes;
+    return a > b ? a : b;
 }
 
 extern "C" int face_embed_bwd(const int32_t* key, const void* dy, int64_t ld_dy, int64_t N, int64_t V, int32_t F, int32_t dtype,

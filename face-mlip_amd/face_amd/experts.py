@@ -20,6 +20,8 @@ synchronises; none has a CPU path. They differentiate once, in training too: all
 inputs take gradients, except those of the 8-bit forms. Forward-mode derivatives are refused. Forward and backward are captured into a graph together,
 as with torch's own operators on leaves of which no eager graph is alive (fresh ones, by detach().requires_grad_()).
 """
+import functools
+
 import torch
 from torch.autograd import forward_ad
 
@@ -77,9 +79,9 @@ _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_d
 
 def _launch(t, name, label, *args):
     """Call entry point `name` with args and the current stream of t's device, as the current device."""
-    idx = t.device.index
+    idx = t.get_device()
     if idx == _get_device():
-        call(name, *args, _lib.stream_of(t), label=label)
+        call(name, *args, _lib.stream_of(t) if _lib._raw_stream is None else _lib._raw_stream(idx), label=label)
     else:
         with torch.cuda.device(idx):
             call(name, *args, _lib.stream_of(t), label=label)
@@ -95,6 +97,12 @@ def _once(name, *grads):
 def _like(t):
     """A dense tensor of t's shape and type (half the host time of torch.empty(t.shape, ...))."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=4096)
+def _work_size(name, *sizes):
+    """Workspace of a call, by its sizes alone."""
+    return getattr(_lib.lib(), name)(*sizes)
 
 
 def _work(n_bytes, device):
@@ -257,7 +265,7 @@ class LayerNorm(torch.autograd.Function):
             dy = _rows(dy, F)
         if ds is not None:
             ds = _rows(ds, F)
-        need = _lib.lib().face_layer_norm_rows_bwd_work(N, F) if need_w or need_b else 0
+        need = _work_size("face_layer_norm_rows_bwd_work", N, F) if need_w or need_b else 0
         work = _work(need, some.device)
         _launch(some, "face_layer_norm_rows_bwd", "layer_norm_bwd", ptr(s2), F if s2 is None else s2.stride(0), ptr(q), ptr(block),
                 mean, stat.data_ptr(), ptr(dy), F if dy is None else dy.stride(0), ptr(ds), F if ds is None else ds.stride(0), N, F,
@@ -389,9 +397,10 @@ class GatedSiLU(torch.autograd.Function):
         x2 = q = scale = None
         if ctx.keep8:
             q, scale = ctx.saved_tensors
+            dx = torch.empty(*dy.shape[:-1], 2 * F, dtype=dy.dtype, device=dy.device)
         else:
-            x2 = _rows(ctx.saved_tensors[0], 2 * F)
-        dx = torch.empty(*dy.shape[:-1], 2 * F, dtype=dy.dtype, device=dy.device)
+            x, = ctx.saved_tensors
+            x2, dx = _rows(x, 2 * F), _like(x)
         _launch(dy, "face_gated_silu_bwd", "gated_silu_bwd", ptr(x2), 2 * F if x2 is None else x2.stride(0), ptr(q), ptr(scale),
                 d2.data_ptr(), d2.stride(0), d2.shape[0], F, _DTYPES[dy.dtype], dx.data_ptr())
         return dx, None
@@ -439,7 +448,7 @@ class Embed(torch.autograd.Function):
         V, F, N = ctx.rows, dy.shape[-1], key.numel()
         d2 = _rows(dy, F)
         dt = torch.empty(V, F, dtype=dy.dtype, device=dy.device)
-        need = _lib.lib().face_embed_bwd_work(N, V, F)
+        need = _work_size("face_embed_bwd_work", N, V, F)
         work = _work(need, dy.device)
         _launch(dy, "face_embed_bwd", "embed_bwd", key.data_ptr(), d2.data_ptr(), d2.stride(0), N, V, F, _DTYPES[dy.dtype], ctx.factor,
                 dt.data_ptr(), ptr(work), need)
