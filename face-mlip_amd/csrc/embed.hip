@@ -20,11 +20,11 @@ struct Sixteen {
     static constexpr int E = 16 / (int)sizeof(T);
     v4u a;
 };
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ Sixteen<T> hold16(const T* p, int left) {
     Sixteen<T> r = {};
     if (left >= Sixteen<T>::E) {
-        r.a = ld16(p);
+        r.a = ld16s<NT>(p);
     } else if (left > 0) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -49,16 +49,16 @@ __device__ __forceinline__ void values16(const Sixteen<T>& r, float x[Sixteen<T>
         for (int e = 0; e < 4; ++e) unpack2<T>(r.a[e], x[2 * e], x[2 * e + 1]);
     }
 }
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void store16(T* p, int left, const float x[Sixteen<T>::E]) {
     if (left >= Sixteen<T>::E) {
         if constexpr (sizeof(T) == 4) {
-            st16(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
+            st16s<NT>(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
         } else {
             v4u a;
 #pragma unroll
             for (int e = 0; e < 4; ++e) a[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
-            st16(p, a);
+            st16s<NT>(p, a);
         }
     } else {
 #pragma unroll
@@ -67,9 +67,13 @@ __device__ __forceinline__ void store16(T* p, int left, const float x[Sixteen<T>
     }
 }
 
+// Rows of y and of dy past this pass the caches by (64 MB of pairs' rows, both directions, 77 us for 81 with ordinary accesses, 256 MB
+// 158 for 211).
+constexpr int64_t kEmbedStream = (int64_t)48 << 20;
+
 // R rows per group of lanes, a workgroup's groups side by side, so that the rows' indices, then their entries, are on
 // their way together.
-template <typename T, typename I, int R>
+template <typename T, typename I, int R, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t ld, const I* __restrict__ index,
                                                         int64_t N, int64_t V, int F, float factor, int lg, T* __restrict__ y,
                                                         int32_t* __restrict__ key) {
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
             values16<T>(r[i], x);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = in[i] ? x[e] * factor : 0.f;
-            if (n < N) store16(y + n * F + c, F - c, x);
+            if (n < N) store16<NT>(y + n * F + c, F - c, x);
         }
     }
 }
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(T* __restrict__ out, in
 
 // Groups of LC lanes, C sorted rows each. part (shares, 2, F): a run that comes from the share before (0), one that begins
 // here and goes on (1). The next rows' numbers are on their way while the present ones are added.
-template <typename T, int LC>
+template <typename T, int LC, bool NT>
 __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restrict__ key, const int32_t* __restrict__ row,
                                                          const T* __restrict__ dy, int64_t ld, int64_t N, int64_t C, int V, int F,
                                                          float factor, float* __restrict__ part, T* __restrict__ out) {
@@ -455,7 +459,7 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restri
     for (int64_t p = begin; p < end; p += U) {
         Sixteen<T> r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = hold16(dy + (int64_t)at[u] * ld + c, left);
+        for (int u = 0; u < U; ++u) r[u] = hold16<NT>(dy + (int64_t)at[u] * ld + c, left);
         if (p + U < end) numbers(p + U, next_k, next_at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -667,10 +671,11 @@ static int launch_embed_bwd(const int32_t* key, const T* dy, int64_t ld, int64_t
     embed_sort<T>(key, N, V, F, out, work, keys, rows, st);
     float* part = (float*)(work + p.sort_bytes);
     const dim3 grid((unsigned)((p.shares * p.lanes + 255) / 256), (unsigned)p.tiles);
+    const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream;
 #define FACE_RUNS(L_)                                                                                                     \
     if (p.lanes == L_)                                                                                                    \
-        hipLaunchKernelGGL((embed_runs_kernel<T, L_>), grid, dim3(256), 0, st, keys, rows, dy, ld, N, p.C, (int)V, F, factor, \
-                           part, out);
+        hipLaunchKernelGGL((nt ? embed_runs_kernel<T, L_, true> : embed_runs_kernel<T, L_, false>), grid, dim3(256), 0, st, keys, rows, \
+                           dy, ld, N, p.C, (int)V, F, factor, part, out);
     FACE_RUNS(8) FACE_RUNS(16) FACE_RUNS(32) FACE_RUNS(64)
 #undef FACE_RUNS
     if (p.shares > 1)
@@ -703,15 +708,18 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
         const int64_t sixteens = ((int64_t)F * sizeof(T) + 15) / 16;
         int lg = 0;
         while (lg < 6 && (1 << lg) < sixteens) ++lg;
-        const int64_t groups = 256 >> lg, many = N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
+        const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream;
+        const int64_t groups = 256 >> lg, many = nt || N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
         const dim3 grid((unsigned)((N + groups * many - 1) / (groups * many)));
         auto launch = [&](auto* kern, auto* i) {
             hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T*)table, ld_t, i, N, V, F, factor, lg, (T*)y, key);
         };
         if (wide)
-            launch(many > 1 ? embed_fwd_kernel<T, int64_t, 4> : embed_fwd_kernel<T, int64_t, 1>, (const int64_t*)index);
+            launch(nt ? embed_fwd_kernel<T, int64_t, 4, true> : many > 1 ? embed_fwd_kernel<T, int64_t, 4, false> : embed_fwd_kernel<T, int64_t, 1, false>,
+                   (const int64_t*)index);
         else
-            launch(many > 1 ? embed_fwd_kernel<T, int32_t, 4> : embed_fwd_kernel<T, int32_t, 1>, (const int32_t*)index);
+            launch(nt ? embed_fwd_kernel<T, int32_t, 4, true> : many > 1 ? embed_fwd_kernel<T, int32_t, 4, false> : embed_fwd_kernel<T, int32_t, 1, false>,
+                   (const int32_t*)index);
         FACE_LAUNCH_CHECK();
         return 0;
     });

@@ -24,7 +24,7 @@ __device__ __forceinline__ RowAt row_at(int lg) {
     return {(int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg), (int)threadIdx.x & ((1 << lg) - 1), 1 << lg};
 }
 
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
     const RowAt r = row_at(lg);
@@ -35,8 +35,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int6
     scale += r.n * kept_blocks(F);
     for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
         float v[kPiece];
-        load_piece(x + c, F - c, v);
-        store_kept(q, scale, c, F, v);
+        load_row<NT>(x + c, F - c, v);
+        store_kept<NT>(q, scale, c, F, v);
     }
 }
 
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int6
 template <typename T>
 constexpr float kLargest = __is_same(T, f16) ? 65504.f : (__is_same(T, bf16) ? 0x1.fep127f : 0x1.fffffep127f);
 
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__ q, int64_t ld_q,
                                                      const uint8_t* __restrict__ scale, int64_t ld_s, int64_t N, int F, int lg,
                                                      T* __restrict__ x) {
@@ -56,15 +56,15 @@ __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__
 #pragma unroll 4
     for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
         float v[kPiece];
-        kept_values(hold_kept(q, scale, c, F), v);
+        kept_values(hold_kept<NT>(q, scale, c, F), v);
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) v[e] = within(v[e], kLargest<T>);
-        store_piece(x + c, F - c, v);
+        store_row<NT>(x + c, F - c, v);
     }
 }
 
 // q (N, 2 F) and scale (N, 2, blocks of F), or null.
-template <typename T, bool KEEP>
+template <typename T, bool KEEP, bool NT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                         T* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
     const RowAt r = row_at(lg);
@@ -76,19 +76,19 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x,
     scale += r.n * 2 * blocks;
     for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
         float a[kPiece], b[kPiece];
-        load_piece(x + c, F - c, a);
-        load_piece(x + F + c, F - c, b);
+        load_row<NT>(x + c, F - c, a);
+        load_row<NT>(x + F + c, F - c, b);
         if constexpr (KEEP) {
-            store_kept(q, scale, c, F, a);
-            store_kept(q + F, scale + blocks, c, F, b);
+            store_kept<NT>(q, scale, c, F, a);
+            store_kept<NT>(q + F, scale + blocks, c, F, b);
         }
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) a[e] = silu(a[e]) * b[e];
-        store_piece(y + c, F - c, a);
+        store_row<NT>(y + c, F - c, a);
     }
 }
 
-template <typename T, bool KEPT>
+template <typename T, bool KEPT, bool NT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x, int64_t ld, const uint8_t* __restrict__ q,
                                                         const uint8_t* __restrict__ scale, const T* __restrict__ dy,
                                                         int64_t ld_dy, int64_t N, int F, int lg, T* __restrict__ dx) {
@@ -103,13 +103,13 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x,
 #pragma unroll 2
     for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
         float a[kPiece], b[kPiece], d[kPiece];
-        load_piece(dy + c, F - c, d);
+        load_row<NT>(dy + c, F - c, d);
         if constexpr (KEPT) {
-            kept_values(hold_kept(q, scale, c, F), a);
-            kept_values(hold_kept(q + F, scale + blocks, c, F), b);
+            kept_values(hold_kept<NT>(q, scale, c, F), a);
+            kept_values(hold_kept<NT>(q + F, scale + blocks, c, F), b);
         } else {
-            load_piece(x + c, F - c, a);
-            load_piece(x + F + c, F - c, b);
+            load_row<NT>(x + c, F - c, a);
+            load_row<NT>(x + F + c, F - c, b);
         }
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) {
@@ -117,8 +117,8 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x,
             a[e] = d[e] * b[e] * silu_slope(t);
             b[e] = d[e] * silu(t);
         }
-        store_piece(dx + c, F - c, a);
-        store_piece(dx + F + c, F - c, b);
+        store_row<NT>(dx + c, F - c, a);
+        store_row<NT>(dx + F + c, F - c, b);
     }
 }
 
@@ -144,7 +144,8 @@ extern "C" int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F,
     const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(pack_kernel<T>, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
+        auto* kern = streams<T>(N * F * 3 / 2) ? pack_kernel<T, true> : pack_kernel<T, false>;
+        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
                            (uint8_t*)q, (uint8_t*)scale);
         FACE_LAUNCH_CHECK();
         return 0;
@@ -160,7 +161,8 @@ extern "C" int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, 
     const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(unpack_kernel<T>, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
+        auto* kern = streams<T>(N * F * 3 / 2) ? unpack_kernel<T, true> : unpack_kernel<T, false>;
+        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
                            (const uint8_t*)scale, ld_s, N, F, lg, (T*)x);
         FACE_LAUNCH_CHECK();
         return 0;
@@ -176,7 +178,9 @@ extern "C" int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32
     const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        auto* kern = q ? gated_fwd_kernel<T, true> : gated_fwd_kernel<T, false>;
+        const bool nt = streams<T>(N * F * (q ? 4 : 3));
+        auto* kern = q ? (nt ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
+                       : (nt ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
         hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg, (T*)y,
                            (uint8_t*)q, (uint8_t*)scale);
         FACE_LAUNCH_CHECK();
@@ -193,7 +197,9 @@ extern "C" int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, c
     const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        auto* kern = q ? gated_bwd_kernel<T, true> : gated_bwd_kernel<T, false>;
+        const bool nt = streams<T>(N * F * (q ? 4 : 5));
+        auto* kern = q ? (nt ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
+                       : (nt ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
         hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, (const uint8_t*)q,
                            (const uint8_t*)scale, (const T*)dy, ld_dy, N, F, lg, (T*)dx);
         FACE_LAUNCH_CHECK();

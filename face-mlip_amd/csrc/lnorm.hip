@@ -48,7 +48,7 @@ __device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, floa
     }
 }
 
-template <typename T, int LANES, int U, int MODE>
+template <typename T, int LANES, int U, int MODE, bool NT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
     __shared__ float part[LANES / 32 + 1];
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int c = kPiece * (lane + LANES * u);
-        load_piece(x + c, left_at<U>(u, c, F), v[u]);
+        load_row<NT>(x + c, left_at<U>(u, c, F), v[u]);
     }
     if (a.r) {
         const T* r = (const T*)a.r + n * a.ld_r;
@@ -70,10 +70,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
         for (int u = 0; u < U; ++u) {
             const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
             float t[kPiece];
-            load_piece(r + c, left, t);
+            load_row<NT>(r + c, left, t);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) v[u][e] = to_f(from_f<T>(v[u][e] + t[e]));
-            store_piece(s + c, left, v[u]);
+            store_row<NT>(s + c, left, v[u]);
         }
     }
     float sum = 0.f;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
         const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
         float h[kPiece], y[kPiece];
         ln_piece(v[u], mean, rs, w + c, b ? b + c : nullptr, left, h, y);
-        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, c + left, h);
+        if constexpr (MODE == kLnKept) store_kept<NT>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, c + left, h);
         if constexpr (MODE == kLnQ8) {
             // the magnitudes compare as integers, a NaN above everything: its row gets a NaN scale and no number
 #pragma unroll
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
                 top = m > top ? m : top;
             }
         } else {
-            store_piece((T*)a.y + n * F + c, left, y);
+            store_row<NT>((T*)a.y + n * F + c, left, y);
         }
     }
     if constexpr (MODE == kLnQ8) {
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = kPiece * (lane + LANES * u);
-            store_e4m3(a.q + n * F + c, left_at<U>(u, c, F), v[u], inv);
+            store_e4m3<NT>(a.q + n * F + c, left_at<U>(u, c, F), v[u], inv);
         }
         if (lane == 0) a.scale[n] = sc;
     }
@@ -236,11 +236,11 @@ struct LnBwdArgs {
 };
 
 // h of a piece, from the row as it was normalised or as it was kept.
-template <typename T, bool KEPT>
+template <typename T, bool KEPT, bool NT>
 struct LnRow {
     RawPiece<T> a;
     __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
-        a = hold_raw((const T*)g.s + n * g.ld_s + c, left);
+        a = hold_raw<NT>((const T*)g.s + n * g.ld_s + c, left);
     }
     __device__ __forceinline__ void values(float mean, float rs, float h[kPiece]) const {
         raw_values<T>(a, h);
@@ -248,11 +248,11 @@ struct LnRow {
         for (int e = 0; e < kPiece; ++e) h[e] = (h[e] - mean) * rs;
     }
 };
-template <typename T>
-struct LnRow<T, true> {
+template <typename T, bool NT>
+struct LnRow<T, true, NT> {
     KeptPiece a;
     __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
-        a = hold_kept(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, c + left);
+        a = hold_kept<NT>(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, c + left);
     }
     __device__ __forceinline__ void values(float, float, float h[kPiece]) const { kept_values_near(a, h); }
 };
@@ -261,7 +261,7 @@ struct LnRow<T, true> {
 // all of them; its row of partial sums is joined with the others' by ln_column_sum_kernel in a fixed order: no
 // atomics. All of a row's reads are issued before the first is used. Beyond a row's end dy is 0, and h is finite where
 // the row's is.
-template <typename T, int LANES, int U, bool KEPT>
+template <typename T, int LANES, int U, bool KEPT, bool NT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
     __shared__ float part[LANES / 32 + 1];
@@ -270,14 +270,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
     const float inv_f = 1.f / (float)F;
     float aw[U][kPiece] = {}, ab[U][kPiece] = {};
     for (int64_t n = (int64_t)blockIdx.x * kRows + slot; n < a.N; n += (int64_t)gridDim.x * kRows) {
-        LnRow<T, KEPT> row[U];
+        LnRow<T, KEPT, NT> row[U];
         RawPiece<T> dy[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
             row[u].hold(a, n, c, left);
-            dy[u] = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, left) : RawPiece<T>{};
-            ds[u] = a.ds && a.dx ? hold_raw((const T*)a.ds + n * a.ld_ds + c, left) : RawPiece<T>{};
+            dy[u] = a.dy ? hold_raw<NT>((const T*)a.dy + n * a.ld_dy + c, left) : RawPiece<T>{};
+            ds[u] = a.ds && a.dx ? hold_raw<NT>((const T*)a.ds + n * a.ld_ds + c, left) : RawPiece<T>{};
         }
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
             load_piece((const T*)a.w + c, left_at<U>(u, c, F), w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
-            store_piece((T*)a.dx + n * F + c, left_at<U>(u, c, F), o);
+            store_row<NT>((T*)a.dx + n * F + c, left_at<U>(u, c, F), o);
         }
     }
     if (!a.part) return;
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnBwdArgs a) {
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
         auto load = [&](int c, float h[kPiece], float d[kPiece], float w[kPiece]) {
-            LnRow<T, KEPT> row;
+            LnRow<T, KEPT, false> row;
             row.hold(a, n, c, F - c);
             row.values(mean, rs, h);
             RawPiece<T> r = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
@@ -465,8 +465,11 @@ static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
     if (a.F > kLnHeld) {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);
     }
-#define FACE_ROW(L_, U_) \
-    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, U_, MODE>), grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
+#define FACE_ROW(L_, U_)                                                                                                 \
+    else if (sh.lanes == L_ && sh.units == U_)                                                                          \
+        hipLaunchKernelGGL((streams<T>(a.N * a.F * (a.r ? 4 : 2)) ? ln_fwd_kernel<T, L_, U_, MODE, true>        \
+                                                                           : ln_fwd_kernel<T, L_, U_, MODE, false>),     \
+                           grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
     FACE_LN_ROWS
 #undef FACE_ROW
     FACE_LAUNCH_CHECK();
@@ -482,8 +485,11 @@ static int launch_ln_bwd(const LnBwdArgs& a, T* dw, T* db, hipStream_t st) {
         if (a.F > kLnHeld) {
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, KEPT>), grid, dim3(1024), 0, st, a);
         }
-#define FACE_ROW(L_, U_) \
-    else if (sh.lanes == L_ && sh.units == U_) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, U_, KEPT>), grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
+#define FACE_ROW(L_, U_)                                                                                                 \
+    else if (sh.lanes == L_ && sh.units == U_)                                                                          \
+        hipLaunchKernelGGL((streams<T>(a.N * a.F * (a.ds ? 4 : 3)) ? ln_bwd_kernel<T, L_, U_, KEPT, true>        \
+                                                                           : ln_bwd_kernel<T, L_, U_, KEPT, false>),     \
+                           grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
         FACE_LN_ROWS
 #undef FACE_ROW
         FACE_LAUNCH_CHECK();

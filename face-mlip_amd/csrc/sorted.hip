@@ -7,7 +7,7 @@
 // place is order's inverse, -1 for slots that have none: what leaves rows of x, or gathers into rows of y, goes by
 // rows, reads or writes each of those once, and its other side by whole rows. With one choice per row there is nothing to share:
 // xs is gathered by order, without the inverse. Bound by bytes.
-#include "elem.h"
+#include "kept.h"
 
 namespace face {
 
@@ -44,16 +44,11 @@ __global__ __launch_bounds__(256) void places_kernel(const int32_t* __restrict__
     if (a >= 0 && a < slots) place[a] = (int32_t)p;
 }
 
-// Threads per row: about four pieces each.
-static inline int sorted_lanes_log2(int64_t F) {
-    const int64_t p = (F + kPiece - 1) / kPiece;
-    int lg = 4;
-    while (lg < 8 && ((int64_t)4 << lg) < p) ++lg;
-    return lg;
-}
+// Threads per row.
+static inline int sorted_lanes_log2(int64_t F) { return F <= 512 ? 4 : (F <= 4096 ? 6 : 8); }
 
 // xs[p] = x[order[p] / k].
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restrict__ x, int64_t ld,
                                                               const int32_t* __restrict__ ptr,
                                                               const int32_t* __restrict__ order, int64_t slots, int k, int G,
@@ -66,14 +61,14 @@ __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restric
 #pragma unroll 4
     for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
         float v[kPiece] = {};
-        if (some) load_piece(from + c, F - c, v);
-        store_piece(xs + p * F + c, F - c, v);
+        if (some) load_row<NT>(from + c, F - c, v);
+        store_row<NT>(xs + p * F + c, F - c, v);
     }
 }
 
 // A row's threads write it to the places of its k slots, and zeros to those of the places i k .. i k + k - 1 that
-// have no slot.
-template <typename T>
+// have no slot; four slots per turn, their places known before the row is.
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restrict__ x, int64_t ld,
                                                                const int32_t* __restrict__ ptr,
                                                                const int32_t* __restrict__ order,
@@ -82,23 +77,34 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
     const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
     if (n * k >= slots) return;
     const int64_t m = places_of(ptr, G, slots);
+    constexpr int J = 4;
+    for (int j0 = 0; j0 < k; j0 += J) {
+        int p[J];
+        bool bare[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int64_t i = n * k + j0 + j;
+            const bool in = j0 + j < k;
+            p[j] = in ? place[i] : -1;
+            const int a = in && i < m ? order[i] : -1;
+            bare[j] = in && (a < 0 || a >= slots || place[a] != i);
+        }
 #pragma unroll 2
-    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
-        float v[kPiece];
-        const float none[kPiece] = {};
-        load_piece(x + n * ld + c, F - c, v);
-        for (int j = 0; j < k; ++j) {
-            const int64_t i = n * k + j;
-            const int p = place[i];
-            if (p >= 0) store_piece(xs + (int64_t)p * F + c, F - c, v);
-            const int a = i < m ? order[i] : -1;
-            if (a < 0 || a >= slots || place[a] != i) store_piece(xs + i * F + c, F - c, none);
+        for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
+            float v[kPiece];
+            const float none[kPiece] = {};
+            load_row<NT>(x + n * ld + c, F - c, v);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                if (p[j] >= 0) store_row<NT>(xs + (int64_t)p[j] * F + c, F - c, v);
+                if (bare[j]) store_row<NT>(xs + (n * k + j0 + j) * F + c, F - c, none);
+            }
         }
     }
 }
 
 // out[i] = r[i] + sum_j w[i, j] y[place(i k + j)], in order; w null: ones.
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ place,
                                                          const float* __restrict__ w, const T* __restrict__ r, int64_t ld_r,
                                                          int64_t N, int k, int F, int lg, T* __restrict__ out) {
@@ -106,23 +112,23 @@ __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y
     if (n >= N) return;
     for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
         float s[kPiece] = {};
-        if (r) load_piece(r + n * ld_r + c, F - c, s);
+        if (r) load_row<NT>(r + n * ld_r + c, F - c, s);
 #pragma unroll 4
         for (int j = 0; j < k; ++j) {
             const int p = place[n * k + j];
             if (p < 0) continue;
             float v[kPiece];
-            load_piece(y + (int64_t)p * ld_y + c, F - c, v);
+            load_row<NT>(y + (int64_t)p * ld_y + c, F - c, v);
             const float f = w ? w[n * k + j] : 1.f;
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) s[e] = fmaf(f, v[e], s[e]);
         }
-        store_piece(out + n * F + c, F - c, s);
+        store_row<NT>(out + n * F + c, F - c, s);
     }
 }
 
 // dy[p] = w dout and dw = dout . y[p] at the places of the row's slots; zeros at places without a slot.
-template <typename T, int LANES>
+template <typename T, int LANES, bool NT>
 __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ dout, int64_t ld_d, const T* __restrict__ y,
                                                          int64_t ld_y, const int32_t* __restrict__ ptr,
                                                          const int32_t* __restrict__ order,
@@ -150,12 +156,12 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
         }
         for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
             float d[kPiece];
-            load_piece(dout + n * ld_d + c, F - c, d);
+            load_row<NT>(dout + n * ld_d + c, F - c, d);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 float v[kPiece];
                 if (dw && p[j] >= 0) {
-                    load_piece(y + (int64_t)p[j] * ld_y + c, F - c, v);
+                    load_row<NT>(y + (int64_t)p[j] * ld_y + c, F - c, v);
 #pragma unroll
                     for (int e = 0; e < kPiece; ++e) s[j] = fmaf(d[e], v[e], s[j]);
                 }
@@ -163,11 +169,11 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
                 if (p[j] >= 0) {
 #pragma unroll
                     for (int e = 0; e < kPiece; ++e) v[e] = f[j] * d[e];
-                    store_piece(dy + (int64_t)p[j] * F + c, F - c, v);
+                    store_row<NT>(dy + (int64_t)p[j] * F + c, F - c, v);
                 }
                 if (bare[j]) {
                     const float none[kPiece] = {};
-                    store_piece(dy + (n * k + j0 + j) * F + c, F - c, none);
+                    store_row<NT>(dy + (n * k + j0 + j) * F + c, F - c, none);
                 }
             }
         }
@@ -222,11 +228,12 @@ extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, cons
     const int64_t slots = N * k;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const bool nt = streams<T>((slots + N) * F);
         if (place)
-            hipLaunchKernelGGL(dispatch_scatter_kernel<T>, sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x,
+            hipLaunchKernelGGL((nt ? dispatch_scatter_kernel<T, true> : dispatch_scatter_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x,
                                ld_x, ptr, order, place, slots, k, G, F, lg, (T*)xs);
         else
-            hipLaunchKernelGGL(dispatch_gather_kernel<T>, sorted_grid(slots, lg), dim3(256), 0, (hipStream_t)stream,
+            hipLaunchKernelGGL((nt ? dispatch_gather_kernel<T, true> : dispatch_gather_kernel<T, false>), sorted_grid(slots, lg), dim3(256), 0, (hipStream_t)stream,
                                (const T*)x, ld_x, ptr, order, slots, k, G, F, lg, (T*)xs);
         FACE_LAUNCH_CHECK();
         return 0;
@@ -242,7 +249,8 @@ extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t
     const int lg = sorted_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(return_fwd_kernel<T>, sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, place,
+        const bool nt = streams<T>((N * k + N * (r ? 2 : 1)) * F);
+        hipLaunchKernelGGL((nt ? return_fwd_kernel<T, true> : return_fwd_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, place,
                            weight, (const T*)r, ld_r, N, k, F, lg, (T*)out);
         FACE_LAUNCH_CHECK();
         return 0;
@@ -260,7 +268,10 @@ extern "C" int face_expert_return_bwd(const void* dout, int64_t ld_d, const void
     const dim3 grid((unsigned)((N + rows - 1) / rows));
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        auto* kern = L == 16 ? return_bwd_kernel<T, 16> : (L == 64 ? return_bwd_kernel<T, 64> : return_bwd_kernel<T, 256>);
+        const bool nt = streams<T>((2 * N * k + N) * F);
+        auto* kern = L == 16 ? (nt ? return_bwd_kernel<T, 16, true> : return_bwd_kernel<T, 16, false>)
+                   : L == 64 ? (nt ? return_bwd_kernel<T, 64, true> : return_bwd_kernel<T, 64, false>)
+                             : (nt ? return_bwd_kernel<T, 256, true> : return_bwd_kernel<T, 256, false>);
         hipLaunchKernelGGL(kern, grid, dim3(256), 0, (hipStream_t)stream, (const T*)dout, ld_d, (const T*)y, ld_y, ptr, order,
                            place, weight, N, k, G, F, (T*)dy, dweight);
         FACE_LAUNCH_CHECK();
