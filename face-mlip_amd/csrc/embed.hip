@@ -14,59 +14,6 @@
 
 namespace face {
 
-// Sixteen bytes of a row, so that neighbouring lanes move neighbouring bytes whatever the type.
-template <typename T>
-struct Sixteen {
-    static constexpr int E = 16 / (int)sizeof(T);
-    v4u a;
-};
-template <bool NT = false, typename T>
-__device__ __forceinline__ Sixteen<T> hold16(const T* p, int left) {
-    Sixteen<T> r = {};
-    if (left >= Sixteen<T>::E) {
-        r.a = ld16s<NT>(p);
-    } else if (left > 0) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < left) r.a[e] = __builtin_bit_cast(uint32_t, p[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < left) r.a[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
-        }
-    }
-    return r;
-}
-template <typename T>
-__device__ __forceinline__ void values16(const Sixteen<T>& r, float x[Sixteen<T>::E]) {
-    if constexpr (sizeof(T) == 4) {
-        const v4f v = __builtin_bit_cast(v4f, r.a);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = v[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) unpack2<T>(r.a[e], x[2 * e], x[2 * e + 1]);
-    }
-}
-template <bool NT = false, typename T>
-__device__ __forceinline__ void store16(T* p, int left, const float x[Sixteen<T>::E]) {
-    if (left >= Sixteen<T>::E) {
-        if constexpr (sizeof(T) == 4) {
-            st16s<NT>(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
-        } else {
-            v4u a;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
-            st16s<NT>(p, a);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < Sixteen<T>::E; ++e)
-            if (e < left) p[e] = from_f<T>(x[e]);
-    }
-}
-
 // Rows of y and of dy past this pass the caches by (64 MB of pairs' rows, both directions, 77 us for 81 with ordinary accesses, 256 MB
 // 158 for 211).
 constexpr int64_t kEmbedStream = (int64_t)48 << 20;
@@ -92,7 +39,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
     for (int c = E * lane; c < F; c += E << lg) {
         Sixteen<T> r[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) r[i] = hold16(table + (in[i] ? (int64_t)v[i] : 0) * ld + c, in[i] ? F - c : 0);
+        for (int i = 0; i < R; ++i) r[i] = hold16<false>(table + (in[i] ? (int64_t)v[i] : 0) * ld + c, in[i] ? F - c : 0);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int64_t n = n0 + i * groups;
@@ -106,52 +53,60 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
 }
 
 // ---------------------------------------------------------------- few entries or few rows
-// A wave: rows [chunk R, chunk R + R), entries [block TV, block TV + TV), 64 pieces of the columns. Partial sums
+// A lane's sums in fp32.
+template <int E>
+__device__ __forceinline__ void store_sums(float* p, int left, const float x[E]) {
+    if constexpr (E == 8) store_piece(p, left, x);
+    else store16<false>(p, left, x);
+}
+
+// A wave: rows [chunk R, chunk R + R), entries [block TV, block TV + TV), 64 times sixteen bytes of the columns. Partial sums
 // (chunks, V, F), or with one chunk the result.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_scan_kernel(const int32_t* __restrict__ key, const T* __restrict__ dy, int64_t ld,
                                                          int64_t N, int64_t R, int64_t chunks, int64_t V, int64_t TV,
                                                          int64_t blocks, int F, float factor, float* __restrict__ part,
                                                          T* __restrict__ out) {
+    constexpr int E = Sixteen<T>::E;
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (id >= chunks * blocks) return;
     const int64_t chunk = id / blocks, b = id - chunk * blocks;
     const int64_t n0 = chunk * R, n1 = n0 + R < N ? n0 + R : N;
     const int64_t v1 = (b + 1) * TV < V ? (b + 1) * TV : V;
-    const int c = kPiece * (lane + 64 * (int)blockIdx.y), left = F - c;
+    const int c = E * (lane + 64 * (int)blockIdx.y), left = F - c;
     for (int64_t v = b * TV; v < v1; ++v) {
-        float s[kPiece] = {};
+        float s[E] = {};
         for (int64_t a = n0; a < n1; a += 64) {
             uint64_t m = __ballot(a + lane < n1 && key[a + lane < n1 ? a + lane : a] == (int32_t)v);
             while (m) {
                 constexpr int U = 8;
-                RawPiece<T> r[U];
+                Sixteen<T> r[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     r[u] = {};
                     if (m) {
                         const int i = __builtin_ctzll(m);
                         m &= m - 1;
-                        r[u] = hold_raw(dy + (a + i) * ld + c, left);
+                        r[u] = hold16<false>(dy + (a + i) * ld + c, left);
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    float x[kPiece];
-                    raw_values<T>(r[u], x);
+                    float x[E];
+                    values16<T>(r[u], x);
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e) s[e] += x[e];
+                    for (int e = 0; e < E; ++e) s[e] += x[e];
                 }
             }
         }
         if (left <= 0) continue;
         if (part) {
-            store_piece(part + (chunk * V + v) * F + c, left, s);
+            store_sums<E>(part + (chunk * V + v) * F + c, left, s);
         } else {
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) s[e] *= factor;
-            store_piece(out + v * F + c, left, s);
+            for (int e = 0; e < E; ++e) s[e] *= factor;
+            store16<false>(out + v * F + c, left, s);
         }
     }
 }
@@ -434,15 +389,12 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restri
     float acc[E] = {};
     auto flush = [&](bool goes_on) {
         if (from_before || goes_on) {
-            float* p = part + (2 * s + (from_before ? 0 : 1)) * F + c;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < left) p[e] = acc[e];
+            store_sums<E>(part + (2 * s + (from_before ? 0 : 1)) * F + c, left, acc);
         } else {
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = factor * acc[e];
-            store16(out + (int64_t)cur * F + c, left, o);
+            store16<false>(out + (int64_t)cur * F + c, left, o);
         }
     };
     int k[U], next_k[U];
@@ -584,7 +536,7 @@ static inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 static EmbedPlan embed_plan(int64_t N, int64_t V, int F, int size) {
     EmbedPlan p = {};
-    const int64_t pieces = (F + kPiece - 1) / kPiece, sixteens = ((int64_t)F * size + 15) / 16;
+    const int64_t sixteens = ((int64_t)F * size + 15) / 16;
     if (V <= 16 || N <= 512) {
         p.scan = true;
         if (N <= 512) {
@@ -592,7 +544,7 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int F, int size) {
             p.chunks = 1;
             p.TV = 1;
         } else {
-            const int64_t tiles = (pieces + 63) / 64, r = N * tiles / 2048 / 64 * 64;
+            const int64_t tiles = (sixteens + 63) / 64, r = N * tiles / 2048 / 64 * 64;
             p.R = r < 64 ? 64 : (r > 1024 ? 1024 : r);
             p.chunks = (N + p.R - 1) / p.R;
             p.TV = V;
@@ -658,7 +610,7 @@ static int launch_embed_bwd(const int32_t* key, const T* dy, int64_t ld, int64_t
     const EmbedPlan p = embed_plan(N, V, F, (int)sizeof(T));
     if (p.scan) {
         float* part = p.chunks > 1 ? (float*)work : nullptr;
-        const dim3 grid((unsigned)((p.chunks * p.blocks + 3) / 4), (unsigned)((F + 64 * kPiece - 1) / (64 * kPiece)));
+        const dim3 grid((unsigned)((p.chunks * p.blocks + 3) / 4), (unsigned)((F + 64 * Sixteen<T>::E - 1) / (64 * Sixteen<T>::E)));
         hipLaunchKernelGGL(embed_scan_kernel<T>, grid, dim3(256), 0, st, key, dy, ld, N, p.R, p.chunks, V, p.TV, p.blocks, F, factor,
                            part, out);
         if (part)

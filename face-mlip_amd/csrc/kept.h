@@ -5,8 +5,8 @@
 // The scale is a byte, e + 127, which is a float's exponent field: x 2^-e and q 2^e are exact, so what a value is
 // kept as hangs on no order of operations, and the rounding to e4m3 (to nearest, ties to even, half a step 2^-4) is the only
 // one. It may pass a type's largest value by half a step: what it stands for is cut to that. A NaN or an infinity is kept as NaN
-// and leaves the others of its block as they are. A block's 32 columns lie in a quad
-// of lanes, a piece each: its maximum is two cross-lane moves.
+// and leaves the others of its block as they are. A block's 32 columns lie in 4 or
+// 8 lanes side by side: its maximum is two or three cross-lane moves.
 #pragma once
 #include "elem.h"
 
@@ -15,94 +15,106 @@ namespace face {
 constexpr int kKeptBlock = 32;
 static __host__ __device__ __forceinline__ int64_t kept_blocks(int64_t F) { return (F + kKeptBlock - 1) / kKeptBlock; }
 
-// The scale's byte of the quad's 32 values (zeros beyond the row's end). All lanes of a quad are active.
-__device__ __forceinline__ uint32_t kept_scale(const float x[kPiece]) {
+// A lane has E values, 4 or 8, so that 32 / E lanes side by side have a block; all of them are active.
+// The scale's byte of the lanes' 32 values (zeros beyond the row's end).
+template <int E>
+__device__ __forceinline__ uint32_t kept_scale(const float x[E]) {
     uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < kPiece; ++e) {
+    for (int e = 0; e < E; ++e) {
         const uint32_t m = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu;
         top = m < 0x7f800000u && m > top ? m : top;
     }
-    const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false);   // lane ^ 1
-    top = a > top ? a : top;
-    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false);   // lane ^ 2
-    top = b > top ? b : top;
-    const int s = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);     // 448 = 1.75 2^8
+    auto step = [&](uint32_t v) { top = v > top ? v : top; };
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));              // lane ^ 1
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));              // lane ^ 2
+    if constexpr (E == 4) step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, false));   // the other quad
+    const int s = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);                         // 448 = 1.75 2^8
     return (uint32_t)(s < 1 ? 1 : s);
 }
 
-// Eight values times `inv` in e4m3. The instruction turns what rounds past 448 (infinities) into NaN.
-template <bool NT = false>
-__device__ __forceinline__ void store_e4m3(uint8_t* p, int left, const float x[kPiece], float inv) {
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, lo, true);
-    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * inv, x[5] * inv, 0, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * inv, x[7] * inv, hi, true);
-    if (left >= kPiece) {
-        typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
-        if constexpr (NT) __builtin_nontemporal_store((v2i_any){lo, hi}, reinterpret_cast<v2i_any*>(p));
-        else *reinterpret_cast<v2i_any*>(p) = (v2i_any){lo, hi};
+// E values times `inv` in e4m3. The instruction turns what rounds past 448 (infinities) into NaN.
+template <int E, bool NT>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, int left, const float x[E], float inv) {
+    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
+    typedef words words_any __attribute__((aligned(1)));
+    uint32_t v[E / 4];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+        v[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, lo, true);
+    }
+    if (left >= E) {
+        words w;
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) w[i] = v[i];
+        if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<words_any*>(p));
+        else *reinterpret_cast<words_any*>(p) = w;
     } else {
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e)
-            if (e < left) p[e] = (uint8_t)((uint32_t)(e < 4 ? lo : hi) >> (8 * (e & 3)));
+        for (int e = 0; e < E; ++e)
+            if (e < left) p[e] = (uint8_t)(v[e / 4] >> (8 * (e & 3)));
     }
 }
 
-// Piece c / 8 of a row: its eight bytes at q + c, and its block's scale, written by the first lane of the quad.
-template <bool NT = false>
-__device__ __forceinline__ void store_kept(uint8_t* q, uint8_t* scale, int c, int F, const float x[kPiece]) {
-    const uint32_t s = kept_scale(x);
-    store_e4m3<NT>(q + c, F - c, x, __builtin_bit_cast(float, (254u - s) << 23));
+// The lane's columns from c on of a row: their bytes at q + c, and the block's scale, written by its first lane.
+template <int E, bool NT>
+__device__ __forceinline__ void store_kept(uint8_t* q, uint8_t* scale, int c, int F, const float x[E]) {
+    const uint32_t s = kept_scale<E>(x);
+    store_e4m3<E, NT>(q + c, F - c, x, __builtin_bit_cast(float, (254u - s) << 23));
     if ((c & (kKeptBlock - 1)) == 0 && c < F) scale[c / kKeptBlock] = (uint8_t)s;
 }
 
 // v within [-top, top]; a NaN stays one.
 __device__ __forceinline__ float within(float v, float top) { return v > top ? top : (v < -top ? -top : v); }
 
-// A kept piece on its way: its bytes and its scale.
+// Kept values on their way: their bytes and their scale.
+template <int E>
 struct KeptPiece {
-    uint32_t lo, hi, scale;
+    uint32_t v[E / 4], scale;
 };
-template <bool NT = false>
-__device__ __forceinline__ KeptPiece hold_kept(const uint8_t* q, const uint8_t* scale, int c, int F) {
-    KeptPiece k = {0, 0, 0};
-    if (c + kPiece <= F) {
-        typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(1)));
-        const v2u_any* p = reinterpret_cast<const v2u_any*>(q + c);
-        const v2u_any v = NT ? __builtin_nontemporal_load(p) : *p;
-        k.lo = v[0];
-        k.hi = v[1];
+template <int E, bool NT>
+__device__ __forceinline__ KeptPiece<E> hold_kept(const uint8_t* q, const uint8_t* scale, int c, int F) {
+    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
+    typedef words words_any __attribute__((aligned(1)));
+    KeptPiece<E> k = {};
+    if (c + E <= F) {
+        const words_any* p = reinterpret_cast<const words_any*>(q + c);
+        const words w = NT ? __builtin_nontemporal_load(p) : *p;
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) k.v[i] = w[i];
     } else if (c < F) {
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e)
-            if (c + e < F) (e < 4 ? k.lo : k.hi) |= (uint32_t)q[c + e] << (8 * (e & 3));
+        for (int e = 0; e < E; ++e)
+            if (c + e < F) k.v[e / 4] |= (uint32_t)q[c + e] << (8 * (e & 3));
     }
     if (c < F) k.scale = scale[c / kKeptBlock];
     return k;
 }
-// Its values at scale s; zeros beyond the row's end.
-__device__ __forceinline__ void kept_values_at(const KeptPiece& k, float s, float x[kPiece]) {
-    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.lo, true);
-    const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.hi, true);
+// The values at scale s; zeros beyond the row's end.
+template <int E>
+__device__ __forceinline__ void kept_values_at(const KeptPiece<E>& k, float s, float x[E]) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        x[e] = a[e] * s;
-        x[2 + e] = b[e] * s;
-        x[4 + e] = c[e] * s;
-        x[6 + e] = d[e] * s;
+    for (int i = 0; i < E / 4; ++i) {
+        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.v[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)k.v[i], true);
+        x[4 * i] = a[0] * s;
+        x[4 * i + 1] = a[1] * s;
+        x[4 * i + 2] = b[0] * s;
+        x[4 * i + 3] = b[1] * s;
     }
 }
 // Those of a row that a kernel kept, far from the largest float.
-__device__ __forceinline__ void kept_values_near(const KeptPiece& k, float x[kPiece]) {
+template <int E>
+__device__ __forceinline__ void kept_values_near(const KeptPiece<E>& k, float x[E]) {
     kept_values_at(k, __builtin_bit_cast(float, k.scale << 23), x);
 }
 // Those of any row. Of the scales that store_kept does not write, 0 stands for 2^-127 and 255 for NaN.
-__device__ __forceinline__ void kept_values(const KeptPiece& k, float x[kPiece]) {
+template <int E>
+__device__ __forceinline__ void kept_values(const KeptPiece<E>& k, float x[E]) {
     kept_values_at(k, __builtin_bit_cast(float, k.scale - 1 < 254u ? k.scale << 23 : (k.scale ? 0x7fc00000u : 0x00400000u)), x);
     if (k.scale >= 247u) {                       // 256 2^120: what the largest floats round to
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) x[e] = within(x[e], 0x1.fffffep127f);
+        for (int e = 0; e < E; ++e) x[e] = within(x[e], 0x1.fffffep127f);
     }
 }
 
@@ -119,60 +131,23 @@ __device__ __forceinline__ void st16s(T* p, v4u v) {
     else st16(p, v);
 }
 constexpr int64_t kStreamBytes = (int64_t)256 << 20;                 // the last level of cache
-// Whether a call that moves n elements of T in pieces of eight does. bf16, both ways (us): norm of 64 MB rows (256 MB in all)
+// Whether a call that moves n elements of T does. bf16, both ways (us): norm of 64 MB rows (256 MB in all)
 // 53 for 51 with ordinary accesses, of 96 MB 75 for 82, of 256 MB 185 for 197; a gate that keeps 128 MB rows 104 for 100, 192 MB
-// 151 for 157. Not in fp32, whose piece is two accesses that each cover half of a stretch of memory: 24,000 x 1440, forward
-// 124 us for 112, unpacked 42 for 31.
+// 151 for 157. Only where neighbouring lanes' accesses lie side by side: with fp32 rows in pieces of eight, two accesses that
+// each cover half of a stretch of memory, the norm of 24,000 x 1440 took 124 us for 112.
 template <typename T>
-static inline bool streams(int64_t n) { return sizeof(T) == 2 && n * (int64_t)sizeof(T) > kStreamBytes; }
-// load_piece and store_piece of such rows.
-template <bool NT, typename T>
-__device__ __forceinline__ void load_row(const T* p, int left, float x[kPiece]) {
-    if (NT && left >= kPiece) {
-        if constexpr (sizeof(T) == 4) {
-            const v4f a = __builtin_bit_cast(v4f, ld16s<NT>(p)), b = __builtin_bit_cast(v4f, ld16s<NT>(p + 4));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = a[e];
-                x[4 + e] = b[e];
-            }
-        } else {
-            const v4u a = ld16s<NT>(p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) unpack2<T>(a[e], x[2 * e], x[2 * e + 1]);
-        }
-    } else {
-        load_piece(p, left, x);
-    }
-}
-template <bool NT, typename T>
-__device__ __forceinline__ void store_row(T* p, int left, const float x[kPiece]) {
-    if (NT && left >= kPiece) {
-        if constexpr (sizeof(T) == 4) {
-            st16s<NT>(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
-            st16s<NT>(p + 4, __builtin_bit_cast(v4u, (v4f){x[4], x[5], x[6], x[7]}));
-        } else {
-            v4u a;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
-            st16s<NT>(p, a);
-        }
-    } else {
-        store_piece(p, left, x);
-    }
-}
-
+static inline bool streams(int64_t n) { return n * (int64_t)sizeof(T) > kStreamBytes; }
 // A piece of a row in its memory's type, on its way: half the registers of its values where they are 16-bit.
 template <typename T>
 struct RawPiece {
     v4u a[sizeof(T) / 2];
 };
-template <bool NT = false, typename T>
+template <typename T>
 __device__ __forceinline__ RawPiece<T> hold_raw(const T* p, int left) {
     RawPiece<T> r = {};
     if (left >= kPiece) {
-        r.a[0] = ld16s<NT>(p);
-        if constexpr (sizeof(T) == 4) r.a[1] = ld16s<NT>(p + 4);
+        r.a[0] = ld16(p);
+        if constexpr (sizeof(T) == 4) r.a[1] = ld16(p + 4);
     } else if (left > 0) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -198,6 +173,63 @@ __device__ __forceinline__ void raw_values(const RawPiece<T>& r, float x[kPiece]
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) unpack2<T>(r.a[0][e], x[2 * e], x[2 * e + 1]);
+    }
+}
+
+// Sixteen bytes of a row, so that neighbouring lanes move neighbouring bytes whatever the type.
+template <typename T>
+struct Sixteen {
+    static constexpr int E = 16 / (int)sizeof(T);
+    v4u a;
+};
+template <bool NT, typename T>
+__device__ __forceinline__ Sixteen<T> hold16(const T* p, int left) {
+    Sixteen<T> r = {};
+    if (left >= Sixteen<T>::E) {
+        r.a = ld16s<NT>(p);
+    } else if (left > 0) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) r.a[e] = __builtin_bit_cast(uint32_t, p[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) r.a[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void values16(const Sixteen<T>& r, float x[Sixteen<T>::E]) {
+    if constexpr (sizeof(T) == 4) {
+        const v4f v = __builtin_bit_cast(v4f, r.a);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpack2<T>(r.a[e], x[2 * e], x[2 * e + 1]);
+    }
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void load16(const T* p, int left, float x[Sixteen<T>::E]) {
+    values16<T>(hold16<NT>(p, left), x);
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void store16(T* p, int left, const float x[Sixteen<T>::E]) {
+    if (left >= Sixteen<T>::E) {
+        if constexpr (sizeof(T) == 4) {
+            st16s<NT>(p, __builtin_bit_cast(v4u, (v4f){x[0], x[1], x[2], x[3]}));
+        } else {
+            v4u a;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
+            st16s<NT>(p, a);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < Sixteen<T>::E; ++e)
+            if (e < left) p[e] = from_f<T>(x[e]);
     }
 }
 

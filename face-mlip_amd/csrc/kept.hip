@@ -3,15 +3,15 @@
 //   y = silu(a) b,  a = x[:F], b = x[F:]
 //   da = dy b silu'(a),  db = dy silu(a);   kept: of a and b as 8 bits hold them, each half in blocks of its own
 //
-// A row's pieces are spread over a power of two of threads; a block's four pieces lie in a quad of lanes. Bound by bytes.
+// A row is spread over a power of two of threads, sixteen bytes each at a time. Bound by bytes.
 #include "kept.h"
 
 namespace face {
 
-// Threads per row (a power of two, whole quads): about four pieces each.
-static inline int kept_lanes_log2(int64_t F) {
-    const int64_t p = 4 * kept_blocks(F);
-    int lg = 2;
+// Threads per row of E values each at a time (a power of two, whole blocks): about four times each.
+static inline int kept_lanes_log2(int64_t F, int E) {
+    const int64_t p = kept_blocks(F) * (kKeptBlock / E);
+    int lg = E == 4 ? 3 : 2;
     while (lg < 8 && ((int64_t)4 << lg) < p) ++lg;
     return lg;
 }
@@ -27,16 +27,17 @@ __device__ __forceinline__ RowAt row_at(int lg) {
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+    constexpr int E = Sixteen<T>::E;
     const RowAt r = row_at(lg);
     if (r.n >= N) return;
     const int end = kKeptBlock * (int)kept_blocks(F);                    // whole quads
     x += r.n * ld;
     q += r.n * F;
     scale += r.n * kept_blocks(F);
-    for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
-        float v[kPiece];
-        load_row<NT>(x + c, F - c, v);
-        store_kept<NT>(q, scale, c, F, v);
+    for (int c = E * r.lane; c < end; c += E * r.lanes) {
+        float v[E];
+        load16<NT>(x + c, F - c, v);
+        store_kept<E, NT>(q, scale, c, F, v);
     }
 }
 
@@ -48,18 +49,18 @@ template <typename T, bool NT>
 __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__ q, int64_t ld_q,
                                                      const uint8_t* __restrict__ scale, int64_t ld_s, int64_t N, int F, int lg,
                                                      T* __restrict__ x) {
+    constexpr int E = Sixteen<T>::E;
     const RowAt r = row_at(lg);
     if (r.n >= N) return;
     q += r.n * ld_q;
     scale += r.n * ld_s;
     x += r.n * F;
-#pragma unroll 4
-    for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
-        float v[kPiece];
-        kept_values(hold_kept<NT>(q, scale, c, F), v);
+    for (int c = E * r.lane; c < F; c += E * r.lanes) {
+        float v[E];
+        kept_values(hold_kept<E, NT>(q, scale, c, F), v);
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) v[e] = within(v[e], kLargest<T>);
-        store_row<NT>(x + c, F - c, v);
+        for (int e = 0; e < E; ++e) v[e] = within(v[e], kLargest<T>);
+        store16<NT>(x + c, F - c, v);
     }
 }
 
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__
 template <typename T, bool KEEP, bool NT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                         T* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+    constexpr int E = Sixteen<T>::E;
     const RowAt r = row_at(lg);
     if (r.n >= N) return;
     const int blocks = (int)kept_blocks(F), end = KEEP ? kKeptBlock * blocks : F;
@@ -74,17 +76,17 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x,
     y += r.n * F;
     q += r.n * 2 * F;
     scale += r.n * 2 * blocks;
-    for (int c = kPiece * r.lane; c < end; c += kPiece * r.lanes) {
-        float a[kPiece], b[kPiece];
-        load_row<NT>(x + c, F - c, a);
-        load_row<NT>(x + F + c, F - c, b);
+    for (int c = E * r.lane; c < end; c += E * r.lanes) {
+        float a[E], b[E];
+        load16<NT>(x + c, F - c, a);
+        load16<NT>(x + F + c, F - c, b);
         if constexpr (KEEP) {
-            store_kept<NT>(q, scale, c, F, a);
-            store_kept<NT>(q + F, scale + blocks, c, F, b);
+            store_kept<E, NT>(q, scale, c, F, a);
+            store_kept<E, NT>(q + F, scale + blocks, c, F, b);
         }
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) a[e] = silu(a[e]) * b[e];
-        store_row<NT>(y + c, F - c, a);
+        for (int e = 0; e < E; ++e) a[e] = silu(a[e]) * b[e];
+        store16<NT>(y + c, F - c, a);
     }
 }
 
@@ -92,6 +94,7 @@ template <typename T, bool KEPT, bool NT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x, int64_t ld, const uint8_t* __restrict__ q,
                                                         const uint8_t* __restrict__ scale, const T* __restrict__ dy,
                                                         int64_t ld_dy, int64_t N, int F, int lg, T* __restrict__ dx) {
+    constexpr int E = Sixteen<T>::E;
     const RowAt r = row_at(lg);
     if (r.n >= N) return;
     const int blocks = (int)kept_blocks(F);
@@ -100,25 +103,24 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x,
     scale += r.n * 2 * blocks;
     dy += r.n * ld_dy;
     dx += r.n * 2 * F;
-#pragma unroll 2
-    for (int c = kPiece * r.lane; c < F; c += kPiece * r.lanes) {
-        float a[kPiece], b[kPiece], d[kPiece];
-        load_row<NT>(dy + c, F - c, d);
+    for (int c = E * r.lane; c < F; c += E * r.lanes) {
+        float a[E], b[E], d[E];
+        load16<NT>(dy + c, F - c, d);
         if constexpr (KEPT) {
-            kept_values(hold_kept<NT>(q, scale, c, F), a);
-            kept_values(hold_kept<NT>(q + F, scale + blocks, c, F), b);
+            kept_values(hold_kept<E, NT>(q, scale, c, F), a);
+            kept_values(hold_kept<E, NT>(q + F, scale + blocks, c, F), b);
         } else {
-            load_row<NT>(x + c, F - c, a);
-            load_row<NT>(x + F + c, F - c, b);
+            load16<NT>(x + c, F - c, a);
+            load16<NT>(x + F + c, F - c, b);
         }
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) {
+        for (int e = 0; e < E; ++e) {
             const float t = a[e];
             a[e] = d[e] * b[e] * silu_slope(t);
             b[e] = d[e] * silu(t);
         }
-        store_row<NT>(dx + c, F - c, a);
-        store_row<NT>(dx + F + c, F - c, b);
+        store16<NT>(dx + c, F - c, a);
+        store16<NT>(dx + F + c, F - c, b);
     }
 }
 
@@ -141,9 +143,9 @@ extern "C" int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F,
     if (ld_x < F) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!x || !q || !scale) return FACE_ERR_ARG;
-    const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
         auto* kern = streams<T>(N * F * 3 / 2) ? pack_kernel<T, true> : pack_kernel<T, false>;
         hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
                            (uint8_t*)q, (uint8_t*)scale);
@@ -158,9 +160,9 @@ extern "C" int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, 
     if (ld_q < F || ld_s < kept_blocks(F)) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!x || !q || !scale) return FACE_ERR_ARG;
-    const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
         auto* kern = streams<T>(N * F * 3 / 2) ? unpack_kernel<T, true> : unpack_kernel<T, false>;
         hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
                            (const uint8_t*)scale, ld_s, N, F, lg, (T*)x);
@@ -175,9 +177,9 @@ extern "C" int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32
     if (ld_x < 2 * (int64_t)F || !q != !scale) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!x || !y) return FACE_ERR_ARG;
-    const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
         const bool nt = streams<T>(N * F * (q ? 4 : 3));
         auto* kern = q ? (nt ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
                        : (nt ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
@@ -194,9 +196,9 @@ extern "C" int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, c
     if ((x && ld_x < 2 * (int64_t)F) || ld_dy < F) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if ((x ? q || scale : !q || !scale) || !dy || !dx) return FACE_ERR_ARG;
-    const int lg = kept_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
         const bool nt = streams<T>(N * F * (q ? 4 : 5));
         auto* kern = q ? (nt ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
                        : (nt ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);

@@ -31,49 +31,70 @@ struct LnFwdArgs {
     float *mean, *rstd;                // may be null
 };
 
-// Columns of a row that are left at a lane's piece u of U: only its last may be cut short.
-template <int U>
-__device__ __forceinline__ int left_at(int u, int c, int F) { return u + 1 < U ? kPiece : F - c; }
-
-template <typename T>
-__device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, float rs, const T* w, const T* b, int left,
-                                         float h[kPiece], float y[kPiece]) {
-    float g[kPiece], o[kPiece] = {};
-    load_piece(w, left, g);
-    if (b) load_piece(b, left, o);
-#pragma unroll
-    for (int e = 0; e < kPiece; ++e) {
-        h[e] = e < left ? (v[e] - mean) * rs : 0.f;
-        y[e] = fmaf(h[e], g[e], o[e]);
+// Which columns of a row a lane has as its piece u of U: eight neighbouring ones of 16-bit rows; of fp32 rows twice four, LANES
+// chunks of four apart, so that the lanes of an access lie side by side. Only the last unit may be cut short.
+template <typename T, int LANES, int U>
+struct LnUnit {
+    static constexpr int E = Sixteen<T>::E, H = kPiece / E;
+    int c, left;                       // first column, columns of the row from there on
+    __device__ __forceinline__ LnUnit(int u, int lane, int F) {
+        c = kPiece * LANES * u + E * lane;
+        left = u + 1 < U ? kPiece * LANES : F - c;
     }
-}
+    __device__ __forceinline__ bool inside(int e) const { return (e < E ? e : E * LANES + e - E) < left; }
+    template <bool NT>
+    __device__ __forceinline__ RawPiece<T> hold(const T* row) const {
+        RawPiece<T> r;
+#pragma unroll
+        for (int h = 0; h < H; ++h) r.a[h] = hold16<NT>(row + c + E * LANES * h, left - E * LANES * h).a;
+        return r;
+    }
+    template <bool NT>
+    __device__ __forceinline__ void load(const T* row, float x[kPiece]) const {
+        raw_values<T>(hold<NT>(row), x);
+    }
+    template <bool NT, typename Y>
+    __device__ __forceinline__ void store(Y* row, const float x[kPiece]) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int at = E * LANES * h;
+            if constexpr (sizeof(Y) == sizeof(T)) store16<NT>(row + c + at, left - at, x + E * h);
+            else store_piece(row + c + at, left - at, x + E * h);       // fp32 sums of 16-bit rows
+        }
+    }
+    template <bool NT>
+    __device__ __forceinline__ void store_8bit(uint8_t* q, const float x[kPiece], float inv) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h) store_e4m3<E, NT>(q + c + E * LANES * h, left - E * LANES * h, x + E * h, inv);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void keep(uint8_t* q, uint8_t* scale, const float x[kPiece]) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h) store_kept<E, NT>(q, scale, c + E * LANES * h, c + left, x + E * h);
+    }
+};
 
 template <typename T, int LANES, int U, int MODE, bool NT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
+    using Unit = LnUnit<T, LANES, U>;
     __shared__ float part[LANES / 32 + 1];
     const int lane = threadIdx.x % LANES, F = a.F;
     const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
     if (n >= a.N) return;                        // a whole row's threads; rows of several waves have a workgroup each
-    const T* x = (const T*)a.x + n * a.ld_x;
     const T *w = (const T*)a.w, *b = (const T*)a.b;
     float v[U][kPiece];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int c = kPiece * (lane + LANES * u);
-        load_row<NT>(x + c, left_at<U>(u, c, F), v[u]);
-    }
+    for (int u = 0; u < U; ++u) Unit(u, lane, F).template load<NT>((const T*)a.x + n * a.ld_x, v[u]);
     if (a.r) {
-        const T* r = (const T*)a.r + n * a.ld_r;
-        T* s = (T*)a.s + n * F;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
+            const Unit at(u, lane, F);
             float t[kPiece];
-            load_row<NT>(r + c, left, t);
+            at.template load<NT>((const T*)a.r + n * a.ld_r, t);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) v[u][e] = to_f(from_f<T>(v[u][e] + t[e]));
-            store_row<NT>(s + c, left, v[u]);
+            at.template store<NT>((T*)a.s + n * F, v[u]);
         }
     }
     float sum = 0.f;
@@ -86,10 +107,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
     float d1 = 0.f, d2 = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int left = left_at<U>(u, kPiece * (lane + LANES * u), F);
+        const Unit at(u, lane, F);
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) {
-            const float d = e < left ? v[u][e] - mean : 0.f;
+            const float d = at.inside(e) ? v[u][e] - mean : 0.f;
             d1 += d;
             d2 = fmaf(d, d, d2);
         }
@@ -106,10 +127,16 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
     uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
-        float h[kPiece], y[kPiece];
-        ln_piece(v[u], mean, rs, w + c, b ? b + c : nullptr, left, h, y);
-        if constexpr (MODE == kLnKept) store_kept<NT>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, c + left, h);
+        const Unit at(u, lane, F);
+        float h[kPiece], g[kPiece], y[kPiece] = {};
+        at.template load<false>(w, g);
+        if (b) at.template load<false>(b, y);
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) {
+            h[e] = at.inside(e) ? (v[u][e] - mean) * rs : 0.f;
+            y[e] = fmaf(h[e], g[e], y[e]);
+        }
+        if constexpr (MODE == kLnKept) at.template keep<NT>(a.q + n * F, a.block_scale + n * kept_blocks(F), h);
         if constexpr (MODE == kLnQ8) {
             // the magnitudes compare as integers, a NaN above everything: its row gets a NaN scale and no number
 #pragma unroll
@@ -119,7 +146,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
                 top = m > top ? m : top;
             }
         } else {
-            store_row<NT>((T*)a.y + n * F + c, left, y);
+            at.template store<NT>((T*)a.y + n * F, y);
         }
     }
     if constexpr (MODE == kLnQ8) {
@@ -128,16 +155,25 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
         if (sc < 0x1p-126f) sc = 0x1p-126f;
         const float inv = 1.f / sc;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u);
-            store_e4m3<NT>(a.q + n * F + c, left_at<U>(u, c, F), v[u], inv);
-        }
+        for (int u = 0; u < U; ++u) Unit(u, lane, F).template store_8bit<NT>(a.q + n * F, v[u], inv);
         if (lane == 0) a.scale[n] = sc;
     }
 }
 
 // Rows of any length, a workgroup each: read for the mean, for the squares and for the result (and for the largest
 // magnitude of rows in 8 bits); a thread reads back only what it wrote itself.
+template <typename T>
+__device__ __forceinline__ void ln_piece(const float v[kPiece], float mean, float rs, const T* w, const T* b, int left,
+                                         float h[kPiece], float y[kPiece]) {
+    float g[kPiece], o[kPiece] = {};
+    load_piece(w, left, g);
+    if (b) load_piece(b, left, o);
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+        h[e] = e < left ? (v[e] - mean) * rs : 0.f;
+        y[e] = fmaf(h[e], g[e], o[e]);
+    }
+}
 template <typename T, int MODE>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
     constexpr int LANES = 1024;
@@ -196,7 +232,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
         float v[kPiece], h[kPiece], y[kPiece];
         load_piece(x + c, F - c, v);
         ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
-        if constexpr (MODE == kLnKept) store_kept(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
+        if constexpr (MODE == kLnKept) store_kept<kPiece, false>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
         if constexpr (MODE == kLnQ8) {
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
@@ -216,7 +252,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
             float v[kPiece], h[kPiece], y[kPiece];
             load_piece(x + c, F - c, v);
             ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
-            store_e4m3(a.q + n * F + c, F - c, y, inv);
+            store_e4m3<kPiece, false>(a.q + n * F + c, F - c, y, inv);
         }
         if (lane == 0) a.scale[n] = sc;
     }
@@ -235,26 +271,29 @@ struct LnBwdArgs {
     float* part;                       // (workgroups, 2 F): sums of dw, of db; may be null
 };
 
-// h of a piece, from the row as it was normalised or as it was kept.
-template <typename T, bool KEPT, bool NT>
+// h of a piece, from the row as it was normalised or as it was kept: chunks of E values, `apart` columns apart.
+template <typename T, bool KEPT, int E>
 struct LnRow {
     RawPiece<T> a;
-    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
-        a = hold_raw<NT>((const T*)g.s + n * g.ld_s + c, left);
-    }
     __device__ __forceinline__ void values(float mean, float rs, float h[kPiece]) const {
         raw_values<T>(a, h);
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) h[e] = (h[e] - mean) * rs;
     }
 };
-template <typename T, bool NT>
-struct LnRow<T, true, NT> {
-    KeptPiece a;
-    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int left) {
-        a = hold_kept<NT>(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c, c + left);
+template <typename T, int E>
+struct LnRow<T, true, E> {
+    KeptPiece<E> a[kPiece / E];
+    template <bool NT>
+    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int apart, int end) {
+#pragma unroll
+        for (int h = 0; h < kPiece / E; ++h)
+            a[h] = hold_kept<E, NT>(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c + apart * h, end);
     }
-    __device__ __forceinline__ void values(float, float, float h[kPiece]) const { kept_values_near(a, h); }
+    __device__ __forceinline__ void values(float, float, float h[kPiece]) const {
+#pragma unroll
+        for (int i = 0; i < kPiece / E; ++i) kept_values_near(a[i], h + E * i);
+    }
 };
 
 // A workgroup takes rows blockIdx, blockIdx + grid, ... and keeps its columns' sums of dw and db in registers over
@@ -264,30 +303,32 @@ struct LnRow<T, true, NT> {
 template <typename T, int LANES, int U, bool KEPT, bool NT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
+    using Unit = LnUnit<T, LANES, U>;
     __shared__ float part[LANES / 32 + 1];
     __shared__ float sums[kRows > 1 ? 2 * LANES * U * kPiece : 1];
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, F = a.F;
     const float inv_f = 1.f / (float)F;
     float aw[U][kPiece] = {}, ab[U][kPiece] = {};
     for (int64_t n = (int64_t)blockIdx.x * kRows + slot; n < a.N; n += (int64_t)gridDim.x * kRows) {
-        LnRow<T, KEPT, NT> row[U];
+        LnRow<T, KEPT, Unit::E> row[U];
         RawPiece<T> dy[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u), left = left_at<U>(u, c, F);
-            row[u].hold(a, n, c, left);
-            dy[u] = a.dy ? hold_raw<NT>((const T*)a.dy + n * a.ld_dy + c, left) : RawPiece<T>{};
-            ds[u] = a.ds && a.dx ? hold_raw<NT>((const T*)a.ds + n * a.ld_ds + c, left) : RawPiece<T>{};
+            const Unit at(u, lane, F);
+            if constexpr (KEPT) row[u].template hold<NT>(a, n, at.c, Unit::E * LANES, at.c + at.left);
+            else row[u].a = at.template hold<NT>((const T*)a.s + n * a.ld_s);
+            dy[u] = a.dy ? at.template hold<NT>((const T*)a.dy + n * a.ld_dy) : RawPiece<T>{};
+            ds[u] = a.ds && a.dx ? at.template hold<NT>((const T*)a.ds + n * a.ld_ds) : RawPiece<T>{};
         }
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u);
+            const Unit at(u, lane, F);
             float h[kPiece], d[kPiece], w[kPiece];
             row[u].values(mean, rs, h);
             raw_values<T>(dy[u], d);
-            load_piece((const T*)a.w + c, left_at<U>(u, c, F), w);
+            at.template load<false>((const T*)a.w, w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
                 ab[u][e] += d[e];
@@ -303,15 +344,15 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
         sh *= inv_f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = kPiece * (lane + LANES * u);
+            const Unit at(u, lane, F);
             float h[kPiece], d[kPiece], w[kPiece], o[kPiece];
             row[u].values(mean, rs, h);
             raw_values<T>(dy[u], d);
             raw_values<T>(ds[u], o);
-            load_piece((const T*)a.w + c, left_at<U>(u, c, F), w);
+            at.template load<false>((const T*)a.w, w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
-            store_row<NT>((T*)a.dx + n * F + c, left_at<U>(u, c, F), o);
+            at.template store<NT>((T*)a.dx + n * F, o);
         }
     }
     if (!a.part) return;
@@ -341,10 +382,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int c = kPiece * (lane + LANES * u);
+        const Unit at(u, lane, F);
         float* p = a.part + (int64_t)blockIdx.x * 2 * F;
-        store_piece(p + c, left_at<U>(u, c, F), aw[u]);
-        store_piece(p + F + c, left_at<U>(u, c, F), ab[u]);
+        at.template store<false>(p, aw[u]);
+        at.template store<false>(p + F, ab[u]);
     }
 }
 
@@ -362,8 +403,9 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnBwdArgs a) {
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
         auto load = [&](int c, float h[kPiece], float d[kPiece], float w[kPiece]) {
-            LnRow<T, KEPT, false> row;
-            row.hold(a, n, c, F - c);
+            LnRow<T, KEPT, kPiece> row;
+            if constexpr (KEPT) row.template hold<false>(a, n, c, 0, F);
+            else row.a = hold_raw((const T*)a.s + n * a.ld_s + c, F - c);
             row.values(mean, rs, h);
             RawPiece<T> r = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
             raw_values<T>(r, d);
@@ -462,12 +504,13 @@ static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
     const int64_t rows = ln_rows(a.F), blocks = (a.N + rows - 1) / rows;
     if (blocks > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks);
+    const bool nt = streams<T>(a.N * a.F * (a.r ? 4 : 2));
     if (a.F > kLnHeld) {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);
     }
 #define FACE_ROW(L_, U_)                                                                                                 \
     else if (sh.lanes == L_ && sh.units == U_)                                                                          \
-        hipLaunchKernelGGL((streams<T>(a.N * a.F * (a.r ? 4 : 2)) ? ln_fwd_kernel<T, L_, U_, MODE, true>        \
+        hipLaunchKernelGGL((nt ? ln_fwd_kernel<T, L_, U_, MODE, true>        \
                                                                            : ln_fwd_kernel<T, L_, U_, MODE, false>),     \
                            grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
     FACE_LN_ROWS
@@ -482,12 +525,13 @@ static int launch_ln_bwd(const LnBwdArgs& a, T* dw, T* db, hipStream_t st) {
     const int64_t blocks = ln_bwd_grid(a.N, a.F, sizeof(T) == 4);
     if (blocks) {
         const dim3 grid((unsigned)blocks);
+        const bool nt = streams<T>(a.N * a.F * (a.ds ? 4 : 3));
         if (a.F > kLnHeld) {
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, KEPT>), grid, dim3(1024), 0, st, a);
         }
 #define FACE_ROW(L_, U_)                                                                                                 \
     else if (sh.lanes == L_ && sh.units == U_)                                                                          \
-        hipLaunchKernelGGL((streams<T>(a.N * a.F * (a.ds ? 4 : 3)) ? ln_bwd_kernel<T, L_, U_, KEPT, true>        \
+        hipLaunchKernelGGL((nt ? ln_bwd_kernel<T, L_, U_, KEPT, true>        \
                                                                            : ln_bwd_kernel<T, L_, U_, KEPT, false>),     \
                            grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
         FACE_LN_ROWS

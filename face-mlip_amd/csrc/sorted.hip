@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void places_kernel(const int32_t* __restrict__
 }
 
 // Threads per row.
-static inline int sorted_lanes_log2(int64_t F) { return F <= 512 ? 4 : (F <= 4096 ? 6 : 8); }
+static inline int sorted_lanes_log2(int64_t F, int size) { return F * size <= 1024 ? 4 : (F * size <= 8192 ? 6 : 8); }
 
 // xs[p] = x[order[p] / k].
 template <typename T, bool NT>
@@ -53,16 +53,16 @@ __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restric
                                                               const int32_t* __restrict__ ptr,
                                                               const int32_t* __restrict__ order, int64_t slots, int k, int G,
                                                               int F, int lg, T* __restrict__ xs) {
+    constexpr int E = Sixteen<T>::E;
     const int64_t p = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
     if (p >= slots) return;
     const int a = p < places_of(ptr, G, slots) ? order[p] : -1;
     const bool some = a >= 0 && a < slots;
     const T* from = x + (int64_t)(some ? a / k : 0) * ld;
-#pragma unroll 4
-    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
-        float v[kPiece] = {};
-        if (some) load_row<NT>(from + c, F - c, v);
-        store_row<NT>(xs + p * F + c, F - c, v);
+    for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
+        float v[E] = {};
+        if (some) load16<NT>(from + c, F - c, v);
+        store16<NT>(xs + p * F + c, F - c, v);
     }
 }
 
@@ -74,6 +74,7 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
                                                                const int32_t* __restrict__ order,
                                                                const int32_t* __restrict__ place, int64_t slots, int k, int G,
                                                                int F, int lg, T* __restrict__ xs) {
+    constexpr int E = Sixteen<T>::E;
     const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
     if (n * k >= slots) return;
     const int64_t m = places_of(ptr, G, slots);
@@ -89,41 +90,59 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
             const int a = in && i < m ? order[i] : -1;
             bare[j] = in && (a < 0 || a >= slots || place[a] != i);
         }
-#pragma unroll 2
-        for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
-            float v[kPiece];
-            const float none[kPiece] = {};
-            load_row<NT>(x + n * ld + c, F - c, v);
+        for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
+            float v[E];
+            const float none[E] = {};
+            load16<NT>(x + n * ld + c, F - c, v);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                if (p[j] >= 0) store_row<NT>(xs + (int64_t)p[j] * F + c, F - c, v);
-                if (bare[j]) store_row<NT>(xs + (n * k + j0 + j) * F + c, F - c, none);
+                if (p[j] >= 0) store16<NT>(xs + (int64_t)p[j] * F + c, F - c, v);
+                if (bare[j]) store16<NT>(xs + (n * k + j0 + j) * F + c, F - c, none);
             }
         }
     }
 }
 
-// out[i] = r[i] + sum_j w[i, j] y[place(i k + j)], in order; w null: ones.
+// out[i] = r[i] + sum_j w[i, j] y[place(i k + j)], in order; w null: ones. Four slots per turn, their rows on the way
+// together; the first four's places are known before any row is asked for.
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ place,
                                                          const float* __restrict__ w, const T* __restrict__ r, int64_t ld_r,
                                                          int64_t N, int k, int F, int lg, T* __restrict__ out) {
+    constexpr int E = Sixteen<T>::E;
     const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
     if (n >= N) return;
-    for (int c = kPiece * (threadIdx.x & ((1 << lg) - 1)); c < F; c += kPiece << lg) {
-        float s[kPiece] = {};
-        if (r) load_row<NT>(r + n * ld_r + c, F - c, s);
-#pragma unroll 4
-        for (int j = 0; j < k; ++j) {
-            const int p = place[n * k + j];
-            if (p < 0) continue;
-            float v[kPiece];
-            load_row<NT>(y + (int64_t)p * ld_y + c, F - c, v);
-            const float f = w ? w[n * k + j] : 1.f;
+    constexpr int J = 4;
+    int p[J];
+    float f[J];
+    auto turn = [&](int j0) {
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) s[e] = fmaf(f, v[e], s[e]);
+        for (int j = 0; j < J; ++j) {
+            const int64_t i = n * k + j0 + j;
+            p[j] = j0 + j < k ? place[i] : -1;
+            f[j] = j0 + j < k && w ? w[i] : 1.f;
         }
-        store_row<NT>(out + n * F + c, F - c, s);
+    };
+    turn(0);
+    for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
+        float s[E] = {};
+        if (r) load16<NT>(r + n * ld_r + c, F - c, s);
+        for (int j0 = 0; j0 < k; j0 += J) {
+            if (k > J) turn(j0);
+            Sixteen<T> v[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (p[j] >= 0) v[j] = hold16<NT>(y + (int64_t)p[j] * ld_y + c, F - c);
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (p[j] >= 0) {
+                    float x[E];
+                    values16<T>(v[j], x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) s[e] = fmaf(f[j], x[e], s[e]);
+                }
+        }
+        store16<NT>(out + n * F + c, F - c, s);
     }
 }
 
@@ -135,6 +154,7 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
                                                          const int32_t* __restrict__ place, const float* __restrict__ w,
                                                          int64_t N, int k, int G, int F, T* __restrict__ dy,
                                                          float* __restrict__ dw) {
+    constexpr int E = Sixteen<T>::E;
     __shared__ float part[LANES / 64 + 1];
     const int lane = threadIdx.x % LANES;
     const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -154,26 +174,26 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
             const int a = in && i < m ? order[i] : -1;
             bare[j] = in && (a < 0 || a >= slots || place[a] != i);
         }
-        for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
-            float d[kPiece];
-            load_row<NT>(dout + n * ld_d + c, F - c, d);
+        for (int c = E * lane; c < F; c += E * LANES) {
+            float d[E];
+            load16<NT>(dout + n * ld_d + c, F - c, d);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                float v[kPiece];
+                float v[E];
                 if (dw && p[j] >= 0) {
-                    load_row<NT>(y + (int64_t)p[j] * ld_y + c, F - c, v);
+                    load16<NT>(y + (int64_t)p[j] * ld_y + c, F - c, v);
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e) s[j] = fmaf(d[e], v[e], s[j]);
+                    for (int e = 0; e < E; ++e) s[j] = fmaf(d[e], v[e], s[j]);
                 }
                 if (!dy) continue;
                 if (p[j] >= 0) {
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e) v[e] = f[j] * d[e];
-                    store_row<NT>(dy + (int64_t)p[j] * F + c, F - c, v);
+                    for (int e = 0; e < E; ++e) v[e] = f[j] * d[e];
+                    store16<NT>(dy + (int64_t)p[j] * F + c, F - c, v);
                 }
                 if (bare[j]) {
-                    const float none[kPiece] = {};
-                    store_row<NT>(dy + (n * k + j0 + j) * F + c, F - c, none);
+                    const float none[E] = {};
+                    store16<NT>(dy + (n * k + j0 + j) * F + c, F - c, none);
                 }
             }
         }
@@ -224,10 +244,10 @@ extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, cons
     if (ld_x < F) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!x || !ptr || !order || !xs) return FACE_ERR_ARG;
-    const int lg = sorted_lanes_log2(F);
     const int64_t slots = N * k;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = sorted_lanes_log2(F, sizeof(T));
         const bool nt = streams<T>((slots + N) * F);
         if (place)
             hipLaunchKernelGGL((nt ? dispatch_scatter_kernel<T, true> : dispatch_scatter_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x,
@@ -246,9 +266,9 @@ extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t
     if (ld_y < F || (r && ld_r < F)) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!y || !place || !out) return FACE_ERR_ARG;
-    const int lg = sorted_lanes_log2(F);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int lg = sorted_lanes_log2(F, sizeof(T));
         const bool nt = streams<T>((N * k + N * (r ? 2 : 1)) * F);
         hipLaunchKernelGGL((nt ? return_fwd_kernel<T, true> : return_fwd_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, place,
                            weight, (const T*)r, ld_r, N, k, F, lg, (T*)out);
@@ -264,10 +284,10 @@ extern "C" int face_expert_return_bwd(const void* dout, int64_t ld_d, const void
     if (ld_d < F || (dweight && ld_y < F)) return FACE_ERR_ARG;
     if (N == 0 || (!dy && !dweight)) return 0;
     if (!dout || !ptr || !order || !place || (dweight && !y)) return FACE_ERR_ARG;
-    const int L = F <= 512 ? 16 : (F <= 4096 ? 64 : 256), rows = 256 / L;
-    const dim3 grid((unsigned)((N + rows - 1) / rows));
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        const int L = 1 << sorted_lanes_log2(F, sizeof(T)), rows = 256 / L;
+        const dim3 grid((unsigned)((N + rows - 1) / rows));
         const bool nt = streams<T>((2 * N * k + N) * F);
         auto* kern = L == 16 ? (nt ? return_bwd_kernel<T, 16, true> : return_bwd_kernel<T, 16, false>)
                    : L == 64 ? (nt ? return_bwd_kernel<T, 64, true> : return_bwd_kernel<T, 64, false>)

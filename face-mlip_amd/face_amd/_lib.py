@@ -194,7 +194,13 @@ def record_order(on=True, after=None):
     return _order
 
 
-def _raise(name, code):
+def listening():
+    """Whether calls are timed or logged."""
+    return _timing is not None or _order is not None
+
+
+def fail(name, code):
+    """Raise what a call of `name` that returned `code` stands for."""
     msg = lib().face_hip_error_string(code).decode()
     raise RuntimeError(f"{name} failed: {msg} (code {code})")
 
@@ -202,12 +208,7 @@ def _raise(name, code):
 def call(name, *args, label=None):
     """Call entry point `name`; raise RuntimeError on a non-zero status. `label` names the
     launch for time_calls (defaults to the entry-point name)."""
-    fn = getattr(_lib or lib(), name)
-    if _timing is None and _order is None:       # nobody listens
-        code = fn(*args)
-        if code != 0:
-            _raise(name, code)
-        return
+    fn = getattr(lib(), name)
     key = label or name
     # "name*n": a launch doing the work of n calls of "name" (passes or moment sets merged)
     if _timing is not None and key.split("*")[0] in _timing:
@@ -219,7 +220,7 @@ def call(name, *args, label=None):
     else:
         code = fn(*args)
     if code != 0:
-        _raise(name, code)
+        fail(name, code)
     if _order is not None:
         _order.append(key)
         if _after_call is not None:

@@ -67,29 +67,37 @@ def _check(name, ref, **tensors):
 def _rows(t, width):
     """t as (rows, width) with unit column stride and rows one after the other: a view where its
     strides allow one, else a copy."""
-    if t.dim() != 2:
+    strides = t.stride()
+    if len(strides) != 2:
         t = t.reshape(-1, width)
-    if t.stride(1) == 1 and t.stride(0) >= width:
+        strides = t.stride()
+    if strides[1] == 1 and strides[0] >= width:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = _lib._raw_stream
 
 
 def _launch(t, name, label, *args):
     """Call entry point `name` with args and the current stream of t's device, as the current device."""
     idx = t.get_device()
-    if idx == _get_device():
-        call(name, *args, _lib.stream_of(t) if _lib._raw_stream is None else _lib._raw_stream(idx), label=label)
-    else:
+    if idx != _get_device():
         with torch.cuda.device(idx):
             call(name, *args, _lib.stream_of(t), label=label)
+    elif _raw_stream is None or _lib.listening():
+        call(name, *args, _lib.stream_of(t), label=label)
+    else:                                        # call() for nobody that listens, half its host time
+        code = getattr(_lib.lib(), name)(*args, _raw_stream(idx))
+        if code:
+            _lib.fail(name, code)
 
 
 def _once(name, *grads):
     """A backward that is itself recorded, or whose incoming gradients have tangents, would need second derivatives."""
-    _no_tangents(name + "'s gradient", *grads)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents(name + "'s gradient", *grads)
     if torch.is_grad_enabled():
         raise NotImplementedError("the expert layer's operators differentiate once (create_graph=False)")
 
