@@ -213,38 +213,29 @@ static int sorted_args(int64_t N, int32_t k, int32_t G, int32_t F, int32_t dtype
     if (F > (1 << 28) || N > (int64_t)0x7fffffff || N * k > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
     return 0;
 }
+static void launch_places(const int32_t* ptr, const int32_t* order, int64_t slots, int G, int32_t* place, hipStream_t st) {
+    if (slots <= kPlacesOne) {
+        hipLaunchKernelGGL(places_one_kernel, dim3(1), dim3(1024), 0, st, ptr, order, (int)slots, G, place);
+        return;
+    }
+    const dim3 grid((unsigned)((slots + 255) / 256));
+    hipLaunchKernelGGL(places_none_kernel, grid, dim3(256), 0, st, slots, place);
+    hipLaunchKernelGGL(places_kernel, grid, dim3(256), 0, st, ptr, order, slots, G, place);
+}
 static dim3 sorted_grid(int64_t rows, int lg) { return dim3((unsigned)((rows + (256 >> lg) - 1) >> (8 - lg))); }
 
 }  // namespace face
 
 using namespace face;
 
-extern "C" int face_expert_places(const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t* place,
-                                  void* stream) {
-    if (slots < 0 || G <= 0) return FACE_ERR_ARG;
-    if (slots > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    if (slots == 0) return 0;
-    if (!ptr || !order || !place) return FACE_ERR_ARG;
-    const hipStream_t st = (hipStream_t)stream;
-    if (slots <= kPlacesOne) {
-        hipLaunchKernelGGL(places_one_kernel, dim3(1), dim3(1024), 0, st, ptr, order, (int)slots, G, place);
-    } else {
-        const dim3 grid((unsigned)((slots + 255) / 256));
-        hipLaunchKernelGGL(places_none_kernel, grid, dim3(256), 0, st, slots, place);
-        hipLaunchKernelGGL(places_kernel, grid, dim3(256), 0, st, ptr, order, slots, G, place);
-    }
-    FACE_LAUNCH_CHECK();
-    return 0;
-}
-
 extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, const int32_t* ptr, const int32_t* order,
-                                    const int32_t* place, int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs,
-                                    void* stream) {
+                                    int32_t* place, int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs, void* stream) {
     if (int rc = sorted_args(N, k, G, F, dtype)) return rc;
     if (ld_x < F) return FACE_ERR_ARG;
     if (N == 0) return 0;
     if (!x || !ptr || !order || !xs) return FACE_ERR_ARG;
     const int64_t slots = N * k;
+    if (place) launch_places(ptr, order, slots, G, place, (hipStream_t)stream);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = sorted_lanes_log2(F, sizeof(T));
@@ -260,12 +251,14 @@ extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, cons
     });
 }
 
-extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* place, const float* weight, const void* r,
-                                      int64_t ld_r, int64_t N, int32_t k, int32_t F, int32_t dtype, void* out, void* stream) {
-    if (int rc = sorted_args(N, k, 1, F, dtype)) return rc;
+extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* ptr, const int32_t* order, int32_t* place,
+                                      int32_t placed, const float* weight, const void* r, int64_t ld_r, int64_t N, int32_t k,
+                                      int32_t G, int32_t F, int32_t dtype, void* out, void* stream) {
+    if (int rc = sorted_args(N, k, G, F, dtype)) return rc;
     if (ld_y < F || (r && ld_r < F)) return FACE_ERR_ARG;
     if (N == 0) return 0;
-    if (!y || !place || !out) return FACE_ERR_ARG;
+    if (!y || !place || !out || (!placed && (!ptr || !order))) return FACE_ERR_ARG;
+    if (!placed) launch_places(ptr, order, N * k, G, place, (hipStream_t)stream);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = sorted_lanes_log2(F, sizeof(T));

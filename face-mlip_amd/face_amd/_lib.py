@@ -115,9 +115,8 @@ _SIGS = {
     "face_embed_fwd": (ctypes.c_int, [P, I64, P, I32, I64, I64, I32, I32, F32, P, P, P]),
     "face_embed_bwd_work": (I64, [I64, I64, I32]),
     "face_embed_bwd": (ctypes.c_int, [P, P, I64, I64, I64, I32, I32, F32, P, P, I64, P]),
-    "face_expert_places": (ctypes.c_int, [P, P, I64, I32, P, P]),
     "face_expert_dispatch": (ctypes.c_int, [P, I64, I32, P, P, P, I64, I32, I32, I32, P, P]),
-    "face_expert_return_fwd": (ctypes.c_int, [P, I64, P, P, P, I64, I64, I32, I32, I32, P, P]),
+    "face_expert_return_fwd": (ctypes.c_int, [P, I64, P, P, P, I32, P, P, I64, I64, I32, I32, I32, I32, P, P]),
     "face_expert_return_bwd": (ctypes.c_int, [P, I64, P, I64, P, P, P, P, I64, I32, I32, I32, I32, P, P, P]),
 }
 

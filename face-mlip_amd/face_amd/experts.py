@@ -794,13 +794,6 @@ def expert_combine(y, weight, residual=None):
 
 
 # ----------------------------------------------------------------------------- rows by expert and back
-def _places(like, p, order, slots):
-    """The inverse of a plan's order: the place of every slot, -1 of one that has none."""
-    place = torch.empty(slots, dtype=torch.int32, device=order.device)
-    _launch(like, "face_expert_places", "expert_places", p.data_ptr(), order.data_ptr(), slots, p.shape[0] - 1, place.data_ptr())
-    return place
-
-
 def _by_rows(slots, k, F):
     """Whether rows are read once and written to their k places, which takes the order's inverse first, or gathered by
     the order, read k times."""
@@ -810,7 +803,7 @@ def _by_rows(slots, k, F):
 def _dispatch_fwd(x, p, order, k):
     F, slots = x.shape[1], order.shape[0]
     x2 = _rows(x, F)
-    place = _places(x, p, order, slots) if _by_rows(slots, k, F) else None
+    place = torch.empty_like(order) if _by_rows(slots, k, F) else None
     xs = torch.empty(slots, F, dtype=x.dtype, device=x.device)
     _launch(x, "face_expert_dispatch", "expert_dispatch", x2.data_ptr(), x2.stride(0), k, p.data_ptr(), order.data_ptr(), ptr(place),
             x.shape[0], p.shape[0] - 1, F, _DTYPES[x.dtype], xs.data_ptr())
@@ -829,9 +822,7 @@ class ExpertDispatch(torch.autograd.Function):
     def backward(ctx, dxs):
         _once("expert_dispatch", dxs)
         p, order, place = ctx.saved_tensors
-        if place is None:
-            place = _places(dxs, p, order, order.shape[0])
-        return _return_fwd(dxs, place, None, None, ctx.rows, ctx.k), None, None, None
+        return _return_fwd(dxs, p, order, place, None, None, ctx.rows, ctx.k)[0], None, None, None
 
 
 def expert_dispatch(x, plan):
@@ -851,24 +842,29 @@ def expert_dispatch(x, plan):
     return _dispatch_fwd(x, plan.ptr, plan.order, k)[0]
 
 
-def _return_fwd(y, place, weight, residual, N, k):
+def _return_fwd(y, p, order, place, weight, residual, N, k):
+    """(out, place): place, the inverse of the plan's order, is made here if it is None."""
     F = y.shape[1]
     y2, w = _rows(y, F), None if weight is None else weight.contiguous()
     r = None if residual is None else _rows(residual, F)
+    placed = place is not None
+    if not placed:
+        place = torch.empty_like(order)
     out = torch.empty(N, F, dtype=y.dtype, device=y.device)
-    _launch(y, "face_expert_return_fwd", "expert_return_fwd", y2.data_ptr(), y2.stride(0), place.data_ptr(), ptr(w), ptr(r),
-            F if r is None else r.stride(0), N, k, F, _DTYPES[y.dtype], out.data_ptr())
-    return out
+    _launch(y, "face_expert_return_fwd", "expert_return_fwd", y2.data_ptr(), y2.stride(0), p.data_ptr(), order.data_ptr(),
+            place.data_ptr(), int(placed), ptr(w), ptr(r), F if r is None else r.stride(0), N, k, p.shape[0] - 1, F,
+            _DTYPES[y.dtype], out.data_ptr())
+    return out, place
 
 
 class ExpertReturn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weight, residual, p, order, rows, k):
-        place = _places(y, p, order, order.shape[0])
+        out, place = _return_fwd(y, p, order, None, weight, residual, rows, k)
         # without a gradient of the weights the backward reads no row of y
         ctx.save_for_backward(y if weight is not None and ctx.needs_input_grad[1] else None, weight, p, order, place)
         ctx.rows, ctx.k = rows, k
-        return _return_fwd(y, place, weight, residual, rows, k)
+        return out
 
     @staticmethod
     def backward(ctx, dout):
@@ -908,4 +904,4 @@ def expert_return(y, plan, weight=None, residual=None):
     _check(name, y, plan=plan.ptr, weight=weight, residual=residual)
     if _wants_grad(y, weight, residual):
         return ExpertReturn.apply(y, weight, residual, plan.ptr, plan.order, plan.rows, plan.k)
-    return _return_fwd(y, _places(y, plan.ptr, plan.order, plan.slots), weight, residual, plan.rows, plan.k)
+    return _return_fwd(y, plan.ptr, plan.order, None, weight, residual, plan.rows, plan.k)[0]

@@ -658,16 +658,16 @@ int64_t face_embed_bwd_work(int64_t N, int64_t V, int32_t F);
 int face_embed_bwd(const int32_t* key, const void* dy, int64_t ld_dy, int64_t N, int64_t V, int32_t F, int32_t dtype,
                    float factor, void* dtable, void* work, int64_t work_bytes, void* stream);
 
-/* place (slots) = the inverse of a plan's order: where in it, before ptr[G], a slot is, -1 for slots that are not. */
-int face_expert_places(const int32_t* ptr, const int32_t* order, int64_t slots, int32_t G, int32_t* place, void* stream);
-/* xs[p] (N k, F) = x[order[p] / k], 0 for the places that hold no slot, from ptr[G] on; place NULL: gathered by order, else
- * scattered by it. */
-int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, const int32_t* ptr, const int32_t* order,
-                         const int32_t* place, int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs, void* stream);
+/* xs[p] (N k, F) = x[order[p] / k], 0 for the places that hold no slot, from ptr[G] on. place (N k) or NULL: gathered by
+ * order, or scattered by its inverse, written to place: where in order, before ptr[G], a slot is, -1 for slots that are
+ * not. */
+int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, const int32_t* ptr, const int32_t* order, int32_t* place,
+                         int64_t N, int32_t G, int32_t F, int32_t dtype, void* xs, void* stream);
 /* out[i] (N, F) = r[i] + sum_j weight[i, j] y[place[i k + j]]; r NULL: 0, weight (N, k) NULL: 1. With weight and r NULL
- * the gradient of face_expert_dispatch. */
-int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* place, const float* weight, const void* r,
-                           int64_t ld_r, int64_t N, int32_t k, int32_t F, int32_t dtype, void* out, void* stream);
+ * the gradient of face_expert_dispatch. placed 0: place (N k) is written first, from ptr and order (else not read). */
+int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t* ptr, const int32_t* order, int32_t* place,
+                           int32_t placed, const float* weight, const void* r, int64_t ld_r, int64_t N, int32_t k, int32_t G,
+                           int32_t F, int32_t dtype, void* out, void* stream);
 /* dy (N k, F) = weight dout at the slots' places, 0 elsewhere, dweight (N, k) = dout . y; either may be NULL. */
 int face_expert_return_bwd(const void* dout, int64_t ld_d, const void* y, int64_t ld_y, const int32_t* ptr,
                            const int32_t* order, const int32_t* place, const float* weight, int64_t N, int32_t k, int32_t G,

@@ -117,12 +117,11 @@ def test_entry_points_refuse_bad_arguments():
     eb = lambda N=5000, V=100, ld=8, n=need, work=ok, d=ok, key=ok: L.face_embed_bwd(key, ok, ld, N, V, 8, 0, 1.0, d, work, n, None)
     assert need > 0 and eb(N=-1) == eb(V=0) == eb(ld=7) == eb(n=need - 1) == eb(work=None) == eb(d=None) == eb(key=None) == -1
     assert L.face_embed_bwd_work(100, 100, 8) == 0
-    pl = lambda slots=4, G=2, p=ok: L.face_expert_places(p, ok, slots, G, ok, None)
-    assert pl(slots=-1) == pl(G=0) == pl(p=None) == -1 and pl(slots=0) == 0 and pl(slots=1 << 31) == -2
     dp = lambda N=4, k=2, G=2, F=8, ld=8, dt=0, x=ok: L.face_expert_dispatch(x, ld, k, ok, ok, None, N, G, F, dt, ok, None)
     assert dp(N=-1) == dp(k=0) == dp(G=0) == dp(F=0) == dp(ld=7) == dp(dt=3) == dp(x=None) == -1 and dp(N=0) == 0
     assert dp(N=1 << 30, k=2) == -2
-    rf = lambda N=4, k=2, F=8, ld=8, p=ok, r=None: L.face_expert_return_fwd(ok, ld, p, ok, r, 7, N, k, F, 0, ok, None)
-    assert rf(N=-1) == rf(k=0) == rf(F=0) == rf(ld=7) == rf(p=None) == rf(r=ok) == -1 and rf(N=0) == 0
+    rf = lambda N=4, k=2, F=8, ld=8, p=ok, r=None, o=ok, G=2: L.face_expert_return_fwd(ok, ld, o, o, p, 0, ok, r, 7, N, k, G, F, 0, ok,
+                                                                                     None)
+    assert rf(N=-1) == rf(k=0) == rf(F=0) == rf(ld=7) == rf(p=None) == rf(r=ok) == rf(o=None) == rf(G=0) == -1 and rf(N=0) == 0
     rb = lambda dy=ok, dw=ok, y=ok, ld=8: L.face_expert_return_bwd(ok, ld, y, 8, ok, ok, ok, ok, 4, 2, 2, 8, 0, dy, dw, None)
     assert rb(y=None) == rb(ld=7) == -1 and rb(dy=None, dw=None) == 0
