@@ -193,11 +193,6 @@ def record_order(on=True, after=None):
     return _order
 
 
-def listening():
-    """Whether calls are timed or logged."""
-    return _timing is not None or _order is not None
-
-
 def fail(name, code):
     """Raise what a call of `name` that returned `code` stands for."""
     msg = lib().face_hip_error_string(code).decode()
