@@ -20,7 +20,7 @@ constexpr int64_t kEmbedStream = (int64_t)48 << 20;
 
 // R rows per group of lanes, a workgroup's groups side by side, so that the rows' indices, then their entries, are on
 // their way together.
-template <typename T, typename I, int R, bool NT>
+template <typename T, typename I, int R, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t ld, const I* __restrict__ index,
                                                         int64_t N, int64_t V, int F, float factor, int lg, T* __restrict__ y,
                                                         int32_t* __restrict__ key) {
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
     for (int c = E * lane; c < F; c += E << lg) {
         Sixteen<T> r[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) r[i] = hold16<false>(table + (in[i] ? (int64_t)v[i] : 0) * ld + c, in[i] ? F - c : 0);
+        for (int i = 0; i < R; ++i) r[i] = hold16<false, CUT>(table + (in[i] ? (int64_t)v[i] : 0) * ld, c, in[i] ? F : 0);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int64_t n = n0 + i * groups;
@@ -47,17 +47,17 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
             values16<T>(r[i], x);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = in[i] ? x[e] * factor : 0.f;
-            if (n < N) store16<NT>(y + n * F + c, F - c, x);
+            if (n < N) store16<NT, CUT>(y + n * F, c, F, x);
         }
     }
 }
 
 // ---------------------------------------------------------------- few entries or few rows
-// A lane's sums in fp32.
+// A lane's sums in fp32, to columns [c, c + E) of a row of F.
 template <int E>
-__device__ __forceinline__ void store_sums(float* p, int left, const float x[E]) {
-    if constexpr (E == 8) store_piece(p, left, x);
-    else store16<false>(p, left, x);
+__device__ __forceinline__ void store_sums(float* row, int c, int F, const float x[E]) {
+    store16<false, true>(row, c, F, x);
+    if constexpr (E == 8) store16<false, true>(row, c + 4, F, x + 4);
 }
 
 // A wave: rows [chunk R, chunk R + R), entries [block TV, block TV + TV), 64 times sixteen bytes of the columns. Partial sums
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const int32_t* __restri
                     if (m) {
                         const int i = __builtin_ctzll(m);
                         m &= m - 1;
-                        r[u] = hold16<false>(dy + (a + i) * ld + c, left);
+                        r[u] = hold16<false, true>(dy + (a + i) * ld, c, F);
                     }
                 }
 #pragma unroll
@@ -102,11 +102,11 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const int32_t* __restri
         }
         if (left <= 0) continue;
         if (part) {
-            store_sums<E>(part + (chunk * V + v) * F + c, left, s);
+            store_sums<E>(part + (chunk * V + v) * F, c, F, s);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) s[e] *= factor;
-            store16<false>(out + v * F + c, left, s);
+            store16<false, true>(out + v * F, c, F, s);
         }
     }
 }
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(T* __restrict__ out, in
 
 // Groups of LC lanes, C sorted rows each. part (shares, 2, F): a run that comes from the share before (0), one that begins
 // here and goes on (1). The next rows' numbers are on their way while the present ones are added.
-template <typename T, int LC, bool NT>
+template <typename T, int LC, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restrict__ key, const int32_t* __restrict__ row,
                                                          const T* __restrict__ dy, int64_t ld, int64_t N, int64_t C, int V, int F,
                                                          float factor, float* __restrict__ part, T* __restrict__ out) {
@@ -389,12 +389,12 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restri
     float acc[E] = {};
     auto flush = [&](bool goes_on) {
         if (from_before || goes_on) {
-            store_sums<E>(part + (2 * s + (from_before ? 0 : 1)) * F + c, left, acc);
+            store_sums<E>(part + (2 * s + (from_before ? 0 : 1)) * F, c, F, acc);
         } else {
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = factor * acc[e];
-            store16<false>(out + (int64_t)cur * F + c, left, o);
+            store16<false, true>(out + (int64_t)cur * F, c, F, o);
         }
     };
     int k[U], next_k[U];
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const int32_t* __restri
     for (int64_t p = begin; p < end; p += U) {
         Sixteen<T> r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = hold16<NT>(dy + (int64_t)at[u] * ld + c, left);
+        for (int u = 0; u < U; ++u) r[u] = hold16<NT, CUT>(dy + (int64_t)at[u] * ld, c, F);
         if (p + U < end) numbers(p + U, next_k, next_at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -626,8 +626,10 @@ static int launch_embed_bwd(const int32_t* key, const T* dy, int64_t ld, int64_t
     const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream;
 #define FACE_RUNS(L_)                                                                                                     \
     if (p.lanes == L_)                                                                                                    \
-        hipLaunchKernelGGL((nt ? embed_runs_kernel<T, L_, true> : embed_runs_kernel<T, L_, false>), grid, dim3(256), 0, st, keys, rows, \
-                           dy, ld, N, p.C, (int)V, F, factor, part, out);
+        with_forms(nt, F % Sixteen<T>::E, [&](auto nt_, auto cut_) {                                                      \
+            hipLaunchKernelGGL((embed_runs_kernel<T, L_, nt_.value, cut_.value>), grid, dim3(256), 0, st, keys, rows, dy, ld, N, p.C, \
+                               (int)V, F, factor, part, out);                                                             \
+        });
     FACE_RUNS(8) FACE_RUNS(16) FACE_RUNS(32) FACE_RUNS(64)
 #undef FACE_RUNS
     if (p.shares > 1)
@@ -660,18 +662,20 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
         const int64_t sixteens = ((int64_t)F * sizeof(T) + 15) / 16;
         int lg = 0;
         while (lg < 6 && (1 << lg) < sixteens) ++lg;
-        const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream;
+        const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream, cut = F % Sixteen<T>::E;
         const int64_t groups = 256 >> lg, many = nt || N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
         const dim3 grid((unsigned)((N + groups * many - 1) / (groups * many)));
-        auto launch = [&](auto* kern, auto* i) {
-            hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T*)table, ld_t, i, N, V, F, factor, lg, (T*)y, key);
+        auto launch = [&](auto* i) {
+            using I = std::remove_cv_t<std::remove_pointer_t<decltype(i)>>;
+            with_forms(nt, cut, [&](auto nt_, auto cut_) {
+                auto* kern = many > 1 ? embed_fwd_kernel<T, I, 4, nt_.value, cut_.value> : embed_fwd_kernel<T, I, 1, false, cut_.value>;
+                hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T*)table, ld_t, i, N, V, F, factor, lg, (T*)y, key);
+            });
         };
         if (wide)
-            launch(nt ? embed_fwd_kernel<T, int64_t, 4, true> : many > 1 ? embed_fwd_kernel<T, int64_t, 4, false> : embed_fwd_kernel<T, int64_t, 1, false>,
-                   (const int64_t*)index);
+            launch((const int64_t*)index);
         else
-            launch(nt ? embed_fwd_kernel<T, int32_t, 4, true> : many > 1 ? embed_fwd_kernel<T, int32_t, 4, false> : embed_fwd_kernel<T, int32_t, 1, false>,
-                   (const int32_t*)index);
+            launch((const int32_t*)index);
         FACE_LAUNCH_CHECK();
         return 0;
     });

@@ -24,7 +24,7 @@ __device__ __forceinline__ RowAt row_at(int lg) {
     return {(int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg), (int)threadIdx.x & ((1 << lg) - 1), 1 << lg};
 }
 
-template <typename T, bool NT>
+template <typename T, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
     constexpr int E = Sixteen<T>::E;
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int6
     scale += r.n * kept_blocks(F);
     for (int c = E * r.lane; c < end; c += E * r.lanes) {
         float v[E];
-        load16<NT>(x + c, F - c, v);
-        store_kept<E, NT>(q, scale, c, F, v);
+        load16<NT, CUT>(x, c, F, v);
+        store_kept<E, NT, CUT>(q, scale, c, F, v);
     }
 }
 
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, int6
 template <typename T>
 constexpr float kLargest = __is_same(T, f16) ? 65504.f : (__is_same(T, bf16) ? 0x1.fep127f : 0x1.fffffep127f);
 
-template <typename T, bool NT>
+template <typename T, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__ q, int64_t ld_q,
                                                      const uint8_t* __restrict__ scale, int64_t ld_s, int64_t N, int F, int lg,
                                                      T* __restrict__ x) {
@@ -57,15 +57,15 @@ __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__
     x += r.n * F;
     for (int c = E * r.lane; c < F; c += E * r.lanes) {
         float v[E];
-        kept_values(hold_kept<E, NT>(q, scale, c, F), v);
+        kept_values(hold_kept<E, NT, CUT>(q, scale, c, F), v);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = within(v[e], kLargest<T>);
-        store16<NT>(x + c, F - c, v);
+        store16<NT, CUT>(x, c, F, v);
     }
 }
 
 // q (N, 2 F) and scale (N, 2, blocks of F), or null.
-template <typename T, bool KEEP, bool NT>
+template <typename T, bool KEEP, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x, int64_t ld, int64_t N, int F, int lg,
                                                         T* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
     constexpr int E = Sixteen<T>::E;
@@ -78,19 +78,19 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const T* __restrict__ x,
     scale += r.n * 2 * blocks;
     for (int c = E * r.lane; c < end; c += E * r.lanes) {
         float a[E], b[E];
-        load16<NT>(x + c, F - c, a);
-        load16<NT>(x + F + c, F - c, b);
+        load16<NT, CUT>(x, c, F, a);
+        load16<NT, CUT>(x + F, c, F, b);
         if constexpr (KEEP) {
-            store_kept<E, NT>(q, scale, c, F, a);
-            store_kept<E, NT>(q + F, scale + blocks, c, F, b);
+            store_kept<E, NT, CUT>(q, scale, c, F, a);
+            store_kept<E, NT, CUT>(q + F, scale + blocks, c, F, b);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) a[e] = silu(a[e]) * b[e];
-        store16<NT>(y + c, F - c, a);
+        store16<NT, CUT>(y, c, F, a);
     }
 }
 
-template <typename T, bool KEPT, bool NT>
+template <typename T, bool KEPT, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x, int64_t ld, const uint8_t* __restrict__ q,
                                                         const uint8_t* __restrict__ scale, const T* __restrict__ dy,
                                                         int64_t ld_dy, int64_t N, int F, int lg, T* __restrict__ dx) {
@@ -105,13 +105,13 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x,
     dx += r.n * 2 * F;
     for (int c = E * r.lane; c < F; c += E * r.lanes) {
         float a[E], b[E], d[E];
-        load16<NT>(dy + c, F - c, d);
+        load16<NT, CUT>(dy, c, F, d);
         if constexpr (KEPT) {
-            kept_values(hold_kept<E, NT>(q, scale, c, F), a);
-            kept_values(hold_kept<E, NT>(q + F, scale + blocks, c, F), b);
+            kept_values(hold_kept<E, NT, CUT>(q, scale, c, F), a);
+            kept_values(hold_kept<E, NT, CUT>(q + F, scale + blocks, c, F), b);
         } else {
-            load16<NT>(x + c, F - c, a);
-            load16<NT>(x + F + c, F - c, b);
+            load16<NT, CUT>(x, c, F, a);
+            load16<NT, CUT>(x + F, c, F, b);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const T* __restrict__ x,
             a[e] = d[e] * b[e] * silu_slope(t);
             b[e] = d[e] * silu(t);
         }
-        store16<NT>(dx + c, F - c, a);
-        store16<NT>(dx + F + c, F - c, b);
+        store16<NT, CUT>(dx, c, F, a);
+        store16<NT, CUT>(dx + F, c, F, b);
     }
 }
 
@@ -146,9 +146,10 @@ extern "C" int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F,
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = kept_lanes_log2(F, Sixteen<T>::E);
-        auto* kern = streams<T>(N * F * 3 / 2) ? pack_kernel<T, true> : pack_kernel<T, false>;
-        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
+        with_forms(streams<T>(N * F * 3 / 2), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            hipLaunchKernelGGL((pack_kernel<T, nt.value, cut.value>), kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
                            (uint8_t*)q, (uint8_t*)scale);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -163,9 +164,10 @@ extern "C" int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, 
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = kept_lanes_log2(F, Sixteen<T>::E);
-        auto* kern = streams<T>(N * F * 3 / 2) ? unpack_kernel<T, true> : unpack_kernel<T, false>;
-        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
+        with_forms(streams<T>(N * F * 3 / 2), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            hipLaunchKernelGGL((unpack_kernel<T, nt.value, cut.value>), kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
                            (const uint8_t*)scale, ld_s, N, F, lg, (T*)x);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -180,11 +182,11 @@ extern "C" int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = kept_lanes_log2(F, Sixteen<T>::E);
-        const bool nt = streams<T>(N * F * (q ? 4 : 3));
-        auto* kern = q ? (nt ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
-                       : (nt ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
-        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg, (T*)y,
+        with_forms(streams<T>(N * F * (q ? 4 : 3)), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            auto* kern = q ? gated_fwd_kernel<T, true, nt.value, cut.value> : gated_fwd_kernel<T, false, nt.value, cut.value>;
+            hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg, (T*)y,
                            (uint8_t*)q, (uint8_t*)scale);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -199,11 +201,11 @@ extern "C" int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, c
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = kept_lanes_log2(F, Sixteen<T>::E);
-        const bool nt = streams<T>(N * F * (q ? 4 : 5));
-        auto* kern = q ? (nt ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
-                       : (nt ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
-        hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, (const uint8_t*)q,
+        with_forms(streams<T>(N * F * (q ? 4 : 5)), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            auto* kern = q ? gated_bwd_kernel<T, true, nt.value, cut.value> : gated_bwd_kernel<T, false, nt.value, cut.value>;
+            hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, (const uint8_t*)q,
                            (const uint8_t*)scale, (const T*)dy, ld_dy, N, F, lg, (T*)dx);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });

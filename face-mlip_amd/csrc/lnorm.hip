@@ -31,53 +31,78 @@ struct LnFwdArgs {
     float *mean, *rstd;                // may be null
 };
 
+// A lane's eight values of a row, on their way in the row's type.
+template <typename T>
+struct LnPiece {
+    Sixteen<T> a[kPiece / Sixteen<T>::E];
+    __device__ __forceinline__ void values(float x[kPiece]) const {
+#pragma unroll
+        for (int h = 0; h < kPiece / Sixteen<T>::E; ++h) values16<T>(a[h], x + Sixteen<T>::E * h);
+    }
+};
+template <bool NT, typename T>
+__device__ __forceinline__ LnPiece<T> hold_eight(const T* row, int c, int F) {
+    LnPiece<T> r;
+#pragma unroll
+    for (int h = 0; h < kPiece / Sixteen<T>::E; ++h) r.a[h] = hold16<NT, true>(row, c + Sixteen<T>::E * h, F);
+    return r;
+}
+
 // Which columns of a row a lane has as its piece u of U: eight neighbouring ones of 16-bit rows; of fp32 rows twice four, LANES
 // chunks of four apart, so that the lanes of an access lie side by side. Only the last unit may be cut short.
-template <typename T, int LANES, int U>
+template <typename T, int LANES, int U, bool CUT>
 struct LnUnit {
     static constexpr int E = Sixteen<T>::E, H = kPiece / E;
-    int c, left;                       // first column, columns of the row from there on
-    __device__ __forceinline__ LnUnit(int u, int lane, int F) {
-        c = kPiece * LANES * u + E * lane;
-        left = u + 1 < U ? kPiece * LANES : F - c;
-    }
-    __device__ __forceinline__ bool inside(int e) const { return (e < E ? e : E * LANES + e - E) < left; }
+    bool whole;                        // known when the loop over u is unrolled
+    int c, F;                          // first column, columns of the row
+    __device__ __forceinline__ LnUnit(int u, int lane, int F_) : whole(u + 1 < U), c(kPiece * LANES * u + E * lane), F(F_) {}
+    __device__ __forceinline__ int at(int h) const { return c + E * LANES * h; }
+    __device__ __forceinline__ bool inside(int e) const { return whole || at(e / E) + e % E < F; }
     template <bool NT>
-    __device__ __forceinline__ RawPiece<T> hold(const T* row) const {
-        RawPiece<T> r;
+    __device__ __forceinline__ LnPiece<T> hold(const T* row) const {
+        LnPiece<T> r;
 #pragma unroll
-        for (int h = 0; h < H; ++h) r.a[h] = hold16<NT>(row + c + E * LANES * h, left - E * LANES * h).a;
+        for (int h = 0; h < H; ++h) {
+            if (whole) r.a[h] = {ld16s<NT>(row + at(h)), 0};
+            else r.a[h] = hold16<NT, CUT>(row, at(h), F);
+        }
         return r;
     }
     template <bool NT>
     __device__ __forceinline__ void load(const T* row, float x[kPiece]) const {
-        raw_values<T>(hold<NT>(row), x);
+        hold<NT>(row).values(x);
     }
     template <bool NT, typename Y>
     __device__ __forceinline__ void store(Y* row, const float x[kPiece]) const {
+        const int end = whole ? c + kPiece * LANES : F;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            const int at = E * LANES * h;
-            if constexpr (sizeof(Y) == sizeof(T)) store16<NT>(row + c + at, left - at, x + E * h);
-            else store_piece(row + c + at, left - at, x + E * h);       // fp32 sums of 16-bit rows
+            store16<NT, CUT>(row, at(h), end, x + E * h);
+            if constexpr (sizeof(Y) != sizeof(T)) store16<NT, CUT>(row, at(h) + 4, end, x + 4);   // fp32 sums of 16-bit rows
         }
     }
     template <bool NT>
     __device__ __forceinline__ void store_8bit(uint8_t* q, const float x[kPiece], float inv) const {
 #pragma unroll
-        for (int h = 0; h < H; ++h) store_e4m3<E, NT>(q + c + E * LANES * h, left - E * LANES * h, x + E * h, inv);
+        for (int h = 0; h < H; ++h) store_e4m3<E, NT, CUT>(q, at(h), whole ? c + kPiece * LANES : F, x + E * h, inv);
     }
     template <bool NT>
     __device__ __forceinline__ void keep(uint8_t* q, uint8_t* scale, const float x[kPiece]) const {
 #pragma unroll
-        for (int h = 0; h < H; ++h) store_kept<E, NT>(q, scale, c + E * LANES * h, c + left, x + E * h);
+        for (int h = 0; h < H; ++h) store_kept<E, NT, CUT>(q, scale, at(h), whole ? c + kPiece * LANES : F, x + E * h);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void hold_kept_row(const uint8_t* q, const uint8_t* scale, KeptPiece<E> k[H]) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            k[h] = whole ? hold_kept<E, NT, false>(q, scale, at(h), at(h) + E) : hold_kept<E, NT, CUT>(q, scale, at(h), F);
     }
 };
 
-template <typename T, int LANES, int U, int MODE, bool NT>
+template <typename T, int LANES, int U, int MODE, bool NT, bool CUT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
-    using Unit = LnUnit<T, LANES, U>;
+    using Unit = LnUnit<T, LANES, U, CUT>;
     __shared__ float part[LANES / 32 + 1];
     const int lane = threadIdx.x % LANES, F = a.F;
     const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
@@ -232,7 +257,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
         float v[kPiece], h[kPiece], y[kPiece];
         load_piece(x + c, F - c, v);
         ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
-        if constexpr (MODE == kLnKept) store_kept<kPiece, false>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
+        if constexpr (MODE == kLnKept) store_kept<kPiece, false, true>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F, h);
         if constexpr (MODE == kLnQ8) {
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
@@ -252,7 +277,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
             float v[kPiece], h[kPiece], y[kPiece];
             load_piece(x + c, F - c, v);
             ln_piece(v, mean, rs, w + c, b ? b + c : nullptr, F - c, h, y);
-            store_e4m3<kPiece, false>(a.q + n * F + c, F - c, y, inv);
+            store_e4m3<kPiece, false, true>(a.q + n * F, c, F, y, inv);
         }
         if (lane == 0) a.scale[n] = sc;
     }
@@ -271,12 +296,12 @@ struct LnBwdArgs {
     float* part;                       // (workgroups, 2 F): sums of dw, of db; may be null
 };
 
-// h of a piece, from the row as it was normalised or as it was kept: chunks of E values, `apart` columns apart.
+// h of a piece, from the row as it was normalised or as it was kept.
 template <typename T, bool KEPT, int E>
 struct LnRow {
-    RawPiece<T> a;
+    LnPiece<T> a;
     __device__ __forceinline__ void values(float mean, float rs, float h[kPiece]) const {
-        raw_values<T>(a, h);
+        a.values(h);
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) h[e] = (h[e] - mean) * rs;
     }
@@ -284,12 +309,6 @@ struct LnRow {
 template <typename T, int E>
 struct LnRow<T, true, E> {
     KeptPiece<E> a[kPiece / E];
-    template <bool NT>
-    __device__ __forceinline__ void hold(const LnBwdArgs& g, int64_t n, int c, int apart, int end) {
-#pragma unroll
-        for (int h = 0; h < kPiece / E; ++h)
-            a[h] = hold_kept<E, NT>(g.q + n * g.F, g.block_scale + n * kept_blocks(g.F), c + apart * h, end);
-    }
     __device__ __forceinline__ void values(float, float, float h[kPiece]) const {
 #pragma unroll
         for (int i = 0; i < kPiece / E; ++i) kept_values_near(a[i], h + E * i);
@@ -300,10 +319,10 @@ struct LnRow<T, true, E> {
 // all of them; its row of partial sums is joined with the others' by ln_column_sum_kernel in a fixed order: no
 // atomics. All of a row's reads are issued before the first is used. Beyond a row's end dy is 0, and h is finite where
 // the row's is.
-template <typename T, int LANES, int U, bool KEPT, bool NT>
+template <typename T, int LANES, int U, bool KEPT, bool NT, bool CUT>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwdArgs a) {
     constexpr int kRows = LANES > 256 ? 1 : 256 / LANES;
-    using Unit = LnUnit<T, LANES, U>;
+    using Unit = LnUnit<T, LANES, U, CUT>;
     __shared__ float part[LANES / 32 + 1];
     __shared__ float sums[kRows > 1 ? 2 * LANES * U * kPiece : 1];
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, F = a.F;
@@ -311,14 +330,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
     float aw[U][kPiece] = {}, ab[U][kPiece] = {};
     for (int64_t n = (int64_t)blockIdx.x * kRows + slot; n < a.N; n += (int64_t)gridDim.x * kRows) {
         LnRow<T, KEPT, Unit::E> row[U];
-        RawPiece<T> dy[U], ds[U];
+        LnPiece<T> dy[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const Unit at(u, lane, F);
-            if constexpr (KEPT) row[u].template hold<NT>(a, n, at.c, Unit::E * LANES, at.c + at.left);
+            if constexpr (KEPT) at.template hold_kept_row<NT>(a.q + n * F, a.block_scale + n * kept_blocks(F), row[u].a);
             else row[u].a = at.template hold<NT>((const T*)a.s + n * a.ld_s);
-            dy[u] = a.dy ? at.template hold<NT>((const T*)a.dy + n * a.ld_dy) : RawPiece<T>{};
-            ds[u] = a.ds && a.dx ? at.template hold<NT>((const T*)a.ds + n * a.ld_ds) : RawPiece<T>{};
+            dy[u] = a.dy ? at.template hold<NT>((const T*)a.dy + n * a.ld_dy) : LnPiece<T>{};
+            ds[u] = a.ds && a.dx ? at.template hold<NT>((const T*)a.ds + n * a.ld_ds) : LnPiece<T>{};
         }
         const float mean = KEPT ? 0.f : a.mean[n], rs = a.rstd[n];
         float sg = 0.f, sh = 0.f;
@@ -327,7 +346,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
             const Unit at(u, lane, F);
             float h[kPiece], d[kPiece], w[kPiece];
             row[u].values(mean, rs, h);
-            raw_values<T>(dy[u], d);
+            dy[u].values(d);
             at.template load<false>((const T*)a.w, w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
@@ -347,8 +366,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(LnBwd
             const Unit at(u, lane, F);
             float h[kPiece], d[kPiece], w[kPiece], o[kPiece];
             row[u].values(mean, rs, h);
-            raw_values<T>(dy[u], d);
-            raw_values<T>(ds[u], o);
+            dy[u].values(d);
+            ds[u].values(o);
             at.template load<false>((const T*)a.w, w);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) o[e] = fmaf(rs, fmaf(d[e], w[e], -sg) - h[e] * sh, o[e]);
@@ -404,11 +423,11 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnBwdArgs a) {
         float sg = 0.f, sh = 0.f;
         auto load = [&](int c, float h[kPiece], float d[kPiece], float w[kPiece]) {
             LnRow<T, KEPT, kPiece> row;
-            if constexpr (KEPT) row.template hold<false>(a, n, c, 0, F);
-            else row.a = hold_raw((const T*)a.s + n * a.ld_s + c, F - c);
+            if constexpr (KEPT) row.a[0] = hold_kept<kPiece, false, true>(a.q + n * F, a.block_scale + n * kept_blocks(F), c, F);
+            else row.a = hold_eight<false>((const T*)a.s + n * a.ld_s, c, F);
             row.values(mean, rs, h);
-            RawPiece<T> r = a.dy ? hold_raw((const T*)a.dy + n * a.ld_dy + c, F - c) : RawPiece<T>{};
-            raw_values<T>(r, d);
+            LnPiece<T> r = a.dy ? hold_eight<false>((const T*)a.dy + n * a.ld_dy, c, F) : LnPiece<T>{};
+            r.values(d);
             load_piece((const T*)a.w + c, F - c, w);
         };
         for (int c = kPiece * lane; c < F; c += kPiece * LANES) {
@@ -479,7 +498,8 @@ __global__ __launch_bounds__(1024) void ln_column_sum_kernel(const float* __rest
 constexpr int kLnHeld = 16384;                   // longest row that stays in registers
 constexpr int kLnMax = 65536;
 
-// The variants: lanes per row and pieces per lane, the fewest that hold the row.
+// The variants: lanes per row and pieces per lane, the fewest that hold the row. Large calls have a form for rows of whole sixteen
+// bytes: the shifts of others cost registers (100,000 x 2304 bf16 kept in 8 bits, both directions, 819 us with them, 709 without).
 #define FACE_LN_ROWS                                                                                                 \
     FACE_ROW(16, 1) FACE_ROW(16, 2) FACE_ROW(64, 1) FACE_ROW(64, 2) FACE_ROW(64, 3) FACE_ROW(64, 4) FACE_ROW(64, 5) \
     FACE_ROW(256, 2) FACE_ROW(256, 3) FACE_ROW(256, 4) FACE_ROW(256, 5) FACE_ROW(512, 3) FACE_ROW(512, 4)
@@ -504,14 +524,14 @@ static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
     const int64_t rows = ln_rows(a.F), blocks = (a.N + rows - 1) / rows;
     if (blocks > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks);
-    const bool nt = streams<T>(a.N * a.F * (a.r ? 4 : 2));
+    const bool nt = streams<T>(a.N * a.F * (a.r ? 4 : 2)), cut = a.F % Sixteen<T>::E;
     if (a.F > kLnHeld) {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);
     }
 #define FACE_ROW(L_, U_)                                                                                                 \
     else if (sh.lanes == L_ && sh.units == U_)                                                                          \
-        hipLaunchKernelGGL((nt ? ln_fwd_kernel<T, L_, U_, MODE, true>        \
-                                                                           : ln_fwd_kernel<T, L_, U_, MODE, false>),     \
+        hipLaunchKernelGGL((!nt ? ln_fwd_kernel<T, L_, U_, MODE, false, true>                                           \
+                            : cut ? ln_fwd_kernel<T, L_, U_, MODE, true, true> : ln_fwd_kernel<T, L_, U_, MODE, true, false>), \
                            grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
     FACE_LN_ROWS
 #undef FACE_ROW
@@ -525,14 +545,14 @@ static int launch_ln_bwd(const LnBwdArgs& a, T* dw, T* db, hipStream_t st) {
     const int64_t blocks = ln_bwd_grid(a.N, a.F, sizeof(T) == 4);
     if (blocks) {
         const dim3 grid((unsigned)blocks);
-        const bool nt = streams<T>(a.N * a.F * (a.ds ? 4 : 3));
+        const bool nt = streams<T>(a.N * a.F * (a.ds ? 4 : 3)), cut = a.F % Sixteen<T>::E;
         if (a.F > kLnHeld) {
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, KEPT>), grid, dim3(1024), 0, st, a);
         }
 #define FACE_ROW(L_, U_)                                                                                                 \
     else if (sh.lanes == L_ && sh.units == U_)                                                                          \
-        hipLaunchKernelGGL((nt ? ln_bwd_kernel<T, L_, U_, KEPT, true>        \
-                                                                           : ln_bwd_kernel<T, L_, U_, KEPT, false>),     \
+        hipLaunchKernelGGL((!nt ? ln_bwd_kernel<T, L_, U_, KEPT, false, true>                                           \
+                            : cut ? ln_bwd_kernel<T, L_, U_, KEPT, true, true> : ln_bwd_kernel<T, L_, U_, KEPT, true, false>), \
                            grid, dim3(L_ > 256 ? L_ : 256), 0, st, a);
         FACE_LN_ROWS
 #undef FACE_ROW

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void places_kernel(const int32_t* __restrict__
 static inline int sorted_lanes_log2(int64_t F, int size) { return F * size <= 1024 ? 4 : (F * size <= 8192 ? 6 : 8); }
 
 // xs[p] = x[order[p] / k].
-template <typename T, bool NT>
+template <typename T, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restrict__ x, int64_t ld,
                                                               const int32_t* __restrict__ ptr,
                                                               const int32_t* __restrict__ order, int64_t slots, int k, int G,
@@ -61,14 +61,14 @@ __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restric
     const T* from = x + (int64_t)(some ? a / k : 0) * ld;
     for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
         float v[E] = {};
-        if (some) load16<NT>(from + c, F - c, v);
-        store16<NT>(xs + p * F + c, F - c, v);
+        if (some) load16<NT, CUT>(from, c, F, v);
+        store16<NT, CUT>(xs + p * F, c, F, v);
     }
 }
 
 // A row's threads write it to the places of its k slots, and zeros to those of the places i k .. i k + k - 1 that
 // have no slot; four slots per turn, their places known before the row is.
-template <typename T, bool NT>
+template <typename T, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restrict__ x, int64_t ld,
                                                                const int32_t* __restrict__ ptr,
                                                                const int32_t* __restrict__ order,
@@ -93,11 +93,11 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
         for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
             float v[E];
             const float none[E] = {};
-            load16<NT>(x + n * ld + c, F - c, v);
+            load16<NT, CUT>(x + n * ld, c, F, v);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                if (p[j] >= 0) store16<NT>(xs + (int64_t)p[j] * F + c, F - c, v);
-                if (bare[j]) store16<NT>(xs + (n * k + j0 + j) * F + c, F - c, none);
+                if (p[j] >= 0) store16<NT, CUT>(xs + (int64_t)p[j] * F, c, F, v);
+                if (bare[j]) store16<NT, CUT>(xs + (n * k + j0 + j) * F, c, F, none);
             }
         }
     }
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
 
 // out[i] = r[i] + sum_j w[i, j] y[place(i k + j)], in order; w null: ones. Four slots per turn, their rows on the way
 // together; the first four's places are known before any row is asked for.
-template <typename T, bool NT>
+template <typename T, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ place,
                                                          const float* __restrict__ w, const T* __restrict__ r, int64_t ld_r,
                                                          int64_t N, int k, int F, int lg, T* __restrict__ out) {
@@ -126,13 +126,13 @@ __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y
     turn(0);
     for (int c = E * (threadIdx.x & ((1 << lg) - 1)); c < F; c += E << lg) {
         float s[E] = {};
-        if (r) load16<NT>(r + n * ld_r + c, F - c, s);
+        if (r) load16<NT, CUT>(r + n * ld_r, c, F, s);
         for (int j0 = 0; j0 < k; j0 += J) {
             if (k > J) turn(j0);
             Sixteen<T> v[J];
 #pragma unroll
             for (int j = 0; j < J; ++j)
-                if (p[j] >= 0) v[j] = hold16<NT>(y + (int64_t)p[j] * ld_y + c, F - c);
+                if (p[j] >= 0) v[j] = hold16<NT, CUT>(y + (int64_t)p[j] * ld_y, c, F);
 #pragma unroll
             for (int j = 0; j < J; ++j)
                 if (p[j] >= 0) {
@@ -142,12 +142,12 @@ __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y
                     for (int e = 0; e < E; ++e) s[e] = fmaf(f[j], x[e], s[e]);
                 }
         }
-        store16<NT>(out + n * F + c, F - c, s);
+        store16<NT, CUT>(out + n * F, c, F, s);
     }
 }
 
 // dy[p] = w dout and dw = dout . y[p] at the places of the row's slots; zeros at places without a slot.
-template <typename T, int LANES, bool NT>
+template <typename T, int LANES, bool NT, bool CUT>
 __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ dout, int64_t ld_d, const T* __restrict__ y,
                                                          int64_t ld_y, const int32_t* __restrict__ ptr,
                                                          const int32_t* __restrict__ order,
@@ -176,12 +176,12 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
         }
         for (int c = E * lane; c < F; c += E * LANES) {
             float d[E];
-            load16<NT>(dout + n * ld_d + c, F - c, d);
+            load16<NT, CUT>(dout + n * ld_d, c, F, d);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 float v[E];
                 if (dw && p[j] >= 0) {
-                    load16<NT>(y + (int64_t)p[j] * ld_y + c, F - c, v);
+                    load16<NT, CUT>(y + (int64_t)p[j] * ld_y, c, F, v);
 #pragma unroll
                     for (int e = 0; e < E; ++e) s[j] = fmaf(d[e], v[e], s[j]);
                 }
@@ -189,11 +189,11 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
                 if (p[j] >= 0) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = f[j] * d[e];
-                    store16<NT>(dy + (int64_t)p[j] * F + c, F - c, v);
+                    store16<NT, CUT>(dy + (int64_t)p[j] * F, c, F, v);
                 }
                 if (bare[j]) {
                     const float none[E] = {};
-                    store16<NT>(dy + (n * k + j0 + j) * F + c, F - c, none);
+                    store16<NT, CUT>(dy + (n * k + j0 + j) * F, c, F, none);
                 }
             }
         }
@@ -239,13 +239,14 @@ extern "C" int face_expert_dispatch(const void* x, int64_t ld_x, int32_t k, cons
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = sorted_lanes_log2(F, sizeof(T));
-        const bool nt = streams<T>((slots + N) * F);
-        if (place)
-            hipLaunchKernelGGL((nt ? dispatch_scatter_kernel<T, true> : dispatch_scatter_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x,
-                               ld_x, ptr, order, place, slots, k, G, F, lg, (T*)xs);
-        else
-            hipLaunchKernelGGL((nt ? dispatch_gather_kernel<T, true> : dispatch_gather_kernel<T, false>), sorted_grid(slots, lg), dim3(256), 0, (hipStream_t)stream,
-                               (const T*)x, ld_x, ptr, order, slots, k, G, F, lg, (T*)xs);
+        with_forms(streams<T>((slots + N) * F), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            if (place)
+                hipLaunchKernelGGL((dispatch_scatter_kernel<T, nt.value, cut.value>), sorted_grid(N, lg), dim3(256), 0,
+                                   (hipStream_t)stream, (const T*)x, ld_x, ptr, order, place, slots, k, G, F, lg, (T*)xs);
+            else
+                hipLaunchKernelGGL((dispatch_gather_kernel<T, nt.value, cut.value>), sorted_grid(slots, lg), dim3(256), 0,
+                                   (hipStream_t)stream, (const T*)x, ld_x, ptr, order, slots, k, G, F, lg, (T*)xs);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -262,9 +263,10 @@ extern "C" int face_expert_return_fwd(const void* y, int64_t ld_y, const int32_t
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int lg = sorted_lanes_log2(F, sizeof(T));
-        const bool nt = streams<T>((N * k + N * (r ? 2 : 1)) * F);
-        hipLaunchKernelGGL((nt ? return_fwd_kernel<T, true> : return_fwd_kernel<T, false>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)y, ld_y, place,
-                           weight, (const T*)r, ld_r, N, k, F, lg, (T*)out);
+        with_forms(streams<T>((N * k + N * (r ? 2 : 1)) * F), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            hipLaunchKernelGGL((return_fwd_kernel<T, nt.value, cut.value>), sorted_grid(N, lg), dim3(256), 0, (hipStream_t)stream,
+                               (const T*)y, ld_y, place, weight, (const T*)r, ld_r, N, k, F, lg, (T*)out);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });
@@ -281,12 +283,12 @@ extern "C" int face_expert_return_bwd(const void* dout, int64_t ld_d, const void
         using T = decltype(t);
         const int L = 1 << sorted_lanes_log2(F, sizeof(T)), rows = 256 / L;
         const dim3 grid((unsigned)((N + rows - 1) / rows));
-        const bool nt = streams<T>((2 * N * k + N) * F);
-        auto* kern = L == 16 ? (nt ? return_bwd_kernel<T, 16, true> : return_bwd_kernel<T, 16, false>)
-                   : L == 64 ? (nt ? return_bwd_kernel<T, 64, true> : return_bwd_kernel<T, 64, false>)
-                             : (nt ? return_bwd_kernel<T, 256, true> : return_bwd_kernel<T, 256, false>);
-        hipLaunchKernelGGL(kern, grid, dim3(256), 0, (hipStream_t)stream, (const T*)dout, ld_d, (const T*)y, ld_y, ptr, order,
-                           place, weight, N, k, G, F, (T*)dy, dweight);
+        with_forms(streams<T>((2 * N * k + N) * F), F % Sixteen<T>::E, [&](auto nt, auto cut) {
+            auto* kern = L == 16 ? return_bwd_kernel<T, 16, nt.value, cut.value>
+                       : L == 64 ? return_bwd_kernel<T, 64, nt.value, cut.value> : return_bwd_kernel<T, 256, nt.value, cut.value>;
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, (hipStream_t)stream, (const T*)dout, ld_d, (const T*)y, ld_y, ptr, order,
+                               place, weight, N, k, G, F, (T*)dy, dweight);
+        });
         FACE_LAUNCH_CHECK();
         return 0;
     });

@@ -398,27 +398,34 @@ class GatedSiLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, keep8):
         y, q, scale = _gated_fwd(x, keep8)
-        ctx.save_for_backward(*((q, scale) if keep8 else (x,)))
+        if keep8:
+            ctx.save_for_backward(q, scale)
+        else:
+            ctx.save_for_backward(x)
         F = y.shape[-1]
-        ctx.known = y.numel() // F, F, _DTYPES[x.dtype], keep8
+        ctx.known = y.numel() // F, F, _DTYPES[x.dtype], keep8, x.is_contiguous()
         return y
 
     @staticmethod
     def backward(ctx, dy):
         _once("gated_silu", dy)
-        N, F, code, keep8 = ctx.known
-        d2 = _rows(dy, F)
-        x2 = q = scale = None
-        ld = 2 * F
+        N, F, code, keep8, dense = ctx.known
+        ld, ld_dy = 2 * F, F
+        if not dy.is_contiguous():
+            dy = _rows(dy, F)
+            ld_dy = dy.stride(0)
+        x = q = scale = None
         if keep8:
-            q, scale = ctx.saved_tensors
+            q, scale = (ptr(t) for t in ctx.saved_tensors)
             dx = torch.empty(*dy.shape[:-1], ld, dtype=dy.dtype, device=dy.device)
         else:
             x, = ctx.saved_tensors
-            x2, dx = _rows(x, ld), _like(x)
-            ld = x2.stride(0)
-        _launch(dy, "face_gated_silu_bwd", "gated_silu_bwd", ptr(x2), ld, ptr(q), ptr(scale), d2.data_ptr(), d2.stride(0), N, F, code,
-                dx.data_ptr())
+            dx = torch.empty_like(x) if dense else _like(x)
+            if not dense:
+                x = _rows(x, ld)
+                ld = x.stride(0)
+            x = x.data_ptr()
+        _launch(dx, "face_gated_silu_bwd", "gated_silu_bwd", x, ld, q, scale, dy.data_ptr(), ld_dy, N, F, code, dx.data_ptr())
         return dx, None
 
 
@@ -464,11 +471,14 @@ class Embed(torch.autograd.Function):
         _once("embed", dy)
         key, = ctx.saved_tensors
         N, V, F, code, factor, need = ctx.known
-        d2 = _rows(dy, F)
+        ld = F
+        if not dy.is_contiguous():
+            dy = _rows(dy, F)
+            ld = dy.stride(0)
         dt = torch.empty(V, F, dtype=dy.dtype, device=dy.device)
         work = _work(need, dy.device)
-        _launch(dy, "face_embed_bwd", "embed_bwd", key.data_ptr(), d2.data_ptr(), d2.stride(0), N, V, F, code, factor, dt.data_ptr(),
-                ptr(work), need)
+        _launch(dt, "face_embed_bwd", "embed_bwd", key.data_ptr(), dy.data_ptr(), ld, N, V, F, code, factor, dt.data_ptr(), ptr(work),
+                need)
         return dt, None, None
 
 
