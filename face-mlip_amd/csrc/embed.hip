@@ -661,7 +661,7 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
         using T = decltype(t);
         const int64_t sixteens = ((int64_t)F * sizeof(T) + 15) / 16;
         int lg = 0;
-        while (lg < 6 && (1 << lg) < sixteens) ++lg;
+        while (lg < 8 && (1 << lg) < sixteens) ++lg;
         const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream, cut = F % Sixteen<T>::E;
         const int64_t groups = 256 >> lg, many = nt || N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
         const dim3 grid((unsigned)((N + groups * many - 1) / (groups * many)));

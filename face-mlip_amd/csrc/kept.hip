@@ -8,11 +8,13 @@
 
 namespace face {
 
-// Threads per row of E values each at a time (a power of two, whole blocks): about four times each.
-static inline int kept_lanes_log2(int64_t F, int E) {
+// Threads per row of E values each at a time (a power of two, whole blocks): about `turns` times each. The gate, with three
+// to five rows on their way, takes one turn (165,864 x 97 fp32 kept, both directions, 100 us for 177 of four), the single row of
+// a packing four (100,000 x 2304 bf16 there and back 224 us for 241 of one).
+static inline int kept_lanes_log2(int64_t F, int E, int turns) {
     const int64_t p = kept_blocks(F) * (kKeptBlock / E);
     int lg = E == 4 ? 3 : 2;
-    while (lg < 8 && ((int64_t)4 << lg) < p) ++lg;
+    while (lg < 8 && ((int64_t)turns << lg) < p) ++lg;
     return lg;
 }
 
@@ -145,7 +147,7 @@ extern "C" int face_pack_rows(const void* x, int64_t ld_x, int64_t N, int32_t F,
     if (!x || !q || !scale) return FACE_ERR_ARG;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E, 4);
         with_forms(streams<T>(N * F * 3 / 2), F % Sixteen<T>::E, [&](auto nt, auto cut) {
             hipLaunchKernelGGL((pack_kernel<T, nt.value, cut.value>), kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg,
                            (uint8_t*)q, (uint8_t*)scale);
@@ -163,7 +165,7 @@ extern "C" int face_unpack_rows(const void* q, int64_t ld_q, const void* scale, 
     if (!x || !q || !scale) return FACE_ERR_ARG;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E, 4);
         with_forms(streams<T>(N * F * 3 / 2), F % Sixteen<T>::E, [&](auto nt, auto cut) {
             hipLaunchKernelGGL((unpack_kernel<T, nt.value, cut.value>), kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, ld_q,
                            (const uint8_t*)scale, ld_s, N, F, lg, (T*)x);
@@ -181,7 +183,7 @@ extern "C" int face_gated_silu_fwd(const void* x, int64_t ld_x, int64_t N, int32
     if (!x || !y) return FACE_ERR_ARG;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E, 1);
         with_forms(streams<T>(N * F * (q ? 4 : 3)), F % Sixteen<T>::E, [&](auto nt, auto cut) {
             auto* kern = q ? gated_fwd_kernel<T, true, nt.value, cut.value> : gated_fwd_kernel<T, false, nt.value, cut.value>;
             hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, N, F, lg, (T*)y,
@@ -200,7 +202,7 @@ extern "C" int face_gated_silu_bwd(const void* x, int64_t ld_x, const void* q, c
     if ((x ? q || scale : !q || !scale) || !dy || !dx) return FACE_ERR_ARG;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const int lg = kept_lanes_log2(F, Sixteen<T>::E);
+        const int lg = kept_lanes_log2(F, Sixteen<T>::E, 1);
         with_forms(streams<T>(N * F * (q ? 4 : 5)), F % Sixteen<T>::E, [&](auto nt, auto cut) {
             auto* kern = q ? gated_bwd_kernel<T, true, nt.value, cut.value> : gated_bwd_kernel<T, false, nt.value, cut.value>;
             hipLaunchKernelGGL(kern, kept_grid(N, lg), dim3(256), 0, (hipStream_t)stream, (const T*)x, ld_x, (const uint8_t*)q,
