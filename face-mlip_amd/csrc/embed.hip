@@ -6,7 +6,7 @@
 // atomics, the same bits every time. Two ways:
 //   * few entries, or few rows: a wave takes a chunk of rows and, entry by entry, finds the chunk's rows of it with a
 //     ballot per 64 indices; partial sums per chunk and entry, joined by columns. Nothing is sorted.
-//   * else the indices are sorted first (a stable radix sort of 8 bits a pass, or one workgroup up to 4096 rows); groups of
+//   * else the indices are sorted first (a stable radix sort of 8 bits a pass, or one workgroup up to 1024 rows); groups of
 //     lanes sum equal shares of the sorted rows, entry after entry. What begins and ends within a share is done; the
 //     sums that go on into the next share are joined afterwards, short runs by a few lanes, long ones by a workgroup.
 // Sums in fp32. Bound by bytes: the rows of dy, read once each.
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const float* __restric
 // ---------------------------------------------------------------- sort
 // (key, row) pairs by key, stably; a key outside [0, V) counts as V. Pairs come from the indices in the first pass.
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortBits = 8;
-constexpr int64_t kSortOne = 4096;               // one workgroup does it all up to here
+constexpr int64_t kSortOne = 1024;               // one workgroup does it all up to here (24 us with the sums; 48 for 4000, in passes 26)
 
 __device__ __forceinline__ uint32_t sort_key(const int32_t* key, int64_t a, uint32_t V) {
     const uint32_t k = (uint32_t)key[a];
@@ -537,14 +537,19 @@ static inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 static EmbedPlan embed_plan(int64_t N, int64_t V, int F, int size) {
     EmbedPlan p = {};
     const int64_t sixteens = ((int64_t)F * size + 15) / 16;
-    if (V <= 16 || N <= 512) {
+    // Few rows: a wave per entry looks through all of them. Few entries: a wave per chunk looks for all of them. Else sorted.
+    // us, this way / sorted: 1024 rows x 96 fp32 of 200 entries 7 / 24, 2048 of 14,161 16 / 32, but x 2304 bf16 76 / 42; 100,000
+    // rows x 96 fp32 of 8 entries 22 / 33, of 16 28 / 33, of 64 65 / 34, x 1440 118 / 119, 157 / 127, 325 / 121.
+    const int64_t tiles = (sixteens + 63) / 64;
+    const bool few_rows = N <= 512 || (V > 8 && N <= 2048 && V * tiles * N <= (int64_t)36 << 20);
+    if (V <= 8 || few_rows) {
         p.scan = true;
-        if (N <= 512) {
+        if (few_rows) {
             p.R = N < 1 ? 1 : N;
             p.chunks = 1;
             p.TV = 1;
         } else {
-            const int64_t tiles = (sixteens + 63) / 64, r = N * tiles / 2048 / 64 * 64;
+            const int64_t r = N * tiles / 2048 / 64 * 64;
             p.R = r < 64 ? 64 : (r > 1024 ? 1024 : r);
             p.chunks = (N + p.R - 1) / p.R;
             p.TV = V;

@@ -494,6 +494,8 @@ def embed(table, index, scale=1.0):
         _fail(name, f"int32 or int64 index, got {index.dtype}")
     if index.numel() >= 1 << 31:
         _fail(name, f"fewer than 2^31 rows, got {index.numel()}")
+    if isinstance(scale, torch.Tensor):
+        _fail(name, "scale: a number, got a tensor (no gradient would reach it)")
     factor = float(scale)
     _check(name, table, index=index)
     if _wants_grad(table):

@@ -480,7 +480,7 @@ def check_embed(table, index, scale, dy):
 @pytest.mark.parametrize("N,V,F", [(1, 1, 1), (1, 5, 96), (21, 3, 96), (21, 119, 7), (64, 2, 8), (65, 3, 2304), (300, 20000, 40),
                                    (512, 17, 130), (513, 17, 130), (700, 3, 33), (4096, 40, 65), (4097, 300, 64), (5000, 16, 520),
                                    (9000, 255, 96), (9000, 256, 97), (3000, 70000, 24), (30000, 70000, 24), (40000, 14161, 64),
-                                   (100000, 3, 256), (50000, 20, 600), (20000, 17, 2304), (200000, 1000, 16)])
+                                   (100000, 3, 256), (900, 70000, 40), (2048, 9, 70), (2049, 9, 70), (50000, 20, 600), (20000, 17, 2304), (200000, 1000, 16)])
 def test_embed(dtype, N, V, F):
     say("embed", dtype, N, V, F)
     g = gen(N + V + F)
@@ -500,8 +500,8 @@ def test_embed_runs_of_every_length():
     for lengths in ([1] * 60, [16] * 60, [15, 17] * 30, [32, 1, 31] * 20, [100, 3, 129, 128, 127] * 12, [8000, 1, 1, 500] * 15,
                     [0, 0, 4000, 0, 130, 144, 145] * 8, [60000] + [0] * 58 + [7]):
         index = torch.cat([torch.full((n,), v, device=DEV) for v, n in enumerate(lengths)])
-        if index.numel() <= 512:
-            index = index.repeat(20)
+        if index.numel() <= 2048:
+            index = index.repeat(2048 // index.numel() + 2)
         index = index[torch.randperm(index.numel(), generator=g, device=DEV)]
         say("runs", index.numel())
         check_embed(rand(g, V, F), index.to(torch.int32), 0.5, rand(g, index.numel(), F))
@@ -533,6 +533,31 @@ def test_embed_shapes_strides_and_far_indices():
         dy[5, 3] = math.nan
         d, = torch.autograd.grad([ex.embed(t := leaf(table), index)], [t], [dy])
         assert d.isnan().sum() == 1 and d[index[5], 3].isnan()
+
+
+def test_embed_of_millions():
+    """Segments of the sort that are longer than what is loaded at once, three passes."""
+    g = gen(7)
+    N, V = 5000003, 70001
+    index = (torch.rand(N, generator=g, device=DEV) ** 3 * V).to(torch.int32)
+    check_embed(rand(g, V, 9), index, 1.0, rand(g, N, 9))
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_rows_in_both_directions(dtype, keep8):
+    none = lambda *s: torch.empty(0, *s, dtype=dtype, device=DEV)
+    w, b = torch.ones(7, dtype=dtype, device=DEV), torch.ones(7, dtype=dtype, device=DEV)
+    l = [leaf(none(7)), leaf(w), leaf(b), leaf(none(7))]
+    y, s = ex.layer_norm(l[0], l[1], l[2], residual=l[3], keep8=keep8)
+    dx, dw, db, dr = torch.autograd.grad([y, s], l, [none(7), none(7)])
+    assert dx.shape == dr.shape == (0, 7) and not dw.any() and not db.any()
+    l = leaf(none(6))
+    assert torch.autograd.grad([ex.gated_silu(l, keep8)], [l], [none(3)])[0].shape == (0, 6)
+    plan = ex.group_plan(torch.empty(0, 2, dtype=torch.int32, device=DEV), 3)
+    l = [leaf(none(5)), leaf(torch.ones(3, 4, 5, dtype=dtype, device=DEV))]
+    dx, dw = torch.autograd.grad([ex.grouped_linear(*l, plan, keep8=keep8)], l, [none(4)])
+    assert dx.shape == (0, 5) and not dw.any()
 
 
 # ----------------------------------------------------------------------------- rows by expert

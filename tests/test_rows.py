@@ -74,6 +74,7 @@ def test_embed_refusals():
     bad("table", ex.embed, torch.zeros(1, 65537), I)
     bad("int32 or int64", ex.embed, X, I.float())
     bad("int32 or int64", ex.embed, X, I.to(torch.uint8))
+    bad("a number", ex.embed, X, I, torch.ones(()))
 
 
 def test_rows_by_expert_refusals():
