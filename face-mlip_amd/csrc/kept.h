@@ -165,10 +165,11 @@ constexpr int64_t kStreamBytes = (int64_t)256 << 20;                 // the last
 // each cover half of a stretch of memory, the norm of 24,000 x 1440 took 124 us for 112.
 template <typename T>
 static inline bool streams(int64_t n) { return n * (int64_t)sizeof(T) > kStreamBytes; }
+
 // Sixteen bytes of a row, so that neighbouring lanes move neighbouring bytes whatever the type: columns [c, c + E) of F, zeros
-// beyond. What ends before the sixteen bytes do is read as the row's last sixteen and shifted by `s` bits when its values are
-// asked for, so that no load waits for another (CUT; without it rows are whole multiples. Element by element, rows of odd widths took up to twice as long: 77,737 x
-// 2876 fp16, norm kept in 8 bits, 1269 us for 948); only a row that is shorter than that goes by elements.
+// beyond. CUT: rows of any width; what ends before the sixteen bytes do is read as the row's last sixteen and shifted by `s` bits
+// when its values are asked for, so that no load waits for another (element by element, 77,737 x 2876 fp16, norm kept in 8 bits,
+// both directions, took 1269 us for 934). Only a row that is shorter than that goes by elements. Not CUT: whole multiples.
 template <typename T>
 struct Sixteen {
     static constexpr int E = 16 / (int)sizeof(T);

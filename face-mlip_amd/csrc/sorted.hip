@@ -6,7 +6,8 @@
 //
 // place is order's inverse, -1 for slots that have none: what leaves rows of x, or gathers into rows of y, goes by
 // rows, reads or writes each of those once, and its other side by whole rows. With one choice per row there is nothing to share:
-// xs is gathered by order, without the inverse. Bound by bytes.
+// xs is gathered by order, without the inverse, as in small calls. Bound by bytes: 100,000 x 2304 bf16 to two of eight experts: out
+// 246 us (1.4 GB: 5.6 TB/s), its gradient 207, back 286 (1.8 GB), its gradients 412 (2.3 GB), the inverse 2 x 5.
 #include "kept.h"
 
 namespace face {

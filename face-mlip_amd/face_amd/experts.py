@@ -329,6 +329,11 @@ def quantize_rows(x, x_op=None):
 
 
 # ----------------------------------------------------------------------------- rows kept in 8 bits
+def _row_count(name, x):
+    if x.numel() >= x.shape[-1] << 31:
+        _fail(name, f"fewer than 2^31 rows, got {tuple(x.shape)}")
+
+
 def _blocks(F):
     """Scales of a kept row: one for each 32 columns."""
     return (F + 31) // 32
@@ -362,6 +367,7 @@ def pack_rows(x):
     _dtype("pack_rows", x)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_PACKED:
         _fail("pack_rows", f"rows of 1 to {MAX_PACKED} columns, got {tuple(x.shape)}")
+    _row_count("pack_rows", x)
     _check("pack_rows", x)
     return _pack(x)
 
@@ -374,6 +380,7 @@ def unpack_rows(q, scale, dtype=torch.bfloat16):
         _fail(name, f"float8_e4m3fn rows of 1 to {MAX_PACKED} columns, got {tuple(q.shape)} {q.dtype}")
     if dtype not in _DTYPES:
         _fail(name, f"dtype float32, bfloat16 or float16, got {dtype}")
+    _row_count(name, q)
     shape = (*q.shape[:-1], _blocks(q.shape[-1]))
     if scale.shape != shape or scale.dtype != _E8M0:
         _fail(name, f"scale {shape} float8_e8m0fnu, got {tuple(scale.shape)} {scale.dtype}")
@@ -436,6 +443,7 @@ def gated_silu(x, keep8=False):
     _dtype("gated_silu", x)
     if x.dim() < 1 or x.shape[-1] % 2 or not 2 <= x.shape[-1] <= 2 * MAX_PACKED:
         _fail("gated_silu", f"x (..., 2 F), F <= {MAX_PACKED}, got {tuple(x.shape)}")
+    _row_count("gated_silu", x)
     _check("gated_silu", x)
     if _wants_grad(x):
         return GatedSiLU.apply(x, bool(keep8))
@@ -817,8 +825,9 @@ def expert_combine(y, weight, residual=None):
 # ----------------------------------------------------------------------------- rows by expert and back
 def _by_rows(slots, k, F):
     """Whether rows are read once and written to their k places, which takes the order's inverse first, or gathered by
-    the order, read k times."""
-    return k > 1 and slots * F >= 1 << 22
+    the order, read k times. bf16, k = 2, us: 2^25 elements out gathered 21, by rows 22; 2^26 of 2304 columns 40 / 37, 2^28 182 /
+    148, but of 96 columns 213 / 226."""
+    return k > 1 and F >= 256 and slots * F >= 1 << 26
 
 
 def _dispatch_fwd(x, p, order, k):

@@ -570,8 +570,10 @@ def sort_case(g, N, k, G, F, dtype, closed=0.1):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,k,G,F", [(0, 2, 3, 8), (1, 1, 1, 1), (1, 3, 2, 96), (21, 2, 8, 96), (50, 5, 3, 257), (301, 8, 64, 513),
                                      (4096, 2, 8, 40), (5000, 3, 8, 300), (9000, 1, 3, 800), (3000, 4, 16, 4100)])
-def test_rows_by_expert_and_back(dtype, N, k, G, F):
-    say("sort", dtype, N, k, G, F)
+@pytest.mark.parametrize("by_rows", [False, True])
+def test_rows_by_expert_and_back(dtype, N, k, G, F, by_rows, monkeypatch):
+    say("sort", dtype, N, k, G, F, by_rows)
+    monkeypatch.setattr(ex, "_by_rows", lambda *a: by_rows)          # either way at every size
     g = gen(N + k + F)
     plan, weight = sort_case(g, N, k, G, F, dtype)
     slots, m = N * k, int(plan.ptr[-1])
@@ -620,9 +622,11 @@ def test_rows_by_expert_and_back(dtype, N, k, G, F):
     assert not dz[other].any()
 
 
-@pytest.mark.parametrize("N,F", [(40, 33), (3000, 700)])
-def test_rows_by_a_kept_plan_of_some_slots(N, F):
+@pytest.mark.parametrize("N,F", [(40, 33), (3000, 700), (9000, 20)])
+@pytest.mark.parametrize("by_rows", [False, True])
+def test_rows_by_a_kept_plan_of_some_slots(N, F, by_rows, monkeypatch):
     """Plans that a program keeps: places that name no slot, slots that have none, ends past the order."""
+    monkeypatch.setattr(ex, "_by_rows", lambda *a: by_rows)
     g = gen(N)
     k, slots = 2, 2 * N
     perm = torch.randperm(slots, generator=g, device=DEV).to(torch.int32)
@@ -916,6 +920,86 @@ def test_rows_past_two_to_the_31_elements(keep8):
         out = ex.expert_return(xs, plan)
         assert torch.equal(out[-3000:], (k * x[:N // k][-3000:].float()).to(BF16))
         del xs, out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("F", [901, 904])
+def test_large_calls_give_the_rows_of_small_ones(dtype, F):
+    """Past 256 MB rows are read and written by other accesses, whole pieces and cut ones: bit for bit the same rows, and sums
+    over all rows within their bound."""
+    g = gen(F)
+    N = 48001 if dtype != F32 else 24001
+    x, r, dy, ds = (rand(g, N, F, dtype=dtype) for _ in range(4))
+    w, b = (1 + 0.1 * rand(g, F)).to(dtype), rand(g, F, dtype=dtype)
+    parts = (slice(0, 700), slice(N - 700, N))
+
+    def same(big, f):
+        for p in parts:
+            for a, c in zip(big, f(p)):
+                assert torch.equal(a[p].view(torch.uint8), c.view(torch.uint8))
+
+    for keep8 in (False, True):
+        say("norm", dtype, F, keep8)
+
+        def norm(p):
+            l = [leaf(t) for t in (x[p], r[p], w, b)]
+            y, s = ex.layer_norm(l[0], l[2], l[3], residual=l[1], keep8=keep8)
+            return (y.detach(), s.detach(), *torch.autograd.grad([y, s], l, [dy[p], ds[p]]))
+
+        out = norm(slice(0, N))
+        same(out[:4], lambda p: norm(p)[:4])
+        d = dy.double()
+        near(out[5], d.sum(0), (N + 8) * U32 * d.abs().sum(0), "db")
+        if not keep8:
+            s, h, rstd, eh = ln64(x, r, w, b, 1e-5)
+            near(out[4], (d * h).sum(0), (N + 8) * U32 * (d * h).abs().sum(0) + (d.abs() * eh).sum(0), "dw")
+            del s, h, rstd, eh
+        del d
+        say("gate", dtype, F, keep8)
+        M = N // 2
+        z = torch.stack([x[:M], r[:M]], 1).reshape(M, 2 * F).repeat(3, 1)
+        dz = dy[:M].repeat(3, 1)
+        parts = (slice(0, 700), slice(3 * M - 700, 3 * M))
+
+        def gate(p):
+            l = leaf(z[p])
+            y = ex.gated_silu(l, keep8)
+            return y.detach(), torch.autograd.grad([y], [l], [dz[p]])[0]
+
+        same(gate(slice(0, 3 * M)), gate)
+        parts = (slice(0, 700), slice(N - 700, N))
+    say("norm in 8 bits, pack")
+    same(ex.layer_norm_q8(x, w, b, residual=r), lambda p: ex.layer_norm_q8(x[p], w, b, residual=r[p]))
+    z = torch.cat([x, r, dy, ds])
+    parts = (slice(0, 700), slice(4 * N - 700, 4 * N))
+    same(ex.pack_rows(z), lambda p: ex.pack_rows(z[p]))
+    q, scale = ex.pack_rows(z)
+    same([ex.unpack_rows(q, scale, dtype)], lambda p: [ex.unpack_rows(q[p], scale[p], dtype)])
+    say("by expert")
+    k = 2
+    plan, weight = sort_case(g, N, k, 5, F, dtype)
+    m = int(plan.ptr[-1])
+    at, i = plan.order[:m].long(), plan.order[:m].long() // k
+    lx, ly, lw = leaf(x), leaf(z[:N * k]), leaf(weight)
+    xs = ex.expert_dispatch(lx, plan)
+    assert torch.equal(xs[:m], x[i]) and not xs[m:].any()
+    out = ex.expert_return(ly, plan, lw, residual=r)
+    dx, dys, dw = torch.autograd.grad([xs, out], [lx, ly, lw], [z[N * k:], dy])
+    v = torch.zeros(N * k, F, dtype=dtype, device=DEV)
+    v[at] = z[:m]                                                    # by slot, summed as the join does
+    want = r.float()
+    for j in range(k):
+        want = torch.addcmul(want, weight[:, j:j + 1], v.view(N, k, F)[:, j].float())
+    near(out, want.double(), 4 * U32 * (r.double().abs() + v.view(N, k, F).double().abs().sum(1)), "out")
+    v.zero_()
+    v[at] = z[N * k:][:m]
+    near(dx, v.view(N, k, F).double().sum(1), 2 * U32 * v.view(N, k, F).double().abs().sum(1), "dx")
+    wd = weight.reshape(-1)[at][:, None] * dy[i].float()
+    assert torch.equal(dys[:m], wd.to(dtype)) and not dys[m:].any()
+    say("embed")
+    for V in (5, 3000):
+        index = torch.randint(0, V, (N,), generator=g, device=DEV, dtype=torch.int32)
+        check_embed(x[:V].contiguous(), index, 1.0, dy)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

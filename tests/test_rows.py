@@ -64,6 +64,10 @@ def test_kept_rows_refusals():
     bad("float32, bfloat16 or float16", ex.gated_silu, X.double())
     bad("x .* 2 F", ex.gated_silu, torch.zeros(4, 7))
     bad("x .* 2 F", ex.gated_silu, torch.zeros(4, 0))
+    many = torch.empty(1 << 31, 2, device="meta")
+    bad("2\\^31 rows", ex.pack_rows, many)
+    bad("2\\^31 rows", ex.gated_silu, many)
+    bad("2\\^31 rows", ex.unpack_rows, many.to(torch.float8_e4m3fn), many)
 
 
 def test_embed_refusals():
