@@ -13,11 +13,22 @@ operators: the FACE model itself calls none of them):
 
 and, for serving in 8 bits, rms_norm_q8 and quantize_rows in front of grouped_linear_q8.
 
+Around it, for whole models of such layers:
+
+    x = embed(table, species, scale)                       rows of a table, by species or pair of species
+    y, s = layer_norm(x, w, b, eps, residual=r)            the norm with the mean taken out, and layer_norm_q8
+    xs = expert_dispatch(y, plan)                          rows laid out by expert, for code of the user's own
+    h = gated_silu(u)                                      silu of one half of the hidden rows times the other
+    out = expert_return(v, plan, weight, residual=s)       such rows joined in the order of the atoms
+
+and training in less memory: layer_norm, gated_silu and grouped_linear with keep8=True keep what their backward reads in
+8 bits (pack_rows, unpack_rows).
+
 Rows are float32, bfloat16 or float16 (all tensors of a call alike, gate weights and scales float32); sums,
 softmax and norm statistics are float32. Every operator launches the kernels of
 libface_hip.so on torch's current stream of its tensors' device, allocates its results and workspaces with torch and never
 synchronises; none has a CPU path. They differentiate once, in training too: all of their floating
-inputs take gradients, except those of the 8-bit forms. Forward-mode derivatives are refused. Forward and backward are captured into a graph together,
+inputs take gradients, except those of the 8-bit forms for serving and of pack_rows. Forward-mode derivatives are refused. Forward and backward are captured into a graph together,
 as with torch's own operators on leaves of which no eager graph is alive (fresh ones, by detach().requires_grad_()).
 """
 import functools
