@@ -181,7 +181,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool some, int bits) 
     return m;
 }
 // A segment is shared out to the waves, a wave's share taken 64 keys at a time; up to kSortHeld of these are loaded together
-// (each load by itself was a trip to memory: 15 us a pass for 9 with a million keys).
+// (one by one, a million keys were placed in 16.6 us a pass for 15.4).
 constexpr int kSortHeld = 8;
 struct SortShare {
     int64_t begin, end;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void sort_count(const int32_t* key, const SortShare& 
         }
     }
 }
-// Workgroups behind the segments' clear the table's gradient, `zero` of 16-byte pieces each.
+// Workgroups behind the segments' clear the table's gradient: entries without a row.
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int32_t* __restrict__ key, int64_t N, int64_t seg, int segs,
                                                                   uint32_t V, int shift, int bits, int32_t* __restrict__ count,
                                                                   char* __restrict__ out, int64_t out_bytes) {

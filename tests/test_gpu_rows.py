@@ -689,6 +689,42 @@ def test_rows_by_expert_strides_and_some_gradients():
     assert torch.equal(a, b)
 
 
+def test_gradients_against_differences():
+    """Rows of a table, rows by expert and back: linear in each operand, so that a difference of any length is exact in 64 bits;
+    what is left is float32's rounding of sums of m terms."""
+    g = gen(14)
+    N, k, F = 70, 2, 50
+    plan, weight = sort_case(g, N, k, 4, F, F32)
+    m = int(plan.ptr[-1])
+    a = plan.order[:m].long()
+    i = a // k
+    index = torch.randint(-1, 6, (N,), generator=g, device=DEV)
+    table, ys, r = rand(g, 6, F), rand(g, N * k, F), rand(g, N, F)
+    d1, d2, d3 = rand(g, N, F), rand(g, N * k, F), rand(g, N, F)
+
+    def loss(table, ys, weight, r):
+        y = torch.where(index[:, None] >= 0, table[index.clamp_min(0)], 0.0) * 3.0
+        xs = torch.zeros(N * k, F, dtype=torch.float64, device=DEV)
+        xs[:m] = y[i]
+        out = r.index_add(0, i, ys[:m] * weight.reshape(-1)[a][:, None])
+        return (y * d1.double()).sum() + (xs * d2.double()).sum() + (out * d3.double()).sum()
+
+    l = [leaf(t) for t in (table, ys, weight, r)]
+    y = ex.embed(l[0], index, 3.0)
+    xs = ex.expert_dispatch(y, plan)
+    out = ex.expert_return(l[1], plan, l[2], residual=l[3])
+    grads = torch.autograd.grad([y, xs, out], l, [d1, d2, d3])
+    for j, t in enumerate(l):
+        v = rand(g, *t.shape).double()
+        at = [z.detach().double() for z in l]
+        hi, lo = list(at), list(at)
+        hi[j], lo[j] = at[j] + v, at[j] - v
+        want = (loss(*hi) - loss(*lo)) / 2
+        # a gradient's element is a sum of at most 3 N terms of order 3 x 3, each direction's element of order 3
+        n = t.numel()
+        assert abs((grads[j].double() * v).sum() - want) <= 3 * N * U32 * 27 * n ** 0.5 * 10, j
+
+
 # ----------------------------------------------------------------------------- together
 class Layer:
     """Species rows, norm, rows by expert, one product per expert, the gate, a product by group, and back."""
