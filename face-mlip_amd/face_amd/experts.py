@@ -404,7 +404,7 @@ def _gated_fwd(x, keep8=False):
     F = x.shape[-1] // 2
     x2 = _rows(x, 2 * F)
     N = x2.shape[0]
-    y = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], F))
     q = _work(N * 2 * F, x.device) if keep8 else None
     scale = _work(N * 2 * _blocks(F), x.device) if keep8 else None
     _launch(x, "face_gated_silu_fwd", "gated_silu_fwd", x2.data_ptr(), x2.stride(0), N, F, _DTYPES[x.dtype], y.data_ptr(), ptr(q),
@@ -435,7 +435,7 @@ class GatedSiLU(torch.autograd.Function):
         x = q = scale = None
         if keep8:
             q, scale = (ptr(t) for t in ctx.saved_tensors)
-            dx = torch.empty(*dy.shape[:-1], ld, dtype=dy.dtype, device=dy.device)
+            dx = dy.new_empty((*dy.shape[:-1], ld))
         else:
             x, = ctx.saved_tensors
             dx = torch.empty_like(x) if dense else _like(x)
@@ -465,7 +465,7 @@ def gated_silu(x, keep8=False):
 def _embed_fwd(table, index, factor, keys):
     V, F = table.shape
     t2, i = _rows(table, F), index.contiguous()
-    y = torch.empty(*index.shape, F, dtype=table.dtype, device=table.device)
+    y = table.new_empty((*index.shape, F))
     key = None
     wide = i.dtype == torch.int64
     if keys:
@@ -494,7 +494,7 @@ class Embed(torch.autograd.Function):
         if not dy.is_contiguous():
             dy = _rows(dy, F)
             ld = dy.stride(0)
-        dt = torch.empty(V, F, dtype=dy.dtype, device=dy.device)
+        dt = dy.new_empty((V, F))
         work = _work(need, dy.device)
         _launch(dt, "face_embed_bwd", "embed_bwd", key.data_ptr(), dy.data_ptr(), ld, N, V, F, code, factor, dt.data_ptr(), ptr(work),
                 need)
@@ -845,7 +845,7 @@ def _dispatch_fwd(x, p, order, k):
     F, slots = x.shape[1], order.shape[0]
     x2 = _rows(x, F)
     place = torch.empty_like(order) if _by_rows(slots, k, F) else None
-    xs = torch.empty(slots, F, dtype=x.dtype, device=x.device)
+    xs = x.new_empty((slots, F))
     _launch(x, "face_expert_dispatch", "expert_dispatch", x2.data_ptr(), x2.stride(0), k, p.data_ptr(), order.data_ptr(), ptr(place),
             x.shape[0], p.shape[0] - 1, F, _DTYPES[x.dtype], xs.data_ptr())
     return xs, place
@@ -891,7 +891,7 @@ def _return_fwd(y, p, order, place, weight, residual, N, k):
     placed = place is not None
     if not placed:
         place = torch.empty_like(order)
-    out = torch.empty(N, F, dtype=y.dtype, device=y.device)
+    out = y.new_empty((N, F))
     _launch(y, "face_expert_return_fwd", "expert_return_fwd", y2.data_ptr(), y2.stride(0), p.data_ptr(), order.data_ptr(),
             place.data_ptr(), int(placed), ptr(w), ptr(r), F if r is None else r.stride(0), N, k, p.shape[0] - 1, F,
             _DTYPES[y.dtype], out.data_ptr())
@@ -916,9 +916,9 @@ class ExpertReturn(torch.autograd.Function):
             y, weight, p, order, place = ctx.saved_tensors
             N, k, F, G, code = ctx.known
             if need_y:
-                dy = torch.empty(N * k, F, dtype=dout.dtype, device=dout.device)
+                dy = dout.new_empty((N * k, F))
             if need_w:
-                dw = torch.empty(N, k, dtype=torch.float32, device=dout.device)
+                dw = dout.new_empty((N, k), dtype=torch.float32)
             d2, w = _rows(dout, F), None if weight is None else weight.contiguous()
             y2 = _rows(y, F) if need_w else None
             _launch(dout, "face_expert_return_bwd", "expert_return_bwd", d2.data_ptr(), d2.stride(0), ptr(y2),
