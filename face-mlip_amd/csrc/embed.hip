@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
                                                         int32_t* __restrict__ key) {
     constexpr int E = Sixteen<T>::E;
     const int groups = 256 >> lg, lane = threadIdx.x & ((1 << lg) - 1);
-    const int64_t n0 = (int64_t)blockIdx.x * groups * R + (threadIdx.x >> lg);
+    const int64_t n0 = row_block() * groups * R + (threadIdx.x >> lg);
     I v[R];
     bool in[R];
 #pragma unroll
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
 // ---------------------------------------------------------------- sums of sorted rows
 template <typename T>
 __global__ __launch_bounds__(256) void embed_zero_kernel(T* __restrict__ out, int64_t n) {
-    const int64_t i = kPiece * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    const int64_t i = kPiece * (row_block() * 256 + threadIdx.x);
     if (i >= n) return;
     const float none[kPiece] = {};
     store_piece(out + i, n - i < kPiece ? (int)(n - i) : kPiece, none);
@@ -549,7 +549,7 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int F, int size) {
         if (few_rows) {
             p.R = N < 1 ? 1 : N;
             p.chunks = 1;
-            p.TV = 1;
+            p.TV = (V + (1 << 22) - 1) >> 22;        // one, but for millions of entries: a grid's dimension ends at 2^32 threads
         } else {
             const int64_t r = N * tiles / 2048 / 64 * 64;
             p.R = r < 64 ? 64 : (r > 1024 ? 1024 : r);
@@ -584,7 +584,7 @@ static void embed_sort(const int32_t* key, int64_t N, int64_t V, int F, T* out, 
         int n2 = 2;
         while (n2 < N) n2 *= 2;
         hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(1024), 0, st, key, (int)N, (uint32_t)V, n2, k[0], r[0]);
-        hipLaunchKernelGGL(embed_zero_kernel<T>, dim3((unsigned)((V * F + 256 * kPiece - 1) / (256 * kPiece))), dim3(256), 0, st, out,
+        hipLaunchKernelGGL(embed_zero_kernel<T>, row_grid((V * F + 256 * kPiece - 1) / (256 * kPiece)), dim3(256), 0, st, out,
                            V * F);
         key_out = k[0];
         row_out = r[0];
@@ -671,7 +671,7 @@ extern "C" int face_embed_fwd(const void* table, int64_t ld_t, const void* index
         while (lg < 8 && (1 << lg) < sixteens) ++lg;
         const bool nt = N * F * (int64_t)sizeof(T) > kEmbedStream, cut = F % Sixteen<T>::E;
         const int64_t groups = 256 >> lg, many = nt || N >= groups * 4096 ? 4 : 1;   // four rows a group once that fills the card
-        const dim3 grid((unsigned)((N + groups * many - 1) / (groups * many)));
+        const dim3 grid = row_grid((N + groups * many - 1) / (groups * many));
         auto launch = [&](auto* i) {
             using I = std::remove_cv_t<std::remove_pointer_t<decltype(i)>>;
             with_forms(nt, cut, [&](auto nt_, auto cut_) {

@@ -251,6 +251,13 @@ __device__ __forceinline__ void store16(T* row, int c, int F, const float x[Sixt
     }
 }
 
+// Workgroups in two dimensions: one of them holds fewer than 2^32 threads.
+static inline dim3 row_grid(int64_t blocks) {
+    constexpr int64_t kSide = 1 << 22;
+    return blocks <= kSide ? dim3((unsigned)blocks) : dim3((unsigned)kSide, (unsigned)((blocks + kSide - 1) / kSide));
+}
+__device__ __forceinline__ int64_t row_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Sum over a wave in a fixed order, the same in every lane, without a trip through LDS.
 __device__ __forceinline__ float wave_sum(float v) {
     v = row16_sum(v);

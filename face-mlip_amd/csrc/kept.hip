@@ -24,7 +24,7 @@ struct RowAt {
     int lane, lanes;
 };
 __device__ __forceinline__ RowAt row_at(int lg) {
-    return {(int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg), (int)threadIdx.x & ((1 << lg) - 1), 1 << lg};
+    return {row_block() * (256 >> lg) + (threadIdx.x >> lg), (int)threadIdx.x & ((1 << lg) - 1), 1 << lg};
 }
 
 template <typename T, bool NT, bool CUT>
@@ -134,7 +134,7 @@ static int kept_args(int64_t N, int32_t F, int32_t dtype) {
     if (F > kKeptMax || N > (int64_t)0x7fffffff) return FACE_ERR_UNSUPPORTED;
     return 0;
 }
-static dim3 kept_grid(int64_t N, int lg) { return dim3((unsigned)((N + (256 >> lg) - 1) >> (8 - lg))); }
+static dim3 kept_grid(int64_t N, int lg) { return row_grid((N + (256 >> lg) - 1) >> (8 - lg)); }
 
 }  // namespace face
 

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(LnFwd
     using Unit = LnUnit<T, LANES, U, CUT>;
     __shared__ float part[LANES / 32 + 1];
     const int lane = threadIdx.x % LANES, F = a.F;
-    const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
+    const int64_t n = row_block() * kRows + threadIdx.x / LANES;
     if (n >= a.N) return;                        // a whole row's threads; rows of several waves have a workgroup each
     const T *w = (const T*)a.w, *b = (const T*)a.b;
     float v[U][kPiece];
@@ -207,7 +207,8 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnFwdArgs a) {
     constexpr int LANES = 1024;
     __shared__ float part[LANES / 32 + 1];
     const int lane = threadIdx.x, F = a.F;
-    const int64_t n = blockIdx.x;
+    const int64_t n = row_block();
+    if (n >= a.N) return;
     const T *w = (const T*)a.w, *b = (const T*)a.b;
     const T* x = (const T*)a.x + n * a.ld_x;
     const int end = (F + kKeptBlock - 1) / kKeptBlock * kKeptBlock;      // whole quads
@@ -526,7 +527,7 @@ static int launch_ln_fwd(const LnFwdArgs& a, hipStream_t st) {
     const RowShape sh = ln_shape(a.F);
     const int64_t rows = ln_rows(a.F), blocks = (a.N + rows - 1) / rows;
     if (blocks > 0x7fffffff) return FACE_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid = row_grid(blocks);
     const bool nt = streams<T>(a.N * a.F * (a.r ? 4 : 2)), cut = a.F % Sixteen<T>::E;
     if (a.F > kLnHeld) {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, MODE>), grid, dim3(1024), 0, st, a);

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void dispatch_gather_kernel(const T* __restric
                                                               const int32_t* __restrict__ order, int64_t slots, int k, int G,
                                                               int F, int lg, T* __restrict__ xs) {
     constexpr int E = Sixteen<T>::E;
-    const int64_t p = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    const int64_t p = row_block() * (256 >> lg) + (threadIdx.x >> lg);
     if (p >= slots) return;
     const int a = p < places_of(ptr, G, slots) ? order[p] : -1;
     const bool some = a >= 0 && a < slots;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(const T* __restri
                                                                const int32_t* __restrict__ place, int64_t slots, int k, int G,
                                                                int F, int lg, T* __restrict__ xs) {
     constexpr int E = Sixteen<T>::E;
-    const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    const int64_t n = row_block() * (256 >> lg) + (threadIdx.x >> lg);
     if (n * k >= slots) return;
     const int64_t m = places_of(ptr, G, slots);
     constexpr int J = 4;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void return_fwd_kernel(const T* __restrict__ y
                                                          const float* __restrict__ w, const T* __restrict__ r, int64_t ld_r,
                                                          int64_t N, int k, int F, int lg, T* __restrict__ out) {
     constexpr int E = Sixteen<T>::E;
-    const int64_t n = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    const int64_t n = row_block() * (256 >> lg) + (threadIdx.x >> lg);
     if (n >= N) return;
     constexpr int J = 4;
     int p[J];
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void return_bwd_kernel(const T* __restrict__ d
     constexpr int E = Sixteen<T>::E;
     __shared__ float part[LANES / 64 + 1];
     const int lane = threadIdx.x % LANES;
-    const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t n = row_block() * (256 / LANES) + threadIdx.x / LANES;
     if (n >= N) return;
     const int64_t slots = N * k, m = places_of(ptr, G, slots);
     constexpr int J = 4;
@@ -229,7 +229,7 @@ static void launch_places(const int32_t* ptr, const int32_t* order, int64_t slot
     hipLaunchKernelGGL(places_none_kernel, grid, dim3(256), 0, st, slots, place);
     hipLaunchKernelGGL(places_kernel, grid, dim3(256), 0, st, ptr, order, slots, G, place);
 }
-static dim3 sorted_grid(int64_t rows, int lg) { return dim3((unsigned)((rows + (256 >> lg) - 1) >> (8 - lg))); }
+static dim3 sorted_grid(int64_t rows, int lg) { return row_grid((rows + (256 >> lg) - 1) >> (8 - lg)); }
 
 }  // namespace face
 
@@ -290,7 +290,7 @@ extern "C" int face_expert_return_bwd(const void* dout, int64_t ld_d, const void
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int L = F * sizeof(T) <= 256 ? 16 : (F * sizeof(T) <= 8192 ? 64 : 256), rows = 256 / L;
-        const dim3 grid((unsigned)((N + rows - 1) / rows));
+        const dim3 grid = row_grid((N + rows - 1) / rows);
         with_forms(streams<T>((2 * N * k + N) * F), F % Sixteen<T>::E, [&](auto nt, auto cut) {
             auto* kern = L == 16 ? return_bwd_kernel<T, 16, nt.value, cut.value>
                        : L == 64 ? return_bwd_kernel<T, 64, nt.value, cut.value> : return_bwd_kernel<T, 256, nt.value, cut.value>;

@@ -1038,6 +1038,60 @@ def test_large_calls_give_the_rows_of_small_ones(dtype, F):
         check_embed(x[:V].contiguous(), index, 1.0, dy)
 
 
+@pytest.mark.parametrize("keep8", [False, True])
+def test_more_rows_than_one_dimension_of_a_grid(keep8):
+    """Hundreds of millions of narrow rows, more workgroups than a grid takes side by side: the last rows are those of a
+    small call."""
+    g = gen(4)
+    N = 71000003
+    base = rand(g, 4099, 2, dtype=BF16)
+    x = base.repeat(N // 4099 + 1, 1)[:N]
+    tail = slice(N - 5000, N)
+    w, b = rand(g, 2, dtype=BF16), rand(g, 2, dtype=BF16)
+    say("norm")
+    l, t = leaf(x), leaf(x[tail])
+    y, yt = ex.layer_norm(l, w, b, 1e-2, keep8=keep8), ex.layer_norm(t, w, b, 1e-2, keep8=keep8)
+    assert torch.equal(y[tail], yt)
+    dx, = torch.autograd.grad([y], [l], [x])
+    dt, = torch.autograd.grad([yt], [t], [x[tail]])
+    assert torch.equal(dx[tail], dt)
+    del y, dx
+    say("by expert")
+    order = torch.arange(N - 1, -1, -1, dtype=torch.int32, device=DEV)
+    plan = ex.GroupPlan(torch.tensor([0, N], dtype=torch.int32, device=DEV), order, N)
+    xs = ex.expert_dispatch(x, plan)
+    assert torch.equal(xs[tail], x[:5000].flip(0)) and torch.equal(xs[:5000], x[tail].flip(0))
+    out = ex.expert_return(xs, plan)
+    assert torch.equal(out, x)
+    del xs, out, order, plan
+    say("gate")
+    z = x.repeat(4, 1)
+    tail = slice(4 * N - 5000, 4 * N)
+    l, t = leaf(z), leaf(z[tail])
+    y, yt = ex.gated_silu(l, keep8), ex.gated_silu(t, keep8)
+    assert torch.equal(y[tail], yt)
+    dx, = torch.autograd.grad([y], [l], [y.detach()])
+    dt, = torch.autograd.grad([yt], [t], [yt.detach()])
+    assert torch.equal(dx[tail], dt)
+    del y, dx
+    say("pack")
+    q, scale = ex.pack_rows(z)
+    q2, scale2 = ex.pack_rows(z[tail])
+    assert torch.equal(q[tail].view(torch.uint8), q2.view(torch.uint8))
+    assert torch.equal(ex.unpack_rows(q, scale)[tail], ex.unpack_rows(q2, scale2))
+
+
+def test_a_table_of_millions_of_entries():
+    """Few rows of it: every other entry's gradient is zero."""
+    g = gen(5)
+    V, F = 9000001, 3
+    table, index = rand(g, V, F), torch.randint(0, V, (300,), generator=g, device=DEV)
+    index[:40] = V - 1
+    check_embed(table, index, 2.0, rand(g, 300, F))
+    index = torch.randint(0, V, (900,), generator=g, device=DEV)
+    check_embed(table, index, 2.0, rand(g, 900, F))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_wide_embedding_gradient(dtype):
     """Rows of many column tiles, and of a width that no lane's piece divides."""
