@@ -273,7 +273,7 @@ class LayerNorm(torch.autograd.Function):
         N, F, code, keep8, need = ctx.known
         if keep8:
             w, q, block, stat = ctx.saved_tensors
-            mean, s, ld, q, block = None, None, F, q.data_ptr(), ptr(block)
+            mean, s, ld = None, None, F
         else:
             w, stat, s = ctx.saved_tensors
             s = _rows(s, F)
@@ -291,7 +291,7 @@ class LayerNorm(torch.autograd.Function):
             dy = _rows(dy, F)
         if ds is not None:
             ds = _rows(ds, F)
-        _launch(some, "face_layer_norm_rows_bwd", "layer_norm_bwd", ptr(s), ld, q, block, mean, stat.data_ptr(), ptr(dy),
+        _launch(some, "face_layer_norm_rows_bwd", "layer_norm_bwd", ptr(s), ld, ptr(q), ptr(block), mean, stat.data_ptr(), ptr(dy),
                 F if dy is None else dy.stride(0), ptr(ds), F if ds is None else ds.stride(0), N, F, code, w.data_ptr(), ptr(dx),
                 ptr(dw), ptr(db), ptr(work), need)
         return dx if need_x else None, dw, db, None, dx if need_r else None, None
@@ -434,7 +434,7 @@ class GatedSiLU(torch.autograd.Function):
             ld_dy = dy.stride(0)
         x = q = scale = None
         if keep8:
-            q, scale = (ptr(t) for t in ctx.saved_tensors)
+            q, scale = ctx.saved_tensors
             dx = dy.new_empty((*dy.shape[:-1], ld))
         else:
             x, = ctx.saved_tensors
@@ -442,8 +442,8 @@ class GatedSiLU(torch.autograd.Function):
             if not dense:
                 x = _rows(x, ld)
                 ld = x.stride(0)
-            x = x.data_ptr()
-        _launch(dx, "face_gated_silu_bwd", "gated_silu_bwd", x, ld, q, scale, dy.data_ptr(), ld_dy, N, F, code, dx.data_ptr())
+        _launch(dx, "face_gated_silu_bwd", "gated_silu_bwd", ptr(x), ld, ptr(q), ptr(scale), dy.data_ptr(), ld_dy, N, F, code,
+                dx.data_ptr())
         return dx, None
 
 

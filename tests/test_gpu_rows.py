@@ -689,6 +689,35 @@ def test_rows_by_expert_strides_and_some_gradients():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_operands_that_lie_by_columns(dtype):
+    """Operands whose rows are not one after the other are copied for the call: the same results as of the copies."""
+    g = gen(15)
+    cols = lambda n, f: rand(g, f, n, dtype=dtype).t()
+    plan, weight = sort_case(g, 40, 2, 4, 66, dtype)
+    index = torch.randint(0, 40, (90,), generator=g, device=DEV)
+    w, b = rand(g, 66, dtype=dtype), rand(g, 66, dtype=dtype)
+    wt = weight.t().contiguous().t()
+    x, r, ys, dy, dys, d3 = cols(40, 66), cols(40, 66), cols(80, 66), cols(40, 66), cols(80, 66), cols(90, 66)
+    lin = rand(g, 4, 5, 66, dtype=dtype)
+    calls = [(lambda x, r: ex.layer_norm(x, w, b, residual=r)[0], (x, r), dy),
+             (lambda x, r: ex.layer_norm(x, w, b, residual=r, keep8=True)[0], (x, r), dy),
+             (lambda x: ex.gated_silu(x), (x,), cols(40, 33)), (lambda x: ex.gated_silu(x, True), (x,), cols(40, 33)),
+             (lambda x: ex.embed(x, index, 2.0), (x,), d3), (lambda x: ex.expert_dispatch(x, plan), (x,), dys),
+             (lambda y, v, r: ex.expert_return(y, plan, v, residual=r), (ys, wt, r), dy),
+             (lambda x: ex.grouped_linear(x, lin, plan, keep8=True), (x,), cols(80, 5))]
+    for i, (f, operands, d) in enumerate(calls):
+        say("columns", dtype, i)
+        l, c = [leaf(t) for t in operands], [leaf(t.contiguous()) for t in operands]
+        y, yc = f(*l), f(*c)
+        assert torch.equal(y, yc), i
+        got = torch.autograd.grad([y], l, [d])
+        for a, o in zip(got, torch.autograd.grad([yc], c, [d.contiguous()])):
+            assert torch.equal(a, o), i
+    for a, o in zip(ex.pack_rows(x), ex.pack_rows(x.contiguous())):
+        assert torch.equal(a.view(torch.uint8), o.view(torch.uint8))
+
+
 def test_gradients_against_differences():
     """Rows of a table, rows by expert and back: linear in each operand, so that a difference of any length is exact in 64 bits;
     what is left is float32's rounding of sums of m terms."""
