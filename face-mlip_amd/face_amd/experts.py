@@ -373,8 +373,8 @@ def _unpack(q, scale, dtype):
 def pack_rows(x):
     """x (..., F) -> (q (..., F) float8_e4m3fn, scale (..., ceil(F / 32)) float8_e8m0fnu): rows as a backward pass
     keeps them in 8 bits, 1.03 bytes a value. Each 32 columns share a power of two, the least (>= 2^-126) that
-    keeps their largest magnitude within 448: a value is off by at most 2^-4 of itself or 2^-18 of the block's
-    largest. A NaN or an infinity is kept as NaN and leaves the others as they are. No gradients."""
+    keeps their largest magnitude within 448: a value is off by at most 2^-4 of itself or 2^-17 of the block's
+    largest (2^-136 where that is below 2^-118). A NaN or an infinity is kept as NaN and leaves the others as they are. No gradients."""
     _dtype("pack_rows", x)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_PACKED:
         _fail("pack_rows", f"rows of 1 to {MAX_PACKED} columns, got {tuple(x.shape)}")
